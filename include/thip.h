@@ -400,6 +400,87 @@ thip_status_t thip_hl_table(thip_program_t *program, const thip_hl_table_t *op);
 thip_status_t thip_hl_act(thip_program_t *program, const thip_hl_act_t *op);
 thip_status_t thip_hl_elementwisebinary(thip_program_t *program, const thip_hl_elementwisebinary_t *op);
 
+/* ---- Attention and its cache -------------------------------------------------------------------------------------
+ * Operators that no TorqHL op stands for (the reference has neither a softmax nor a cache): what a decoder needs
+ * between its linears.  Element types: queries, keys, values and results BF16; a cache BF16, or I8 with one F32 scale
+ * for each position and head.  Sums, softmax statistics and scores are held in 32 bits.
+ *
+ * Rows are packed: a tensor of T rows holds those of S sequences one behind the other.  row_starts is I32[S + 1],
+ * ascending: sequence s has the n_s rows row_starts[s] .. row_starts[s + 1] - 1.  Rows behind the last sequence's are
+ * neither read nor written.  A sequence may have no row.
+ *
+ * lengths is I32[S]: the positions that sequence s has, its n_s new rows among them, so that row i of them stands at
+ * position lengths[s] - n_s + i.  (A row at a position below 0 is not there: it is not stored, is read as zeros and
+ * attends to nothing.)
+ *
+ * A cache is a tensor [pages, kv_heads, page_size, D] of keys and another of values, with scales [pages, kv_heads,
+ * page_size].  pages is I32[S, P]: position p of sequence s lies in page pages[s][p / page_size], at p % page_size of
+ * it.  A position at or above P * page_size, or whose entry is no page of the cache, is not there either: what is
+ * written to it is dropped, it is read as zeros, and no row attends to it.
+ *
+ * row_starts, lengths and pages are read on the device when the dispatch runs (bindings, or constants), so one program
+ * serves every step of a batch whose lengths change; what they may hold is bounded by the tensors' sizes only.  The caches and
+ * scales are bindings, or views of them: they outlive a dispatch, and are written in place.  D is a multiple of 16 up to 256,
+ * and views start at multiples of 16 bytes. */
+
+/* Stores row i of key and value [T, kv_heads, D] at its position.  An I8 cache holds, for a row x of D elements with
+ * a = max(max |x|, 2^-100): scale = a / 127 and round(x * (127 / a)), to nearest with ties to even, all in 32 bits; a row
+ * with an infinity or a NaN has a NaN scale.  key_scales and value_scales are THIP_NO_VALUE for a BF16 cache.  Two
+ * rows of one call must not have the same place. */
+typedef struct thip_lm_cache_write_t {
+    thip_value_t key_cache;
+    thip_value_t value_cache;
+    thip_value_t key_scales;
+    thip_value_t value_scales;
+    thip_value_t key;
+    thip_value_t value;
+    thip_value_t pages;
+    thip_value_t row_starts;
+    thip_value_t lengths;
+} thip_lm_cache_write_t;
+
+/* Reads rows back into key and value [T, kv_heads, D], BF16: row i of sequence s is what the cache holds at position
+ * lengths[s] - n_s + i, from I8 as the product of value and scale, rounded once. */
+typedef struct thip_lm_cache_read_t {
+    thip_value_t key;
+    thip_value_t value;
+    thip_value_t key_cache;
+    thip_value_t value_cache;
+    thip_value_t key_scales;
+    thip_value_t value_scales;
+    thip_value_t pages;
+    thip_value_t row_starts;
+    thip_value_t lengths;
+} thip_lm_cache_read_t;
+
+/* Attention of packed rows: init and query [T, heads, D]; heads is a multiple of kv_heads, and query head h reads the
+ * key / value head h / (heads / kv_heads).  A row at position p sees position j of its own sequence where j <= p and
+ * (window == 0, or j > p - window, or j < sinks):
+ *     init = sum_j w_j value_j / sum_j w_j,  w_j = exp(scale * (query . key_j) - max over the seen ones),
+ * and zeros where it sees nothing.  What lies at positions that a row does not see has no influence on it, whatever its
+ * bits.  Either over the rows themselves -- key and value [T, kv_heads, D], pages and lengths THIP_NO_VALUE: row i of
+ * a sequence stands at position i, a prompt without a cache -- or over a cache, where key and value are the caches
+ * (and key_scales, value_scales those of an I8 cache) and the new rows' keys and values are there already (thip_lm_cache_write
+ * before it).  init may be the query's own bytes; no other operand may share bytes with init. */
+typedef struct thip_lm_attention_t {
+    thip_value_t init;
+    thip_value_t query;
+    thip_value_t key;
+    thip_value_t value;
+    thip_value_t key_scales;
+    thip_value_t value_scales;
+    thip_value_t pages;
+    thip_value_t row_starts;
+    thip_value_t lengths;
+    float scale;
+    int32_t window;
+    int32_t sinks;
+} thip_lm_attention_t;
+
+thip_status_t thip_lm_cache_write(thip_program_t *program, const thip_lm_cache_write_t *op);
+thip_status_t thip_lm_cache_read(thip_program_t *program, const thip_lm_cache_read_t *op);
+thip_status_t thip_lm_attention(thip_program_t *program, const thip_lm_attention_t *op);
+
 /* Serialises the program (role of TargetBackend::serializeExecutable,
  * compiler/torq/Target/TorqTarget.cpp:115-151, and serializeTorqHW,
  * compiler/torq/Serialization/Serialization.cpp:265-302): picks a kernel

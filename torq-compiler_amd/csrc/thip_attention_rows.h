@@ -1,0 +1,59 @@
+// Device side of the packed rows and of the paged cache: whose a row is, at which position it stands, and where a position lies.
+#pragma once
+
+#include "thip_attention.h"
+#include "thip_kernels_common.h"
+
+namespace thip {
+
+struct RowPlace {
+    int seq;    // -1: no sequence's
+    int begin;  // its first row
+    int count;  // its rows
+    int pos;    // the row's position
+};
+
+// Rows [begin, begin + count) of sequence s; kept inside the tensors whatever row_starts holds.
+__device__ __forceinline__ void rowsOf(const CacheArgs &c, const int32_t *starts, int s, int *begin, int *count) {
+    const int b = min(max(starts[s], 0), c.T), e = min(max(starts[s + 1], b), c.T);
+    *begin = b;
+    *count = e - b;
+}
+
+// The position of a sequence's row 0 (rows stand behind one another).
+__device__ __forceinline__ int firstPosition(const CacheArgs &c, int s, int count) { return c.lengths ? max(c.lengths[s], 0) - count : 0; }
+
+// The last sequence that starts at or before the row (those without rows start where the next one does), if the row is one of its.
+__device__ __forceinline__ RowPlace placeOf(const CacheArgs &c, const int32_t *starts, int row) {
+    int lo = 0, hi = c.S;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    RowPlace p{-1, 0, 0, 0};
+    rowsOf(c, starts, lo, &p.begin, &p.count);
+    if (row < p.begin || row >= p.begin + p.count) return p;
+    p.seq = lo;
+    p.pos = firstPosition(c, lo, p.count) + (row - p.begin);
+    return p;
+}
+
+// Row of the cache that holds a position, -1: none does.
+__device__ __forceinline__ int64_t cacheRow(const CacheArgs &c, int seq, int head, int pos) {
+    if ((uint32_t)pos >= (uint32_t)c.capacity) return -1;
+    const uint32_t entry = fastDiv((uint32_t)pos, c.ps), slot = (uint32_t)pos - entry * c.ps.d;
+    const int32_t page = c.pages[(int64_t)seq * c.P + entry];
+    if ((uint32_t)page >= (uint32_t)c.NP) return -1;
+    return (int64_t)(((uint32_t)page * (uint32_t)c.KVH + (uint32_t)head) * (uint32_t)c.PS + slot);
+}
+
+// The starts in LDS, where they fit `most` sequences; every thread of the workgroup calls it.
+__device__ __forceinline__ const int32_t *holdStarts(const CacheArgs &c, int32_t *held, int most) {
+    if (c.S > most) return c.starts;
+    for (int i = threadIdx.x; i <= c.S; i += blockDim.x) held[i] = c.starts[i];
+    __syncthreads();
+    return held;
+}
+
+}  // namespace thip

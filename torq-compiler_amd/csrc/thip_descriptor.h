@@ -102,7 +102,22 @@ enum Kind : uint32_t {
     // every batch), weights = [TB][Nn][K] (w1 != 0: shared), out [TB][M][Nn]; M <= 32; bias0 = float bits of the one
     // bias, output_min / output_max = float bits of the clamp.
     kKindDecMatmul = 16,
+    // Rows to and from a paged cache, and attention (thip_lm_*).  M = rows T, N = sequences S, W = kv heads, C = D, H = heads
+    // (attention), OH = pages of the cache, KH = page size, KW = P, gran = bytes of a cache element (1: I8, 2: BF16); weights / bias
+    // = keys / values (the caches, or rows), scale = row_starts, table = a CacheExt in the constant segment.
+    // write: in0 / in1 = key / value rows, out = the key cache again.  read: out / in1 = key / value rows, both written.
+    kKindCacheWrite = 17,
+    kKindCacheRead = 18,
+    // in0 = query, out, bias0 = float bits of the scale, K = window, Kp = sinks, w0 = 1: over a cache (0: over the rows, no CacheExt),
+    // in1 = an intermediate of the record's own for partial results (attentionWorkspaceBytes; none where that is 0)
+    kKindAttention = 19,
 };
+
+// Operands of a record on a cache; bindings or constants, or none.
+struct CacheExt {
+    DescRef key_scales, value_scales, pages, lengths;
+};
+static_assert(sizeof(CacheExt) == 64, "CacheExt layout");
 
 enum DecLinearFlags : int32_t {
     kDecPair = 1,         // two matrices of equal width; a workgroup owns the same columns of both, the add joins them

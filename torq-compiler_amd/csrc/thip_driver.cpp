@@ -28,6 +28,7 @@
 #include <thread>
 #include <vector>
 
+#include "thip_attention.h"
 #include "thip_chain_turn.h"
 #include "thip_descriptor.h"
 #include "thip_host_copy.h"
@@ -139,6 +140,9 @@ static const char *opKernelName(const DescOp &op) {
     case kKindEltwise: return "eltwise_int";
     case kKindDecLinear: return "dec_linear";
     case kKindDecMatmul: return "dec_matmul";
+    case kKindCacheWrite: return "cache_write";
+    case kKindCacheRead: return "cache_read";
+    case kKindAttention: return "attention";
     default: return "unknown";
     }
 }
@@ -346,6 +350,38 @@ static thip_status_t launchOp(thip_executable_t *e, uint32_t i, const DescOp &op
         err = launchDecMatmul(a, ctx);
         break;
     }
+    case kKindCacheWrite: case kKindCacheRead: case kKindAttention: {
+        const bool attends = op.kind == kKindAttention;
+        CacheArgs c;
+        memset(&c, 0, sizeof(c));
+        c.starts = (const int32_t *)resolve(e, op.scale, bp);
+        c.T = op.M; c.S = op.N; c.KVH = op.W; c.D = op.C;
+        CacheExt x;
+        memset(&x, 0, sizeof(x));
+        if (!attends || op.w0 == 1) {
+            memcpy(&x, e->blob.data() + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset, sizeof(x));  // the host copy
+            c.lengths = (const int32_t *)resolve(e, x.lengths, bp);
+            c.pages = (const int32_t *)resolve(e, x.pages, bp);
+            c.P = op.KW; c.NP = op.OH; c.PS = op.KH;
+            c.capacity = op.KW * op.KH;
+            c.ps = makeFastDiv((uint32_t)op.KH);
+        }
+        float *keyScales = (float *)resolve(e, x.key_scales, bp), *valueScales = (float *)resolve(e, x.value_scales, bp);
+        uint8_t *keys = resolve(e, op.weights, bp), *values = resolve(e, op.bias, bp);
+        if (attends) {
+            AttentionArgs a{c, (const uint16_t *)resolve(e, op.in0, bp), (uint16_t *)resolve(e, op.out, bp), keys, values, keyScales, valueScales,
+                            op.H, op.H / op.W, 0.0f, op.K, op.Kp, resolve(e, op.in1, bp), 0};
+            memcpy(&a.scale, &op.bias0, 4);
+            if (op.in1.space == kSpaceTemp) a.work_bytes = (size_t)(e->temps[op.in1.index].size - op.in1.offset);
+            err = launchAttention(a, ctx);
+        } else {
+            const bool write = op.kind == kKindCacheWrite;
+            CacheRowsArgs a{c, (uint16_t *)resolve(e, write ? op.in0 : op.out, bp), (uint16_t *)resolve(e, op.in1, bp), keys, values, keyScales, valueScales,
+                            makeFastDiv((uint32_t)op.W)};
+            err = write ? launchCacheWrite(a, ctx) : launchCacheRead(a, ctx);
+        }
+        break;
+    }
     default: return fail(THIP_INTERNAL, "op %u has unknown kind %u", i, op.kind);
     }
     if (err != hipSuccess) {
@@ -474,6 +510,9 @@ static thip_status_t dumpOpOutput(thip_executable_t *e, uint32_t i, uint8_t *con
     case kKindDepthwiseBf16: shape = {op.N, op.OH, op.OW, op.C}; bf16(); break;
     case kKindAvgPoolBf16: shape = {op.N, op.C}; bf16(); break;
     case kKindExpandWeights: shape = {op.K, op.Nn}; bf16(); break;
+    case kKindCacheWrite: shape = {op.OH, op.W, op.KH, op.C}; if (op.gran == 2) bf16(); break;
+    case kKindCacheRead: shape = {op.M, op.W, op.C}; bf16(); break;
+    case kKindAttention: shape = {op.M, op.H, op.C}; bf16(); break;
     default: return THIP_OK;
     }
     size_t count = 1;

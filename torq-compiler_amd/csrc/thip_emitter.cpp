@@ -22,6 +22,7 @@
 #include <string>
 #include <vector>
 
+#include "thip_attention.h"
 #include "thip_descriptor.h"
 #include "thip_kernels.h"
 #include "thip_status.h"
@@ -48,7 +49,7 @@ struct Value {
     }
 };
 
-enum HlKind { kHlConv2d, kHlDepthwise, kHlFullyConnected, kHlMatmul, kHlMaxPool, kHlAvgPool, kHlAdd, kHlTranspose, kHlExpandWeights, kHlFma, kHlMul, kHlAct, kHlBinary, kHlUnary, kHlShift, kHlTable };
+enum HlKind { kHlConv2d, kHlDepthwise, kHlFullyConnected, kHlMatmul, kHlMaxPool, kHlAvgPool, kHlAdd, kHlTranspose, kHlExpandWeights, kHlFma, kHlMul, kHlAct, kHlBinary, kHlUnary, kHlShift, kHlTable, kLmCacheWrite, kLmCacheRead, kLmAttention };
 
 struct HlOp {
     HlKind kind;
@@ -69,6 +70,9 @@ struct HlOp {
         thip_hl_elementwiseunary_t un;
         thip_hl_elementwiseshift_t sh;
         thip_hl_table_t tab;
+        thip_lm_cache_write_t cw;
+        thip_lm_cache_read_t cr;
+        thip_lm_attention_t at;
     } u;
     std::string name;
     std::vector<int32_t> staticTable;  // torq_hl.table: the caller's static_table, copied
@@ -714,6 +718,15 @@ class Emitter {
     thip_status_t emitShift(const thip_hl_elementwiseshift_t &c);
     thip_status_t emitTable(const thip_hl_table_t &c, const std::vector<int32_t> &staticTable);
     // Operands of an integer elementwise op: element types, and the record's common fields.
+    // Attention and its cache (thip_lm_*).
+    thip_status_t boundPart(thip_value_t id, const char *what, int32_t dtype, int32_t rank, bool written, DescRef *out);
+    thip_status_t indexOperand(thip_value_t id, const char *what, int32_t rank, DescRef *out);
+    thip_status_t batchOperands(thip_value_t starts, thip_value_t lengths, thip_value_t pages, bool cached, DescOp *op, CacheExt *ext);
+    thip_status_t cacheOperands(thip_value_t key, thip_value_t value, thip_value_t keyScales, thip_value_t valueScales, bool written, DescOp *op, CacheExt *ext);
+    thip_status_t rowOperand(thip_value_t id, const char *what, bool written, int64_t T, int64_t heads, int64_t D, DescRef *out);
+    thip_status_t emitCacheWrite(const thip_lm_cache_write_t &c);
+    thip_status_t emitCacheRead(const thip_lm_cache_read_t &c);
+    thip_status_t emitAttention(const thip_lm_attention_t &c);
     thip_status_t eltwiseCommon(const char *what, thip_value_t input, thip_value_t init, DescOp *op);
     thip_status_t emitAvgPoolBf16(const thip_hl_avg_pool2d_t &c);
     // ---- decode-shaped bf16 programs (at most 32 rows per matmul): fewer, wider launches -----------------------
@@ -1937,6 +1950,246 @@ thip_status_t Emitter::emitTransposeOp(const thip_hl_transpose_t &c) {
 // that computes both and adds (gate and up), the add behind a linear moves into its epilogue (residual connections),
 // and a transpose in front of a matmul's input2 is read in place.  THIP_NO_DECODE_FUSION leaves every op its own record.
 
+// ---- attention and its cache ------------------------------------------------------------------------------------------
+
+// A binding, or a view of one, in place.
+thip_status_t Emitter::boundPart(thip_value_t id, const char *what, int32_t dtype, int32_t rank, bool written, DescRef *out) {
+    const Value *v;
+    if (thip_status_t s = checkValue(id, what, &v)) return s;
+    if (v->dtype != dtype) return fail(THIP_INVALID_ARGUMENT, "%s: wrong element type", what);
+    if (v->rank != rank) return fail(THIP_INVALID_ARGUMENT, "%s: rank %d, expected %d", what, v->rank, rank);
+    const Value &root = v->kind == kValueView ? prog_.values[(size_t)v->base] : *v;
+    if (root.kind != kValueBinding) return fail(THIP_INVALID_ARGUMENT, "%s: must be a binding, or a view of one", what);
+    *out = bindingRef(root, false);
+    if (written) *out = bindingRef(root, true);
+    if (v->kind == kValueView) out->offset += (uint64_t)v->viewOffset * elemSize(dtype);
+    return THIP_OK;
+}
+
+// What the device reads to find rows and pages: a binding, a view of one, or a constant.
+thip_status_t Emitter::indexOperand(thip_value_t id, const char *what, int32_t rank, DescRef *out) {
+    const Value *v;
+    if (thip_status_t s = checkValue(id, what, &v)) return s;
+    if (v->kind != kValueConstant) return boundPart(id, what, THIP_DTYPE_I32, rank, false, out);
+    if (v->dtype != THIP_DTYPE_I32) return fail(THIP_INVALID_ARGUMENT, "%s: wrong element type", what);
+    if (v->rank != rank) return fail(THIP_INVALID_ARGUMENT, "%s: rank %d, expected %d", what, v->rank, rank);
+    return literalInput(id, what, out);
+}
+
+thip_status_t Emitter::batchOperands(thip_value_t starts, thip_value_t lengths, thip_value_t pages, bool cached, DescOp *op, CacheExt *ext) {
+    if (thip_status_t s = indexOperand(starts, "row_starts", 1, &op->scale)) return s;
+    const int64_t S = prog_.values[(size_t)starts].shape[0] - 1;
+    if (!fitsInt32(S)) return fail(THIP_INVALID_ARGUMENT, "row_starts: holds %lld values, the sequences and one more are needed", (long long)(S + 1));
+    op->N = (int32_t)S;
+    if (!cached) return THIP_OK;
+    if (thip_status_t s = indexOperand(lengths, "lengths", 1, &ext->lengths)) return s;
+    if (thip_status_t s = indexOperand(pages, "pages", 2, &ext->pages)) return s;
+    const Value &l = prog_.values[(size_t)lengths], &p = prog_.values[(size_t)pages];
+    if (l.shape[0] != S || p.shape[0] != S) {
+        return fail(THIP_INVALID_ARGUMENT, "lengths of %lld sequences and pages of %lld, row_starts has %lld", (long long)l.shape[0], (long long)p.shape[0], (long long)S);
+    }
+    if (!fitsInt32(p.shape[1])) return fail(THIP_UNIMPLEMENTED, "pages: %lld entries for a sequence", (long long)p.shape[1]);
+    op->KW = (int32_t)p.shape[1];
+    return THIP_OK;
+}
+
+thip_status_t Emitter::cacheOperands(thip_value_t key, thip_value_t value, thip_value_t keyScales, thip_value_t valueScales, bool written, DescOp *op, CacheExt *ext) {
+    const Value *k, *v;
+    if (thip_status_t s = checkValue(key, "key_cache", &k)) return s;
+    if (thip_status_t s = checkValue(value, "value_cache", &v)) return s;
+    if (k->dtype != THIP_DTYPE_I8 && k->dtype != THIP_DTYPE_BF16) return fail(THIP_UNIMPLEMENTED, "key_cache: a cache is int8 or bf16");
+    if (thip_status_t s = boundPart(key, "key_cache", k->dtype, 4, written, &op->weights)) return s;
+    if (thip_status_t s = boundPart(value, "value_cache", k->dtype, 4, written, &op->bias)) return s;
+    for (int i = 0; i < 4; i++) {
+        if (k->shape[i] != v->shape[i]) return fail(THIP_INVALID_ARGUMENT, "key_cache and value_cache differ in dimension %d", i);
+    }
+    if ((op->weights.offset | op->bias.offset) & 15) return fail(THIP_UNIMPLEMENTED, "a cache that starts at no multiple of 16 bytes");
+    const int64_t D = k->shape[3];
+    if (D % 16 != 0 || D > kMaxHeadDim) return fail(THIP_UNIMPLEMENTED, "rows of %lld elements: multiples of 16 up to %d", (long long)D, kMaxHeadDim);
+    // one by one: the product of three is then below 2^31 too
+    if (!fitsInt32(k->shape[0]) || !fitsInt32(k->shape[1]) || !fitsInt32(k->shape[2]) || !fitsInt32(k->shape[0] * k->shape[1]) || !fitsInt32(k->shape[0] * k->shape[1] * k->shape[2])) {
+        return fail(THIP_UNIMPLEMENTED, "a cache of more than 2^31 rows");
+    }
+    if (!fitsInt32((int64_t)op->KW * k->shape[2])) return fail(THIP_UNIMPLEMENTED, "pages: more than 2^31 positions for a sequence");
+    if (k->dtype == THIP_DTYPE_I8) {
+        if (thip_status_t s = boundPart(keyScales, "key_scales", THIP_DTYPE_F32, 3, written, &ext->key_scales)) return s;
+        if (thip_status_t s = boundPart(valueScales, "value_scales", THIP_DTYPE_F32, 3, written, &ext->value_scales)) return s;
+        for (int i = 0; i < 3; i++) {
+            if (prog_.values[(size_t)keyScales].shape[i] != k->shape[i] || prog_.values[(size_t)valueScales].shape[i] != k->shape[i]) {
+                return fail(THIP_INVALID_ARGUMENT, "the scales differ from the caches in dimension %d", i);
+            }
+        }
+    } else if (keyScales != THIP_NO_VALUE || valueScales != THIP_NO_VALUE) {
+        return fail(THIP_INVALID_ARGUMENT, "a bf16 cache has no scales");
+    }
+    op->gran = (uint32_t)elemSize(k->dtype);
+    op->OH = (int32_t)k->shape[0];
+    op->W = (int32_t)k->shape[1];
+    op->KH = (int32_t)k->shape[2];
+    op->C = (int32_t)D;
+    return THIP_OK;
+}
+
+// Packed rows [T, heads, D], bf16.  Rows of no sequence stay as they are, so what is written is also an input of the dispatch.
+thip_status_t Emitter::rowOperand(thip_value_t id, const char *what, bool written, int64_t T, int64_t heads, int64_t D, DescRef *out) {
+    const Value *v;
+    if (thip_status_t s = checkValue(id, what, &v)) return s;
+    if (v->dtype != THIP_DTYPE_BF16) return fail(THIP_INVALID_ARGUMENT, "%s: rows are bf16", what);
+    if (v->rank != 3 || v->shape[0] != T || v->shape[1] != heads || v->shape[2] != D) {
+        return fail(THIP_INVALID_ARGUMENT, "%s: expected [%lld, %lld, %lld]", what, (long long)T, (long long)heads, (long long)D);
+    }
+    if (v->kind == kValueConstant && written) return fail(THIP_INVALID_ARGUMENT, "%s: cannot be a constant", what);
+    if (!written) {
+        if (thip_status_t s = literalInput(id, what, out)) return s;
+        if (state_[(size_t)id].nhwcOfNchw) return fail(THIP_UNIMPLEMENTED, "%s: an N,C,H,W intermediate", what);
+    } else {
+        if (thip_status_t s = literalOutput(id, what, THIP_DTYPE_BF16, v->numel(), out)) return s;
+        const Value &root = v->kind == kValueView ? prog_.values[(size_t)v->base] : *v;
+        if (root.kind == kValueBinding) bindingRef(root, false);
+    }
+    if (out->offset & 15) return fail(THIP_UNIMPLEMENTED, "%s: a view at an offset that is no multiple of 16 bytes", what);
+    return THIP_OK;
+}
+
+// Operands of one op that may not share bytes: what it writes, with everything else.
+struct Extent {
+    DescRef ref;
+    uint64_t bytes;
+    bool written;
+    const char *what;
+};
+static thip_status_t checkApart(const std::vector<Extent> &all) {
+    for (size_t i = 0; i < all.size(); i++) {
+        for (size_t j = i + 1; j < all.size(); j++) {
+            const Extent &a = all[i], &b = all[j];
+            if (!a.written && !b.written) continue;
+            if (a.ref.space == kSpaceNone || a.ref.space != b.ref.space || a.ref.index != b.ref.index) continue;
+            if (a.ref.offset < b.ref.offset + b.bytes && b.ref.offset < a.ref.offset + a.bytes) {
+                return fail(THIP_INVALID_ARGUMENT, "%s and %s share bytes", a.what, b.what);
+            }
+        }
+    }
+    return THIP_OK;
+}
+
+// What the record's index operands and caches take of their buffers.
+static void addExtents(const DescOp &op, const CacheExt &x, bool cacheWritten, std::vector<Extent> *all) {
+    const uint64_t rows = (uint64_t)op.OH * op.W * op.KH, elems = rows * op.C * op.gran;
+    all->push_back({op.scale, ((uint64_t)op.N + 1) * 4, false, "row_starts"});
+    all->push_back({x.lengths, (uint64_t)op.N * 4, false, "lengths"});
+    all->push_back({x.pages, (uint64_t)op.N * op.KW * 4, false, "pages"});
+    all->push_back({x.key_scales, rows * 4, cacheWritten, "key_scales"});
+    all->push_back({x.value_scales, rows * 4, cacheWritten, "value_scales"});
+    all->push_back({op.weights, elems, cacheWritten, "key_cache"});
+    all->push_back({op.bias, elems, cacheWritten, "value_cache"});
+}
+
+thip_status_t Emitter::emitCacheWrite(const thip_lm_cache_write_t &c) {
+    const Value *k;
+    if (thip_status_t s = checkValue(c.key, "key", &k)) return s;
+    DescOp op;
+    memset(&op, 0, sizeof(op));
+    CacheExt ext{};
+    op.kind = kKindCacheWrite;
+    if (thip_status_t s = batchOperands(c.row_starts, c.lengths, c.pages, true, &op, &ext)) return s;
+    if (thip_status_t s = cacheOperands(c.key_cache, c.value_cache, c.key_scales, c.value_scales, true, &op, &ext)) return s;
+    const int64_t T = k->shape[0];
+    if (!fitsInt32(T) || !fitsInt32(T * op.W)) return fail(THIP_UNIMPLEMENTED, "key: more than 2^31 rows");
+    if (thip_status_t s = rowOperand(c.key, "key", false, T, op.W, op.C, &op.in0)) return s;
+    if (thip_status_t s = rowOperand(c.value, "value", false, T, op.W, op.C, &op.in1)) return s;
+    op.M = (int32_t)T;
+    op.out = op.weights;
+    const uint64_t rows = (uint64_t)T * op.W * op.C * 2;
+    std::vector<Extent> all{{op.in0, rows, false, "key"}, {op.in1, rows, false, "value"}};
+    addExtents(op, ext, true, &all);
+    if (thip_status_t s = checkApart(all)) return s;
+    op.table = newConst(std::vector<CacheExt>{ext});
+    ops_.push_back(op);
+    return THIP_OK;
+}
+
+thip_status_t Emitter::emitCacheRead(const thip_lm_cache_read_t &c) {
+    const Value *k;
+    if (thip_status_t s = checkValue(c.key, "key", &k)) return s;
+    DescOp op;
+    memset(&op, 0, sizeof(op));
+    CacheExt ext{};
+    op.kind = kKindCacheRead;
+    op.out_dtype = THIP_DTYPE_BF16;
+    if (thip_status_t s = batchOperands(c.row_starts, c.lengths, c.pages, true, &op, &ext)) return s;
+    if (thip_status_t s = cacheOperands(c.key_cache, c.value_cache, c.key_scales, c.value_scales, false, &op, &ext)) return s;
+    const int64_t T = k->shape[0];
+    if (!fitsInt32(T) || !fitsInt32(T * op.W)) return fail(THIP_UNIMPLEMENTED, "key: more than 2^31 rows");
+    if (c.key == c.value) return fail(THIP_INVALID_ARGUMENT, "key and value share bytes");
+    if (thip_status_t s = rowOperand(c.key, "key", true, T, op.W, op.C, &op.out)) return s;
+    if (thip_status_t s = rowOperand(c.value, "value", true, T, op.W, op.C, &op.in1)) return s;
+    op.M = (int32_t)T;
+    const uint64_t rows = (uint64_t)T * op.W * op.C * 2;
+    std::vector<Extent> all{{op.out, rows, true, "key"}, {op.in1, rows, true, "value"}};
+    addExtents(op, ext, false, &all);
+    if (thip_status_t s = checkApart(all)) return s;
+    op.table = newConst(std::vector<CacheExt>{ext});
+    ops_.push_back(op);
+    return THIP_OK;
+}
+
+thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
+    const Value *q, *k;
+    if (thip_status_t s = checkValue(c.query, "query", &q)) return s;
+    if (thip_status_t s = checkValue(c.key, "key", &k)) return s;
+    if (q->rank != 3) return fail(THIP_INVALID_ARGUMENT, "query: rank %d, expected 3", q->rank);
+    if (!(c.scale > 0.0f) || c.scale > 3e38f) return fail(THIP_INVALID_ARGUMENT, "scale must be a positive number");
+    if (c.window < 0 || c.sinks < 0) return fail(THIP_INVALID_ARGUMENT, "window %d and sinks %d must not be negative", c.window, c.sinks);
+    const bool cached = c.pages != THIP_NO_VALUE;
+    if (cached != (c.lengths != THIP_NO_VALUE)) return fail(THIP_INVALID_ARGUMENT, "pages and lengths come together");
+    const int64_t T = q->shape[0], H = q->shape[1], D = q->shape[2];
+    DescOp op;
+    memset(&op, 0, sizeof(op));
+    CacheExt ext{};
+    op.kind = kKindAttention;
+    op.out_dtype = THIP_DTYPE_BF16;
+    if (!fitsInt32(T) || !fitsInt32(H) || !fitsInt32(T * H)) return fail(THIP_UNIMPLEMENTED, "query: more than 2^31 rows");
+    if (D % 16 != 0 || D > kMaxHeadDim) return fail(THIP_UNIMPLEMENTED, "rows of %lld elements: multiples of 16 up to %d", (long long)D, kMaxHeadDim);
+    if (thip_status_t s = batchOperands(c.row_starts, c.lengths, c.pages, cached, &op, &ext)) return s;
+    if (cached) {
+        if (thip_status_t s = cacheOperands(c.key, c.value, c.key_scales, c.value_scales, false, &op, &ext)) return s;
+        if (op.C != D) return fail(THIP_INVALID_ARGUMENT, "query: rows of %lld elements, the cache's have %d", (long long)D, op.C);
+    } else {
+        if (c.key_scales != THIP_NO_VALUE || c.value_scales != THIP_NO_VALUE) return fail(THIP_INVALID_ARGUMENT, "rows have no scales");
+        if (k->rank != 3) return fail(THIP_INVALID_ARGUMENT, "key: rank %d, expected 3", k->rank);
+        if (thip_status_t s = rowOperand(c.key, "key", false, T, k->shape[1], D, &op.weights)) return s;
+        if (thip_status_t s = rowOperand(c.value, "value", false, T, k->shape[1], D, &op.bias)) return s;
+        op.W = (int32_t)k->shape[1];
+        op.C = (int32_t)D;
+        op.gran = 2;
+    }
+    if (H % op.W != 0) return fail(THIP_INVALID_ARGUMENT, "%lld query heads over %d key heads", (long long)H, op.W);
+    op.M = (int32_t)T;
+    op.H = (int32_t)H;
+    op.w0 = cached ? 1 : 0;
+    op.K = c.window;
+    op.Kp = c.window ? c.sinks : 0;
+    memcpy(&op.bias0, &c.scale, 4);
+    if (thip_status_t s = rowOperand(c.query, "query", false, T, H, D, &op.in0)) return s;
+    if (thip_status_t s = rowOperand(c.init, "init", true, T, H, D, &op.out)) return s;
+    const uint64_t bytes = (uint64_t)T * H * D * 2;
+    std::vector<Extent> all{{op.out, bytes, true, "init"}};
+    const bool inPlace = op.in0.space == op.out.space && op.in0.index == op.out.index && op.in0.offset == op.out.offset;
+    if (!inPlace) all.push_back({op.in0, bytes, false, "query"});
+    if (cached) {
+        addExtents(op, ext, false, &all);
+        op.table = newConst(std::vector<CacheExt>{ext});
+    } else {
+        all.push_back({op.scale, ((uint64_t)op.N + 1) * 4, false, "row_starts"});
+        all.push_back({op.weights, (uint64_t)T * op.W * D * 2, false, "key"});
+        all.push_back({op.bias, (uint64_t)T * op.W * D * 2, false, "value"});
+    }
+    if (thip_status_t s = checkApart(all)) return s;
+    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T)) op.in1 = newTemp(work);
+    ops_.push_back(op);
+    return THIP_OK;
+}
+
 void Emitter::planDecodeFolding() {
     foldedTranspose_.clear();
     consumed_.assign(prog_.ops.size(), 0);
@@ -2279,6 +2532,9 @@ void Emitter::planChannelPadding() {
         case kHlUnary: bar(op.u.un.input); bar(op.u.un.init); break;
         case kHlShift: bar(op.u.sh.input1); bar(op.u.sh.input2); bar(op.u.sh.init); break;
         case kHlTable: bar(op.u.tab.input); bar(op.u.tab.init); break;
+        case kLmCacheWrite: bar(op.u.cw.key); bar(op.u.cw.value); break;
+        case kLmCacheRead: bar(op.u.cr.key); bar(op.u.cr.value); break;
+        case kLmAttention: bar(op.u.at.query); bar(op.u.at.key); bar(op.u.at.value); bar(op.u.at.init); break;
         }
     }
     // one verdict per group: every member an int8 rank-4 intermediate, all uses agreeing on C
@@ -2335,6 +2591,9 @@ void Emitter::planExpandFolding() {
         case kHlUnary: read(op.u.un.input); break;
         case kHlShift: read(op.u.sh.input1); read(op.u.sh.input2); break;
         case kHlTable: read(op.u.tab.input); break;
+        case kLmCacheWrite: read(op.u.cw.key); read(op.u.cw.value); break;
+        case kLmCacheRead: read(op.u.cr.key_cache); read(op.u.cr.value_cache); break;
+        case kLmAttention: read(op.u.at.query); read(op.u.at.key); read(op.u.at.value); break;
         }
     }
     valueReads_ = reads;
@@ -2424,6 +2683,9 @@ thip_status_t Emitter::run(void **outBlob, size_t *outSize) {
         case kHlUnary: s = emitUnary(op.u.un); break;
         case kHlShift: s = emitShift(op.u.sh); break;
         case kHlTable: s = emitTable(op.u.tab, op.staticTable); break;
+        case kLmCacheWrite: s = emitCacheWrite(op.u.cw); break;
+        case kLmCacheRead: s = emitCacheRead(op.u.cr); break;
+        case kLmAttention: s = emitAttention(op.u.at); break;
         }
         if (s != THIP_OK) return s;
     }
@@ -2612,6 +2874,9 @@ THIP_DEFINE_HL(thip_hl_mul, thip_hl_mul_t, kHlMul, mul)
 THIP_DEFINE_HL(thip_hl_elementwisebinary, thip_hl_elementwisebinary_t, kHlBinary, bin)
 THIP_DEFINE_HL(thip_hl_elementwiseunary, thip_hl_elementwiseunary_t, kHlUnary, un)
 THIP_DEFINE_HL(thip_hl_elementwiseshift, thip_hl_elementwiseshift_t, kHlShift, sh)
+THIP_DEFINE_HL(thip_lm_cache_write, thip_lm_cache_write_t, kLmCacheWrite, cw)
+THIP_DEFINE_HL(thip_lm_cache_read, thip_lm_cache_read_t, kLmCacheRead, cr)
+THIP_DEFINE_HL(thip_lm_attention, thip_lm_attention_t, kLmAttention, at)
 
 thip_status_t thip_hl_table(thip_program_t *program, const thip_hl_table_t *op) {
     if (!program || !op) return fail(THIP_INVALID_ARGUMENT, "thip_hl_table: null argument");

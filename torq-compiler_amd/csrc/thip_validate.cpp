@@ -7,6 +7,7 @@
 
 #include <initializer_list>
 
+#include "thip_attention.h"
 #include "thip_kernels.h"
 #include "thip_status.h"
 
@@ -408,6 +409,62 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
         if ((s = need(op.weights, mul(op.w1 ? 1 : op.TB, op.Nn, op.K) * 2, "in2"))) return s;
         if ((op.in0.offset & 15) || (op.weights.offset & 15) || (op.out.offset & 7)) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
         return need(op.out, mul(op.TB, op.M, op.Nn) * 2, "out");
+    }
+    case kKindCacheWrite: case kKindCacheRead: case kKindAttention: {
+        const bool attends = op.kind == kKindAttention, cached = !attends || op.w0 == 1;
+        if (!positive({op.M, op.N, op.W, op.C}) || op.C % 16 != 0 || op.C > kMaxHeadDim || (op.gran != 2 && !(cached && op.gran == 1)) || mul(op.M, op.W) >= (1ull << 31)) {
+            return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of packed rows", i);
+        }
+        const uint64_t rowBytes = mul(op.M, op.W, op.C) * 2;
+        if ((op.scale.offset & 3) || ((op.in0.offset | op.weights.offset | op.bias.offset | op.out.offset) & 15)) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
+        if ((s = need(op.scale, ((uint64_t)op.N + 1) * 4, "row starts"))) return s;
+        if (cached) {
+            if (!positive({op.OH, op.KH, op.KW}) || mul(op.OH, op.W, op.KH) >= (1ull << 31) || mul(op.KW, op.KH) >= (1ull << 31)) {
+                return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of a cache", i);
+            }
+            if (op.table.space != kSpaceConst) return fail(THIP_INVALID_ARGUMENT, "op %u: the cache's operands must be a constant", i);
+            if ((s = need(op.table, sizeof(CacheExt), "cache operands"))) return s;
+            CacheExt x;
+            memcpy(&x, e->blob + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset, sizeof(x));
+            for (const DescRef *r : {&x.key_scales, &x.value_scales, &x.pages, &x.lengths}) {
+                if ((s = checkLooseRef(e, i, *r))) return s;
+                // intermediates are told by the record's own references
+                if (r->space == kSpaceTemp || (r->offset & 3)) return fail(THIP_INVALID_ARGUMENT, "op %u: bad operand of a cache", i);
+            }
+            const uint64_t rows = mul(op.OH, op.W, op.KH), cacheBytes = rows * (uint64_t)op.C * op.gran;
+            if ((s = need(x.pages, mul(op.N, op.KW) * 4, "pages"))) return s;
+            if ((s = need(x.lengths, (uint64_t)op.N * 4, "lengths"))) return s;
+            if (op.gran == 1) {
+                if ((s = need(x.key_scales, rows * 4, "key scales"))) return s;
+                if ((s = need(x.value_scales, rows * 4, "value scales"))) return s;
+            } else if (x.key_scales.space != kSpaceNone || x.value_scales.space != kSpaceNone) {
+                return fail(THIP_INVALID_ARGUMENT, "op %u: a bf16 cache has no scales", i);
+            }
+            if ((s = need(op.weights, cacheBytes, "key cache"))) return s;
+            if ((s = need(op.bias, cacheBytes, "value cache"))) return s;
+            if (op.kind == kKindCacheWrite && (op.weights.space != kSpaceBinding || op.bias.space != kSpaceBinding || (op.gran == 1 && (x.key_scales.space != kSpaceBinding || x.value_scales.space != kSpaceBinding)))) {
+                return fail(THIP_INVALID_ARGUMENT, "op %u: a cache that is written must be a binding", i);
+            }
+        } else {
+            if ((s = need(op.weights, rowBytes, "key"))) return s;
+            if ((s = need(op.bias, rowBytes, "value"))) return s;
+        }
+        if (attends) {
+            float scale;
+            memcpy(&scale, &op.bias0, 4);
+            if (op.H <= 0 || op.H % op.W != 0 || mul(op.M, op.H) >= (1ull << 31) || op.K < 0 || op.Kp < 0 || (op.w0 != 0 && op.w0 != 1) || !(scale > 0.0f) || scale > 3e38f) {
+                return fail(THIP_INVALID_ARGUMENT, "op %u: bad attention record", i);
+            }
+            if (const uint64_t work = attentionWorkspaceBytes(op.M, op.N, op.H, op.W, op.C, cached ? (int64_t)op.KW * op.KH : op.M)) {
+                if (op.in1.space != kSpaceTemp || (op.in1.offset & 15)) return fail(THIP_INVALID_ARGUMENT, "op %u: bad workspace", i);
+                if ((s = need(op.in1, work, "workspace"))) return s;
+            }
+            if ((s = need(op.in0, mul(op.M, op.H, op.C) * 2, "query"))) return s;
+            return need(op.out, mul(op.M, op.H, op.C) * 2, "out");
+        }
+        if (op.in1.offset & 15) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
+        if ((s = need(op.in1, rowBytes, "value rows"))) return s;
+        return need(op.kind == kKindCacheWrite ? op.in0 : op.out, rowBytes, "key rows");
     }
     default: return fail(THIP_INVALID_ARGUMENT, "op %u has unknown kind %u", i, op.kind);
     }

@@ -42,6 +42,7 @@ EXPORTED_SYMBOLS = [
     "thip_program_tensor", "thip_program_view", "thip_gemm_tile_choice", "thip_hl_conv2d", "thip_hl_depthwise_conv2d", "thip_hl_fully_connected",
     "thip_hl_matmul", "thip_hl_maxpool2d", "thip_hl_avg_pool2d", "thip_hl_add", "thip_hl_transpose", "thip_hl_expand_weights",
     "thip_hl_fma", "thip_hl_mul", "thip_hl_act", "thip_hl_elementwisebinary", "thip_hl_elementwiseunary", "thip_hl_elementwiseshift", "thip_hl_table",
+    "thip_lm_cache_write", "thip_lm_cache_read", "thip_lm_attention",
     "thip_program_serialize", "thip_blob_free",
     "thip_device_create", "thip_device_destroy", "thip_device_name", "thip_device_alloc",
     "thip_device_free", "thip_device_h2d", "thip_device_d2h", "thip_device_synchronize",
@@ -233,6 +234,21 @@ class HlTranspose(ctypes.Structure):
     ]
 
 
+class LmCacheWrite(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("key_cache", "value_cache", "key_scales", "value_scales", "key", "value", "pages", "row_starts",
+                                                    "lengths")]
+
+
+class LmCacheRead(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("key", "value", "key_cache", "value_cache", "key_scales", "value_scales", "pages", "row_starts",
+                                                    "lengths")]
+
+
+class LmAttention(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("init", "query", "key", "value", "key_scales", "value_scales", "pages", "row_starts",
+                                                    "lengths")] + [("scale", ctypes.c_float), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
 _lib = None
 
 
@@ -267,7 +283,8 @@ def lib():
                      ("thip_hl_maxpool2d", HlMaxPool2d), ("thip_hl_avg_pool2d", HlAvgPool2d),
                      ("thip_hl_add", HlAdd), ("thip_hl_transpose", HlTranspose),
                      ("thip_hl_expand_weights", HlExpandWeights), ("thip_hl_fma", HlFma), ("thip_hl_mul", HlMul),
-                     ("thip_hl_act", HlAct), ("thip_hl_elementwisebinary", HlElementwiseBinary)]:
+                     ("thip_hl_act", HlAct), ("thip_hl_elementwisebinary", HlElementwiseBinary),
+                     ("thip_lm_cache_write", LmCacheWrite), ("thip_lm_cache_read", LmCacheRead), ("thip_lm_attention", LmAttention)]:
         getattr(L, name).argtypes = [vp, P(st)]
     L.thip_program_serialize.argtypes = [vp, P(vp), P(sz)]
     L.thip_blob_free.argtypes = [vp]

@@ -319,6 +319,49 @@ class Program:
         rt.check(rt.lib().thip_hl_transpose(self._h, ctypes.byref(op)))
         return init
 
+    # ---- attention and its cache --------------------------------------------
+    # Rows are packed, sequence behind sequence (row_starts, int32 [S + 1]); lengths (int32 [S]) says how many positions each has with
+    # them; a cache is [pages, kv_heads, page_size, D] (bf16, or int8 with float32 scales [pages, kv_heads, page_size]) and pages
+    # (int32 [S, P]) says which page holds which of a sequence's positions.  include/thip.h states what is read and written.
+    def _index_or_none(self, x):
+        return rt.NO_VALUE if x is None else self._as_value(x).index
+
+    def cache_write(self, key, value, key_cache, value_cache, pages, row_starts, lengths, *, key_scales=None, value_scales=None):
+        """Stores the rows key, value [T, kv_heads, D] in the cache, in place; an int8 cache quantises them row by row and head by head."""
+        op = rt.LmCacheWrite(key_cache.index, value_cache.index, self._index_or_none(key_scales), self._index_or_none(value_scales), key.index,
+                             value.index, self._as_value(pages).index, self._as_value(row_starts).index, self._as_value(lengths).index)
+        rt.check(rt.lib().thip_lm_cache_write(self._h, ctypes.byref(op)))
+
+    def cache_read(self, key_cache, value_cache, pages, row_starts, lengths, *, key_scales=None, value_scales=None, key=None, value=None, rows=None):
+        """Reads rows back as bf16 into key, value (new tensors of `rows` rows where they are not given); returns both."""
+        shape = (rows, key_cache.shape[1], key_cache.shape[3])
+        if rows is None and (key is None or value is None):
+            raise rt.ThipError(rt.INVALID_ARGUMENT, "cache_read: key and value, or the number of rows")
+        key, value = self._init_or_new(key, shape, np.uint16), self._init_or_new(value, shape, np.uint16)
+        op = rt.LmCacheRead(key.index, value.index, key_cache.index, value_cache.index, self._index_or_none(key_scales),
+                            self._index_or_none(value_scales), self._as_value(pages).index, self._as_value(row_starts).index, self._as_value(lengths).index)
+        rt.check(rt.lib().thip_lm_cache_read(self._h, ctypes.byref(op)))
+        return key, value
+
+    def attention(self, query, key, value, row_starts, *, scale, window=0, sinks=0, init=None):
+        """Attention of packed prompts: query [T, heads, D] over key, value [T, kv_heads, D] of the same rows; a row sees itself and the rows
+        of its sequence before it, with a window the last `window` of these and the first `sinks`."""
+        init = self._init_or_new(init, query.shape, np.uint16)
+        op = rt.LmAttention(init.index, query.index, key.index, value.index, rt.NO_VALUE, rt.NO_VALUE, rt.NO_VALUE,
+                            self._as_value(row_starts).index, rt.NO_VALUE, scale, int(window), int(sinks))
+        rt.check(rt.lib().thip_lm_attention(self._h, ctypes.byref(op)))
+        return init
+
+    def paged_attention(self, query, key_cache, value_cache, pages, row_starts, lengths, *, scale, window=0, sinks=0, key_scales=None,
+                        value_scales=None, init=None):
+        """Attention of new rows, query [T, heads, D], over a paged cache that holds their keys and values already."""
+        init = self._init_or_new(init, query.shape, np.uint16)
+        op = rt.LmAttention(init.index, query.index, key_cache.index, value_cache.index, self._index_or_none(key_scales),
+                            self._index_or_none(value_scales), self._as_value(pages).index, self._as_value(row_starts).index,
+                            self._as_value(lengths).index, scale, int(window), int(sinks))
+        rt.check(rt.lib().thip_lm_attention(self._h, ctypes.byref(op)))
+        return init
+
     # ---- serialisation ------------------------------------------------------
     def serialize(self):
         """Returns the dispatch descriptor as ``bytes``."""
