@@ -37,13 +37,45 @@ struct AttentionArgs {
     const float *key_scales, *value_scales;  // null: bf16
     int32_t H, G;                          // G: query heads of a key head
     float scale;
+    FastDiv g;
     int32_t window, sinks;                 // window 0: none (and sinks then 0)
     uint8_t *work;                         // attentionWorkspaceBytes
     size_t work_bytes;
 };
 hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx);
 
-// Bytes of partial results that a launch of these sizes may keep.  capacity: positions that a sequence can have.
-inline uint64_t attentionWorkspaceBytes(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity) { return 0; }
+// How a launch shares its work out.  An item is a tile of `rows` of a sequence's rows (a row: one query head of one token, the heads of a key
+// head next to one another) against a run of blocks of `keys` positions; a workgroup has one.  Where that makes too few items, the
+// device cuts the runs of long sequences so that there are about kAttentionItems, and a second launch joins the parts.
+constexpr int kAttentionItems = 512;  // a power of two: two a CU
+struct AttentionPlan {
+    bool tiles;         // attention_tiles, or attention_stream
+    int32_t rows, keys;
+    int32_t minBlocks;  // blocks that a part has at least
+    bool splits;        // runs may be cut
+    int64_t grid;       // items at most
+    int64_t slots;      // parts at most: one that is cut is of more than one run, so there are at most twice as many as asked for
+};
+// capacity: positions that a sequence can have
+inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
+    AttentionPlan p;
+    const int64_t rows = T * (H / KVH);  // of one key head
+    p.tiles = rows > 32 * S;
+    p.rows = p.tiles ? 128 : 16;
+    p.keys = p.tiles && D <= 128 ? 64 : 32;
+    p.minBlocks = p.tiles ? 4 : 4;
+    const int64_t span = window && window + sinks + p.rows < capacity ? window + sinks + p.rows : capacity;
+    const int64_t most = (rows / p.rows + (S < T ? S : T)) * KVH, parts = (span + (int64_t)p.keys * p.minBlocks - 1) / ((int64_t)p.keys * p.minBlocks) + 2;
+    p.splits = parts > 3 && most < kAttentionItems;
+    p.grid = p.splits ? (most * parts < most + 2 * kAttentionItems ? most * parts : most + 2 * kAttentionItems) : most;
+    p.slots = p.splits ? (p.grid < 2 * kAttentionItems ? p.grid : 2 * kAttentionItems) : 0;
+    return p;
+}
+
+// Bytes of partial results that a launch of these sizes may keep: for each row of a slot D sums, a maximum and a sum of weights.
+inline uint64_t attentionWorkspaceBytes(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
+    const AttentionPlan p = attentionPlan(T, S, H, KVH, D, capacity, window, sinks);
+    return (uint64_t)p.slots * (uint64_t)p.rows * (uint64_t)(D + 4) * 4;
+}
 
 }  // namespace thip

@@ -2,6 +2,16 @@
 //
 // o = sum_j w_j v_j / sum_j w_j, w_j = exp(scale (q . k_j) - m), over the positions j that the row sees; one pass over the keys with a
 // running maximum m and a running sum, both scaled down where a later key raises m.  Exponents are to base 2, with log2(e) in the scale.
+//
+// Both products are taken transposed: S^T = K Q^T and O^T = V^T P^T.  A lane then holds scores of ONE query row (the result's column), so
+// the softmax runs in the lane but for the maximum over the lanes that share the row, its scale of O is one number, and the scores it
+// holds are, rounded to bf16, the right operand of the second product as they lie: the keys only have to be taken in the order in which the first
+// product left them, which is the addresses of V's reads.  V's operand has a lane's values along the keys, across the rows that V lies in;
+// ds_read_b64_tr turns them on the way out of LDS.
+//
+// Weights are rounded to bf16 for the second product, by half a step of 2^-8 each, as a result of independent values is off by anyway; their
+// sum is kept of the unrounded ones.  int8 keys and values are whole numbers that bf16 holds, so the scales are applied in fp32: a
+// key's to its score, a value's to its weight.
 #include "thip_attention.h"
 #include "thip_attention_rows.h"
 #include "thip_kernels_common.h"
@@ -10,35 +20,162 @@ namespace thip {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
 // Whether a row at position p sees position j (0 <= j).
 __device__ __forceinline__ bool sees(const AttentionArgs &a, int p, int j) { return j <= p && (a.window == 0 || p - j < a.window || j < a.sinks); }
 
-// Row of the keys (elements / D) that position j of a sequence has; -1: none.
-__device__ __forceinline__ int64_t keyRow(const CacheArgs &c, int seq, int begin, int count, int head, int j) {
-    if (c.pages) return cacheRow(c, seq, head, j);
-    return (uint32_t)j < (uint32_t)count ? (int64_t)(begin + j) * c.KVH + head : -1;
+// ---- the work of a workgroup ----------------------------------------------------------------------------------------
+
+// What sequence `s` brings: its rows, the positions it has, and the blocks that a tile of it can see at most.
+struct SeqWork {
+    int begin, count, first, length, tiles, blocks;
+};
+__device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const AttentionPlan &p, int s) {
+    const CacheArgs &c = a.c;
+    SeqWork w;
+    rowsOf(c, c.starts, s, &w.begin, &w.count);
+    w.first = firstPosition(c, s, w.count);
+    w.length = c.pages ? min(w.first + w.count, c.capacity) : w.count;
+    w.tiles = (int)(((uint32_t)w.count * (uint32_t)a.G + (uint32_t)p.rows - 1) / (uint32_t)p.rows);
+    w.blocks = (w.length + p.keys - 1) / p.keys;
+    if (a.window) {
+        // a tile's window reaches over its own tokens too, and its first and last block need not be whole
+        const int64_t seen = (int64_t)a.window + (p.rows - 1) / a.G + 1;
+        w.blocks = (int)min((int64_t)w.blocks, (int64_t)((a.sinks + (int64_t)p.keys - 1) / p.keys) + (seen + p.keys - 1) / p.keys + 1);
+    }
+    return w;
 }
 
-// One row by one wave, key by key: a lane has the scores of one key of 64, then four of the result's elements.  A value is only touched where
-// the row sees its position, so what other positions hold, NaN and infinity among it, cannot come in.  Leaves in the lanes the elements lane + 64 e of
-// sum_j w_j v_j, and the maximum and the sum, of positions [from, to).
+__device__ __forceinline__ int waveSumBefore(int v) {
+    const int lane = threadIdx.x & 63;
+    int sum = v;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const int up = __shfl_up(sum, step);
+        if (lane >= step) sum += up;
+    }
+    return sum - v;
+}
+
+// Blocks that a part has: so many that about kAttentionItems parts come of all that the tiles can see.  The same for every wave.
+__device__ __forceinline__ int blocksOfPart(const AttentionArgs &a, const AttentionPlan &p) {
+    if (!p.splits) return 0x7fffffff;
+    uint64_t total = 0;
+    for (int s = threadIdx.x & 63; s < a.c.S; s += 64) {
+        const SeqWork w = measureSeq(a, p, s);
+        total += (uint64_t)w.tiles * (uint64_t)w.blocks;
+    }
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        total += ((uint64_t)(uint32_t)__shfl_xor((int)(total >> 32), step) << 32) + (uint32_t)__shfl_xor((int)total, step);
+    }
+    const uint64_t part = (total * (uint64_t)a.c.KVH + kAttentionItems - 1) / kAttentionItems;
+    return (int)min(max(part, (uint64_t)p.minBlocks), (uint64_t)0x7fffffff);
+}
+__device__ __forceinline__ int partsOf(const SeqWork &w, int part) { return w.blocks <= part ? 1 : (int)(((uint32_t)w.blocks + (uint32_t)part - 1) / (uint32_t)part); }
+
+struct Item {
+    SeqWork w;
+    int seq, tile, head, split, splits, part;
+    int slot;  // of its partial result; -1: the item is its rows' only one
+};
+
+// Item `index` of the launch, or the sequence `index` (by sequence: slot is its first one, the tile none).  Items lie sequence by sequence, a sequence's
+// last tiles, which see most, first; key heads are next to one another, so that workgroups of one XCD (every eighth) read the same
+// keys where there are eight heads.  False: there is none.
+template <bool BY_SEQUENCE>
+__device__ __forceinline__ bool findItem(const AttentionArgs &a, const AttentionPlan &p, int index, Item *out) {
+    const int lane = threadIdx.x & 63, part = blocksOfPart(a, p);
+    int items = 0, slots = 0;
+    for (int base = 0; base < a.c.S; base += 64) {
+        SeqWork w{};
+        if (base + lane < a.c.S) w = measureSeq(a, p, base + lane);
+        const int splits = partsOf(w, part), mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
+        const int before = items + waveSumBefore(mine), cutBefore = slots + waveSumBefore(cut);
+        const bool here = BY_SEQUENCE ? base + lane == index : mine > 0 && before <= index && index < before + mine;
+        const uint64_t found = __ballot(here);
+        if (found) {
+            const int l = __builtin_ctzll(found);
+            out->w.begin = __builtin_amdgcn_readlane(w.begin, l);
+            out->w.count = __builtin_amdgcn_readlane(w.count, l);
+            out->w.first = __builtin_amdgcn_readlane(w.first, l);
+            out->w.length = __builtin_amdgcn_readlane(w.length, l);
+            out->w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+            out->w.blocks = __builtin_amdgcn_readlane(w.blocks, l);
+            out->seq = base + l;
+            out->part = part;
+            out->splits = __builtin_amdgcn_readlane(splits, l);
+            const int first = __builtin_amdgcn_readlane(cutBefore, l);
+            if (BY_SEQUENCE) {
+                out->slot = first;
+                return true;
+            }
+            const int local = index - __builtin_amdgcn_readlane(before, l), rest = local / a.c.KVH;
+            out->head = local - rest * a.c.KVH;
+            out->split = rest % out->splits;
+            out->tile = out->w.tiles - 1 - rest / out->splits;
+            out->slot = out->splits > 1 ? first + local : -1;
+            return out->slot < p.slots;  // false: starts that do not ascend
+        }
+        items = __builtin_amdgcn_readlane(before + mine, 63);
+        slots = __builtin_amdgcn_readlane(cutBefore + cut, 63);
+    }
+    return false;
+}
+
+// The blocks that a tile reads: those of the first positions that stay visible, then from its first row's window on.  Blocks [from, to)
+// of that order are the item's.
+struct Span {
+    int rows;          // of the tile
+    int sinkBlocks, windowBlock;
+    int from, to;
+};
+__device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
+    Span s;
+    const int r0 = it.tile * p.rows;
+    s.rows = min(p.rows, it.w.count * a.G - r0);
+    const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
+    const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(top - a.window + 1, 0) : 0;
+    s.sinkBlocks = (min(min(a.sinks, low), high) + p.keys - 1) / p.keys;
+    s.windowBlock = max(low / p.keys, s.sinkBlocks);
+    const int all = s.sinkBlocks + max((high + p.keys - 1) / p.keys - s.windowBlock, 0);
+    s.from = min(it.splits > 1 ? it.split * it.part : 0, all);
+    s.to = it.splits > 1 ? min(all, s.from + it.part) : all;
+    return s;
+}
+__device__ __forceinline__ int blockStart(const AttentionPlan &p, const Span &s, int b) { return (b < s.sinkBlocks ? b : b - s.sinkBlocks + s.windowBlock) * p.keys; }
+
+// Row of the keys (elements / D) that position j of a sequence has; -1: none.
+template <bool PAGED>
+__device__ __forceinline__ int keyRow(const CacheArgs &c, int seq, int begin, int length, int head, int j) {
+    if constexpr (PAGED) return j < length ? (int)cacheRow(c, seq, head, j) : -1;
+    return j < length ? (begin + j) * c.KVH + head : -1;
+}
+
+// ---- one row, key by key ----------------------------------------------------------------------------------------------
+
+// One row by one wave: a lane has the scores of one key of 64, then four of the result's elements (lane + 64 e).  A value is only touched
+// where the row sees its position, so what other positions hold, NaN and infinities among it, cannot come in: the tiles below multiply a
+// masked value by a weight of zero, and hand a row here where that left a NaN.  Adds positions [from, to) to o, m and l.
 // q: D floats of LDS, the row's query.
-template <bool Q8>
-__device__ void attendRow(const AttentionArgs &a, const float *q, int seq, int begin, int count, int head, int pos, int from, int to, float *o, float *m, float *l) {
+template <bool PAGED, bool Q8>
+__device__ __noinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, int pos, int from, int to, float *o, float *m, float *l) {
     const CacheArgs &c = a.c;
     const int lane = threadIdx.x & 63, D = c.D;
-    float most = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = 0.0f;
+    float most = *m, sum = *l;
     for (int base = from; base < to; base += 64) {
         const int j = base + lane;
-        int64_t row = -1;
-        if (j < to && sees(a, pos, j)) row = keyRow(c, seq, begin, count, head, j);
+        int row = -1;
+        if (j < to && sees(a, pos, j)) row = keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j);
         float s = -INFINITY, vs = 1.0f;
         if (row >= 0) {
             float dot = 0.0f;
             if constexpr (Q8) {
-                const int8_t *k = (const int8_t *)a.key + row * D;
+                const int8_t *k = (const int8_t *)a.key + (int64_t)row * D;
                 for (int d = 0; d < D; d += 16) {
                     const v4i w = *(const v4i *)(k + d);
 #pragma unroll
@@ -47,7 +184,7 @@ __device__ void attendRow(const AttentionArgs &a, const float *q, int seq, int b
                 dot *= a.key_scales[row];
                 vs = a.value_scales[row];
             } else {
-                const uint16_t *k = (const uint16_t *)a.key + row * D;
+                const uint16_t *k = (const uint16_t *)a.key + (int64_t)row * D;
                 for (int d = 0; d < D; d += 8) {
                     const v4i w = *(const v4i *)(k + d);
 #pragma unroll
@@ -77,7 +214,7 @@ __device__ void attendRow(const AttentionArgs &a, const float *q, int seq, int b
         while (seen) {
             const int t = __builtin_ctzll(seen);
             seen &= seen - 1;
-            const int64_t r = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), t) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, t);
+            const int64_t r = __builtin_amdgcn_readlane(row, t);
             const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), t));
             const float u = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), t));
 #pragma unroll
@@ -95,30 +232,622 @@ __device__ void attendRow(const AttentionArgs &a, const float *q, int seq, int b
     *l = sum;
 }
 
-// A wave a row and query head.
-template <bool Q8>
-__global__ __launch_bounds__(256) void attention_rows(AttentionArgs a) {
-    __shared__ float q[4][kMaxHeadDim];
-    const CacheArgs &c = a.c;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    const int row = (int)(item / a.H), h = (int)(item % a.H);
-    if (row >= c.T) return;
-    const RowPlace p = placeOf(c, c.starts, row);
-    if (p.seq < 0) return;
-    const uint16_t *query = a.query + ((int64_t)row * a.H + h) * c.D;
-    for (int d = lane; d < c.D; d += 64) q[wave][d] = __uint_as_float((uint32_t)query[d] << 16);
-    __builtin_amdgcn_wave_barrier();
+// A row of an item once more, key by key, and its result or partial result stored.  q: LDS of this wave, kMaxHeadDim floats.
+template <bool PAGED, bool Q8>
+__device__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const Item &it, const Span &span, int r, float *q) {
+    const int lane = threadIdx.x & 63, D = a.c.D;
+    const int inSeq = it.tile * p.rows + r, token = (int)fastDiv((uint32_t)inSeq, a.g), h = it.head * a.G + inSeq - token * a.G;
+    const int64_t at = ((int64_t)(it.w.begin + token) * a.H + h) * D;
+    for (int d = lane; d < D; d += 64) q[d] = __uint_as_float((uint32_t)a.query[at + d] << 16);
     __threadfence_block();
-    float o[4], m, l;
-    const int end = min(p.pos + 1, c.pages ? c.capacity : p.count);
-    attendRow<Q8>(a, q[wave], p.seq, p.begin, p.count, h / a.G, p.pos, 0, end, o, &m, &l);
-    uint16_t *out = a.out + ((int64_t)row * a.H + h) * c.D;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const int d = lane + 64 * e;
-        if (d < c.D) out[d] = bf16Bits(l == 0.0f ? 0.0f : o[e] / l);
+    float o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
+    const int pos = it.w.first + token;
+    for (int b = span.from; b < span.to; b++) {
+        const int j = blockStart(p, span, b);
+        attendRow<PAGED, Q8>(a, q, it, pos, j, j + p.keys, o, &m, &l);
     }
+    if (it.slot < 0) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = lane + 64 * e;
+            if (d < D) a.out[at + d] = bf16Bits(l == 0.0f ? 0.0f : o[e] / l);
+        }
+    } else {
+        float *part = (float *)a.work + ((int64_t)it.slot * p.rows + r) * (D + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = lane + 64 * e;
+            if (d < D) part[d] = o[e];
+        }
+        if (lane == 0) {
+            part[D] = m;
+            part[D + 1] = l;
+        }
+    }
+    __threadfence_block();
+}
+
+// ---- small helpers of the tiles ---------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float maxOverHalves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sumOverHalves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float maxOverQuarters(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return maxOverHalves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sumOverQuarters(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return sumOverHalves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ int packBf16(float lo, float hi) { return __builtin_bit_cast(int, __builtin_convertvector((v2f){lo, hi}, v2bf)); }
+
+// Four int8 as bf16, which holds them: the upper halves of their floats.
+__device__ __forceinline__ v2i wholeBf16(int w) {
+    const uint32_t f0 = __float_as_uint((float)(int8_t)w), f1 = __float_as_uint((float)(int8_t)(w >> 8));
+    const uint32_t f2 = __float_as_uint((float)(int8_t)(w >> 16)), f3 = __float_as_uint((float)(w >> 24));
+    return v2i{(int)__builtin_amdgcn_perm(f1, f0, 0x07060302u), (int)__builtin_amdgcn_perm(f3, f2, 0x07060302u)};
+}
+__device__ __forceinline__ v8bf wholeBf16x8(int lo, int hi) {
+    const v2i a = wholeBf16(lo), b = wholeBf16(hi);
+    return __builtin_bit_cast(v8bf, v4i{a[0], a[1], b[0], b[1]});
+}
+
+// Four rows of 16 elements, a lane's eight bytes of one of them: the lane gets a column (16 lanes a group).
+__device__ __forceinline__ v2i turn16(const int8_t *p) {
+    return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)p));
+}
+// Eight rows of 16 bytes, likewise.
+__device__ __forceinline__ v2i turn8(const int8_t *p) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i *)p); }
+
+// Rows of keys and values in LDS are as long as a head; 16 of them at one 16-byte chunk, or 8 of them at four neighbouring ones, must not meet in the banks.
+// The chunk of a row is stored at chunk ^ swizzle(row): the row's low two bits move it by whole groups of four chunks, the next two
+// within a group.
+template <int ROW_BYTES>
+__device__ __forceinline__ int swizzle(int row) {
+    if constexpr (ROW_BYTES >= 256) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else return ((row & 2) << 1) | ((row >> 2) & 3);  // 128 bytes: rows lie in both halves of the banks in turn
+}
+
+constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the running maximum before all is scaled down: weights stay below 2^8
+
+// ---- tiles of 128 rows ------------------------------------------------------------------------------------------------
+
+// Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is in registers while
+// one is worked on, the rows of the block behind that are being looked up.
+template <int DT, bool PAGED, bool Q8>
+__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(AttentionArgs a, AttentionPlan p) {
+    constexpr int KB = DT == 256 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
+    extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+    float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]
+    uint8_t *const flagRoom = (uint8_t *)(scaleRoom + 4 * KB);      // [2][4 waves]: some row of the block is not there
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const CacheArgs &c = a.c;
+    Item it;
+    if (!findItem<false>(a, p, blockIdx.x, &it)) return;
+    const Span span = spanOf(a, p, it);
+    const int D = c.D, r0 = it.tile * 128 + wave * 32, rowsHere = min(32, span.rows - wave * 32);  // of this wave; none: <= 0
+    const bool active = rowsHere > 0;
+    const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + max(rowsHere, 1) - 1), a.g);
+    const int inSeq = r0 + min(col, max(rowsHere, 1) - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
+    const int pos = it.w.first + token;
+    const int64_t at = ((int64_t)(it.w.begin + min(token, it.w.count - 1)) * a.H + it.head * a.G + inSeq - token * a.G) * D;
+
+    v8bf q[DT / 16];
+#pragma unroll
+    for (int t = 0; t < DT / 16; t++) {
+        v4i w{0, 0, 0, 0};
+        if (active && 16 * t < D) w = *(const v4i *)(a.query + at + 16 * t + 8 * half);
+        q[t] = __builtin_bit_cast(v8bf, w);
+    }
+    v16f o[DT / 32];
+#pragma unroll
+    for (int t = 0; t < DT / 32; t++) o[t] = v16f{0};
+    float m = -INFINITY, l = 0.0f;
+    const float scale = a.scale * kLog2e;
+
+    // this thread's part of a block: chunk `piece` of rows tid / CH + STEP i
+    const int piece = tid % CH, myRow = tid / CH;
+    const bool pieceIn = piece * 8 < D;
+    int rows[PER], scaleRow = -1;
+    v4i kreg[PER], vreg[PER];
+    float sreg = 0.0f;
+    int held[PER];
+    auto lookUp = [&](int b) {
+        const int j0 = blockStart(p, span, b);
+#pragma unroll
+        for (int i = 0; i < PER; i++) rows[i] = b < span.to ? keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j0 + myRow + STEP * i) : -1;
+        if constexpr (Q8) {
+            scaleRow = -1;
+            if (tid < 2 * KB && b < span.to) scaleRow = keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j0 + (tid & (KB - 1)));
+        }
+    };
+    auto fetch = [&]() {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            held[i] = rows[i];
+            kreg[i] = v4i{0, 0, 0, 0};
+            vreg[i] = v4i{0, 0, 0, 0};
+            if (rows[i] >= 0 && pieceIn) {
+                const int64_t from = (int64_t)rows[i] * D + piece * 8;
+                if constexpr (Q8) {
+                    const v2i kw = *(const v2i *)((const int8_t *)a.key + from), vw = *(const v2i *)((const int8_t *)a.value + from);
+                    kreg[i] = v4i{kw[0], kw[1], 0, 0};
+                    vreg[i] = v4i{vw[0], vw[1], 0, 0};
+                } else {
+                    kreg[i] = *(const v4i *)((const uint16_t *)a.key + from);
+                    vreg[i] = *(const v4i *)((const uint16_t *)a.value + from);
+                }
+            }
+        }
+        if constexpr (Q8) {
+            sreg = 0.0f;
+            if (scaleRow >= 0) sreg = (tid < KB ? a.key_scales : a.value_scales)[scaleRow];
+        }
+    };
+    auto put = [&](int stage) {
+        int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
+        bool missing = false;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int row = myRow + STEP * i, where = row * ROW + ((piece ^ swizzle<ROW>(row)) << 4);
+            v4i kw = kreg[i], vw = vreg[i];
+            if constexpr (Q8) {
+                kw = __builtin_bit_cast(v4i, wholeBf16x8(kw[0], kw[1]));
+                vw = __builtin_bit_cast(v4i, wholeBf16x8(vw[0], vw[1]));
+            }
+            *(v4i *)(keys + where) = kw;
+            *(v4i *)(values + where) = vw;
+            missing = missing || held[i] < 0;
+        }
+        if constexpr (Q8) {
+            if (tid < 2 * KB) scaleRoom[stage * 2 * KB + tid] = sreg;
+        }
+        if constexpr (PAGED) {
+            const bool some = __any(missing);
+            if (lane == 0) flagRoom[stage * 4 + wave] = some;
+        }
+    };
+
+    lookUp(span.from);
+    fetch();
+    lookUp(span.from + 1);
+    for (int b = span.from, stage = 0; b < span.to; b++, stage ^= 1) {
+        put(stage);
+        fetch();
+        lookUp(b + 2);
+        __syncthreads();
+        const int j0 = blockStart(p, span, b);
+        if (!active || j0 > bottom) continue;
+        const int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
+        v16f s[KB / 32];
+#pragma unroll
+        for (int k = 0; k < KB / 32; k++) {
+            s[k] = v16f{0};
+            const int row = k * 32 + col;
+#pragma unroll
+            for (int t = 0; t < DT / 16; t++) {
+                const v8bf kw = *(const v8bf *)(keys + row * ROW + (((2 * t + half) ^ swizzle<ROW>(row)) << 4));
+                s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kw, q[t], s[k], 0, 0, 0);
+            }
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int k = 0; k < KB / 32; k++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const v4f u = *(const v4f *)(scaleRoom + stage * 2 * KB + k * 32 + 8 * i + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[k][4 * i + e] *= u[e];
+                }
+            }
+        }
+        bool whole = j0 + KB - 1 <= top && j0 + KB <= it.w.length && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        bool gaps = false;
+        if constexpr (PAGED) gaps = __builtin_amdgcn_readfirstlane(*(const int *)(flagRoom + stage * 4)) != 0;
+        if (!whole || gaps) {
+#pragma unroll
+            for (int k = 0; k < KB / 32; k++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int j = j0 + k * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+                    bool see = sees(a, pos, j) && j < it.w.length;
+                    if constexpr (PAGED) {
+                        if (gaps && see) see = cacheRow(c, it.seq, it.head, j) >= 0;
+                    }
+                    s[k][i] = see ? s[k][i] : -INFINITY;
+                }
+            }
+        }
+        float high = s[0][0];
+#pragma unroll
+        for (int k = 0; k < KB / 32; k++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) high = fmaxf(high, s[k][i]);
+        }
+        high = maxOverHalves(high) * scale;
+        if (__any(high > m + kSlack || (m == -INFINITY && high > m))) {
+            const float now = fmaxf(m, high), down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+            m = now;
+            l *= down;
+#pragma unroll
+            for (int t = 0; t < DT / 32; t++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[t][i] *= down;
+            }
+        }
+        const float shift = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int k = 0; k < KB / 32; k++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[k][i] = __builtin_amdgcn_exp2f(fmaf(s[k][i], scale, -shift));
+                l += s[k][i];
+            }
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int k = 0; k < KB / 32; k++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const v4f u = *(const v4f *)(scaleRoom + stage * 2 * KB + KB + k * 32 + 8 * i + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[k][4 * i + e] = s[k][4 * i + e] == 0.0f ? 0.0f : s[k][4 * i + e] * u[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KB / 32; k++) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                v4i w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = packBf16(s[k][8 * x + 2 * e], s[k][8 * x + 2 * e + 1]);
+                const v8bf weights = __builtin_bit_cast(v8bf, w);
+                const int row = k * 32 + 16 * x + 4 * half + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), low = (lane & 1) * 8;
+#pragma unroll
+                for (int t = 0; t < DT / 32; t++) {
+                    const v2i v0 = turn16(values + row * ROW + (((4 * t + chunk) ^ swizzle<ROW>(row)) << 4) + low);
+                    const v2i v1 = turn16(values + (row + 8) * ROW + (((4 * t + chunk) ^ swizzle<ROW>(row + 8)) << 4) + low);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]}), weights, o[t], 0, 0, 0);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (!active) return;
+    l = sumOverHalves(l);
+    // a masked value that was no number, or a row that sees one
+    bool odd = false;
+    if constexpr (!Q8) {
+#pragma unroll
+        for (int t = 0; t < DT / 32; t++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) odd = odd || o[t][i] != o[t][i];
+        }
+    }
+    const uint64_t odds = __ballot(odd);
+    const uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
+    if (col < rowsHere && !((again >> col) & 1)) {
+        if (it.slot < 0) {
+            const float by = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int t = 0; t < DT / 32; t++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int d = 32 * t + 8 * i + 4 * half;
+                    if (d < D) *(v2i *)(a.out + at + d) = v2i{packBf16(o[t][4 * i] * by, o[t][4 * i + 1] * by), packBf16(o[t][4 * i + 2] * by, o[t][4 * i + 3] * by)};
+                }
+            }
+        } else {
+            float *part = (float *)a.work + ((int64_t)it.slot * 128 + wave * 32 + col) * (D + 4);
+#pragma unroll
+            for (int t = 0; t < DT / 32; t++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int d = 32 * t + 8 * i + 4 * half;
+                    if (d < D) *(v4f *)(part + d) = v4f{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+                }
+            }
+            if (half == 0) {
+                part[D] = m;
+                part[D + 1] = l;
+            }
+        }
+    }
+    if constexpr (!Q8) {
+        for (int r = 0; r < rowsHere; r++) {
+            if ((again >> r) & 1) redoRow<PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)smem + wave * kMaxHeadDim);
+        }
+    }
+}
+
+// ---- few rows: keys and values streamed -----------------------------------------------------------------------------------
+
+// A tile of 16 rows (a token's heads, or a few tokens'); each of the four waves has blocks of 32 keys of its own, every fourth, and joins the
+// others at the end.  A wave waits for nobody: its keys go straight into the matrix operand's registers, its values through LDS of its own.
+// The registers are filled again as soon as their content is used, so a block's 2 x 32 rows are under way while the one before is worked on.
+template <int DT, bool PAGED, bool Q8>
+__global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_stream(AttentionArgs a, AttentionPlan p) {
+    constexpr int KB = 32, STEPS = DT / 32, ROW = DT * (Q8 ? 1 : 2), LOADS = ROW / 64;  // LOADS: 16-byte pieces of a row that one of four lanes has
+    constexpr int JOIN = 16 * (DT + 4);  // floats of a wave's result
+    extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
+    const CacheArgs &c = a.c;
+    Item it;
+    if (!findItem<false>(a, p, blockIdx.x, &it)) return;
+    const Span span = spanOf(a, p, it);
+    const int D = c.D, r0 = it.tile * 16;
+    const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + span.rows - 1), a.g);
+    const int inSeq = r0 + min(col, span.rows - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
+    const int pos = it.w.first + token;
+    int8_t *const values = smem + wave * KB * ROW;
+    float *const scales = (float *)(smem + 4 * KB * ROW) + wave * 2 * KB;
+
+    v8bf q[STEPS];
+    {
+        const int64_t at = ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + inSeq - token * a.G) * D;
+#pragma unroll
+        for (int t = 0; t < STEPS; t++) {
+            // of an int8 row a lane has 16 elements at a time, for two steps
+            const int d = Q8 ? 64 * (t >> 1) + 16 * quarter + 8 * (t & 1) : 32 * t + 8 * quarter;
+            v4i w{0, 0, 0, 0};
+            if (d < D) w = *(const v4i *)(a.query + at + d);
+            q[t] = __builtin_bit_cast(v8bf, w);
+        }
+    }
+    v4f o[DT / 16];
+#pragma unroll
+    for (int t = 0; t < DT / 16; t++) o[t] = v4f{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    const float scale = a.scale * kLog2e;
+
+    int rows[2];         // of the block to be fetched next: keys col and 16 + col
+    bool there[2];       // of the block in the registers
+    v4i kreg[2][LOADS], vreg[2][LOADS];
+    float sreg = 0.0f;
+    auto lookUp = [&](int b) {
+        const int j0 = blockStart(p, span, b);
+#pragma unroll
+        for (int k = 0; k < 2; k++) rows[k] = b < span.to ? keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j0 + 16 * k + col) : -1;
+    };
+    constexpr int ELEMS = Q8 ? 16 : 8;  // of a piece
+    auto fetch = [&](const void *from, v4i(&reg)[2][LOADS]) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int d = (4 * i + quarter) * ELEMS;
+                reg[k][i] = v4i{0, 0, 0, 0};
+                if (rows[k] >= 0 && d < D) reg[k][i] = *(const v4i *)((const int8_t *)from + ((int64_t)rows[k] * D + d) * (Q8 ? 1 : 2));
+            }
+        }
+    };
+    auto fetchScales = [&]() {
+        if constexpr (Q8) {
+            const int row = (lane & 16) ? rows[1] : rows[0];
+            sreg = 0.0f;
+            if (row >= 0) sreg = (lane < 32 ? a.key_scales : a.value_scales)[row];
+        }
+    };
+
+    lookUp(span.from + wave);
+    there[0] = rows[0] >= 0;
+    there[1] = rows[1] >= 0;
+    fetchScales();
+    fetch(a.value, vreg);
+    fetch(a.key, kreg);
+    lookUp(span.from + wave + 4);
+    for (int b = span.from + wave; b < span.to; b += 4) {
+        const int j0 = blockStart(p, span, b);
+        const uint64_t gone0 = __ballot(!there[0]), gone1 = __ballot(!there[1]);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int row = 16 * k + col, chunk = 4 * i + quarter;
+                int at;
+                if constexpr (Q8) at = row * ROW + ((chunk ^ (ROW >= 256 ? row & 15 : ROW == 128 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
+                else at = row * ROW + ((chunk ^ swizzle<ROW>(row)) << 4);
+                *(v4i *)(values + at) = vreg[k][i];
+            }
+        }
+        if constexpr (Q8) scales[lane] = sreg;
+        __builtin_amdgcn_wave_barrier();
+        const bool now0 = rows[0] >= 0, now1 = rows[1] >= 0;
+        fetchScales();
+        fetch(a.value, vreg);
+        v4f s[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            s[k] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < STEPS; t++) {
+                v8bf kw;
+                if constexpr (Q8) kw = (t & 1) ? wholeBf16x8(kreg[k][t >> 1][2], kreg[k][t >> 1][3]) : wholeBf16x8(kreg[k][t >> 1][0], kreg[k][t >> 1][1]);
+                else kw = __builtin_bit_cast(v8bf, kreg[k][t]);
+                s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw, q[t], s[k], 0, 0, 0);
+            }
+        }
+        fetch(a.key, kreg);
+        there[0] = now0;
+        there[1] = now1;
+        lookUp(b + 8);
+        if constexpr (Q8) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const v4f u = *(const v4f *)(scales + 16 * k + 4 * quarter);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[k][i] *= u[i];
+            }
+        }
+        const bool whole = j0 + KB - 1 <= top && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        if (!whole || (gone0 | gone1)) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int key = 4 * quarter + i, j = j0 + 16 * k + key;
+                    const bool see = sees(a, pos, j) && !(((k ? gone1 : gone0) >> key) & 1);
+                    s[k][i] = see ? s[k][i] : -INFINITY;
+                }
+            }
+        }
+        float high = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        high = maxOverQuarters(high) * scale;
+        if (__any(high > m + kSlack || (m == -INFINITY && high > m))) {
+            const float now = fmaxf(m, high), down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+            m = now;
+            l *= down;
+#pragma unroll
+            for (int t = 0; t < DT / 16; t++) o[t] *= down;
+        }
+        const float shift = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[k][i] = __builtin_amdgcn_exp2f(fmaf(s[k][i], scale, -shift));
+                l += s[k][i];
+            }
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const v4f u = *(const v4f *)(scales + 32 + 16 * k + 4 * quarter);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[k][i] = s[k][i] == 0.0f ? 0.0f : s[k][i] * u[i];
+            }
+        }
+        const v8bf weights = __builtin_bit_cast(v8bf, v4i{packBf16(s[0][0], s[0][1]), packBf16(s[0][2], s[0][3]), packBf16(s[1][0], s[1][1]), packBf16(s[1][2], s[1][3])});
+#pragma unroll
+        for (int t = 0; t < DT / 16; t++) {
+            v8bf vw;
+            if constexpr (Q8) {
+                const int row = 4 * quarter + ((col >> 1) & 3) + 16 * (col >> 3), at = row * ROW + ((t ^ (ROW >= 256 ? row & 15 : ROW == 128 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4) + 8 * (col & 1);
+                const v2i w = turn8(values + at);
+                vw = wholeBf16x8(w[0], w[1]);
+            } else {
+                const int row = 4 * quarter + (col >> 2), chunk = 2 * t + ((col & 3) >> 1), low = 8 * (col & 1);
+                const v2i v0 = turn16(values + row * ROW + ((chunk ^ swizzle<ROW>(row)) << 4) + low);
+                const v2i v1 = turn16(values + (row + 16) * ROW + ((chunk ^ swizzle<ROW>(row + 16)) << 4) + low);
+                vw = __builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]});
+            }
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vw, weights, o[t], 0, 0, 0);
+        }
+    }
+    l = sumOverQuarters(l);
+    __syncthreads();
+    // [wave][row][D + 4]: sums, maximum, sum of weights
+    float *const join = (float *)smem;
+#pragma unroll
+    for (int t = 0; t < DT / 16; t++) *(v4f *)(join + wave * JOIN + col * (DT + 4) + 16 * t + 4 * quarter) = o[t];
+    if (quarter == 0) {
+        join[wave * JOIN + col * (DT + 4) + DT] = m;
+        join[wave * JOIN + col * (DT + 4) + DT + 1] = l;
+    }
+    __syncthreads();
+    const int r = tid >> 4;  // 16 threads a row
+    float most = -INFINITY, factor[4], total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) most = fmaxf(most, join[w * JOIN + r * (DT + 4) + DT]);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        factor[w] = __builtin_amdgcn_exp2f(join[w * JOIN + r * (DT + 4) + DT] - (most == -INFINITY ? 0.0f : most));
+        total += factor[w] * join[w * JOIN + r * (DT + 4) + DT + 1];
+    }
+    v4f sum[DT / 64];
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < DT / 64; e++) {
+        sum[e] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) sum[e] += factor[w] * *(const v4f *)(join + w * JOIN + r * (DT + 4) + 64 * e + 4 * col);
+#pragma unroll
+        for (int i = 0; i < 4; i++) odd = odd || sum[e][i] != sum[e][i];
+    }
+    // the rows of this wave that have a NaN: 4 wave .. 4 wave + 3, 16 lanes each
+    const uint64_t odds = Q8 ? 0 : __ballot(odd);
+    if (r < span.rows && !((odds >> (16 * (r & 3))) & 0xffff)) {
+        const int mine = r0 + r, tok = (int)fastDiv((uint32_t)mine, a.g);
+        if (it.slot < 0) {
+            const float by = total == 0.0f ? 0.0f : 1.0f / total;
+            uint16_t *out = a.out + ((int64_t)(it.w.begin + tok) * a.H + it.head * a.G + mine - tok * a.G) * D;
+#pragma unroll
+            for (int e = 0; e < DT / 64; e++) {
+                if (64 * e + 4 * col < D) *(v2i *)(out + 64 * e + 4 * col) = v2i{packBf16(sum[e][0] * by, sum[e][1] * by), packBf16(sum[e][2] * by, sum[e][3] * by)};
+            }
+        } else {
+            float *part = (float *)a.work + ((int64_t)it.slot * 16 + r) * (D + 4);
+#pragma unroll
+            for (int e = 0; e < DT / 64; e++) {
+                if (64 * e + 4 * col < D) *(v4f *)(part + 64 * e + 4 * col) = sum[e];
+            }
+            if (col == 0) {
+                part[D] = most;
+                part[D + 1] = total;
+            }
+        }
+    }
+    if constexpr (!Q8) {
+        __syncthreads();
+        for (int k = 0; k < 4; k++) {
+            if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
+        }
+    }
+}
+
+// ---- the parts of cut runs joined ---------------------------------------------------------------------------------------
+
+// A wave a row and head; a lane has four elements of some of the parts.
+__global__ __launch_bounds__(256) void attention_join(AttentionArgs a, AttentionPlan p) {
+    const CacheArgs &c = a.c;
+    const int lane = threadIdx.x & 63;
+    const int64_t index = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (index >= (int64_t)c.T * a.H) return;
+    const int row = (int)(index / a.H), h = (int)(index - (int64_t)row * a.H), head = (int)fastDiv((uint32_t)h, a.g);
+    const RowPlace place = placeOf(c, c.starts, row);
+    if (place.seq < 0) return;
+    Item it;
+    if (!findItem<true>(a, p, place.seq, &it) || it.splits <= 1) return;
+    if (it.slot + (int64_t)it.w.tiles * it.splits * c.KVH > p.slots) return;  // starts that do not ascend
+    const int inSeq = (row - place.begin) * a.G + h - head * a.G, tile = inSeq / p.rows, D = c.D;
+    const int64_t slot0 = it.slot + (int64_t)(it.w.tiles - 1 - tile) * it.splits * c.KVH + head;
+    const float *base = (const float *)a.work + (slot0 * p.rows + inSeq - tile * p.rows) * (D + 4);
+    const int64_t stride = (int64_t)c.KVH * p.rows * (D + 4);
+    float most = -INFINITY;
+    for (int s = lane; s < it.splits; s += 64) most = fmaxf(most, base[s * stride + D]);
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
+    const float shift = most == -INFINITY ? 0.0f : most;
+    const int lanes = D >> 2, groups = 64 / lanes, group = lane / lanes, piece = lane - group * lanes;
+    v4f sum{0, 0, 0, 0};
+    float total = 0.0f;
+    if (group < groups) {
+        for (int s = group; s < it.splits; s += groups) {
+            const float *part = base + s * stride;
+            const float f = __builtin_amdgcn_exp2f(part[D] - shift);
+            sum += f * *(const v4f *)(part + 4 * piece);
+            total += f * part[D + 1];
+        }
+    }
+    v4f all = sum;
+    float l = total;
+    for (int g = 1; g < groups; g++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) all[i] += __shfl(sum[i], (lane + g * lanes) & 63);
+        l += __shfl(total, (lane + g * lanes) & 63);
+    }
+    if (lane >= lanes) return;
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    *(v2i *)(a.out + index * D + 4 * piece) = v2i{packBf16(all[0] * by, all[1] * by), packBf16(all[2] * by, all[3] * by)};
 }
 
 static hipError_t checkAttention(const AttentionArgs &a) {
@@ -126,23 +855,54 @@ static hipError_t checkAttention(const AttentionArgs &a) {
     if (c.T < 1 || c.S < 1 || c.KVH < 1 || c.D < 16 || c.D > kMaxHeadDim || c.D % 16 != 0 || a.G < 1 || a.H != a.G * c.KVH) return hipErrorInvalidValue;
     if ((int64_t)c.T * a.H >= (1LL << 31) || a.window < 0 || a.sinks < 0) return hipErrorInvalidValue;
     if (!c.starts || !a.query || !a.out || !a.key || !a.value || !c.lengths != !c.pages || !a.key_scales != !a.value_scales) return hipErrorInvalidValue;
-    if (((uintptr_t)a.query | (uintptr_t)a.out | (uintptr_t)a.key | (uintptr_t)a.value) & 15) return hipErrorInvalidValue;
+    if (((uintptr_t)a.query | (uintptr_t)a.out | (uintptr_t)a.key | (uintptr_t)a.value | (uintptr_t)a.work) & 15) return hipErrorInvalidValue;
     if (c.pages) {
         if (c.P < 1 || c.NP < 1 || c.PS < 1 || (int64_t)c.P * c.PS != c.capacity || (int64_t)c.NP * c.KVH * c.PS >= (1LL << 31)) return hipErrorInvalidValue;
     } else if (a.key_scales) {
         return hipErrorInvalidValue;
     }
-    if (a.work_bytes < attentionWorkspaceBytes(c.T, c.S, a.H, c.KVH, c.D, c.pages ? c.capacity : c.T)) return hipErrorInvalidValue;
+    if (a.work_bytes < attentionWorkspaceBytes(c.T, c.S, a.H, c.KVH, c.D, c.pages ? c.capacity : c.T, a.window, a.sinks)) return hipErrorInvalidValue;
     return hipSuccess;
+}
+
+template <int DT, bool PAGED, bool Q8>
+static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &p, const LaunchCtx &ctx) {
+    if (p.grid > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)p.grid);
+    if (p.tiles) {
+        constexpr int KB = DT == 256 ? 32 : 64;
+        constexpr size_t lds = 4 * KB * DT * 2 + 4 * KB * 4 + 16;
+        auto kernel = attention_tiles<DT, PAGED, Q8>;
+        // asked for the kernel's name, as every executable does once on its device, the launcher configures it there
+        if (lds > 64 * 1024 && ctx.name) {
+            if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return e;
+        }
+        THIP_ENQUEUE(ctx, kernelLabel("attention_tiles", {DT, PAGED, Q8}), kernel, grid, dim3(256), lds, a, p);
+    } else {
+        constexpr size_t tiles = 4 * 32 * DT * (Q8 ? 1 : 2) + (Q8 ? 4 * 64 * 4 : 0), join = 4 * 16 * (DT + 4) * 4, lds = tiles > join ? tiles : join;
+        auto kernel = attention_stream<DT, PAGED, Q8>;
+        if (lds > 64 * 1024 && ctx.name) {
+            if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return e;
+        }
+        THIP_ENQUEUE(ctx, kernelLabel("attention_stream", {DT, PAGED, Q8}), kernel, grid, dim3(256), lds, a, p);
+    }
+    return ctx.name ? hipSuccess : hipGetLastError();
+}
+
+template <bool PAGED, bool Q8>
+static hipError_t byHeadDim(const AttentionArgs &a, const AttentionPlan &p, const LaunchCtx &ctx) {
+    if (a.c.D <= 64) return enqueueAttention<64, PAGED, Q8>(a, p, ctx);
+    if (a.c.D <= 128) return enqueueAttention<128, PAGED, Q8>(a, p, ctx);
+    return enqueueAttention<256, PAGED, Q8>(a, p, ctx);
 }
 
 hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx) {
     if (hipError_t e = checkAttention(a)) return e;
-    const int64_t items = (int64_t)a.c.T * a.H;
-    const dim3 grid((unsigned)((items + 3) / 4));
-    if (a.key_scales) THIP_ENQUEUE(ctx, kernelLabel("attention_rows", {1}), attention_rows<true>, grid, dim3(256), 0, a);
-    else THIP_ENQUEUE(ctx, kernelLabel("attention_rows", {0}), attention_rows<false>, grid, dim3(256), 0, a);
-    return ctx.name ? hipSuccess : hipGetLastError();
+    const AttentionPlan p = attentionPlan(a.c.T, a.c.S, a.H, a.c.KVH, a.c.D, a.c.pages ? a.c.capacity : a.c.T, a.window, a.sinks);
+    hipError_t e = !a.c.pages ? byHeadDim<false, false>(a, p, ctx) : a.key_scales ? byHeadDim<true, true>(a, p, ctx) : byHeadDim<true, false>(a, p, ctx);
+    if (e != hipSuccess || !p.splits || ctx.name) return e;
+    THIP_ENQUEUE(ctx, "attention_join", attention_join, dim3((unsigned)(((int64_t)a.c.T * a.H + 3) / 4)), dim3(256), 0, a, p);
+    return hipGetLastError();
 }
 
 }  // namespace thip

@@ -370,7 +370,7 @@ static thip_status_t launchOp(thip_executable_t *e, uint32_t i, const DescOp &op
         uint8_t *keys = resolve(e, op.weights, bp), *values = resolve(e, op.bias, bp);
         if (attends) {
             AttentionArgs a{c, (const uint16_t *)resolve(e, op.in0, bp), (uint16_t *)resolve(e, op.out, bp), keys, values, keyScales, valueScales,
-                            op.H, op.H / op.W, 0.0f, op.K, op.Kp, resolve(e, op.in1, bp), 0};
+                            op.H, op.H / op.W, 0.0f, makeFastDiv((uint32_t)(op.H / op.W)), op.K, op.Kp, resolve(e, op.in1, bp), 0};
             memcpy(&a.scale, &op.bias0, 4);
             if (op.in1.space == kSpaceTemp) a.work_bytes = (size_t)(e->temps[op.in1.index].size - op.in1.offset);
             err = launchAttention(a, ctx);

@@ -2185,7 +2185,7 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
         all.push_back({op.bias, (uint64_t)T * op.W * D * 2, false, "value"});
     }
     if (thip_status_t s = checkApart(all)) return s;
-    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T)) op.in1 = newTemp(work);
+    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T, op.K, op.Kp)) op.in1 = newTemp(work);
     ops_.push_back(op);
     return THIP_OK;
 }

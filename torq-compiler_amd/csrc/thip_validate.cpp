@@ -455,7 +455,7 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
             if (op.H <= 0 || op.H % op.W != 0 || mul(op.M, op.H) >= (1ull << 31) || op.K < 0 || op.Kp < 0 || (op.w0 != 0 && op.w0 != 1) || !(scale > 0.0f) || scale > 3e38f) {
                 return fail(THIP_INVALID_ARGUMENT, "op %u: bad attention record", i);
             }
-            if (const uint64_t work = attentionWorkspaceBytes(op.M, op.N, op.H, op.W, op.C, cached ? (int64_t)op.KW * op.KH : op.M)) {
+            if (const uint64_t work = attentionWorkspaceBytes(op.M, op.N, op.H, op.W, op.C, cached ? (int64_t)op.KW * op.KH : op.M, op.K, op.Kp)) {
                 if (op.in1.space != kSpaceTemp || (op.in1.offset & 15)) return fail(THIP_INVALID_ARGUMENT, "op %u: bad workspace", i);
                 if ((s = need(op.in1, work, "workspace"))) return s;
             }
