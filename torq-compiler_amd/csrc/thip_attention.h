@@ -46,36 +46,51 @@ hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx);
 
 // How a launch shares its work out.  An item is a tile of `rows` of a sequence's rows (a row: one query head of one token, the heads of a key
 // head next to one another) against a run of blocks of `keys` positions; a workgroup has one.  Where that makes too few items, the
-// device cuts the runs of long sequences so that there are about kAttentionItems, and a second launch joins the parts.
-constexpr int kAttentionItems = 512;  // a power of two: two a CU
+// device cuts the runs of long sequences so that there are about `items`, and the last workgroup of a tile to finish joins the parts.
 struct AttentionPlan {
-    bool tiles;         // attention_tiles, or attention_stream
-    int32_t rows, keys;
-    int32_t minBlocks;  // blocks that a part has at least
-    bool splits;        // runs may be cut
-    int64_t grid;       // items at most
-    int64_t slots;      // parts at most: one that is cut is of more than one run, so there are at most twice as many as asked for
+    bool tiles;                  // attention_tiles, or attention_stream
+    int32_t rowsLog, keysLog;
+    int32_t windowBlocks;        // blocks that a tile can see at most (with a window)
+    int32_t minBlocks, maxParts; // blocks that a part has at least, and parts of a run at most
+    bool splits;                 // runs may be cut
+    int32_t items;
+    int64_t grid;                // items at most
+    int64_t slots;               // parts at most: one that is cut is of more than one run, so there are at most twice as many as asked for
+    FastDiv kvh;
+    __host__ __device__ int32_t rows() const { return 1 << rowsLog; }
+    __host__ __device__ int32_t keys() const { return 1 << keysLog; }
 };
 // capacity: positions that a sequence can have
 inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
     AttentionPlan p;
-    const int64_t rows = T * (H / KVH);  // of one key head
+    const int64_t G = H / KVH, rows = T * G;  // of one key head
     p.tiles = rows > 32 * S;
-    p.rows = p.tiles ? 128 : 16;
-    p.keys = p.tiles && D <= 128 ? 64 : 32;
+    p.rowsLog = p.tiles ? 7 : 4;
+    p.keysLog = p.tiles && D <= 128 ? 6 : 5;
+    p.items = p.tiles ? 512 : 1024;
     p.minBlocks = p.tiles ? 4 : 4;
-    const int64_t span = window && window + sinks + p.rows < capacity ? window + sinks + p.rows : capacity;
-    const int64_t most = (rows / p.rows + (S < T ? S : T)) * KVH, parts = (span + (int64_t)p.keys * p.minBlocks - 1) / ((int64_t)p.keys * p.minBlocks) + 2;
-    p.splits = parts > 3 && most < kAttentionItems;
-    p.grid = p.splits ? (most * parts < most + 2 * kAttentionItems ? most * parts : most + 2 * kAttentionItems) : most;
-    p.slots = p.splits ? (p.grid < 2 * kAttentionItems ? p.grid : 2 * kAttentionItems) : 0;
+    p.maxParts = p.tiles ? 16 : 64;
+    const int64_t keys = p.keys();
+    // a tile's window reaches over its own tokens too, and its first and last block need not be whole
+    const int64_t windowed = (sinks + keys - 1) / keys + (window + (p.rows() - 1) / G + keys) / keys + 1;
+    p.windowBlocks = (int32_t)(windowed < 0x7fffffff ? windowed : 0x7fffffff);
+    int64_t blocks = (capacity + keys - 1) / keys;
+    if (window && windowed < blocks) blocks = windowed;
+    const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
+    int64_t parts = (blocks + p.minBlocks - 1) / p.minBlocks;
+    if (parts > p.maxParts) parts = p.maxParts;
+    p.splits = parts > 1 && most < p.items / 2;
+    p.grid = p.splits ? (most * parts < most + 2 * p.items ? most * parts : most + 2 * p.items) : most;
+    p.slots = p.splits ? (p.grid < 2 * p.items ? p.grid : 2 * p.items) : 0;
+    p.kvh = makeFastDiv((uint32_t)KVH);
     return p;
 }
 
-// Bytes of partial results that a launch of these sizes may keep: for each row of a slot D sums, a maximum and a sum of weights.
+// Bytes of partial results that a launch of these sizes may keep: for each row of a slot D sums, a maximum and a sum of weights; and a counter for each
+// slot, 0 before and after every launch.
 inline uint64_t attentionWorkspaceBytes(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
     const AttentionPlan p = attentionPlan(T, S, H, KVH, D, capacity, window, sinks);
-    return (uint64_t)p.slots * (uint64_t)p.rows * (uint64_t)(D + 4) * 4;
+    return (uint64_t)p.slots * ((uint64_t)p.rows() * (uint64_t)(D + 4) * 4 + 4);
 }
 
 }  // namespace thip

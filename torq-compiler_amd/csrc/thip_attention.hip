@@ -26,7 +26,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 // Whether a row at position p sees position j (0 <= j).
-__device__ __forceinline__ bool sees(const AttentionArgs &a, int p, int j) { return j <= p && (a.window == 0 || p - j < a.window || j < a.sinks); }
+__device__ __forceinline__ bool sees(const AttentionArgs &a, int p, int j) { return (j <= p) & ((a.window == 0) | (p - j < a.window) | (j < a.sinks)); }
 
 // ---- the work of a workgroup ----------------------------------------------------------------------------------------
 
@@ -36,47 +36,41 @@ struct SeqWork {
 };
 __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const AttentionPlan &p, int s) {
     const CacheArgs &c = a.c;
-    SeqWork w;
+    SeqWork w{0, 0, 0, 0, 0, 0};
+    if (s >= c.S) return w;
     rowsOf(c, c.starts, s, &w.begin, &w.count);
     w.first = firstPosition(c, s, w.count);
     w.length = c.pages ? min(w.first + w.count, c.capacity) : w.count;
-    w.tiles = (int)(((uint32_t)w.count * (uint32_t)a.G + (uint32_t)p.rows - 1) / (uint32_t)p.rows);
-    w.blocks = (w.length + p.keys - 1) / p.keys;
-    if (a.window) {
-        // a tile's window reaches over its own tokens too, and its first and last block need not be whole
-        const int64_t seen = (int64_t)a.window + (p.rows - 1) / a.G + 1;
-        w.blocks = (int)min((int64_t)w.blocks, (int64_t)((a.sinks + (int64_t)p.keys - 1) / p.keys) + (seen + p.keys - 1) / p.keys + 1);
-    }
+    w.tiles = (int)(((uint32_t)w.count * (uint32_t)a.G + (uint32_t)p.rows() - 1) >> p.rowsLog);
+    w.blocks = (int)(((uint32_t)w.length + (uint32_t)p.keys() - 1) >> p.keysLog);
+    if (a.window) w.blocks = min(w.blocks, p.windowBlocks);
     return w;
 }
 
-__device__ __forceinline__ int waveSumBefore(int v) {
+// Sum of the lanes before this one, of which `lanes` have something.
+__device__ __forceinline__ int sumBefore(int v, int lanes) {
     const int lane = threadIdx.x & 63;
     int sum = v;
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
+    for (int step = 1; step < lanes; step *= 2) {
         const int up = __shfl_up(sum, step);
         if (lane >= step) sum += up;
     }
     return sum - v;
 }
 
-// Blocks that a part has: so many that about kAttentionItems parts come of all that the tiles can see.  The same for every wave.
-__device__ __forceinline__ int blocksOfPart(const AttentionArgs &a, const AttentionPlan &p) {
-    if (!p.splits) return 0x7fffffff;
-    uint64_t total = 0;
-    for (int s = threadIdx.x & 63; s < a.c.S; s += 64) {
-        const SeqWork w = measureSeq(a, p, s);
-        total += (uint64_t)w.tiles * (uint64_t)w.blocks;
+// Blocks that a part has: so many that about p.items parts come of all that the tiles can see, given for the first 64 sequences in
+// `mine`.  The same for every wave; taken for more than it is where a float does not hold it.
+__device__ __forceinline__ int blocksOfPart(const AttentionArgs &a, const AttentionPlan &p, const SeqWork &mine) {
+    float total = (float)mine.tiles * (float)mine.blocks;
+    for (int base = 64; base < a.c.S; base += 64) {
+        const SeqWork w = measureSeq(a, p, base + (threadIdx.x & 63));
+        total += (float)w.tiles * (float)w.blocks;
     }
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        total += ((uint64_t)(uint32_t)__shfl_xor((int)(total >> 32), step) << 32) + (uint32_t)__shfl_xor((int)total, step);
-    }
-    const uint64_t part = (total * (uint64_t)a.c.KVH + kAttentionItems - 1) / kAttentionItems;
-    return (int)min(max(part, (uint64_t)p.minBlocks), (uint64_t)0x7fffffff);
+    for (int step = 1; step < min(a.c.S, 64); step *= 2) total += __shfl_xor(total, step);
+    total = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(total)));
+    const float part = ceilf(total * (float)a.c.KVH * 1.001f / (float)p.items);
+    return max(p.minBlocks, (int)fminf(part, 1e9f));
 }
-__device__ __forceinline__ int partsOf(const SeqWork &w, int part) { return w.blocks <= part ? 1 : (int)(((uint32_t)w.blocks + (uint32_t)part - 1) / (uint32_t)part); }
 
 struct Item {
     SeqWork w;
@@ -84,20 +78,19 @@ struct Item {
     int slot;  // of its partial result; -1: the item is its rows' only one
 };
 
-// Item `index` of the launch, or the sequence `index` (by sequence: slot is its first one, the tile none).  Items lie sequence by sequence, a sequence's
-// last tiles, which see most, first; key heads are next to one another, so that workgroups of one XCD (every eighth) read the same
-// keys where there are eight heads.  False: there is none.
-template <bool BY_SEQUENCE>
+// Item `index` of the launch.  Items lie sequence by sequence, a sequence's last tiles, which see most, first; key heads are next to one another, so
+// that workgroups of one XCD (every eighth) read the same keys where there are eight heads.  False: there is none.
 __device__ __forceinline__ bool findItem(const AttentionArgs &a, const AttentionPlan &p, int index, Item *out) {
-    const int lane = threadIdx.x & 63, part = blocksOfPart(a, p);
+    const int lane = threadIdx.x & 63;
+    SeqWork w = measureSeq(a, p, lane);
+    const int part = p.splits ? blocksOfPart(a, p, w) : 0x7fffffff;
     int items = 0, slots = 0;
-    for (int base = 0; base < a.c.S; base += 64) {
-        SeqWork w{};
-        if (base + lane < a.c.S) w = measureSeq(a, p, base + lane);
-        const int splits = partsOf(w, part), mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
-        const int before = items + waveSumBefore(mine), cutBefore = slots + waveSumBefore(cut);
-        const bool here = BY_SEQUENCE ? base + lane == index : mine > 0 && before <= index && index < before + mine;
-        const uint64_t found = __ballot(here);
+    for (int base = 0;;) {
+        int splits = 1;
+        if (p.splits && w.blocks > part) splits = min(p.maxParts, (int)(((uint32_t)w.blocks + (uint32_t)part - 1) / (uint32_t)part));
+        const int lanes = min(a.c.S - base, 64), mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
+        const int before = items + sumBefore(mine, lanes), cutBefore = p.splits ? slots + sumBefore(cut, lanes) : 0;
+        const uint64_t found = __ballot(mine > 0 && before <= index && index < before + mine);
         if (found) {
             const int l = __builtin_ctzll(found);
             out->w.begin = __builtin_amdgcn_readlane(w.begin, l);
@@ -107,24 +100,29 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
             out->w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
             out->w.blocks = __builtin_amdgcn_readlane(w.blocks, l);
             out->seq = base + l;
-            out->part = part;
             out->splits = __builtin_amdgcn_readlane(splits, l);
-            const int first = __builtin_amdgcn_readlane(cutBefore, l);
-            if (BY_SEQUENCE) {
-                out->slot = first;
-                return true;
+            const uint32_t local = (uint32_t)(index - __builtin_amdgcn_readlane(before, l));
+            uint32_t rest = fastDiv(local, p.kvh);
+            out->head = (int)(local - rest * (uint32_t)a.c.KVH);
+            out->split = 0;
+            out->slot = -1;
+            if (out->splits > 1) {
+                const uint32_t tile = rest / (uint32_t)out->splits;
+                out->split = (int)(rest - tile * (uint32_t)out->splits);
+                rest = tile;
+                out->part = (int)(((uint32_t)out->w.blocks + (uint32_t)out->splits - 1) / (uint32_t)out->splits);
+                out->slot = __builtin_amdgcn_readlane(cutBefore, l) + (int)local;
             }
-            const int local = index - __builtin_amdgcn_readlane(before, l), rest = local / a.c.KVH;
-            out->head = local - rest * a.c.KVH;
-            out->split = rest % out->splits;
-            out->tile = out->w.tiles - 1 - rest / out->splits;
-            out->slot = out->splits > 1 ? first + local : -1;
-            return out->slot < p.slots;  // false: starts that do not ascend
+            out->tile = out->w.tiles - 1 - (int)rest;
+            // starts that do not ascend may make more of them: the parts of a run that would not all have a place are left out
+            return out->splits == 1 || out->slot + (out->splits - 1 - out->split) * a.c.KVH < p.slots;
         }
+        base += 64;
+        if (base >= a.c.S) return false;
         items = __builtin_amdgcn_readlane(before + mine, 63);
         slots = __builtin_amdgcn_readlane(cutBefore + cut, 63);
+        w = measureSeq(a, p, base + lane);
     }
-    return false;
 }
 
 // The blocks that a tile reads: those of the first positions that stay visible, then from its first row's window on.  Blocks [from, to)
@@ -136,24 +134,110 @@ struct Span {
 };
 __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
     Span s;
-    const int r0 = it.tile * p.rows;
-    s.rows = min(p.rows, it.w.count * a.G - r0);
+    const int r0 = it.tile << p.rowsLog, keys = p.keys();
+    s.rows = min(p.rows(), it.w.count * a.G - r0);
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
     const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(top - a.window + 1, 0) : 0;
-    s.sinkBlocks = (min(min(a.sinks, low), high) + p.keys - 1) / p.keys;
-    s.windowBlock = max(low / p.keys, s.sinkBlocks);
-    const int all = s.sinkBlocks + max((high + p.keys - 1) / p.keys - s.windowBlock, 0);
+    s.sinkBlocks = (min(min(a.sinks, low), high) + keys - 1) >> p.keysLog;
+    s.windowBlock = max(low >> p.keysLog, s.sinkBlocks);
+    const int all = s.sinkBlocks + max(((int)((uint32_t)high + (uint32_t)keys - 1) >> p.keysLog) - s.windowBlock, 0);
     s.from = min(it.splits > 1 ? it.split * it.part : 0, all);
     s.to = it.splits > 1 ? min(all, s.from + it.part) : all;
     return s;
 }
-__device__ __forceinline__ int blockStart(const AttentionPlan &p, const Span &s, int b) { return (b < s.sinkBlocks ? b : b - s.sinkBlocks + s.windowBlock) * p.keys; }
+__device__ __forceinline__ int blockStart(const AttentionPlan &p, const Span &s, int b) { return (b < s.sinkBlocks ? b : b - s.sinkBlocks + s.windowBlock) << p.keysLog; }
 
 // Row of the keys (elements / D) that position j of a sequence has; -1: none.
 template <bool PAGED>
 __device__ __forceinline__ int keyRow(const CacheArgs &c, int seq, int begin, int length, int head, int j) {
-    if constexpr (PAGED) return j < length ? (int)cacheRow(c, seq, head, j) : -1;
+    if constexpr (PAGED) return cacheRow(c, seq, head, j < length ? j : -1);
     return j < length ? (begin + j) * c.KVH + head : -1;
+}
+
+// ---- partial results ---------------------------------------------------------------------------------------------------
+
+// A slot holds, for each row of a tile, D sums, then the maximum and the sum of weights.  They go from workgroup to workgroup, which may be on
+// different XCDs, past the caches, by loads and stores at the device's scope (a fence would write the XCD's whole L2 back).
+constexpr int kDeviceScope = 16;  // sc1
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t slotsOf(const AttentionArgs &a, const AttentionPlan &p) {
+    return __builtin_amdgcn_make_buffer_rsrc(a.work, 0, (int)((uint32_t)p.slots * (uint32_t)p.rows() * (uint32_t)(a.c.D + 4) * 4u), 0x00020000);
+}
+__device__ __forceinline__ uint32_t slotRow(const AttentionArgs &a, const AttentionPlan &p, int slot, int r) {
+    return (((uint32_t)slot << p.rowsLog) + (uint32_t)r) * (uint32_t)(a.c.D + 4) * 4u;
+}
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t to, uint32_t at, float x, float y, float z, float w) {
+    __builtin_amdgcn_raw_buffer_store_b128(v4u{__float_as_uint(x), __float_as_uint(y), __float_as_uint(z), __float_as_uint(w)}, to, (int)at, 0, kDeviceScope);
+}
+__device__ __forceinline__ v4f get4(__amdgpu_buffer_rsrc_t from, uint32_t at) {
+    return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, 0, kDeviceScope));
+}
+
+__device__ __forceinline__ int packBf16(float lo, float hi) { return __builtin_bit_cast(int, __builtin_convertvector((v2f){lo, hi}, v2bf)); }
+
+// Every thread of a workgroup that has stored its part: the last one of the run's to come here adds the parts, in their order, scaled to
+// their common maximum.  room: LDS that nobody uses any more, ROWS (PARTS + 1) floats and one.
+template <int ROWS, int PARTS>
+__device__ __forceinline__ void joinParts(const AttentionArgs &a, const AttentionPlan &p, const Item &it, int rows, float *room) {
+    constexpr int LANES = 256 / ROWS, EACH = PARTS / LANES;  // threads of a row, and parts of each
+    const int tid = threadIdx.x, D = a.c.D, first = it.slot - it.split * a.c.KVH;
+    const auto slots = slotsOf(a, p);
+    uint32_t *const counter = (uint32_t *)(a.work + slotRow(a, p, (int)p.slots, 0)) + first;
+    int *const last = (int *)room;
+    float *const factors = room + 1, *const totals = factors + ROWS * PARTS;
+    waitVmcnt<0>();  // this wave's part is where the others will look
+    __syncthreads();
+    if (tid == 0) *last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == (uint32_t)it.splits;
+    __syncthreads();
+    if (!*last) return;
+    if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    {
+        const int r = tid / LANES, mine = tid % LANES;
+        v4f part[EACH];
+        float most = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int s = e * LANES + mine;
+            part[e] = v4f{-INFINITY, 0.0f, 0.0f, 0.0f};
+            if (s < it.splits) part[e] = get4(slots, slotRow(a, p, first + s * a.c.KVH, min(r, rows - 1)) + D * 4);
+        }
+#pragma unroll
+        for (int e = 0; e < EACH; e++) most = fmaxf(most, part[e][0]);
+#pragma unroll
+        for (int step = 1; step < LANES; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
+        const float shift = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const float f = __builtin_amdgcn_exp2f(part[e][0] - shift);
+            factors[r * PARTS + e * LANES + mine] = f;
+            total += f * part[e][1];
+        }
+#pragma unroll
+        for (int step = 1; step < LANES; step *= 2) total += __shfl_xor(total, step);
+        if (mine == 0) totals[r] = total == 0.0f ? 0.0f : 1.0f / total;
+    }
+    __syncthreads();
+    const int pieces = D >> 2;
+    const uint32_t step = slotRow(a, p, a.c.KVH, 0);
+    for (int e = tid; e < rows * pieces; e += 256) {
+        const int r = e / pieces, d = 4 * (e - r * pieces);
+        v4f sum{0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t from = slotRow(a, p, first, r) + d * 4;
+        for (int s = 0; s < it.splits; s += 8) {
+            v4f part[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) part[k] = get4(slots, from + min(s + k, it.splits - 1) * step);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float f = s + k < it.splits ? factors[r * PARTS + s + k] : 0.0f;
+                if (s + k < it.splits) sum += f * part[k];
+            }
+        }
+        const int mine = it.tile * ROWS + r, token = (int)fastDiv((uint32_t)mine, a.g);
+        *(v2i *)(a.out + ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + mine - token * a.G) * D + d) =
+            v2i{packBf16(sum[0] * totals[r], sum[1] * totals[r]), packBf16(sum[2] * totals[r], sum[3] * totals[r])};
+    }
 }
 
 // ---- one row, key by key ----------------------------------------------------------------------------------------------
@@ -163,7 +247,7 @@ __device__ __forceinline__ int keyRow(const CacheArgs &c, int seq, int begin, in
 // masked value by a weight of zero, and hand a row here where that left a NaN.  Adds positions [from, to) to o, m and l.
 // q: D floats of LDS, the row's query.
 template <bool PAGED, bool Q8>
-__device__ __noinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, int pos, int from, int to, float *o, float *m, float *l) {
+__device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, int pos, int from, int to, float *o, float *m, float *l) {
     const CacheArgs &c = a.c;
     const int lane = threadIdx.x & 63, D = c.D;
     float most = *m, sum = *l;
@@ -234,9 +318,9 @@ __device__ __noinline__ void attendRow(const AttentionArgs &a, const float *q, c
 
 // A row of an item once more, key by key, and its result or partial result stored.  q: LDS of this wave, kMaxHeadDim floats.
 template <bool PAGED, bool Q8>
-__device__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const Item &it, const Span &span, int r, float *q) {
+__device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const Item &it, const Span &span, int r, float *q) {
     const int lane = threadIdx.x & 63, D = a.c.D;
-    const int inSeq = it.tile * p.rows + r, token = (int)fastDiv((uint32_t)inSeq, a.g), h = it.head * a.G + inSeq - token * a.G;
+    const int inSeq = (it.tile << p.rowsLog) + r, token = (int)fastDiv((uint32_t)inSeq, a.g), h = it.head * a.G + inSeq - token * a.G;
     const int64_t at = ((int64_t)(it.w.begin + token) * a.H + h) * D;
     for (int d = lane; d < D; d += 64) q[d] = __uint_as_float((uint32_t)a.query[at + d] << 16);
     __threadfence_block();
@@ -244,7 +328,7 @@ __device__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const It
     const int pos = it.w.first + token;
     for (int b = span.from; b < span.to; b++) {
         const int j = blockStart(p, span, b);
-        attendRow<PAGED, Q8>(a, q, it, pos, j, j + p.keys, o, &m, &l);
+        attendRow<PAGED, Q8>(a, q, it, pos, j, j + p.keys(), o, &m, &l);
     }
     if (it.slot < 0) {
 #pragma unroll
@@ -253,16 +337,14 @@ __device__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const It
             if (d < D) a.out[at + d] = bf16Bits(l == 0.0f ? 0.0f : o[e] / l);
         }
     } else {
-        float *part = (float *)a.work + ((int64_t)it.slot * p.rows + r) * (D + 4);
+        const auto slots = slotsOf(a, p);
+        const uint32_t at = slotRow(a, p, it.slot, r);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const int d = lane + 64 * e;
-            if (d < D) part[d] = o[e];
+            if (d < D) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[e]), slots, (int)at + d * 4, 0, kDeviceScope);
         }
-        if (lane == 0) {
-            part[D] = m;
-            part[D + 1] = l;
-        }
+        if (lane == 0) put4(slots, at + D * 4, m, l, 0.0f, 0.0f);
     }
     __threadfence_block();
 }
@@ -285,8 +367,6 @@ __device__ __forceinline__ float sumOverQuarters(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return sumOverHalves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
-
-__device__ __forceinline__ int packBf16(float lo, float hi) { return __builtin_bit_cast(int, __builtin_convertvector((v2f){lo, hi}, v2bf)); }
 
 // Four int8 as bf16, which holds them: the upper halves of their floats.
 __device__ __forceinline__ v2i wholeBf16(int w) {
@@ -319,18 +399,18 @@ constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the 
 
 // ---- tiles of 128 rows ------------------------------------------------------------------------------------------------
 
-// Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is in registers while
+// Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is on its way while
 // one is worked on, the rows of the block behind that are being looked up.
 template <int DT, bool PAGED, bool Q8>
-__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(AttentionArgs a, AttentionPlan p) {
+__global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(AttentionArgs a, AttentionPlan p) {
     constexpr int KB = DT == 256 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]
     uint8_t *const flagRoom = (uint8_t *)(scaleRoom + 4 * KB);      // [2][4 waves]: some row of the block is not there
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const CacheArgs &c = a.c;
     Item it;
-    if (!findItem<false>(a, p, blockIdx.x, &it)) return;
+    if (!findItem(a, p, blockIdx.x, &it)) return;
     const Span span = spanOf(a, p, it);
     const int D = c.D, r0 = it.tile * 128 + wave * 32, rowsHere = min(32, span.rows - wave * 32);  // of this wave; none: <= 0
     const bool active = rowsHere > 0;
@@ -342,8 +422,8 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
     v8bf q[DT / 16];
 #pragma unroll
     for (int t = 0; t < DT / 16; t++) {
-        v4i w{0, 0, 0, 0};
-        if (active && 16 * t < D) w = *(const v4i *)(a.query + at + 16 * t + 8 * half);
+        v4i w = *(const v4i *)(a.query + at + (16 * t < D ? 16 * t : 0) + 8 * half);
+        if (16 * t >= D) w = v4i{0, 0, 0, 0};
         q[t] = __builtin_bit_cast(v8bf, w);
     }
     v16f o[DT / 32];
@@ -352,77 +432,85 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
     float m = -INFINITY, l = 0.0f;
     const float scale = a.scale * kLog2e;
 
-    // this thread's part of a block: chunk `piece` of rows tid / CH + STEP i
-    const int piece = tid % CH, myRow = tid / CH;
-    const bool pieceIn = piece * 8 < D;
+    // this thread's part of a block: chunk `piece` of rows tid / CH + STEP i.  Loads are never skipped: a position that is not there is read
+    // as row 0, and the value taken for zeros, its score for minus infinity; behind D a piece is the first one, against zeros of the query.
+    const int piece = tid % CH, myRow = tid / CH, pieceAt = piece * 8 < D ? piece * 8 : 0;
     int rows[PER], scaleRow = -1;
-    v4i kreg[PER], vreg[PER];
+    v2i kreg[PER], vreg[PER];
     float sreg = 0.0f;
-    int held[PER];
+    uint32_t gone = 0;  // rows of the block in the registers that are not there, a bit each
     auto lookUp = [&](int b) {
-        const int j0 = blockStart(p, span, b);
+        const int j0 = blockStart(p, span, b), length = b < span.to ? it.w.length : 0;
 #pragma unroll
-        for (int i = 0; i < PER; i++) rows[i] = b < span.to ? keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j0 + myRow + STEP * i) : -1;
-        if constexpr (Q8) {
-            scaleRow = -1;
-            if (tid < 2 * KB && b < span.to) scaleRow = keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j0 + (tid & (KB - 1)));
-        }
+        for (int i = 0; i < PER; i++) rows[i] = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + myRow + STEP * i);
+        if constexpr (Q8) scaleRow = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + (tid & (KB - 1)));
     };
-    auto fetch = [&]() {
+    // bf16: straight into LDS, a wave's 64 pieces of 16 bytes one behind the other, so that a lane's place is given and it takes the
+    // piece that belongs there
+    const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t *)smem) + wave * 1024;
+    auto send = [&](int stage) {
+        gone = 0;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            held[i] = rows[i];
-            kreg[i] = v4i{0, 0, 0, 0};
-            vreg[i] = v4i{0, 0, 0, 0};
-            if (rows[i] >= 0 && pieceIn) {
-                const int64_t from = (int64_t)rows[i] * D + piece * 8;
-                if constexpr (Q8) {
-                    const v2i kw = *(const v2i *)((const int8_t *)a.key + from), vw = *(const v2i *)((const int8_t *)a.value + from);
-                    kreg[i] = v4i{kw[0], kw[1], 0, 0};
-                    vreg[i] = v4i{vw[0], vw[1], 0, 0};
-                } else {
-                    kreg[i] = *(const v4i *)((const uint16_t *)a.key + from);
-                    vreg[i] = *(const v4i *)((const uint16_t *)a.value + from);
-                }
-            }
-        }
-        if constexpr (Q8) {
-            sreg = 0.0f;
-            if (scaleRow >= 0) sreg = (tid < KB ? a.key_scales : a.value_scales)[scaleRow];
+            gone |= rows[i] < 0 ? 1u << i : 0u;
+            const int mine = piece ^ swizzle<ROW>(myRow + STEP * i);
+            const int64_t from = ((int64_t)max(rows[i], 0) * D + (mine * 8 < D ? mine * 8 : 0)) * 2;
+            dmaLoad16((const int8_t *)a.key + from, lds + stage * 2 * KB * ROW + i * 4096);
+            dmaLoad16((const int8_t *)a.value + from, lds + stage * 2 * KB * ROW + KB * ROW + i * 4096);
         }
     };
-    auto put = [&](int stage) {
-        int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
-        bool missing = false;
+    auto arrive = [&](int stage) {
+        waitVmcnt<0>();
+        const bool some = __any(gone != 0);
+        if (some) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int row = myRow + STEP * i, where = row * ROW + ((piece ^ swizzle<ROW>(row)) << 4);
-            v4i kw = kreg[i], vw = vreg[i];
-            if constexpr (Q8) {
-                kw = __builtin_bit_cast(v4i, wholeBf16x8(kw[0], kw[1]));
-                vw = __builtin_bit_cast(v4i, wholeBf16x8(vw[0], vw[1]));
+            for (int i = 0; i < PER; i++) {
+                if ((gone >> i) & 1) *(v4i *)(smem + stage * 2 * KB * ROW + KB * ROW + i * 4096 + tid * 16) = v4i{0, 0, 0, 0};
             }
-            *(v4i *)(keys + where) = kw;
-            *(v4i *)(values + where) = vw;
-            missing = missing || held[i] < 0;
-        }
-        if constexpr (Q8) {
-            if (tid < 2 * KB) scaleRoom[stage * 2 * KB + tid] = sreg;
         }
         if constexpr (PAGED) {
-            const bool some = __any(missing);
             if (lane == 0) flagRoom[stage * 4 + wave] = some;
         }
     };
+    // int8: through registers, where they become bf16
+    auto fetch = [&]() {
+        gone = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            gone |= rows[i] < 0 ? 1u << i : 0u;
+            const int64_t from = (int64_t)max(rows[i], 0) * D + pieceAt;
+            kreg[i] = *(const v2i *)((const int8_t *)a.key + from);
+            vreg[i] = *(const v2i *)((const int8_t *)a.value + from);
+        }
+        sreg = (tid & KB ? a.value_scales : a.key_scales)[max(scaleRow, 0)];
+    };
+    auto put = [&](int stage) {
+        int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
+        const bool some = __any(gone != 0);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int row = myRow + STEP * i, where = row * ROW + ((piece ^ swizzle<ROW>(row)) << 4);
+            *(v8bf *)(keys + where) = wholeBf16x8(kreg[i][0], kreg[i][1]);
+            *(v8bf *)(values + where) = wholeBf16x8(vreg[i][0], vreg[i][1]);
+        }
+        if (tid < 2 * KB) scaleRoom[stage * 2 * KB + tid] = sreg;
+        if (lane == 0) flagRoom[stage * 4 + wave] = some;
+    };
 
     lookUp(span.from);
-    fetch();
+    if constexpr (Q8) fetch();
+    else send(0);
     lookUp(span.from + 1);
     for (int b = span.from, stage = 0; b < span.to; b++, stage ^= 1) {
-        put(stage);
-        fetch();
-        lookUp(b + 2);
+        if constexpr (Q8) {
+            put(stage);
+            fetch();
+        } else {
+            arrive(stage);
+        }
         __syncthreads();
+        if constexpr (!Q8) send(stage ^ 1);  // everybody is done with what was there
+        lookUp(b + 2);
         const int j0 = blockStart(p, span, b);
         if (!active || j0 > bottom) continue;
         const int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
@@ -457,7 +545,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int j = j0 + k * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-                    bool see = sees(a, pos, j) && j < it.w.length;
+                    bool see = sees(a, pos, j) & (j < it.w.length);
                     if constexpr (PAGED) {
                         if (gaps && see) see = cacheRow(c, it.seq, it.head, j) >= 0;
                     }
@@ -520,8 +608,8 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
             }
         }
     }
+    waitVmcnt<0>();  // the block behind the last one
     __syncthreads();
-    if (!active) return;
     l = sumOverHalves(l);
     // a masked value that was no number, or a row that sees one
     bool odd = false;
@@ -529,7 +617,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
 #pragma unroll
         for (int t = 0; t < DT / 32; t++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) odd = odd || o[t][i] != o[t][i];
+            for (int i = 0; i < 16; i++) odd |= o[t][i] != o[t][i];
         }
     }
     const uint64_t odds = __ballot(odd);
@@ -546,19 +634,17 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
                 }
             }
         } else {
-            float *part = (float *)a.work + ((int64_t)it.slot * 128 + wave * 32 + col) * (D + 4);
+            const auto slots = slotsOf(a, p);
+            const uint32_t to = slotRow(a, p, it.slot, wave * 32 + col);
 #pragma unroll
             for (int t = 0; t < DT / 32; t++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int d = 32 * t + 8 * i + 4 * half;
-                    if (d < D) *(v4f *)(part + d) = v4f{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+                    if (d < D) put4(slots, to + d * 4, o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
                 }
             }
-            if (half == 0) {
-                part[D] = m;
-                part[D + 1] = l;
-            }
+            if (half == 0) put4(slots, to + D * 4, m, l, 0.0f, 0.0f);
         }
     }
     if constexpr (!Q8) {
@@ -566,6 +652,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
             if ((again >> r) & 1) redoRow<PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)smem + wave * kMaxHeadDim);
         }
     }
+    if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
 }
 
 // ---- few rows: keys and values streamed -----------------------------------------------------------------------------------
@@ -573,15 +660,15 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void attention_tiles(Attent
 // A tile of 16 rows (a token's heads, or a few tokens'); each of the four waves has blocks of 32 keys of its own, every fourth, and joins the
 // others at the end.  A wave waits for nobody: its keys go straight into the matrix operand's registers, its values through LDS of its own.
 // The registers are filled again as soon as their content is used, so a block's 2 x 32 rows are under way while the one before is worked on.
-template <int DT, bool PAGED, bool Q8>
+template <int DT, bool EXACT, bool PAGED, bool Q8>
 __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_stream(AttentionArgs a, AttentionPlan p) {
     constexpr int KB = 32, STEPS = DT / 32, ROW = DT * (Q8 ? 1 : 2), LOADS = ROW / 64;  // LOADS: 16-byte pieces of a row that one of four lanes has
     constexpr int JOIN = 16 * (DT + 4);  // floats of a wave's result
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
     const CacheArgs &c = a.c;
     Item it;
-    if (!findItem<false>(a, p, blockIdx.x, &it)) return;
+    if (!findItem(a, p, blockIdx.x, &it)) return;
     const Span span = spanOf(a, p, it);
     const int D = c.D, r0 = it.tile * 16;
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + span.rows - 1), a.g);
@@ -590,6 +677,34 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
     int8_t *const values = smem + wave * KB * ROW;
     float *const scales = (float *)(smem + 4 * KB * ROW) + wave * 2 * KB;
 
+    // Loads are never skipped: a position that is not there is read as row 0, its value taken for zeros and its score for minus infinity; behind D
+    // (not EXACT) a piece is the first one, against zeros of the query.
+    int row0, row1;      // of the block to be fetched next: keys col and 16 + col
+    bool there0, there1; // of the block in the registers
+    v4i kreg[2][LOADS], vreg[2][LOADS];
+    float sreg = 0.0f;
+    auto lookUp = [&](int b) {
+        const int j0 = blockStart(p, span, b), length = b < span.to ? it.w.length : 0;
+        row0 = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + col);
+        row1 = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + 16 + col);
+    };
+    constexpr int ELEMS = Q8 ? 16 : 8, SIZE = Q8 ? 1 : 2;  // elements of a piece, bytes of an element
+    auto fetch = [&](const void *from, v4i(&reg)[2][LOADS]) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int8_t *const at = (const int8_t *)from + ((int64_t)max(k ? row1 : row0, 0) * D + (EXACT ? quarter * ELEMS : 0)) * SIZE;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int d = (4 * i + quarter) * ELEMS;
+                reg[k][i] = *(const v4i *)(at + (EXACT ? 64 * i : d < D ? d * SIZE : 0));
+            }
+        }
+    };
+    lookUp(span.from + wave);
+    auto fetchScales = [&]() {
+        if constexpr (Q8) sreg = (lane < 32 ? a.key_scales : a.value_scales)[max((lane & 16) ? row1 : row0, 0)];
+    };
+
     v8bf q[STEPS];
     {
         const int64_t at = ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + inSeq - token * a.G) * D;
@@ -597,8 +712,8 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
         for (int t = 0; t < STEPS; t++) {
             // of an int8 row a lane has 16 elements at a time, for two steps
             const int d = Q8 ? 64 * (t >> 1) + 16 * quarter + 8 * (t & 1) : 32 * t + 8 * quarter;
-            v4i w{0, 0, 0, 0};
-            if (d < D) w = *(const v4i *)(a.query + at + d);
+            v4i w = *(const v4i *)(a.query + at + (EXACT || d < D ? d : 0));
+            if (!EXACT && d >= D) w = v4i{0, 0, 0, 0};
             q[t] = __builtin_bit_cast(v8bf, w);
         }
     }
@@ -607,46 +722,22 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
     for (int t = 0; t < DT / 16; t++) o[t] = v4f{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
     const float scale = a.scale * kLog2e;
-
-    int rows[2];         // of the block to be fetched next: keys col and 16 + col
-    bool there[2];       // of the block in the registers
-    v4i kreg[2][LOADS], vreg[2][LOADS];
-    float sreg = 0.0f;
-    auto lookUp = [&](int b) {
-        const int j0 = blockStart(p, span, b);
-#pragma unroll
-        for (int k = 0; k < 2; k++) rows[k] = b < span.to ? keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j0 + 16 * k + col) : -1;
-    };
-    constexpr int ELEMS = Q8 ? 16 : 8;  // of a piece
-    auto fetch = [&](const void *from, v4i(&reg)[2][LOADS]) {
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-#pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int d = (4 * i + quarter) * ELEMS;
-                reg[k][i] = v4i{0, 0, 0, 0};
-                if (rows[k] >= 0 && d < D) reg[k][i] = *(const v4i *)((const int8_t *)from + ((int64_t)rows[k] * D + d) * (Q8 ? 1 : 2));
-            }
-        }
-    };
-    auto fetchScales = [&]() {
-        if constexpr (Q8) {
-            const int row = (lane & 16) ? rows[1] : rows[0];
-            sreg = 0.0f;
-            if (row >= 0) sreg = (lane < 32 ? a.key_scales : a.value_scales)[row];
-        }
-    };
-
-    lookUp(span.from + wave);
-    there[0] = rows[0] >= 0;
-    there[1] = rows[1] >= 0;
+    there0 = row0 >= 0;
+    there1 = row1 >= 0;
     fetchScales();
     fetch(a.value, vreg);
     fetch(a.key, kreg);
     lookUp(span.from + wave + 4);
     for (int b = span.from + wave; b < span.to; b += 4) {
         const int j0 = blockStart(p, span, b);
-        const uint64_t gone0 = __ballot(!there[0]), gone1 = __ballot(!there[1]);
+        const uint64_t gone0 = __ballot(!there0), gone1 = __ballot(!there1);
+        if (gone0 | gone1) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                if (!there0) vreg[0][i] = v4i{0, 0, 0, 0};
+                if (!there1) vreg[1][i] = v4i{0, 0, 0, 0};
+            }
+        }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int k = 0; k < 2; k++) {
@@ -661,7 +752,7 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
         }
         if constexpr (Q8) scales[lane] = sreg;
         __builtin_amdgcn_wave_barrier();
-        const bool now0 = rows[0] >= 0, now1 = rows[1] >= 0;
+        const bool now0 = row0 >= 0, now1 = row1 >= 0;
         fetchScales();
         fetch(a.value, vreg);
         v4f s[2];
@@ -677,8 +768,8 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
             }
         }
         fetch(a.key, kreg);
-        there[0] = now0;
-        there[1] = now1;
+        there0 = now0;
+        there1 = now1;
         lookUp(b + 8);
         if constexpr (Q8) {
 #pragma unroll
@@ -695,7 +786,7 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = 4 * quarter + i, j = j0 + 16 * k + key;
-                    const bool see = sees(a, pos, j) && !(((k ? gone1 : gone0) >> key) & 1);
+                    const bool see = sees(a, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
                     s[k][i] = see ? s[k][i] : -INFINITY;
                 }
             }
@@ -771,7 +862,7 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
 #pragma unroll
         for (int w = 0; w < 4; w++) sum[e] += factor[w] * *(const v4f *)(join + w * JOIN + r * (DT + 4) + 64 * e + 4 * col);
 #pragma unroll
-        for (int i = 0; i < 4; i++) odd = odd || sum[e][i] != sum[e][i];
+        for (int i = 0; i < 4; i++) odd |= sum[e][i] != sum[e][i];
     }
     // the rows of this wave that have a NaN: 4 wave .. 4 wave + 3, 16 lanes each
     const uint64_t odds = Q8 ? 0 : __ballot(odd);
@@ -785,15 +876,13 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
                 if (64 * e + 4 * col < D) *(v2i *)(out + 64 * e + 4 * col) = v2i{packBf16(sum[e][0] * by, sum[e][1] * by), packBf16(sum[e][2] * by, sum[e][3] * by)};
             }
         } else {
-            float *part = (float *)a.work + ((int64_t)it.slot * 16 + r) * (D + 4);
+            const auto slots = slotsOf(a, p);
+            const uint32_t to = slotRow(a, p, it.slot, r);
 #pragma unroll
             for (int e = 0; e < DT / 64; e++) {
-                if (64 * e + 4 * col < D) *(v4f *)(part + 64 * e + 4 * col) = sum[e];
+                if (64 * e + 4 * col < D) put4(slots, to + (64 * e + 4 * col) * 4, sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
             }
-            if (col == 0) {
-                part[D] = most;
-                part[D + 1] = total;
-            }
+            if (col == 0) put4(slots, to + D * 4, most, total, 0.0f, 0.0f);
         }
     }
     if constexpr (!Q8) {
@@ -802,53 +891,13 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
             if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
         }
     }
+    if (it.slot >= 0) {
+        __syncthreads();
+        joinParts<16, 64>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
+    }
 }
 
-// ---- the parts of cut runs joined ---------------------------------------------------------------------------------------
-
-// A wave a row and head; a lane has four elements of some of the parts.
-__global__ __launch_bounds__(256) void attention_join(AttentionArgs a, AttentionPlan p) {
-    const CacheArgs &c = a.c;
-    const int lane = threadIdx.x & 63;
-    const int64_t index = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (index >= (int64_t)c.T * a.H) return;
-    const int row = (int)(index / a.H), h = (int)(index - (int64_t)row * a.H), head = (int)fastDiv((uint32_t)h, a.g);
-    const RowPlace place = placeOf(c, c.starts, row);
-    if (place.seq < 0) return;
-    Item it;
-    if (!findItem<true>(a, p, place.seq, &it) || it.splits <= 1) return;
-    if (it.slot + (int64_t)it.w.tiles * it.splits * c.KVH > p.slots) return;  // starts that do not ascend
-    const int inSeq = (row - place.begin) * a.G + h - head * a.G, tile = inSeq / p.rows, D = c.D;
-    const int64_t slot0 = it.slot + (int64_t)(it.w.tiles - 1 - tile) * it.splits * c.KVH + head;
-    const float *base = (const float *)a.work + (slot0 * p.rows + inSeq - tile * p.rows) * (D + 4);
-    const int64_t stride = (int64_t)c.KVH * p.rows * (D + 4);
-    float most = -INFINITY;
-    for (int s = lane; s < it.splits; s += 64) most = fmaxf(most, base[s * stride + D]);
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
-    const float shift = most == -INFINITY ? 0.0f : most;
-    const int lanes = D >> 2, groups = 64 / lanes, group = lane / lanes, piece = lane - group * lanes;
-    v4f sum{0, 0, 0, 0};
-    float total = 0.0f;
-    if (group < groups) {
-        for (int s = group; s < it.splits; s += groups) {
-            const float *part = base + s * stride;
-            const float f = __builtin_amdgcn_exp2f(part[D] - shift);
-            sum += f * *(const v4f *)(part + 4 * piece);
-            total += f * part[D + 1];
-        }
-    }
-    v4f all = sum;
-    float l = total;
-    for (int g = 1; g < groups; g++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) all[i] += __shfl(sum[i], (lane + g * lanes) & 63);
-        l += __shfl(total, (lane + g * lanes) & 63);
-    }
-    if (lane >= lanes) return;
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
-    *(v2i *)(a.out + index * D + 4 * piece) = v2i{packBf16(all[0] * by, all[1] * by), packBf16(all[2] * by, all[3] * by)};
-}
+// ---- launches -------------------------------------------------------------------------------------------------------------
 
 static hipError_t checkAttention(const AttentionArgs &a) {
     const CacheArgs &c = a.c;
@@ -872,6 +921,7 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
     if (p.tiles) {
         constexpr int KB = DT == 256 ? 32 : 64;
         constexpr size_t lds = 4 * KB * DT * 2 + 4 * KB * 4 + 16;
+        static_assert(lds >= (4 * kMaxHeadDim + 128 * 17 + 1) * 4, "what joins the parts");
         auto kernel = attention_tiles<DT, PAGED, Q8>;
         // asked for the kernel's name, as every executable does once on its device, the launcher configures it there
         if (lds > 64 * 1024 && ctx.name) {
@@ -880,11 +930,17 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
         THIP_ENQUEUE(ctx, kernelLabel("attention_tiles", {DT, PAGED, Q8}), kernel, grid, dim3(256), lds, a, p);
     } else {
         constexpr size_t tiles = 4 * 32 * DT * (Q8 ? 1 : 2) + (Q8 ? 4 * 64 * 4 : 0), join = 4 * 16 * (DT + 4) * 4, lds = tiles > join ? tiles : join;
-        auto kernel = attention_stream<DT, PAGED, Q8>;
-        if (lds > 64 * 1024 && ctx.name) {
-            if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return e;
-        }
-        THIP_ENQUEUE(ctx, kernelLabel("attention_stream", {DT, PAGED, Q8}), kernel, grid, dim3(256), lds, a, p);
+        static_assert(lds >= (4 * kMaxHeadDim + 16 * 65 + 1) * 4, "what joins the parts");
+        auto enqueue = [&](auto exact) -> hipError_t {
+            constexpr bool EXACT = decltype(exact)::value;
+            auto kernel = attention_stream<DT, EXACT, PAGED, Q8>;
+            if (lds > 64 * 1024 && ctx.name) {
+                if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return e;
+            }
+            THIP_ENQUEUE(ctx, kernelLabel("attention_stream", {DT, EXACT, PAGED, Q8}), kernel, grid, dim3(256), lds, a, p);
+            return hipSuccess;
+        };
+        if (hipError_t e = a.c.D == DT ? enqueue(std::true_type{}) : enqueue(std::false_type{})) return e;
     }
     return ctx.name ? hipSuccess : hipGetLastError();
 }
@@ -899,10 +955,7 @@ static hipError_t byHeadDim(const AttentionArgs &a, const AttentionPlan &p, cons
 hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx) {
     if (hipError_t e = checkAttention(a)) return e;
     const AttentionPlan p = attentionPlan(a.c.T, a.c.S, a.H, a.c.KVH, a.c.D, a.c.pages ? a.c.capacity : a.c.T, a.window, a.sinks);
-    hipError_t e = !a.c.pages ? byHeadDim<false, false>(a, p, ctx) : a.key_scales ? byHeadDim<true, true>(a, p, ctx) : byHeadDim<true, false>(a, p, ctx);
-    if (e != hipSuccess || !p.splits || ctx.name) return e;
-    THIP_ENQUEUE(ctx, "attention_join", attention_join, dim3((unsigned)(((int64_t)a.c.T * a.H + 3) / 4)), dim3(256), 0, a, p);
-    return hipGetLastError();
+    return !a.c.pages ? byHeadDim<false, false>(a, p, ctx) : a.key_scales ? byHeadDim<true, true>(a, p, ctx) : byHeadDim<true, false>(a, p, ctx);
 }
 
 }  // namespace thip

@@ -39,13 +39,12 @@ __device__ __forceinline__ RowPlace placeOf(const CacheArgs &c, const int32_t *s
     return p;
 }
 
-// Row of the cache that holds a position, -1: none does.
-__device__ __forceinline__ int64_t cacheRow(const CacheArgs &c, int seq, int head, int pos) {
-    if ((uint32_t)pos >= (uint32_t)c.capacity) return -1;
-    const uint32_t entry = fastDiv((uint32_t)pos, c.ps), slot = (uint32_t)pos - entry * c.ps.d;
-    const int32_t page = c.pages[(int64_t)seq * c.P + entry];
-    if ((uint32_t)page >= (uint32_t)c.NP) return -1;
-    return (int64_t)(((uint32_t)page * (uint32_t)c.KVH + (uint32_t)head) * (uint32_t)c.PS + slot);
+// Row of the cache that holds a position, -1: none does.  Without branches (a position that is none is looked up as the first).
+__device__ __forceinline__ int cacheRow(const CacheArgs &c, int seq, int head, int pos) {
+    const bool in = (uint32_t)pos < (uint32_t)c.capacity;
+    const uint32_t p = in ? (uint32_t)pos : 0u, entry = fastDiv(p, c.ps), slot = p - entry * c.ps.d;
+    const uint32_t page = (uint32_t)c.pages[(int64_t)seq * c.P + entry];
+    return in && page < (uint32_t)c.NP ? (int)((page * (uint32_t)c.KVH + (uint32_t)head) * (uint32_t)c.PS + slot) : -1;
 }
 
 // The starts in LDS, where they fit `most` sequences; every thread of the workgroup calls it.

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void cache_write(CacheRowsArgs a) {
         if (row < rows && piece < pieces) data[u] = streamLoad<v4i>(src + row * a.c.D + piece * 8);
     }
     const int32_t *starts = holdStarts(a.c, held, kStartsInLds);
-    int64_t to[U];
+    int to[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int64_t row = first + (int64_t)u * (256 >> LOG);
@@ -66,12 +66,12 @@ __global__ __launch_bounds__(256) void cache_write(CacheRowsArgs a) {
                 const int32_t hi = finite ? (int32_t)rintf(__uint_as_float(w & 0xffff0000u) * inverse) : 0;
                 q[i >> 1] |= (((uint32_t)lo & 0xffu) | (((uint32_t)hi & 0xffu) << 8)) << (16 * (i & 1));
             }
-            int8_t *cache = (int8_t *)(values ? a.value_cache : a.key_cache) + to[u] * a.c.D + piece * 8;
+            int8_t *cache = (int8_t *)(values ? a.value_cache : a.key_cache) + (int64_t)to[u] * a.c.D + piece * 8;
             *(v2i *)cache = v2i{(int)q[0], (int)q[1]};
             if (piece == 0) (values ? a.value_scales : a.key_scales)[to[u]] = finite ? unit / 127.0f : __uint_as_float(0x7fc00000u);
         } else {
             if (to[u] < 0 || piece >= pieces) continue;
-            uint16_t *cache = (uint16_t *)(values ? a.value_cache : a.key_cache) + to[u] * a.c.D + piece * 8;
+            uint16_t *cache = (uint16_t *)(values ? a.value_cache : a.key_cache) + (int64_t)to[u] * a.c.D + piece * 8;
             *(v4i *)cache = data[u];
         }
     }
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256) void cache_read(CacheRowsArgs a) {
     const int64_t rows = (int64_t)a.c.T * a.c.KVH, first = (int64_t)blockIdx.x * (256 >> LOG) * U + (threadIdx.x >> LOG);
     uint16_t *dst = values ? a.value : a.key;
     const int32_t *starts = holdStarts(a.c, held, kStartsInLds);
-    int64_t from[U];
+    int from[U];
     bool there[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void cache_read(CacheRowsArgs a) {
             q[u] = v2i{0, 0};
             scale[u] = 0.0f;
             if (from[u] < 0) continue;
-            q[u] = streamLoad<v2i>((const int8_t *)(values ? a.value_cache : a.key_cache) + from[u] * a.c.D + piece * 8);
+            q[u] = streamLoad<v2i>((const int8_t *)(values ? a.value_cache : a.key_cache) + (int64_t)from[u] * a.c.D + piece * 8);
             scale[u] = (values ? a.value_scales : a.key_scales)[from[u]];
         }
 #pragma unroll
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void cache_read(CacheRowsArgs a) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             data[u] = v4i{0, 0, 0, 0};
-            if (from[u] >= 0) data[u] = streamLoad<v4i>((const uint16_t *)(values ? a.value_cache : a.key_cache) + from[u] * a.c.D + piece * 8);
+            if (from[u] >= 0) data[u] = streamLoad<v4i>((const uint16_t *)(values ? a.value_cache : a.key_cache) + (int64_t)from[u] * a.c.D + piece * 8);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
