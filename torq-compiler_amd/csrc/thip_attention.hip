@@ -147,11 +147,26 @@ __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPl
 }
 __device__ __forceinline__ int blockStart(const AttentionPlan &p, const Span &s, int b) { return (b < s.sinkBlocks ? b : b - s.sinkBlocks + s.windowBlock) << p.keysLog; }
 
-// Row of the keys (elements / D) that position j of a sequence has; -1: none.
+// Row of the keys (elements / D) that position j of a sequence has; -1: none.  In a loop a position is asked for a block ahead of the loads that
+// need its row, and before the loads of the block before: loads come back in order, and a wait for an entry of the table would be one for all that
+// were sent before it.
 template <bool PAGED>
-__device__ __forceinline__ int keyRow(const CacheArgs &c, int seq, int begin, int length, int head, int j) {
-    if constexpr (PAGED) return cacheRow(c, seq, head, j < length ? j : -1);
-    return j < length ? (begin + j) * c.KVH + head : -1;
+struct KeyAsk {
+    PageAsk page;
+};
+template <>
+struct KeyAsk<false> {
+    int row;
+};
+template <bool PAGED>
+__device__ __forceinline__ KeyAsk<PAGED> askKey(const AttentionArgs &a, const Item &it, int j, bool in) {
+    if constexpr (PAGED) return {askPage(a.c, it.seq, j, in ? it.w.length : 0)};
+    else return {in & (j < it.w.length) ? (it.w.begin + j) * a.c.KVH + it.head : -1};
+}
+template <bool PAGED>
+__device__ __forceinline__ int keyRow(const AttentionArgs &a, const Item &it, const KeyAsk<PAGED> &q) {
+    if constexpr (PAGED) return rowOf(a.c, q.page, it.head);
+    else return q.row;
 }
 
 // ---- partial results ---------------------------------------------------------------------------------------------------
@@ -254,7 +269,7 @@ __device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q
     for (int base = from; base < to; base += 64) {
         const int j = base + lane;
         int row = -1;
-        if (j < to && sees(a, pos, j)) row = keyRow<PAGED>(c, it.seq, it.w.begin, it.w.length, it.head, j);
+        if (j < to && sees(a, pos, j)) row = keyRow(a, it, askKey<PAGED>(a, it, j, true));
         float s = -INFINITY, vs = 1.0f;
         if (row >= 0) {
             float dot = 0.0f;
@@ -436,14 +451,20 @@ __global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(
     // as row 0, and the value taken for zeros, its score for minus infinity; behind D a piece is the first one, against zeros of the query.
     const int piece = tid % CH, myRow = tid / CH, pieceAt = piece * 8 < D ? piece * 8 : 0;
     int rows[PER], scaleRow = -1;
+    KeyAsk<PAGED> asked[PER], scaleAsked;
     v2i kreg[PER], vreg[PER];
     float sreg = 0.0f;
-    uint32_t gone = 0;  // rows of the block in the registers that are not there, a bit each
-    auto lookUp = [&](int b) {
-        const int j0 = blockStart(p, span, b), length = b < span.to ? it.w.length : 0;
+    uint32_t gone = 0;  // rows of the block last sent for that are not there, a bit each
+    auto ask = [&](int b) {
+        const int j0 = blockStart(p, span, b);
 #pragma unroll
-        for (int i = 0; i < PER; i++) rows[i] = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + myRow + STEP * i);
-        if constexpr (Q8) scaleRow = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + (tid & (KB - 1)));
+        for (int i = 0; i < PER; i++) asked[i] = askKey<PAGED>(a, it, j0 + myRow + STEP * i, b < span.to);
+        if constexpr (Q8) scaleAsked = askKey<PAGED>(a, it, j0 + (tid & (KB - 1)), b < span.to);
+    };
+    auto resolve = [&]() {
+#pragma unroll
+        for (int i = 0; i < PER; i++) rows[i] = keyRow(a, it, asked[i]);
+        if constexpr (Q8) scaleRow = keyRow(a, it, scaleAsked);
     };
     // bf16: straight into LDS, a wave's 64 pieces of 16 bytes one behind the other, so that a lane's place is given and it takes the
     // piece that belongs there
@@ -497,20 +518,24 @@ __global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(
         if (lane == 0) flagRoom[stage * 4 + wave] = some;
     };
 
-    lookUp(span.from);
+    ask(span.from);
+    resolve();
+    ask(span.from + 1);
     if constexpr (Q8) fetch();
     else send(0);
-    lookUp(span.from + 1);
     for (int b = span.from, stage = 0; b < span.to; b++, stage ^= 1) {
+        resolve();
         if constexpr (Q8) {
+            ask(b + 2);
             put(stage);
             fetch();
+            __syncthreads();
         } else {
             arrive(stage);
+            __syncthreads();  // and everybody is done with the other buffer
+            ask(b + 2);
+            send(stage ^ 1);
         }
-        __syncthreads();
-        if constexpr (!Q8) send(stage ^ 1);  // everybody is done with what was there
-        lookUp(b + 2);
         const int j0 = blockStart(p, span, b);
         if (!active || j0 > bottom) continue;
         const int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
@@ -681,12 +706,17 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
     // (not EXACT) a piece is the first one, against zeros of the query.
     int row0, row1;      // of the block to be fetched next: keys col and 16 + col
     bool there0, there1; // of the block in the registers
+    KeyAsk<PAGED> asked0, asked1;  // of the block behind that
     v4i kreg[2][LOADS], vreg[2][LOADS];
     float sreg = 0.0f;
-    auto lookUp = [&](int b) {
-        const int j0 = blockStart(p, span, b), length = b < span.to ? it.w.length : 0;
-        row0 = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + col);
-        row1 = keyRow<PAGED>(c, it.seq, it.w.begin, length, it.head, j0 + 16 + col);
+    auto ask = [&](int b) {
+        const int j = blockStart(p, span, b) + col;
+        asked0 = askKey<PAGED>(a, it, j, b < span.to);
+        asked1 = askKey<PAGED>(a, it, j + 16, b < span.to);
+    };
+    auto resolve = [&]() {
+        row0 = keyRow(a, it, asked0);
+        row1 = keyRow(a, it, asked1);
     };
     constexpr int ELEMS = Q8 ? 16 : 8, SIZE = Q8 ? 1 : 2;  // elements of a piece, bytes of an element
     auto fetch = [&](const void *from, v4i(&reg)[2][LOADS]) {
@@ -700,7 +730,7 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
             }
         }
     };
-    lookUp(span.from + wave);
+    ask(span.from + wave);
     auto fetchScales = [&]() {
         if constexpr (Q8) sreg = (lane < 32 ? a.key_scales : a.value_scales)[max((lane & 16) ? row1 : row0, 0)];
     };
@@ -722,14 +752,17 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
     for (int t = 0; t < DT / 16; t++) o[t] = v4f{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
     const float scale = a.scale * kLog2e;
+    resolve();
+    ask(span.from + wave + 4);
     there0 = row0 >= 0;
     there1 = row1 >= 0;
     fetchScales();
     fetch(a.value, vreg);
     fetch(a.key, kreg);
-    lookUp(span.from + wave + 4);
     for (int b = span.from + wave; b < span.to; b += 4) {
         const int j0 = blockStart(p, span, b);
+        resolve();
+        ask(b + 8);
         const uint64_t gone0 = __ballot(!there0), gone1 = __ballot(!there1);
         if (gone0 | gone1) {
 #pragma unroll
@@ -770,7 +803,6 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
         fetch(a.key, kreg);
         there0 = now0;
         there1 = now1;
-        lookUp(b + 8);
         if constexpr (Q8) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {

@@ -39,13 +39,24 @@ __device__ __forceinline__ RowPlace placeOf(const CacheArgs &c, const int32_t *s
     return p;
 }
 
-// Row of the cache that holds a position, -1: none does.  Without branches (a position that is none is looked up as the first).
-__device__ __forceinline__ int cacheRow(const CacheArgs &c, int seq, int head, int pos) {
-    const bool in = (uint32_t)pos < (uint32_t)c.capacity;
-    const uint32_t p = in ? (uint32_t)pos : 0u, entry = fastDiv(p, c.ps), slot = p - entry * c.ps.d;
-    const uint32_t page = (uint32_t)c.pages[(int64_t)seq * c.P + entry];
-    return in && page < (uint32_t)c.NP ? (int)((page * (uint32_t)c.KVH + (uint32_t)head) * (uint32_t)c.PS + slot) : -1;
+// Where a position lies: the table's entry is asked for, and the row of the cache that it makes (-1: none) is taken when that has come.
+// Without branches; a position that is none is asked for as the first.
+struct PageAsk {
+    uint32_t page, slot;
+    bool in;
+};
+__device__ __forceinline__ PageAsk askPage(const CacheArgs &c, int seq, int pos, int length) {
+    PageAsk q;
+    q.in = ((uint32_t)pos < (uint32_t)c.capacity) & (pos < length);
+    const uint32_t p = q.in ? (uint32_t)pos : 0u, entry = fastDiv(p, c.ps);
+    q.slot = p - entry * c.ps.d;
+    q.page = (uint32_t)c.pages[(int64_t)seq * c.P + entry];
+    return q;
 }
+__device__ __forceinline__ int rowOf(const CacheArgs &c, const PageAsk &q, int head) {
+    return q.in & (q.page < (uint32_t)c.NP) ? (int)((q.page * (uint32_t)c.KVH + (uint32_t)head) * (uint32_t)c.PS + q.slot) : -1;
+}
+__device__ __forceinline__ int cacheRow(const CacheArgs &c, int seq, int head, int pos) { return rowOf(c, askPage(c, seq, pos, 0x7fffffff), head); }
 
 // The starts in LDS, where they fit `most` sequences; every thread of the workgroup calls it.
 __device__ __forceinline__ const int32_t *holdStarts(const CacheArgs &c, int32_t *held, int most) {
