@@ -410,6 +410,22 @@ __device__ __forceinline__ int swizzle(int row) {
     else return ((row & 2) << 1) | ((row >> 2) & 3);  // 128 bytes: rows lie in both halves of the banks in turn
 }
 
+// The same for the streams' values.  int8 rows are shorter, and eight bytes of 32 rows are read at a time: a chunk of each.
+template <int ROW_BYTES, bool Q8>
+__device__ __forceinline__ int streamSwizzle(int row) {
+    if constexpr (!Q8) return swizzle<ROW_BYTES>(row);
+    else return ROW_BYTES >= 256 ? row & 15 : ROW_BYTES == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
+// Address of chunk `c` ^ swizzle of a row, given that of chunk `own` ^ swizzle where c has none of own's bits set: of a chunk's number the low four bits are
+// swizzled, and rows start at multiples of theirs, so that is one XOR with a constant.  `hold` keeps the compiler from making all of them before
+// a loop, where they would take registers.
+__device__ __forceinline__ int chunkAt(int base, int c) { return (base ^ ((c & 15) << 4)) + ((c >> 4) << 8); }
+__device__ __forceinline__ int hold(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the running maximum before all is scaled down: weights stay below 2^8
 
 // ---- tiles of 128 rows ------------------------------------------------------------------------------------------------
@@ -538,15 +554,14 @@ __global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(
         }
         const int j0 = blockStart(p, span, b);
         if (!active || j0 > bottom) continue;
-        const int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
+        const int keyAt = hold(stage * 2 * KB * ROW + col * ROW + ((half ^ swizzle<ROW>(col)) << 4));
         v16f s[KB / 32];
 #pragma unroll
         for (int k = 0; k < KB / 32; k++) {
             s[k] = v16f{0};
-            const int row = k * 32 + col;
 #pragma unroll
             for (int t = 0; t < DT / 16; t++) {
-                const v8bf kw = *(const v8bf *)(keys + row * ROW + (((2 * t + half) ^ swizzle<ROW>(row)) << 4));
+                const v8bf kw = *(const v8bf *)(smem + chunkAt(keyAt, 2 * t) + k * 32 * ROW);
                 s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kw, q[t], s[k], 0, 0, 0);
             }
         }
@@ -615,6 +630,8 @@ __global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(
                 }
             }
         }
+        const int valueRow = 4 * half + ((lane & 15) >> 2);
+        const int valueAt = hold((stage * 2 + 1) * KB * ROW + valueRow * ROW + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swizzle<ROW>(valueRow)) << 4) + (lane & 1) * 8);
 #pragma unroll
         for (int k = 0; k < KB / 32; k++) {
 #pragma unroll
@@ -623,11 +640,11 @@ __global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(
 #pragma unroll
                 for (int e = 0; e < 4; e++) w[e] = packBf16(s[k][8 * x + 2 * e], s[k][8 * x + 2 * e + 1]);
                 const v8bf weights = __builtin_bit_cast(v8bf, w);
-                const int row = k * 32 + 16 * x + 4 * half + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), low = (lane & 1) * 8;
 #pragma unroll
                 for (int t = 0; t < DT / 32; t++) {
-                    const v2i v0 = turn16(values + row * ROW + (((4 * t + chunk) ^ swizzle<ROW>(row)) << 4) + low);
-                    const v2i v1 = turn16(values + (row + 8) * ROW + (((4 * t + chunk) ^ swizzle<ROW>(row + 8)) << 4) + low);
+                    // the rows eight on are swizzled by two chunks more
+                    const v2i v0 = turn16(smem + chunkAt(valueAt, 4 * t) + (k * 32 + 16 * x) * ROW);
+                    const v2i v1 = turn16(smem + chunkAt(valueAt, (4 * t) ^ 2) + (k * 32 + 16 * x + 8) * ROW);
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]}), weights, o[t], 0, 0, 0);
                 }
             }
@@ -699,7 +716,6 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + span.rows - 1), a.g);
     const int inSeq = r0 + min(col, span.rows - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
     const int pos = it.w.first + token;
-    int8_t *const values = smem + wave * KB * ROW;
     float *const scales = (float *)(smem + 4 * KB * ROW) + wave * 2 * KB;
 
     // Loads are never skipped: a position that is not there is read as row 0, its value taken for zeros and its score for minus infinity; behind D
@@ -772,16 +788,11 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
             }
         }
         __builtin_amdgcn_wave_barrier();
+        const int storeAt = hold(wave * KB * ROW + col * ROW + ((quarter ^ streamSwizzle<ROW, Q8>(col)) << 4));
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-#pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int row = 16 * k + col, chunk = 4 * i + quarter;
-                int at;
-                if constexpr (Q8) at = row * ROW + ((chunk ^ (ROW >= 256 ? row & 15 : ROW == 128 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
-                else at = row * ROW + ((chunk ^ swizzle<ROW>(row)) << 4);
-                *(v4i *)(values + at) = vreg[k][i];
-            }
+        for (int i = 0; i < LOADS; i++) {
+            *(v4i *)(smem + chunkAt(storeAt, 4 * i)) = vreg[0][i];
+            *(v4i *)(smem + chunkAt(storeAt, 4 * i) + 16 * ROW) = vreg[1][i];
         }
         if constexpr (Q8) scales[lane] = sreg;
         __builtin_amdgcn_wave_barrier();
@@ -850,17 +861,17 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
             }
         }
         const v8bf weights = __builtin_bit_cast(v8bf, v4i{packBf16(s[0][0], s[0][1]), packBf16(s[0][2], s[0][3]), packBf16(s[1][0], s[1][1]), packBf16(s[1][2], s[1][3])});
+        // a lane's part of V: of four rows (quarter) and the four 16 on, eight bytes at a time; of eight rows at once where they are int8
+        const int valueRow = Q8 ? 4 * quarter + ((col >> 1) & 3) + 16 * (col >> 3) : 4 * quarter + (col >> 2);
+        const int valueAt = hold(wave * KB * ROW + valueRow * ROW + (((Q8 ? 0 : (col & 3) >> 1) ^ streamSwizzle<ROW, Q8>(valueRow)) << 4) + 8 * (col & 1));
 #pragma unroll
         for (int t = 0; t < DT / 16; t++) {
             v8bf vw;
             if constexpr (Q8) {
-                const int row = 4 * quarter + ((col >> 1) & 3) + 16 * (col >> 3), at = row * ROW + ((t ^ (ROW >= 256 ? row & 15 : ROW == 128 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4) + 8 * (col & 1);
-                const v2i w = turn8(values + at);
+                const v2i w = turn8(smem + chunkAt(valueAt, t));
                 vw = wholeBf16x8(w[0], w[1]);
             } else {
-                const int row = 4 * quarter + (col >> 2), chunk = 2 * t + ((col & 3) >> 1), low = 8 * (col & 1);
-                const v2i v0 = turn16(values + row * ROW + ((chunk ^ swizzle<ROW>(row)) << 4) + low);
-                const v2i v1 = turn16(values + (row + 16) * ROW + ((chunk ^ swizzle<ROW>(row + 16)) << 4) + low);
+                const v2i v0 = turn16(smem + chunkAt(valueAt, 2 * t)), v1 = turn16(smem + chunkAt(valueAt, 2 * t) + 16 * ROW);
                 vw = __builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]});
             }
             o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vw, weights, o[t], 0, 0, 0);
