@@ -433,7 +433,7 @@ constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the 
 // Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is on its way while
 // one is worked on, the rows of the block behind that are being looked up.
 template <int DT, bool PAGED, bool Q8>
-__global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(AttentionArgs a, AttentionPlan p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 && Q8 ? 1 : 2, DT == 256 && Q8 ? 1 : 2))) void attention_tiles(AttentionArgs a, AttentionPlan p) {
     constexpr int KB = DT == 256 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]
@@ -557,14 +557,24 @@ __global__ __launch_bounds__(256, DT == 256 && Q8 ? 1 : 2) void attention_tiles(
         const int keyAt = hold(stage * 2 * KB * ROW + col * ROW + ((half ^ swizzle<ROW>(col)) << 4));
         v16f s[KB / 32];
 #pragma unroll
-        for (int k = 0; k < KB / 32; k++) {
-            s[k] = v16f{0};
+        for (int k = 0; k < KB / 32; k++) s[k] = v16f{0};
 #pragma unroll
-            for (int t = 0; t < DT / 16; t++) {
+        for (int t = 0; t < DT / 16; t++) {
+#pragma unroll
+            for (int k = 0; k < KB / 32; k++) {
                 const v8bf kw = *(const v8bf *)(smem + chunkAt(keyAt, 2 * t) + k * 32 * ROW);
                 s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kw, q[t], s[k], 0, 0, 0);
             }
         }
+        // reads of LDS run ahead of the products that take them by AHEAD; left alone each is waited for
+        constexpr int PRODUCTS = DT / 16 * (KB / 32), AHEAD = DT == 256 ? 4 : 6;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+        for (int i = 0; i < PRODUCTS - AHEAD; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
         if constexpr (Q8) {
 #pragma unroll
             for (int k = 0; k < KB / 32; k++) {
