@@ -66,20 +66,24 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     const int64_t G = H / KVH, rows = T * G;  // of one key head
     p.tiles = rows > 32 * S;
     p.rowsLog = p.tiles ? 7 : 4;
-    p.keysLog = p.tiles && D <= 128 ? 6 : 5;
+    p.keysLog = p.tiles && D <= 64 ? 6 : 5;
+    // Tiles: a part's results are 34 (head of 64) to 133 KB that are written, read and joined, about as long as 500 to 1000 positions are worked on
+    // when every CU does.  So runs are cut where some CUs would have one workgroup and others two (384: 4 x 512 rows of 24 heads over 8192 positions
+    // 298 us whole, 213 in parts; 392 tiles of shorter runs 53 whole, 60 in parts), in parts of 2048 positions or more, and in short ones
+    // where half the CUs have nothing to do.
     p.items = p.tiles ? 512 : 1024;
-    p.minBlocks = p.tiles ? 4 : 4;
     p.maxParts = p.tiles ? 16 : 64;
     const int64_t keys = p.keys();
+    const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
+    p.minBlocks = p.tiles ? (int32_t)((most < 128 ? 256 : 2048) / keys) : 4;
     // a tile's window reaches over its own tokens too, and its first and last block need not be whole
     const int64_t windowed = (sinks + keys - 1) / keys + (window + (p.rows() - 1) / G + keys) / keys + 1;
     p.windowBlocks = (int32_t)(windowed < 0x7fffffff ? windowed : 0x7fffffff);
     int64_t blocks = (capacity + keys - 1) / keys;
     if (window && windowed < blocks) blocks = windowed;
-    const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
     int64_t parts = (blocks + p.minBlocks - 1) / p.minBlocks;
     if (parts > p.maxParts) parts = p.maxParts;
-    p.splits = parts > 1 && most < p.items / 2;
+    p.splits = parts > 1 && most <= (p.tiles ? 384 : p.items / 2);
     p.grid = p.splits ? (most * parts < most + 2 * p.items ? most * parts : most + 2 * p.items) : most;
     p.slots = p.splits ? (p.grid < 2 * p.items ? p.grid : 2 * p.items) : 0;
     p.kvh = makeFastDiv((uint32_t)KVH);

@@ -433,8 +433,8 @@ constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the 
 // Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is on its way while
 // one is worked on, the rows of the block behind that are being looked up.
 template <int DT, bool PAGED, bool Q8>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 && Q8 ? 1 : 2, DT == 256 && Q8 ? 1 : 2))) void attention_tiles(AttentionArgs a, AttentionPlan p) {
-    constexpr int KB = DT == 256 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ? Q8 ? 1 : 2 : 3, DT == 256 ? Q8 ? 1 : 2 : 3))) void attention_tiles(AttentionArgs a, AttentionPlan p) {
+    constexpr int KB = DT >= 128 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]
     uint8_t *const flagRoom = (uint8_t *)(scaleRoom + 4 * KB);      // [2][4 waves]: some row of the block is not there
@@ -446,11 +446,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 &
     const int D = c.D, r0 = it.tile * 128 + wave * 32, rowsHere = min(32, span.rows - wave * 32);  // of this wave; none: <= 0
     const bool active = rowsHere > 0;
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + max(rowsHere, 1) - 1), a.g);
-    const int inSeq = r0 + min(col, max(rowsHere, 1) - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
-    const int pos = it.w.first + token;
-    const int64_t at = ((int64_t)(it.w.begin + min(token, it.w.count - 1)) * a.H + it.head * a.G + inSeq - token * a.G) * D;
+    // where this lane's row lies; made twice, not kept over the loop
+    auto rowAt = [&](int column) {
+        const int inSeq = r0 + min(column, max(rowsHere, 1) - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
+        return ((int64_t)(it.w.begin + min(token, it.w.count - 1)) * a.H + it.head * a.G + inSeq - token * a.G) * D;
+    };
+    const int pos = it.w.first + (int)fastDiv((uint32_t)(r0 + min(col, max(rowsHere, 1) - 1)), a.g);
 
     v8bf q[DT / 16];
+    const int64_t at = rowAt(col);
 #pragma unroll
     for (int t = 0; t < DT / 16; t++) {
         v4i w = *(const v4i *)(a.query + at + (16 * t < D ? 16 * t : 0) + 8 * half);
@@ -540,8 +544,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 &
     if constexpr (Q8) fetch();
     else send(0);
     for (int b = span.from, stage = 0; b < span.to; b++, stage ^= 1) {
-        resolve();
         if constexpr (Q8) {
+            resolve();
             ask(b + 2);
             put(stage);
             fetch();
@@ -549,6 +553,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 &
         } else {
             arrive(stage);
             __syncthreads();  // and everybody is done with the other buffer
+            resolve();
             ask(b + 2);
             send(stage ^ 1);
         }
@@ -567,7 +572,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 &
             }
         }
         // reads of LDS run ahead of the products that take them by AHEAD; left alone each is waited for
-        constexpr int PRODUCTS = DT / 16 * (KB / 32), AHEAD = DT == 256 ? 4 : 6;
+        constexpr int PRODUCTS = DT / 16 * (KB / 32), AHEAD = 4;
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
         for (int i = 0; i < PRODUCTS - AHEAD; i++) {
@@ -677,6 +682,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 &
     if (col < rowsHere && !((again >> col) & 1)) {
         if (it.slot < 0) {
             const float by = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t at = rowAt(hold(col));
 #pragma unroll
             for (int t = 0; t < DT / 32; t++) {
 #pragma unroll
@@ -972,7 +978,7 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
     if (p.grid > 0x7fffffffLL) return hipErrorInvalidValue;
     const dim3 grid((unsigned)p.grid);
     if (p.tiles) {
-        constexpr int KB = DT == 256 ? 32 : 64;
+        constexpr int KB = DT >= 128 ? 32 : 64;
         constexpr size_t lds = 4 * KB * DT * 2 + 4 * KB * 4 + 16;
         static_assert(lds >= (4 * kMaxHeadDim + 128 * 17 + 1) * 4, "what joins the parts");
         auto kernel = attention_tiles<DT, PAGED, Q8>;
