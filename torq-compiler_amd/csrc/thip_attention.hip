@@ -453,14 +453,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     };
     const int pos = it.w.first + (int)fastDiv((uint32_t)(r0 + min(col, max(rowsHere, 1) - 1)), a.g);
 
-    v8bf q[DT / 16];
-    const int64_t at = rowAt(col);
-#pragma unroll
-    for (int t = 0; t < DT / 16; t++) {
-        v4i w = *(const v4i *)(a.query + at + (16 * t < D ? 16 * t : 0) + 8 * half);
-        if (16 * t >= D) w = v4i{0, 0, 0, 0};
-        q[t] = __builtin_bit_cast(v8bf, w);
-    }
     v16f o[DT / 32];
 #pragma unroll
     for (int t = 0; t < DT / 32; t++) o[t] = v16f{0};
@@ -543,6 +535,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     ask(span.from + 1);
     if constexpr (Q8) fetch();
     else send(0);
+    v8bf q[DT / 16];
+    const int64_t at = rowAt(col);
+#pragma unroll
+    for (int t = 0; t < DT / 16; t++) {
+        v4i w = *(const v4i *)(a.query + at + (16 * t < D ? 16 * t : 0) + 8 * half);
+        if (16 * t >= D) w = v4i{0, 0, 0, 0};
+        q[t] = __builtin_bit_cast(v8bf, w);
+    }
     for (int b = span.from, stage = 0; b < span.to; b++, stage ^= 1) {
         if constexpr (Q8) {
             resolve();
@@ -679,35 +679,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     }
     const uint64_t odds = __ballot(odd);
     const uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
-    if (col < rowsHere && !((again >> col) & 1)) {
-        if (it.slot < 0) {
-            const float by = l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t at = rowAt(hold(col));
+    int8_t *const room = smem + wave * 32 * ROW;  // of this wave
+    if (it.slot < 0) {
+        // by way of LDS, so that what is written lies in whole rows
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+        const int at = col * ROW + half * 8, turn = (col & 7) << 4;
 #pragma unroll
-            for (int t = 0; t < DT / 32; t++) {
+        for (int t = 0; t < DT / 32; t++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int d = 32 * t + 8 * i + 4 * half;
-                    if (d < D) *(v2i *)(a.out + at + d) = v2i{packBf16(o[t][4 * i] * by, o[t][4 * i + 1] * by), packBf16(o[t][4 * i + 2] * by, o[t][4 * i + 3] * by)};
-                }
-            }
-        } else {
-            const auto slots = slotsOf(a, p);
-            const uint32_t to = slotRow(a, p, it.slot, wave * 32 + col);
-#pragma unroll
-            for (int t = 0; t < DT / 32; t++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int d = 32 * t + 8 * i + 4 * half;
-                    if (d < D) put4(slots, to + d * 4, o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
-                }
-            }
-            if (half == 0) put4(slots, to + D * 4, m, l, 0.0f, 0.0f);
+            for (int i = 0; i < 4; i++)
+                *(v2i *)(room + at + (((4 * t + i) << 4) ^ turn)) = v2i{packBf16(o[t][4 * i] * by, o[t][4 * i + 1] * by), packBf16(o[t][4 * i + 2] * by, o[t][4 * i + 3] * by)};
         }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < CH / 2; i++) {
+            const int r = (64 / CH) * i + lane / CH;
+            const v4i w = *(const v4i *)(room + r * ROW + (((lane % CH) ^ (r & 7)) << 4));
+            if (r < rowsHere && !((again >> r) & 1) && (lane % CH) * 8 < D) *(v4i *)(a.out + rowAt(r) + (lane % CH) * 8) = w;
+        }
+        __builtin_amdgcn_wave_barrier();
+    } else if (col < rowsHere && !((again >> col) & 1)) {
+        const auto slots = slotsOf(a, p);
+        const uint32_t to = slotRow(a, p, it.slot, wave * 32 + col);
+#pragma unroll
+        for (int t = 0; t < DT / 32; t++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d = 32 * t + 8 * i + 4 * half;
+                if (d < D) put4(slots, to + d * 4, o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
+            }
+        }
+        if (half == 0) put4(slots, to + D * 4, m, l, 0.0f, 0.0f);
     }
     if constexpr (!Q8) {
         for (int r = 0; r < rowsHere; r++) {
-            if ((again >> r) & 1) redoRow<PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)smem + wave * kMaxHeadDim);
+            if ((again >> r) & 1) redoRow<PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
         }
     }
     if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
