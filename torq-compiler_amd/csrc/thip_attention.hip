@@ -161,7 +161,7 @@ struct KeyAsk<false> {
 template <bool PAGED>
 __device__ __forceinline__ KeyAsk<PAGED> askKey(const AttentionArgs &a, const Item &it, int j, bool in) {
     if constexpr (PAGED) return {askPage(a.c, it.seq, j, in ? it.w.length : 0)};
-    else return {in & (j < it.w.length) ? (it.w.begin + j) * a.c.KVH + it.head : -1};
+    else return {(in & (j < it.w.length)) ? (it.w.begin + j) * a.c.KVH + it.head : -1};
 }
 template <bool PAGED>
 __device__ __forceinline__ int keyRow(const AttentionArgs &a, const Item &it, const KeyAsk<PAGED> &q) {

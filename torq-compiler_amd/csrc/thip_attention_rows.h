@@ -54,7 +54,7 @@ __device__ __forceinline__ PageAsk askPage(const CacheArgs &c, int seq, int pos,
     return q;
 }
 __device__ __forceinline__ int rowOf(const CacheArgs &c, const PageAsk &q, int head) {
-    return q.in & (q.page < (uint32_t)c.NP) ? (int)((q.page * (uint32_t)c.KVH + (uint32_t)head) * (uint32_t)c.PS + q.slot) : -1;
+    return (q.in & (q.page < (uint32_t)c.NP)) ? (int)((q.page * (uint32_t)c.KVH + (uint32_t)head) * (uint32_t)c.PS + q.slot) : -1;
 }
 __device__ __forceinline__ int cacheRow(const CacheArgs &c, int seq, int head, int pos) { return rowOf(c, askPage(c, seq, pos, 0x7fffffff), head); }
 
