@@ -75,12 +75,14 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     p.maxParts = p.tiles ? 16 : 64;
     const int64_t keys = p.keys();
     const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
-    p.minBlocks = p.tiles ? (int32_t)((most < 128 ? 256 : 2048) / keys) : 4;
     // a tile's window reaches over its own tokens too, and its first and last block need not be whole
     const int64_t windowed = (sinks + keys - 1) / keys + (window + (p.rows() - 1) / G + keys) / keys + 1;
     p.windowBlocks = (int32_t)(windowed < 0x7fffffff ? windowed : 0x7fffffff);
     int64_t blocks = (capacity + keys - 1) / keys;
     if (window && windowed < blocks) blocks = windowed;
+    // Streams: a wave of a workgroup has a block at least, but two of them none where all the parts then still are few (a token of one sequence of
+    // 1024 positions with one head of 256: 12.3 us in parts of four blocks, 11.2 of two; of 32 such with a window of 512: 12 and 13.5)
+    p.minBlocks = p.tiles ? (int32_t)((most < 128 ? 256 : 2048) / keys) : most * blocks <= 256 ? 2 : 4;
     int64_t parts = (blocks + p.minBlocks - 1) / p.minBlocks;
     if (parts > p.maxParts) parts = p.maxParts;
     p.splits = parts > 1 && most <= (p.tiles ? 384 : p.items / 2);

@@ -207,42 +207,48 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     __syncthreads();
     if (!*last) return;
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // the first sums are under way while the factors are made
+    const int pieces = D >> 2;
+    const uint32_t step = slotRow(a, p, a.c.KVH, 0);
+    v4f part[8];
+    auto getParts = [&](int e, int s) {
+        const int r = e / pieces;
+        const uint32_t from = slotRow(a, p, first, r) + (e - r * pieces) * 16;
+#pragma unroll
+        for (int k = 0; k < 8; k++) part[k] = get4(slots, from + min(s + k, it.splits - 1) * step);
+    };
+    getParts(min(tid, rows * pieces - 1), 0);
     {
         const int r = tid / LANES, mine = tid % LANES;
-        v4f part[EACH];
+        v4f stats[EACH];
         float most = -INFINITY, total = 0.0f;
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
             const int s = e * LANES + mine;
-            part[e] = v4f{-INFINITY, 0.0f, 0.0f, 0.0f};
-            if (s < it.splits) part[e] = get4(slots, slotRow(a, p, first + s * a.c.KVH, min(r, rows - 1)) + D * 4);
+            stats[e] = get4(slots, slotRow(a, p, first + min(s, it.splits - 1) * a.c.KVH, min(r, rows - 1)) + D * 4);
+            if (s >= it.splits) stats[e] = v4f{-INFINITY, 0.0f, 0.0f, 0.0f};
         }
 #pragma unroll
-        for (int e = 0; e < EACH; e++) most = fmaxf(most, part[e][0]);
+        for (int e = 0; e < EACH; e++) most = fmaxf(most, stats[e][0]);
 #pragma unroll
         for (int step = 1; step < LANES; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
         const float shift = most == -INFINITY ? 0.0f : most;
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            const float f = __builtin_amdgcn_exp2f(part[e][0] - shift);
+            const float f = __builtin_amdgcn_exp2f(stats[e][0] - shift);
             factors[r * PARTS + e * LANES + mine] = f;
-            total += f * part[e][1];
+            total += f * stats[e][1];
         }
 #pragma unroll
         for (int step = 1; step < LANES; step *= 2) total += __shfl_xor(total, step);
         if (mine == 0) totals[r] = total == 0.0f ? 0.0f : 1.0f / total;
     }
     __syncthreads();
-    const int pieces = D >> 2;
-    const uint32_t step = slotRow(a, p, a.c.KVH, 0);
     for (int e = tid; e < rows * pieces; e += 256) {
         const int r = e / pieces, d = 4 * (e - r * pieces);
         v4f sum{0.0f, 0.0f, 0.0f, 0.0f};
-        const uint32_t from = slotRow(a, p, first, r) + d * 4;
         for (int s = 0; s < it.splits; s += 8) {
-            v4f part[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) part[k] = get4(slots, from + min(s + k, it.splits - 1) * step);
+            if (e != tid || s != 0) getParts(e, s);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const float f = s + k < it.splits ? factors[r * PARTS + s + k] : 0.0f;
