@@ -52,6 +52,7 @@ struct AttentionPlan {
     int32_t rowsLog, keysLog;
     int32_t windowBlocks;        // blocks that a tile can see at most (with a window)
     int32_t minBlocks, maxParts; // blocks that a part has at least, and parts of a run at most
+    int32_t fewBlocks;           // the same where the tile has few rows
     bool splits;                 // runs may be cut
     int32_t items;
     int64_t grid;                // items at most
@@ -64,7 +65,7 @@ struct AttentionPlan {
 inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
     AttentionPlan p;
     const int64_t G = H / KVH, rows = T * G;  // of one key head
-    p.tiles = rows > 32 * S;
+    p.tiles = rows > 32 * S && (D <= 128 || rows * KVH > 2048);
     p.rowsLog = p.tiles ? 7 : 4;
     p.keysLog = p.tiles && D <= 64 ? 6 : 5;
     // Tiles: a part's results are 34 (head of 64) to 133 KB that are written, read and joined, about as long as 500 to 1000 positions are worked on
@@ -82,8 +83,9 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     if (window && windowed < blocks) blocks = windowed;
     // Streams: a wave of a workgroup has a block at least, but two of them none where all the parts then still are few (a token of one sequence of
     // 1024 positions with one head of 256: 12.3 us in parts of four blocks, 11.2 of two; of 32 such with a window of 512: 12 and 13.5)
-    p.minBlocks = p.tiles ? (int32_t)((most < 128 ? 256 : 2048) / keys) : most * blocks <= 256 ? 2 : 4;
-    int64_t parts = (blocks + p.minBlocks - 1) / p.minBlocks;
+    p.minBlocks = p.tiles ? (int32_t)(2048 / keys) : most * blocks <= 256 ? 2 : 4;
+    p.fewBlocks = p.tiles ? (int32_t)(256 / keys) : p.minBlocks;
+    int64_t parts = (blocks + p.fewBlocks - 1) / p.fewBlocks;
     if (parts > p.maxParts) parts = p.maxParts;
     p.splits = parts > 1 && most <= (p.tiles ? 384 : p.items / 2);
     p.grid = p.splits ? (most * parts < most + 2 * p.items ? most * parts : most + 2 * p.items) : most;

@@ -58,18 +58,31 @@ __device__ __forceinline__ int sumBefore(int v, int lanes) {
     return sum - v;
 }
 
-// Blocks that a part has: so many that about p.items parts come of all that the tiles can see, given for the first 64 sequences in
-// `mine`.  The same for every wave; taken for more than it is where a float does not hold it.
-__device__ __forceinline__ int blocksOfPart(const AttentionArgs &a, const AttentionPlan &p, const SeqWork &mine) {
-    float total = (float)mine.tiles * (float)mine.blocks;
-    for (int base = 64; base < a.c.S; base += 64) {
-        const SeqWork w = measureSeq(a, p, base + (threadIdx.x & 63));
+constexpr int kFewRows = 32;  // one wave's of a tile
+
+// Blocks that a part has at least, of a tile with few rows and of another: so many that about p.items parts come of all that the tiles can see,
+// given for the first 64 sequences in `mine`; and no fewer than the plan says.  The same for every wave; a float that does not hold a sum makes it more.
+struct PartBlocks {
+    int few, many;
+};
+__device__ __forceinline__ PartBlocks blocksOfPart(const AttentionArgs &a, const AttentionPlan &p, const SeqWork &mine) {
+    float total = 0.0f, full = 0.0f;  // blocks; tiles with more than a few rows
+    SeqWork w = mine;
+    for (int base = 0;;) {
         total += (float)w.tiles * (float)w.blocks;
+        if (w.count * a.G > kFewRows) full += (float)w.tiles;
+        base += 64;
+        if (base >= a.c.S) break;
+        w = measureSeq(a, p, base + (threadIdx.x & 63));
     }
-    for (int step = 1; step < min(a.c.S, 64); step *= 2) total += __shfl_xor(total, step);
+    for (int step = 1; step < min(a.c.S, 64); step *= 2) {
+        total += __shfl_xor(total, step);
+        full += __shfl_xor(full, step);
+    }
     total = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(total)));
-    const float part = ceilf(total * (float)a.c.KVH * 1.001f / (float)p.items);
-    return max(p.minBlocks, (int)fminf(part, 1e9f));
+    full = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(full)));
+    const int part = (int)fminf(ceilf(total * (float)a.c.KVH * 1.001f / (float)p.items), 1e9f);
+    return {max(part, p.fewBlocks), max(part, full * (float)a.c.KVH < 128.0f ? p.fewBlocks : p.minBlocks)};
 }
 
 struct Item {
@@ -83,11 +96,12 @@ struct Item {
 __device__ __forceinline__ bool findItem(const AttentionArgs &a, const AttentionPlan &p, int index, Item *out) {
     const int lane = threadIdx.x & 63;
     SeqWork w = measureSeq(a, p, lane);
-    const int part = p.splits ? blocksOfPart(a, p, w) : 0x7fffffff;
+    const PartBlocks part = p.splits ? blocksOfPart(a, p, w) : PartBlocks{0x7fffffff, 0x7fffffff};
     int items = 0, slots = 0;
     for (int base = 0;;) {
         int splits = 1;
-        if (p.splits && w.blocks > part) splits = min(p.maxParts, (int)(((uint32_t)w.blocks + (uint32_t)part - 1) / (uint32_t)part));
+        const int own = w.count * a.G <= kFewRows ? part.few : part.many;
+        if (p.splits && w.blocks > own) splits = min(p.maxParts, (int)(((uint32_t)w.blocks + (uint32_t)own - 1) / (uint32_t)own));
         const int lanes = min(a.c.S - base, 64), mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
         const int before = items + sumBefore(mine, lanes), cutBefore = p.splits ? slots + sumBefore(cut, lanes) : 0;
         const uint64_t found = __ballot(mine > 0 && before <= index && index < before + mine);
@@ -443,7 +457,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     constexpr int KB = DT >= 128 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]
-    uint8_t *const flagRoom = (uint8_t *)(scaleRoom + 4 * KB);      // [2][4 waves]: some row of the block is not there
+    uint8_t *const flagRoom = (uint8_t *)(scaleRoom + 4 * KB);      // [2][4 waves]: some position of the block has no page
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const CacheArgs &c = a.c;
     Item it;
@@ -473,6 +487,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     v2i kreg[PER], vreg[PER];
     float sreg = 0.0f;
     uint32_t gone = 0;  // rows of the block last sent for that are not there, a bit each
+    bool holes = false, unpaged = false;  // of those resolved, of those last sent for: some that the sequence has, but no page
     auto ask = [&](int b) {
         const int j0 = blockStart(p, span, b);
 #pragma unroll
@@ -480,8 +495,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
         if constexpr (Q8) scaleAsked = askKey<PAGED>(a, it, j0 + (tid & (KB - 1)), b < span.to);
     };
     auto resolve = [&]() {
+        holes = false;
 #pragma unroll
-        for (int i = 0; i < PER; i++) rows[i] = keyRow(a, it, asked[i]);
+        for (int i = 0; i < PER; i++) {
+            rows[i] = keyRow(a, it, asked[i]);
+            if constexpr (PAGED) holes |= asked[i].page.in & (rows[i] < 0);
+        }
         if constexpr (Q8) scaleRow = keyRow(a, it, scaleAsked);
     };
     // bf16: straight into LDS, a wave's 64 pieces of 16 bytes one behind the other, so that a lane's place is given and it takes the
@@ -489,6 +508,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t *)smem) + wave * 1024;
     auto send = [&](int stage) {
         gone = 0;
+        unpaged = holes;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             gone |= rows[i] < 0 ? 1u << i : 0u;
@@ -500,20 +520,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     };
     auto arrive = [&](int stage) {
         waitVmcnt<0>();
-        const bool some = __any(gone != 0);
-        if (some) {
+        if (__any(gone != 0)) {
 #pragma unroll
             for (int i = 0; i < PER; i++) {
                 if ((gone >> i) & 1) *(v4i *)(smem + stage * 2 * KB * ROW + KB * ROW + i * 4096 + tid * 16) = v4i{0, 0, 0, 0};
             }
         }
         if constexpr (PAGED) {
+            const bool some = __any(unpaged);
             if (lane == 0) flagRoom[stage * 4 + wave] = some;
         }
     };
     // int8: through registers, where they become bf16
     auto fetch = [&]() {
         gone = 0;
+        unpaged = holes;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             gone |= rows[i] < 0 ? 1u << i : 0u;
@@ -525,7 +546,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     };
     auto put = [&](int stage) {
         int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
-        const bool some = __any(gone != 0);
+        const bool some = __any(unpaged);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int row = myRow + STEP * i, where = row * ROW + ((piece ^ swizzle<ROW>(row)) << 4);
