@@ -25,8 +25,10 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
-// Whether a row at position p sees position j (0 <= j).
-__device__ __forceinline__ bool sees(const AttentionArgs &a, int p, int j) { return (j <= p) & ((a.window == 0) | (p - j < a.window) | (j < a.sinks)); }
+// Whether a row at position p sees position j (0 <= j): those of its window up to itself, and those before sinksOf(p).
+__device__ __forceinline__ uint32_t windowOf(const AttentionArgs &a) { return a.window ? (uint32_t)a.window : 0x80000000u; }
+__device__ __forceinline__ int sinksOf(const AttentionArgs &a, int p) { return min(a.sinks, p + 1); }
+__device__ __forceinline__ bool sees(uint32_t window, int sinks, int p, int j) { return ((uint32_t)(p - j) < window) | (j < sinks); }
 
 // ---- the work of a workgroup ----------------------------------------------------------------------------------------
 
@@ -289,7 +291,7 @@ __device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q
     for (int base = from; base < to; base += 64) {
         const int j = base + lane;
         int row = -1;
-        if (j < to && sees(a, pos, j)) row = keyRow(a, it, askKey<PAGED>(a, it, j, true));
+        if (j < to && sees(windowOf(a), sinksOf(a, pos), pos, j)) row = keyRow(a, it, askKey<PAGED>(a, it, j, true));
         float s = -INFINITY, vs = 1.0f;
         if (row >= 0) {
             float dot = 0.0f;
@@ -403,6 +405,9 @@ __device__ __forceinline__ float sumOverQuarters(float v) {
     return sumOverHalves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// A weight times its value's scale; 0 where the weight is 0, whatever the scale of a masked position is.
+__device__ __forceinline__ float weigh(float weight, float scale) { return weight == 0.0f ? 0.0f : weight * scale; }
+
 // Four int8 as bf16, which holds them: the upper halves of their floats.
 __device__ __forceinline__ v2i wholeBf16(int w) {
     const uint32_t f0 = __float_as_uint((float)(int8_t)w), f1 = __float_as_uint((float)(int8_t)(w >> 8));
@@ -458,6 +463,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]
     uint8_t *const flagRoom = (uint8_t *)(scaleRoom + 4 * KB);      // [2][4 waves]: some position of the block has no page
+    uint8_t *const absentRoom = flagRoom + 16;                       // [2][KB]: the position has no row
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const CacheArgs &c = a.c;
     Item it;
@@ -518,6 +524,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
             dmaLoad16((const int8_t *)a.value + from, lds + stage * 2 * KB * ROW + KB * ROW + i * 4096);
         }
     };
+    auto flag = [&](int stage) {
+        const bool some = __any(unpaged);
+        if (lane == 0) flagRoom[stage * 4 + wave] = some;
+        if (piece == 0) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) absentRoom[stage * KB + myRow + STEP * i] = (gone >> i) & 1;
+        }
+    };
     auto arrive = [&](int stage) {
         waitVmcnt<0>();
         if (__any(gone != 0)) {
@@ -526,10 +540,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
                 if ((gone >> i) & 1) *(v4i *)(smem + stage * 2 * KB * ROW + KB * ROW + i * 4096 + tid * 16) = v4i{0, 0, 0, 0};
             }
         }
-        if constexpr (PAGED) {
-            const bool some = __any(unpaged);
-            if (lane == 0) flagRoom[stage * 4 + wave] = some;
-        }
+        if constexpr (PAGED) flag(stage);
     };
     // int8: through registers, where they become bf16
     auto fetch = [&]() {
@@ -546,7 +557,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     };
     auto put = [&](int stage) {
         int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
-        const bool some = __any(unpaged);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int row = myRow + STEP * i, where = row * ROW + ((piece ^ swizzle<ROW>(row)) << 4);
@@ -554,7 +564,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
             *(v8bf *)(values + where) = wholeBf16x8(vreg[i][0], vreg[i][1]);
         }
         if (tid < 2 * KB) scaleRoom[stage * 2 * KB + tid] = sreg;
-        if (lane == 0) flagRoom[stage * 4 + wave] = some;
+        flag(stage);
     };
 
     ask(span.from);
@@ -622,16 +632,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
         bool gaps = false;
         if constexpr (PAGED) gaps = __builtin_amdgcn_readfirstlane(*(const int *)(flagRoom + stage * 4)) != 0;
         if (!whole || gaps) {
+            const int at = hold(pos), sinks = sinksOf(a, at);
+            const uint32_t window = windowOf(a);
 #pragma unroll
             for (int k = 0; k < KB / 32; k++) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int j = j0 + k * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-                    bool see = sees(a, pos, j) & (j < it.w.length);
-                    if constexpr (PAGED) {
-                        if (gaps && see) see = cacheRow(c, it.seq, it.head, j) >= 0;
+                for (int i = 0; i < 4; i++) {
+                    const int j = j0 + k * 32 + 8 * i + 4 * half;
+                    uint32_t missing = 0;  // a byte a position
+                    if constexpr (PAGED) missing = *(const uint32_t *)(absentRoom + stage * KB + k * 32 + 8 * i + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool there = PAGED ? !(missing & (0xffu << (8 * e))) : j + e < it.w.length;
+                        s[k][4 * i + e] = (sees(window, sinks, at, j + e) & there) ? s[k][4 * i + e] : -INFINITY;
                     }
-                    s[k][i] = see ? s[k][i] : -INFINITY;
                 }
             }
         }
@@ -668,7 +682,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
                 for (int i = 0; i < 4; i++) {
                     const v4f u = *(const v4f *)(scaleRoom + stage * 2 * KB + KB + k * 32 + 8 * i + 4 * half);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[k][4 * i + e] = s[k][4 * i + e] == 0.0f ? 0.0f : s[k][4 * i + e] * u[e];
+                    for (int e = 0; e < 4; e++) s[k][4 * i + e] = weigh(s[k][4 * i + e], u[e]);
                 }
             }
         }
@@ -873,12 +887,14 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
         }
         const bool whole = j0 + KB - 1 <= top && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
         if (!whole || (gone0 | gone1)) {
+            const uint32_t window = windowOf(a);
+            const int sinks = sinksOf(a, pos);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = 4 * quarter + i, j = j0 + 16 * k + key;
-                    const bool see = sees(a, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
+                    const bool see = sees(window, sinks, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
                     s[k][i] = see ? s[k][i] : -INFINITY;
                 }
             }
@@ -906,7 +922,7 @@ __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_strea
             for (int k = 0; k < 2; k++) {
                 const v4f u = *(const v4f *)(scales + 32 + 16 * k + 4 * quarter);
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[k][i] = s[k][i] == 0.0f ? 0.0f : s[k][i] * u[i];
+                for (int i = 0; i < 4; i++) s[k][i] = weigh(s[k][i], u[i]);
             }
         }
         const v8bf weights = __builtin_bit_cast(v8bf, v4i{packBf16(s[0][0], s[0][1]), packBf16(s[0][2], s[0][3]), packBf16(s[1][0], s[1][1]), packBf16(s[1][2], s[1][3])});
@@ -1012,7 +1028,7 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
     const dim3 grid((unsigned)p.grid);
     if (p.tiles) {
         constexpr int KB = DT >= 128 ? 32 : 64;
-        constexpr size_t lds = 4 * KB * DT * 2 + 4 * KB * 4 + 16;
+        constexpr size_t lds = 4 * KB * DT * 2 + 4 * KB * 4 + 16 + 2 * KB;
         static_assert(lds >= (4 * kMaxHeadDim + 128 * 17 + 1) * 4, "what joins the parts");
         auto kernel = attention_tiles<DT, PAGED, Q8>;
         // asked for the kernel's name, as every executable does once on its device, the launcher configures it there
