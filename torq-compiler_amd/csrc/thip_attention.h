@@ -52,7 +52,7 @@ struct AttentionPlan {
     int32_t rowsLog, keysLog;
     int32_t windowBlocks;        // blocks that a tile can see at most (with a window)
     int32_t minBlocks, maxParts; // blocks that a part has at least, and parts of a run at most
-    int32_t fewBlocks;           // the same where the tile has few rows
+    int32_t fewBlocks;           // the same where few tiles are full, and of a stream among tiles
     bool splits;                 // runs may be cut
     int32_t items;
     int64_t grid;                // items at most

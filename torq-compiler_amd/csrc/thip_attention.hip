@@ -60,18 +60,23 @@ __device__ __forceinline__ int sumBefore(int v, int lanes) {
     return sum - v;
 }
 
-constexpr int kFewRows = 32;  // one wave's of a tile
+constexpr int kFewRows = 16;  // a stream's
 
-// Blocks that a part has at least, of a tile with few rows and of another: so many that about p.items parts come of all that the tiles can see,
-// given for the first 64 sequences in `mine`; and no fewer than the plan says.  The same for every wave; a float that does not hold a sum makes it more.
+// Among tiles, a sequence with few rows goes as a stream does, four blocks at once.
+__device__ __forceinline__ bool goesByStream(const AttentionArgs &a, int count) { return a.c.pages && a.c.D <= 128 && count * a.G <= kFewRows; }
+
+// Blocks that a part has at least, of a tile and of a stream among tiles: so many that about p.items parts come of all that the tiles can see, given
+// for the first 64 sequences in `mine`; and no fewer than the plan says, which is fewer where full tiles leave half the CUs without any.
+// The same for every wave; a float that does not hold a sum makes it more.
 struct PartBlocks {
-    int few, many;
+    int tile, stream;
 };
 __device__ __forceinline__ PartBlocks blocksOfPart(const AttentionArgs &a, const AttentionPlan &p, const SeqWork &mine) {
-    float total = 0.0f, full = 0.0f;  // blocks; tiles with more than a few rows
+    float total = 0.0f, full = 0.0f;  // blocks; tiles of more than a few rows
     SeqWork w = mine;
     for (int base = 0;;) {
-        total += (float)w.tiles * (float)w.blocks;
+        const bool light = p.tiles && goesByStream(a, w.count);
+        total += (float)w.tiles * (float)w.blocks * (light ? 0.25f : 1.0f);
         if (w.count * a.G > kFewRows) full += (float)w.tiles;
         base += 64;
         if (base >= a.c.S) break;
@@ -83,8 +88,8 @@ __device__ __forceinline__ PartBlocks blocksOfPart(const AttentionArgs &a, const
     }
     total = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(total)));
     full = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(full)));
-    const int part = (int)fminf(ceilf(total * (float)a.c.KVH * 1.001f / (float)p.items), 1e9f);
-    return {max(part, p.fewBlocks), max(part, full * (float)a.c.KVH < 128.0f ? p.fewBlocks : p.minBlocks)};
+    const int part = (int)fminf(ceilf(total * (float)a.c.KVH * 1.001f / (float)p.items), 1e8f);
+    return {max(part, full * (float)a.c.KVH < 128.0f ? p.fewBlocks : p.minBlocks), max(4 * part, p.fewBlocks)};
 }
 
 struct Item {
@@ -102,7 +107,7 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
     int items = 0, slots = 0;
     for (int base = 0;;) {
         int splits = 1;
-        const int own = w.count * a.G <= kFewRows ? part.few : part.many;
+        const int own = p.tiles && goesByStream(a, w.count) ? part.stream : part.tile;
         if (p.splits && w.blocks > own) splits = min(p.maxParts, (int)(((uint32_t)w.blocks + (uint32_t)own - 1) / (uint32_t)own));
         const int lanes = min(a.c.S - base, 64), mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
         const int before = items + sumBefore(mine, lanes), cutBefore = p.splits ? slots + sumBefore(cut, lanes) : 0;
@@ -453,6 +458,249 @@ __device__ __forceinline__ int hold(int v) {
 
 constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the running maximum before all is scaled down: weights stay below 2^8
 
+// ---- few rows: keys and values streamed -----------------------------------------------------------------------------------
+
+// A tile of 16 rows (a token's heads, or a few tokens'); each of the four waves has blocks of 32 keys of its own, every fourth, and joins the
+// others at the end.  A wave waits for nobody: its keys go straight into the matrix operand's registers, its values through LDS of its own.
+// The registers are filled again as soon as their content is used, so a block's 2 x 32 rows are under way while the one before is worked on.
+template <int DT, bool EXACT, bool PAGED, bool Q8>
+__device__ __forceinline__ void streamItem(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
+    constexpr int KB = 32, STEPS = DT / 32, ROW = DT * (Q8 ? 1 : 2), LOADS = ROW / 64;  // LOADS: 16-byte pieces of a row that one of four lanes has
+    constexpr int JOIN = 16 * (DT + 4);  // floats of a wave's result
+    extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
+    const CacheArgs &c = a.c;
+    const Span span = spanOf(a, p, it);
+    const int D = c.D, r0 = it.tile * 16;
+    const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + span.rows - 1), a.g);
+    const int inSeq = r0 + min(col, span.rows - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
+    const int pos = it.w.first + token;
+    float *const scales = (float *)(smem + 4 * KB * ROW) + wave * 2 * KB;
+
+    // Loads are never skipped: a position that is not there is read as row 0, its value taken for zeros and its score for minus infinity; behind D
+    // (not EXACT) a piece is the first one, against zeros of the query.
+    int row0, row1;      // of the block to be fetched next: keys col and 16 + col
+    bool there0, there1; // of the block in the registers
+    KeyAsk<PAGED> asked0, asked1;  // of the block behind that
+    v4i kreg[2][LOADS], vreg[2][LOADS];
+    float sreg = 0.0f;
+    auto ask = [&](int b) {
+        const int j = blockStart(p, span, b) + col;
+        asked0 = askKey<PAGED>(a, it, j, b < span.to);
+        asked1 = askKey<PAGED>(a, it, j + 16, b < span.to);
+    };
+    auto resolve = [&]() {
+        row0 = keyRow(a, it, asked0);
+        row1 = keyRow(a, it, asked1);
+    };
+    constexpr int ELEMS = Q8 ? 16 : 8, SIZE = Q8 ? 1 : 2;  // elements of a piece, bytes of an element
+    auto fetch = [&](const void *from, v4i(&reg)[2][LOADS]) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int8_t *const at = (const int8_t *)from + ((int64_t)max(k ? row1 : row0, 0) * D + (EXACT ? quarter * ELEMS : 0)) * SIZE;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int d = (4 * i + quarter) * ELEMS;
+                reg[k][i] = *(const v4i *)(at + (EXACT ? 64 * i : d < D ? d * SIZE : 0));
+            }
+        }
+    };
+    ask(span.from + wave);
+    auto fetchScales = [&]() {
+        if constexpr (Q8) sreg = (lane < 32 ? a.key_scales : a.value_scales)[max((lane & 16) ? row1 : row0, 0)];
+    };
+
+    v8bf q[STEPS];
+    {
+        const int64_t at = ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + inSeq - token * a.G) * D;
+#pragma unroll
+        for (int t = 0; t < STEPS; t++) {
+            // of an int8 row a lane has 16 elements at a time, for two steps
+            const int d = Q8 ? 64 * (t >> 1) + 16 * quarter + 8 * (t & 1) : 32 * t + 8 * quarter;
+            v4i w = *(const v4i *)(a.query + at + (EXACT || d < D ? d : 0));
+            if (!EXACT && d >= D) w = v4i{0, 0, 0, 0};
+            q[t] = __builtin_bit_cast(v8bf, w);
+        }
+    }
+    v4f o[DT / 16];
+#pragma unroll
+    for (int t = 0; t < DT / 16; t++) o[t] = v4f{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    const float scale = a.scale * kLog2e;
+    resolve();
+    ask(span.from + wave + 4);
+    there0 = row0 >= 0;
+    there1 = row1 >= 0;
+    fetchScales();
+    fetch(a.value, vreg);
+    fetch(a.key, kreg);
+    for (int b = span.from + wave; b < span.to; b += 4) {
+        const int j0 = blockStart(p, span, b);
+        resolve();
+        ask(b + 8);
+        const uint64_t gone0 = __ballot(!there0), gone1 = __ballot(!there1);
+        if (gone0 | gone1) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                if (!there0) vreg[0][i] = v4i{0, 0, 0, 0};
+                if (!there1) vreg[1][i] = v4i{0, 0, 0, 0};
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        const int storeAt = hold(wave * KB * ROW + col * ROW + ((quarter ^ streamSwizzle<ROW, Q8>(col)) << 4));
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            *(v4i *)(smem + chunkAt(storeAt, 4 * i)) = vreg[0][i];
+            *(v4i *)(smem + chunkAt(storeAt, 4 * i) + 16 * ROW) = vreg[1][i];
+        }
+        if constexpr (Q8) scales[lane] = sreg;
+        __builtin_amdgcn_wave_barrier();
+        const bool now0 = row0 >= 0, now1 = row1 >= 0;
+        fetchScales();
+        fetch(a.value, vreg);
+        v4f s[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            s[k] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < STEPS; t++) {
+                v8bf kw;
+                if constexpr (Q8) kw = (t & 1) ? wholeBf16x8(kreg[k][t >> 1][2], kreg[k][t >> 1][3]) : wholeBf16x8(kreg[k][t >> 1][0], kreg[k][t >> 1][1]);
+                else kw = __builtin_bit_cast(v8bf, kreg[k][t]);
+                s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw, q[t], s[k], 0, 0, 0);
+            }
+        }
+        fetch(a.key, kreg);
+        there0 = now0;
+        there1 = now1;
+        if constexpr (Q8) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const v4f u = *(const v4f *)(scales + 16 * k + 4 * quarter);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[k][i] *= u[i];
+            }
+        }
+        const bool whole = j0 + KB - 1 <= top && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        if (!whole || (gone0 | gone1)) {
+            const uint32_t window = windowOf(a);
+            const int sinks = sinksOf(a, pos);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int key = 4 * quarter + i, j = j0 + 16 * k + key;
+                    const bool see = sees(window, sinks, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
+                    s[k][i] = see ? s[k][i] : -INFINITY;
+                }
+            }
+        }
+        float high = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        high = maxOverQuarters(high) * scale;
+        if (__any(high > m + kSlack || (m == -INFINITY && high > m))) {
+            const float now = fmaxf(m, high), down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+            m = now;
+            l *= down;
+#pragma unroll
+            for (int t = 0; t < DT / 16; t++) o[t] *= down;
+        }
+        const float shift = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[k][i] = __builtin_amdgcn_exp2f(fmaf(s[k][i], scale, -shift));
+                l += s[k][i];
+            }
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const v4f u = *(const v4f *)(scales + 32 + 16 * k + 4 * quarter);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[k][i] = weigh(s[k][i], u[i]);
+            }
+        }
+        const v8bf weights = __builtin_bit_cast(v8bf, v4i{packBf16(s[0][0], s[0][1]), packBf16(s[0][2], s[0][3]), packBf16(s[1][0], s[1][1]), packBf16(s[1][2], s[1][3])});
+        // a lane's part of V: of four rows (quarter) and the four 16 on, eight bytes at a time; of eight rows at once where they are int8
+        const int valueRow = Q8 ? 4 * quarter + ((col >> 1) & 3) + 16 * (col >> 3) : 4 * quarter + (col >> 2);
+        const int valueAt = hold(wave * KB * ROW + valueRow * ROW + (((Q8 ? 0 : (col & 3) >> 1) ^ streamSwizzle<ROW, Q8>(valueRow)) << 4) + 8 * (col & 1));
+#pragma unroll
+        for (int t = 0; t < DT / 16; t++) {
+            v8bf vw;
+            if constexpr (Q8) {
+                const v2i w = turn8(smem + chunkAt(valueAt, t));
+                vw = wholeBf16x8(w[0], w[1]);
+            } else {
+                const v2i v0 = turn16(smem + chunkAt(valueAt, 2 * t)), v1 = turn16(smem + chunkAt(valueAt, 2 * t) + 16 * ROW);
+                vw = __builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]});
+            }
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vw, weights, o[t], 0, 0, 0);
+        }
+    }
+    l = sumOverQuarters(l);
+    __syncthreads();
+    // [wave][row][D + 4]: sums, maximum, sum of weights
+    float *const join = (float *)smem;
+#pragma unroll
+    for (int t = 0; t < DT / 16; t++) *(v4f *)(join + wave * JOIN + col * (DT + 4) + 16 * t + 4 * quarter) = o[t];
+    if (quarter == 0) {
+        join[wave * JOIN + col * (DT + 4) + DT] = m;
+        join[wave * JOIN + col * (DT + 4) + DT + 1] = l;
+    }
+    __syncthreads();
+    const int r = tid >> 4;  // 16 threads a row
+    float most = -INFINITY, factor[4], total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) most = fmaxf(most, join[w * JOIN + r * (DT + 4) + DT]);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        factor[w] = __builtin_amdgcn_exp2f(join[w * JOIN + r * (DT + 4) + DT] - (most == -INFINITY ? 0.0f : most));
+        total += factor[w] * join[w * JOIN + r * (DT + 4) + DT + 1];
+    }
+    v4f sum[DT / 64];
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < DT / 64; e++) {
+        sum[e] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) sum[e] += factor[w] * *(const v4f *)(join + w * JOIN + r * (DT + 4) + 64 * e + 4 * col);
+#pragma unroll
+        for (int i = 0; i < 4; i++) odd |= sum[e][i] != sum[e][i];
+    }
+    // the rows of this wave that have a NaN: 4 wave .. 4 wave + 3, 16 lanes each
+    const uint64_t odds = Q8 ? 0 : __ballot(odd);
+    if (r < span.rows && !((odds >> (16 * (r & 3))) & 0xffff)) {
+        const int mine = r0 + r, tok = (int)fastDiv((uint32_t)mine, a.g);
+        if (it.slot < 0) {
+            const float by = total == 0.0f ? 0.0f : 1.0f / total;
+            uint16_t *out = a.out + ((int64_t)(it.w.begin + tok) * a.H + it.head * a.G + mine - tok * a.G) * D;
+#pragma unroll
+            for (int e = 0; e < DT / 64; e++) {
+                if (64 * e + 4 * col < D) *(v2i *)(out + 64 * e + 4 * col) = v2i{packBf16(sum[e][0] * by, sum[e][1] * by), packBf16(sum[e][2] * by, sum[e][3] * by)};
+            }
+        } else {
+            const auto slots = slotsOf(a, p);
+            const uint32_t to = slotRow(a, p, it.slot, r);
+#pragma unroll
+            for (int e = 0; e < DT / 64; e++) {
+                if (64 * e + 4 * col < D) put4(slots, to + (64 * e + 4 * col) * 4, sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
+            }
+            if (col == 0) put4(slots, to + D * 4, most, total, 0.0f, 0.0f);
+        }
+    }
+    if constexpr (!Q8) {
+        __syncthreads();
+        for (int k = 0; k < 4; k++) {
+            if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
+        }
+    }
+    if (it.slot >= 0) {
+        __syncthreads();
+        joinParts<16, 64>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
+    }
+}
+
 // ---- tiles of 128 rows ------------------------------------------------------------------------------------------------
 
 // Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is on its way while
@@ -468,6 +716,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     const CacheArgs &c = a.c;
     Item it;
     if (!findItem(a, p, blockIdx.x, &it)) return;
+    // single tokens among prompts: a tile would have one wave at work, and that for one row of 32 in its products
+    if constexpr (PAGED && DT <= 128) {
+        if (goesByStream(a, it.w.count)) {
+            AttentionPlan stream = p;
+            stream.keysLog = 5;
+            it.part <<= p.keysLog - 5;
+            return streamItem<DT, false, PAGED, Q8>(a, stream, it);
+        }
+    }
     const Span span = spanOf(a, p, it);
     const int D = c.D, r0 = it.tile * 128 + wave * 32, rowsHere = min(32, span.rows - wave * 32);  // of this wave; none: <= 0
     const bool active = rowsHere > 0;
@@ -760,249 +1017,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ?
     if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
 }
 
-// ---- few rows: keys and values streamed -----------------------------------------------------------------------------------
-
-// A tile of 16 rows (a token's heads, or a few tokens'); each of the four waves has blocks of 32 keys of its own, every fourth, and joins the
-// others at the end.  A wave waits for nobody: its keys go straight into the matrix operand's registers, its values through LDS of its own.
-// The registers are filled again as soon as their content is used, so a block's 2 x 32 rows are under way while the one before is worked on.
 template <int DT, bool EXACT, bool PAGED, bool Q8>
 __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_stream(AttentionArgs a, AttentionPlan p) {
-    constexpr int KB = 32, STEPS = DT / 32, ROW = DT * (Q8 ? 1 : 2), LOADS = ROW / 64;  // LOADS: 16-byte pieces of a row that one of four lanes has
-    constexpr int JOIN = 16 * (DT + 4);  // floats of a wave's result
-    extern __shared__ __attribute__((aligned(16))) int8_t smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
-    const CacheArgs &c = a.c;
     Item it;
-    if (!findItem(a, p, blockIdx.x, &it)) return;
-    const Span span = spanOf(a, p, it);
-    const int D = c.D, r0 = it.tile * 16;
-    const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + span.rows - 1), a.g);
-    const int inSeq = r0 + min(col, span.rows - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
-    const int pos = it.w.first + token;
-    float *const scales = (float *)(smem + 4 * KB * ROW) + wave * 2 * KB;
-
-    // Loads are never skipped: a position that is not there is read as row 0, its value taken for zeros and its score for minus infinity; behind D
-    // (not EXACT) a piece is the first one, against zeros of the query.
-    int row0, row1;      // of the block to be fetched next: keys col and 16 + col
-    bool there0, there1; // of the block in the registers
-    KeyAsk<PAGED> asked0, asked1;  // of the block behind that
-    v4i kreg[2][LOADS], vreg[2][LOADS];
-    float sreg = 0.0f;
-    auto ask = [&](int b) {
-        const int j = blockStart(p, span, b) + col;
-        asked0 = askKey<PAGED>(a, it, j, b < span.to);
-        asked1 = askKey<PAGED>(a, it, j + 16, b < span.to);
-    };
-    auto resolve = [&]() {
-        row0 = keyRow(a, it, asked0);
-        row1 = keyRow(a, it, asked1);
-    };
-    constexpr int ELEMS = Q8 ? 16 : 8, SIZE = Q8 ? 1 : 2;  // elements of a piece, bytes of an element
-    auto fetch = [&](const void *from, v4i(&reg)[2][LOADS]) {
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int8_t *const at = (const int8_t *)from + ((int64_t)max(k ? row1 : row0, 0) * D + (EXACT ? quarter * ELEMS : 0)) * SIZE;
-#pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int d = (4 * i + quarter) * ELEMS;
-                reg[k][i] = *(const v4i *)(at + (EXACT ? 64 * i : d < D ? d * SIZE : 0));
-            }
-        }
-    };
-    ask(span.from + wave);
-    auto fetchScales = [&]() {
-        if constexpr (Q8) sreg = (lane < 32 ? a.key_scales : a.value_scales)[max((lane & 16) ? row1 : row0, 0)];
-    };
-
-    v8bf q[STEPS];
-    {
-        const int64_t at = ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + inSeq - token * a.G) * D;
-#pragma unroll
-        for (int t = 0; t < STEPS; t++) {
-            // of an int8 row a lane has 16 elements at a time, for two steps
-            const int d = Q8 ? 64 * (t >> 1) + 16 * quarter + 8 * (t & 1) : 32 * t + 8 * quarter;
-            v4i w = *(const v4i *)(a.query + at + (EXACT || d < D ? d : 0));
-            if (!EXACT && d >= D) w = v4i{0, 0, 0, 0};
-            q[t] = __builtin_bit_cast(v8bf, w);
-        }
-    }
-    v4f o[DT / 16];
-#pragma unroll
-    for (int t = 0; t < DT / 16; t++) o[t] = v4f{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
-    const float scale = a.scale * kLog2e;
-    resolve();
-    ask(span.from + wave + 4);
-    there0 = row0 >= 0;
-    there1 = row1 >= 0;
-    fetchScales();
-    fetch(a.value, vreg);
-    fetch(a.key, kreg);
-    for (int b = span.from + wave; b < span.to; b += 4) {
-        const int j0 = blockStart(p, span, b);
-        resolve();
-        ask(b + 8);
-        const uint64_t gone0 = __ballot(!there0), gone1 = __ballot(!there1);
-        if (gone0 | gone1) {
-#pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                if (!there0) vreg[0][i] = v4i{0, 0, 0, 0};
-                if (!there1) vreg[1][i] = v4i{0, 0, 0, 0};
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-        const int storeAt = hold(wave * KB * ROW + col * ROW + ((quarter ^ streamSwizzle<ROW, Q8>(col)) << 4));
-#pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-            *(v4i *)(smem + chunkAt(storeAt, 4 * i)) = vreg[0][i];
-            *(v4i *)(smem + chunkAt(storeAt, 4 * i) + 16 * ROW) = vreg[1][i];
-        }
-        if constexpr (Q8) scales[lane] = sreg;
-        __builtin_amdgcn_wave_barrier();
-        const bool now0 = row0 >= 0, now1 = row1 >= 0;
-        fetchScales();
-        fetch(a.value, vreg);
-        v4f s[2];
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            s[k] = v4f{0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < STEPS; t++) {
-                v8bf kw;
-                if constexpr (Q8) kw = (t & 1) ? wholeBf16x8(kreg[k][t >> 1][2], kreg[k][t >> 1][3]) : wholeBf16x8(kreg[k][t >> 1][0], kreg[k][t >> 1][1]);
-                else kw = __builtin_bit_cast(v8bf, kreg[k][t]);
-                s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw, q[t], s[k], 0, 0, 0);
-            }
-        }
-        fetch(a.key, kreg);
-        there0 = now0;
-        there1 = now1;
-        if constexpr (Q8) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const v4f u = *(const v4f *)(scales + 16 * k + 4 * quarter);
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[k][i] *= u[i];
-            }
-        }
-        const bool whole = j0 + KB - 1 <= top && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
-        if (!whole || (gone0 | gone1)) {
-            const uint32_t window = windowOf(a);
-            const int sinks = sinksOf(a, pos);
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int key = 4 * quarter + i, j = j0 + 16 * k + key;
-                    const bool see = sees(window, sinks, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
-                    s[k][i] = see ? s[k][i] : -INFINITY;
-                }
-            }
-        }
-        float high = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        high = maxOverQuarters(high) * scale;
-        if (__any(high > m + kSlack || (m == -INFINITY && high > m))) {
-            const float now = fmaxf(m, high), down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
-            m = now;
-            l *= down;
-#pragma unroll
-            for (int t = 0; t < DT / 16; t++) o[t] *= down;
-        }
-        const float shift = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[k][i] = __builtin_amdgcn_exp2f(fmaf(s[k][i], scale, -shift));
-                l += s[k][i];
-            }
-        }
-        if constexpr (Q8) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const v4f u = *(const v4f *)(scales + 32 + 16 * k + 4 * quarter);
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[k][i] = weigh(s[k][i], u[i]);
-            }
-        }
-        const v8bf weights = __builtin_bit_cast(v8bf, v4i{packBf16(s[0][0], s[0][1]), packBf16(s[0][2], s[0][3]), packBf16(s[1][0], s[1][1]), packBf16(s[1][2], s[1][3])});
-        // a lane's part of V: of four rows (quarter) and the four 16 on, eight bytes at a time; of eight rows at once where they are int8
-        const int valueRow = Q8 ? 4 * quarter + ((col >> 1) & 3) + 16 * (col >> 3) : 4 * quarter + (col >> 2);
-        const int valueAt = hold(wave * KB * ROW + valueRow * ROW + (((Q8 ? 0 : (col & 3) >> 1) ^ streamSwizzle<ROW, Q8>(valueRow)) << 4) + 8 * (col & 1));
-#pragma unroll
-        for (int t = 0; t < DT / 16; t++) {
-            v8bf vw;
-            if constexpr (Q8) {
-                const v2i w = turn8(smem + chunkAt(valueAt, t));
-                vw = wholeBf16x8(w[0], w[1]);
-            } else {
-                const v2i v0 = turn16(smem + chunkAt(valueAt, 2 * t)), v1 = turn16(smem + chunkAt(valueAt, 2 * t) + 16 * ROW);
-                vw = __builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]});
-            }
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vw, weights, o[t], 0, 0, 0);
-        }
-    }
-    l = sumOverQuarters(l);
-    __syncthreads();
-    // [wave][row][D + 4]: sums, maximum, sum of weights
-    float *const join = (float *)smem;
-#pragma unroll
-    for (int t = 0; t < DT / 16; t++) *(v4f *)(join + wave * JOIN + col * (DT + 4) + 16 * t + 4 * quarter) = o[t];
-    if (quarter == 0) {
-        join[wave * JOIN + col * (DT + 4) + DT] = m;
-        join[wave * JOIN + col * (DT + 4) + DT + 1] = l;
-    }
-    __syncthreads();
-    const int r = tid >> 4;  // 16 threads a row
-    float most = -INFINITY, factor[4], total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) most = fmaxf(most, join[w * JOIN + r * (DT + 4) + DT]);
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        factor[w] = __builtin_amdgcn_exp2f(join[w * JOIN + r * (DT + 4) + DT] - (most == -INFINITY ? 0.0f : most));
-        total += factor[w] * join[w * JOIN + r * (DT + 4) + DT + 1];
-    }
-    v4f sum[DT / 64];
-    bool odd = false;
-#pragma unroll
-    for (int e = 0; e < DT / 64; e++) {
-        sum[e] = v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < 4; w++) sum[e] += factor[w] * *(const v4f *)(join + w * JOIN + r * (DT + 4) + 64 * e + 4 * col);
-#pragma unroll
-        for (int i = 0; i < 4; i++) odd |= sum[e][i] != sum[e][i];
-    }
-    // the rows of this wave that have a NaN: 4 wave .. 4 wave + 3, 16 lanes each
-    const uint64_t odds = Q8 ? 0 : __ballot(odd);
-    if (r < span.rows && !((odds >> (16 * (r & 3))) & 0xffff)) {
-        const int mine = r0 + r, tok = (int)fastDiv((uint32_t)mine, a.g);
-        if (it.slot < 0) {
-            const float by = total == 0.0f ? 0.0f : 1.0f / total;
-            uint16_t *out = a.out + ((int64_t)(it.w.begin + tok) * a.H + it.head * a.G + mine - tok * a.G) * D;
-#pragma unroll
-            for (int e = 0; e < DT / 64; e++) {
-                if (64 * e + 4 * col < D) *(v2i *)(out + 64 * e + 4 * col) = v2i{packBf16(sum[e][0] * by, sum[e][1] * by), packBf16(sum[e][2] * by, sum[e][3] * by)};
-            }
-        } else {
-            const auto slots = slotsOf(a, p);
-            const uint32_t to = slotRow(a, p, it.slot, r);
-#pragma unroll
-            for (int e = 0; e < DT / 64; e++) {
-                if (64 * e + 4 * col < D) put4(slots, to + (64 * e + 4 * col) * 4, sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
-            }
-            if (col == 0) put4(slots, to + D * 4, most, total, 0.0f, 0.0f);
-        }
-    }
-    if constexpr (!Q8) {
-        __syncthreads();
-        for (int k = 0; k < 4; k++) {
-            if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
-        }
-    }
-    if (it.slot >= 0) {
-        __syncthreads();
-        joinParts<16, 64>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
-    }
+    if (findItem(a, p, blockIdx.x, &it)) streamItem<DT, EXACT, PAGED, Q8>(a, p, it);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------
@@ -1022,13 +1040,18 @@ static hipError_t checkAttention(const AttentionArgs &a) {
     return hipSuccess;
 }
 
+constexpr size_t streamLds(int DT, bool Q8) {
+    const size_t tiles = 4 * 32 * DT * (Q8 ? 1 : 2) + (Q8 ? 4 * 64 * 4 : 0), join = 4 * 16 * (DT + 4) * 4;
+    return tiles > join ? tiles : join;
+}
+
 template <int DT, bool PAGED, bool Q8>
 static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &p, const LaunchCtx &ctx) {
     if (p.grid > 0x7fffffffLL) return hipErrorInvalidValue;
     const dim3 grid((unsigned)p.grid);
     if (p.tiles) {
         constexpr int KB = DT >= 128 ? 32 : 64;
-        constexpr size_t lds = 4 * KB * DT * 2 + 4 * KB * 4 + 16 + 2 * KB;
+        constexpr size_t tiles = 4 * KB * DT * 2 + 4 * KB * 4 + 16 + 2 * KB, streams = PAGED && DT <= 128 ? streamLds(DT, Q8) : 0, lds = tiles > streams ? tiles : streams;
         static_assert(lds >= (4 * kMaxHeadDim + 128 * 17 + 1) * 4, "what joins the parts");
         auto kernel = attention_tiles<DT, PAGED, Q8>;
         // asked for the kernel's name, as every executable does once on its device, the launcher configures it there
@@ -1037,7 +1060,7 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
         }
         THIP_ENQUEUE(ctx, kernelLabel("attention_tiles", {DT, PAGED, Q8}), kernel, grid, dim3(256), lds, a, p);
     } else {
-        constexpr size_t tiles = 4 * 32 * DT * (Q8 ? 1 : 2) + (Q8 ? 4 * 64 * 4 : 0), join = 4 * 16 * (DT + 4) * 4, lds = tiles > join ? tiles : join;
+        constexpr size_t lds = streamLds(DT, Q8);
         static_assert(lds >= (4 * kMaxHeadDim + 16 * 65 + 1) * 4, "what joins the parts");
         auto enqueue = [&](auto exact) -> hipError_t {
             constexpr bool EXACT = decltype(exact)::value;
