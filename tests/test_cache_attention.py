@@ -478,6 +478,44 @@ def test_gpu_chunks(device, case, see, quantised):
     check_attention(b, built.run(device)["out"], before, want)
 
 
+MIXED = [
+    dict(sequences=[(300, 900), (1, 2000), (2, 700), (1, 1), (0, 50), (4, 300), (5, 333), (1, 130)], D=64, H=8, KVH=2, page=24, tail=3),
+    dict(sequences=[(1, 1500), (260, 260), (3, 90), (1, 0)], D=80, H=4, KVH=1, page=7),
+    dict(sequences=[(40, 5000), (1, 4100), (170, 600)], D=128, H=4, KVH=1, page=64),
+    dict(sequences=[(1, 800), (200, 1300), (4, 500), (9, 20)], D=256, H=16, KVH=1, page=16, tail=1),
+    dict(sequences=[(1, 400)] * 70 + [(500, 1100)] + [(1, 300)] * 5, D=32, H=16, KVH=1, page=40),
+    dict(sequences=[(1, 600)] * 100, D=64, H=2, KVH=1, page=16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("see", [dict(), dict(window=200, sinks=3), dict(window=1000, sinks=70)], ids=_id)
+@pytest.mark.parametrize("case", MIXED, ids=_id)
+def test_gpu_single_tokens_among_prompts(device, case, see, quantised):
+    """Sequences of few rows and of many in one batch, their runs of keys cut into parts; twice, as the second run finds what the first left."""
+    b = Batch(quantised=quantised, **case)
+    built, before, want = attend(b, True, **see)
+    first = built.run(device)["out"]
+    check_attention(b, first, before, want)
+    assert np.array_equal(built.run(device, dispatches=3)["out"], first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_gpu_holes_in_long_tables(device, D, quantised):
+    """Entries in the middle of a sequence that are no page, in tiles; two sequences with the same pages."""
+    b = Batch([(150, 700), (90, 300), (1, 650), (140, 700)], D=D, H=16, KVH=1, page=16, quantised=quantised)
+    b.pages[3] = b.pages[0]
+    for s, entries in ((0, (0, 5, 6, 20, 42)), (1, (18,)), (2, (3, 30)), (3, (5, 41))):
+        for e in entries:
+            b.pages[s, e] = (-1, b.caches[0].shape[0], 2 ** 31 - 1)[e % 3]
+    for see in (dict(), dict(window=100, sinks=20)):
+        built, before, want = attend(b, True, **see)
+        check_attention(b, built.run(device)["out"], before, want)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
 def test_gpu_tables_that_name_no_page(device, quantised):

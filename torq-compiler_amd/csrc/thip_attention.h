@@ -65,13 +65,16 @@ struct AttentionPlan {
 inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
     AttentionPlan p;
     const int64_t G = H / KVH, rows = T * G;  // of one key head
+    // Streams read a sequence's keys once for every 16 of its rows, tiles once for 128, at the rate of one wave's row block.  With 32 rows a sequence both
+    // take the same, with 64 streams took a third more (16 sequences of 4096 positions, four heads of 128: 56 us and 43); heads of 256 have the
+    // slower tiles, and few rows of them too few (64 tokens over 4096 positions, four heads: 79 us in tiles, 42 in streams).
     p.tiles = rows > 32 * S && (D <= 128 || rows * KVH > 2048);
     p.rowsLog = p.tiles ? 7 : 4;
     p.keysLog = p.tiles && D <= 64 ? 6 : 5;
-    // Tiles: a part's results are 34 (head of 64) to 133 KB that are written, read and joined, about as long as 500 to 1000 positions are worked on
-    // when every CU does.  So runs are cut where some CUs would have one workgroup and others two (384: 4 x 512 rows of 24 heads over 8192 positions
-    // 298 us whole, 213 in parts; 392 tiles of shorter runs 53 whole, 60 in parts), in parts of 2048 positions or more, and in short ones
-    // where half the CUs have nothing to do.
+    // Tiles: a part's results are 34 (heads of 64) to 133 KB that are written, read and joined.  So runs are cut only where some CUs would have one
+    // workgroup and others two (384 tiles: four chunks of up to 512 tokens, 32 heads of 128, over up to 8192 positions: 298 us whole, 213 in
+    // parts), and in parts of 2048 positions or more (parts of 512 cost a prompt of 2048 tokens with 16 heads of 128 another 13 us, with a
+    // window of 512 another 28); in shorter ones where full tiles leave half the CUs without any.
     p.items = p.tiles ? 512 : 1024;
     p.maxParts = p.tiles ? 16 : 64;
     const int64_t keys = p.keys();

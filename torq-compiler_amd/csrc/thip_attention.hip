@@ -9,6 +9,8 @@
 // product left them, which is the addresses of V's reads.  V's operand has a lane's values along the keys, across the rows that V lies in;
 // ds_read_b64_tr turns them on the way out of LDS.
 //
+// Times below are medians of the kernels in a trace.
+//
 // Weights are rounded to bf16 for the second product, by half a step of 2^-8 each, as a result of independent values is off by anyway; their
 // sum is kept of the unrounded ones.  int8 keys and values are whole numbers that bf16 holds, so the scales are applied in fp32: a
 // key's to its score, a value's to its weight.
@@ -125,7 +127,7 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
             const uint32_t local = (uint32_t)(index - __builtin_amdgcn_readlane(before, l));
             uint32_t rest = fastDiv(local, p.kvh);
             out->head = (int)(local - rest * (uint32_t)a.c.KVH);
-            out->split = 0;
+            out->split = out->part = 0;
             out->slot = -1;
             if (out->splits > 1) {
                 const uint32_t tile = rest / (uint32_t)out->splits;
@@ -463,6 +465,9 @@ constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the 
 // A tile of 16 rows (a token's heads, or a few tokens'); each of the four waves has blocks of 32 keys of its own, every fourth, and joins the
 // others at the end.  A wave waits for nobody: its keys go straight into the matrix operand's registers, its values through LDS of its own.
 // The registers are filled again as soon as their content is used, so a block's 2 x 32 rows are under way while the one before is worked on.
+// Bound by memory where there is much to read (a token for each of 16 sequences of up to 32768 positions, 32 heads of 128 over 8, int8, 770 MB: 157 us,
+// 4.9 TB/s, what a large copy reaches), else by a chain of loads: starts, table, keys, and what the parts wrote (1024 positions of one head
+// of 256: 10 us, of which 2 are the join).
 template <int DT, bool EXACT, bool PAGED, bool Q8>
 __device__ __forceinline__ void streamItem(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
     constexpr int KB = 32, STEPS = DT / 32, ROW = DT * (Q8 ? 1 : 2), LOADS = ROW / 64;  // LOADS: 16-byte pieces of a row that one of four lanes has
@@ -703,10 +708,23 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
 
 // ---- tiles of 128 rows ------------------------------------------------------------------------------------------------
 
+// Waves of a SIMD: so many that what a wave keeps over the loop has its registers (int8 on the way to bf16 among it).  In memory a register would be
+// waited for with all that is under way.
+template <int DT, bool Q8>
+constexpr int kTileWaves = DT == 256 ? Q8 ? 1 : 2 : 3;
+
 // Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is on its way while
-// one is worked on, the rows of the block behind that are being looked up.
+// one is worked on, the rows of the block behind that are being looked up.  A wave's keys and values feed one product each from LDS, which gives
+// just what the matrix units take; 64 rows a wave halve that, but leave two waves a SIMD where three hide each other's softmax (8192 tokens,
+// 32 heads of 128, a window of 1024: 230 us for 195).  Blocks are as long as three workgroups a CU allow: 32 keys, 64 with heads of 64
+// (64 with heads of 128: 214 us).
+//
+// Bound by the waits of a wave for itself (products, the softmax of their results, products) and by vector instructions next to matrix ones: that
+// prompt takes 187 us, 690 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 197, 630.  Heads of 256 leave two waves a SIMD and LDS busy with the
+// blocks that come (six prompts of up to 2048 tokens: 106 us, 360 TFLOP/s, where the longest tile alone takes 100 of them).
 template <int DT, bool PAGED, bool Q8>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == 256 ? Q8 ? 1 : 2 : 3, DT == 256 ? Q8 ? 1 : 2 : 3))) void attention_tiles(AttentionArgs a, AttentionPlan p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
+void attention_tiles(AttentionArgs a, AttentionPlan p) {
     constexpr int KB = DT >= 128 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]

@@ -15,7 +15,7 @@ __device__ __forceinline__ float rowUnit(uint32_t magnitude) { return fmaxf(__ui
 // by, 64 >> LOG of them at a time, D / 8 pieces of 8 elements, each a lane's, 2^LOG lanes a row (those behind its last piece idle).
 // Memory bound; what the work is cut for is that lookups (a chain of four loads: the starts, the length, the table's entry, the row) are few and
 // overlap.  With every lane of a row looking up for itself the arithmetic of that took the time (four sequences of 8192 positions with
-// eight heads of 128 read from int8, 164 MB: 49 us; so 31, 5.3 TB/s.  Five prompts of 12738 tokens together written as bf16, 104 MB:
+// eight heads of 128 read from int8, 164 MB: 49 us; so 30, 5.4 TB/s.  Five prompts of 12738 tokens together written as bf16, 104 MB:
 // 19 us, 5.5 TB/s; 23 before).
 constexpr int kBatch = 4;  // rows of a lane at most, all under way together
 
