@@ -556,6 +556,28 @@ def test_gpu_starts_that_reach_outside(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sequences", [[(60, 2500), (50, 2000), (40, 2000), (1, 900)], [(1, 2500)] * 5 + [(2, 1500)]], ids=["tiles", "streams"])
+def test_gpu_after_starts_that_do_not_ascend(device, sequences):
+    """What a dispatch leaves does not touch the next one's results, even where the first one's starts were not ascending."""
+    b = Batch(sequences, D=64, H=8, KVH=2, page=16)
+    built, before, want = attend(b, True)
+    exe = thip.Executable(device, built.program.serialize())
+    ptrs = [device.upload(x) for _, x in built.arrays]
+    try:
+        names = [name for name, _ in built.arrays]
+        starts, out = ptrs[names.index("row_starts")], ptrs[names.index("out")]
+        odd = np.where(np.arange(len(b.starts)) % 2, b.T, 0).astype(np.int32)
+        for x in (odd, b.starts, odd[::-1].copy(), b.starts):
+            rt.check(rt.lib().thip_device_h2d(device._h, ctypes.c_void_p(starts), x.ctypes.data_as(ctypes.c_void_p), x.nbytes))
+            exe.run_device(ptrs, [a.nbytes for _, a in built.arrays])
+        check_attention(b, device.download(out, before.shape, before.dtype), before, want)
+    finally:
+        for p in ptrs:
+            device.free(p)
+        exe.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("case", [dict(sequences=[(50, 50), (70, 70)], D=64, H=4, KVH=2), dict(sequences=[(130, 130)], D=128, H=2, KVH=1),
                                   dict(sequences=[(90, 90)], D=256, H=4, KVH=1)], ids=_id)
 @pytest.mark.parametrize("cached", [False, True], ids=["rows", "cache"])

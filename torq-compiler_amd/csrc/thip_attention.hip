@@ -137,8 +137,10 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
                 out->slot = __builtin_amdgcn_readlane(cutBefore, l) + (int)local;
             }
             out->tile = out->w.tiles - 1 - (int)rest;
-            // starts that do not ascend may make more of them: the parts of a run that would not all have a place are left out
-            return out->splits == 1 || out->slot + (out->splits - 1 - out->split) * a.c.KVH < p.slots;
+            // starts that do not ascend may make more of them: a run whose parts would not all have a place, or a workgroup, is left out whole, or its
+            // counter would not come back to 0
+            const int behind = (out->splits - 1 - out->split) * a.c.KVH;
+            return out->splits == 1 || (out->slot + behind < p.slots && (int64_t)index + behind < p.grid);
         }
         base += 64;
         if (base >= a.c.S) return false;
