@@ -51,16 +51,25 @@ __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const Atte
     return w;
 }
 
-// Sum of the lanes before this one, of which `lanes` have something.
-__device__ __forceinline__ int sumBefore(int v, int lanes) {
-    const int lane = threadIdx.x & 63;
-    int sum = v;
-    for (int step = 1; step < lanes; step *= 2) {
-        const int up = __shfl_up(sum, step);
-        if (lane >= step) sum += up;
-    }
-    return sum - v;
+// A value moved within a wave's vector registers (what ds_bpermute does takes a trip to LDS, which counts where a workgroup's whole call is a few us);
+// 0 where there is none to come.
+template <int CONTROL, int ROWS = 0xf>
+__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, true); }
+template <int CONTROL, int ROWS = 0xf>
+__device__ __forceinline__ float moved(float v) { return __uint_as_float((uint32_t)moved<CONTROL, ROWS>((int)__float_as_uint(v))); }
+
+// Sum of the lanes up to this one.
+template <typename T>
+__device__ __forceinline__ T sumUpTo(T v) {
+    v += moved<0x111>(v);       // from 1, 2, 4, 8 lanes down in the row of 16
+    v += moved<0x112>(v);
+    v += moved<0x114>(v);
+    v += moved<0x118>(v);
+    v += moved<0x142, 0xa>(v);  // the last of rows 0 and 2 to rows 1 and 3
+    v += moved<0x143, 0xc>(v);  // the last of row 1 to rows 2 and 3
+    return v;
 }
+__device__ __forceinline__ float sumOfWave(float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sumUpTo(v)), 63)); }
 
 constexpr int kFewRows = 16;  // a stream's
 
@@ -84,12 +93,8 @@ __device__ __forceinline__ PartBlocks blocksOfPart(const AttentionArgs &a, const
         if (base >= a.c.S) break;
         w = measureSeq(a, p, base + (threadIdx.x & 63));
     }
-    for (int step = 1; step < min(a.c.S, 64); step *= 2) {
-        total += __shfl_xor(total, step);
-        full += __shfl_xor(full, step);
-    }
-    total = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(total)));
-    full = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(full)));
+    total = sumOfWave(total);
+    full = sumOfWave(full);
     const int part = (int)fminf(ceilf(total * (float)a.c.KVH * 1.001f / (float)p.items), 1e8f);
     return {max(part, full * (float)a.c.KVH < 128.0f ? p.fewBlocks : p.minBlocks), max(4 * part, p.fewBlocks)};
 }
@@ -111,8 +116,8 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
         int splits = 1;
         const int own = p.tiles && goesByStream(a, w.count) ? part.stream : part.tile;
         if (p.splits && w.blocks > own) splits = min(p.maxParts, (int)(((uint32_t)w.blocks + (uint32_t)own - 1) / (uint32_t)own));
-        const int lanes = min(a.c.S - base, 64), mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
-        const int before = items + sumBefore(mine, lanes), cutBefore = p.splits ? slots + sumBefore(cut, lanes) : 0;
+        const int mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
+        const int before = items + sumUpTo(mine) - mine, cutBefore = p.splits ? slots + sumUpTo(cut) - cut : 0;
         const uint64_t found = __ballot(mine > 0 && before <= index && index < before + mine);
         if (found) {
             const int l = __builtin_ctzll(found);
@@ -216,6 +221,19 @@ __device__ __forceinline__ v4f get4(__amdgpu_buffer_rsrc_t from, uint32_t at) {
 
 __device__ __forceinline__ int packBf16(float lo, float hi) { return __builtin_bit_cast(int, __builtin_convertvector((v2f){lo, hi}, v2bf)); }
 
+// Of 2 or 16 lanes next to one another, the same in each.
+template <int LANES, typename F>
+__device__ __forceinline__ float overLanes(float v, F &&f) {
+    static_assert(LANES == 2 || LANES == 16);
+    v = f(v, moved<0xb1>(v));  // the neighbour
+    if constexpr (LANES == 16) {
+        v = f(v, moved<0x4e>(v));   // the other pair of four
+        v = f(v, moved<0x141>(v));  // the other four of eight, backwards
+        v = f(v, moved<0x140>(v));  // the other eight of 16, backwards
+    }
+    return v;
+}
+
 // Every thread of a workgroup that has stored its part: the last one of the run's to come here adds the parts, in their order, scaled to
 // their common maximum.  room: LDS that nobody uses any more, ROWS (PARTS + 1) floats and one.
 template <int ROWS, int PARTS>
@@ -255,8 +273,7 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
         }
 #pragma unroll
         for (int e = 0; e < EACH; e++) most = fmaxf(most, stats[e][0]);
-#pragma unroll
-        for (int step = 1; step < LANES; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
+        most = overLanes<LANES>(most, [](float x, float y) { return fmaxf(x, y); });
         const float shift = most == -INFINITY ? 0.0f : most;
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
@@ -264,8 +281,7 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
             factors[r * PARTS + e * LANES + mine] = f;
             total += f * stats[e][1];
         }
-#pragma unroll
-        for (int step = 1; step < LANES; step *= 2) total += __shfl_xor(total, step);
+        total = overLanes<LANES>(total, [](float x, float y) { return x + y; });
         if (mine == 0) totals[r] = total == 0.0f ? 0.0f : 1.0f / total;
     }
     __syncthreads();
