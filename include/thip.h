@@ -472,7 +472,7 @@ typedef struct thip_lm_attention_t {
     thip_value_t pages;
     thip_value_t row_starts;
     thip_value_t lengths;
-    float scale;
+    float scale; /* positive, at most 2e38 */
     int32_t window;
     int32_t sinks;
 } thip_lm_attention_t;

@@ -217,6 +217,17 @@ def test_refused_attributes(see):
     assert _serialize_error(lambda p: _paged(p, _operands(p), **see))[0] == rt.INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("scale,taken", [(2.5e38, False), (1.9e38, True)])
+def test_scales_that_are_no_number_in_powers_of_two(scale, taken):
+    """Exponents are taken to base 2: the scale times log2(e) has to be a number, or a score of 0 were none."""
+    if taken:
+        p = thip.Program()
+        _paged(p, _operands(p), scale=scale)
+        p.serialize()
+    else:
+        assert _serialize_error(lambda p: _paged(p, _operands(p), scale=scale))[0] == rt.INVALID_ARGUMENT
+
+
 def test_refused_operands():
     def scales_of_bf16(p):
         _paged(p, _operands(p), scales=True)

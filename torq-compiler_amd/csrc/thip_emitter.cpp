@@ -2138,7 +2138,7 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
     if (thip_status_t s = checkValue(c.query, "query", &q)) return s;
     if (thip_status_t s = checkValue(c.key, "key", &k)) return s;
     if (q->rank != 3) return fail(THIP_INVALID_ARGUMENT, "query: rank %d, expected 3", q->rank);
-    if (!(c.scale > 0.0f) || c.scale > 3e38f) return fail(THIP_INVALID_ARGUMENT, "scale must be a positive number");
+    if (!(c.scale > 0.0f) || c.scale > 2e38f) return fail(THIP_INVALID_ARGUMENT, "scale must be a positive number of at most 2e38");
     if (c.window < 0 || c.sinks < 0) return fail(THIP_INVALID_ARGUMENT, "window %d and sinks %d must not be negative", c.window, c.sinks);
     const bool cached = c.pages != THIP_NO_VALUE;
     if (cached != (c.lengths != THIP_NO_VALUE)) return fail(THIP_INVALID_ARGUMENT, "pages and lengths come together");
