@@ -781,40 +781,68 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
     // this thread's part of a block: chunk `piece` of rows tid / CH + STEP i.  Loads are never skipped: a position that is not there is read
     // as row 0, and the value taken for zeros, its score for minus infinity; behind D a piece is the first one, against zeros of the query.
     const int piece = tid % CH, myRow = tid / CH, pieceAt = piece * 8 < D ? piece * 8 : 0;
-    int rows[PER], scaleRow = -1;
-    KeyAsk<PAGED> asked[PER], scaleAsked;
-    v2i kreg[PER], vreg[PER];
-    float sreg = 0.0f;
     uint32_t gone = 0;  // rows of the block last sent for that are not there, a bit each
-    bool holes = false, unpaged = false;  // of those resolved, of those last sent for: some that the sequence has, but no page
-    auto ask = [&](int b) {
-        const int j0 = blockStart(p, span, b);
-#pragma unroll
-        for (int i = 0; i < PER; i++) asked[i] = askKey<PAGED>(a, it, j0 + myRow + STEP * i, b < span.to);
-        if constexpr (Q8) scaleAsked = askKey<PAGED>(a, it, j0 + (tid & (KB - 1)), b < span.to);
-    };
-    auto resolve = [&]() {
-        holes = false;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            rows[i] = keyRow(a, it, asked[i]);
-            if constexpr (PAGED) holes |= asked[i].page.in & (rows[i] < 0);
-        }
-        if constexpr (Q8) scaleRow = keyRow(a, it, scaleAsked);
-    };
+    bool unpaged = false;  // some of them, or of those that were fetched, are the sequence's, but have no page
     // bf16: straight into LDS, a wave's 64 pieces of 16 bytes one behind the other, so that a lane's place is given and it takes the
     // piece that belongs there
     const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t *)smem) + wave * 1024;
-    auto send = [&](int stage) {
-        gone = 0;
-        unpaged = holes;
+    // Where the rows that one load of a wave brings (64 / CH, at most 8) lie behind one another, their place is a scalar's, and a lane's among them stays the
+    // same; in pages of a multiple of 8 positions they do.  Else, and in a block that is not whole, each lane looks its rows up.
+    constexpr int TURNS = DT == 256 ? 2 : 1;  // STEP rows on, the swizzle is another one (rows eight apart)
+    const int waveRow = wave * (64 / CH);
+    const int64_t rowElems = PAGED ? D : (int64_t)c.KVH * D;  // from one position to the next
+    const bool together = PAGED ? c.PS % 8 == 0 : rowElems < 1 << 24;
+    auto pieceOf = [&](int i) {
+        const int mine = piece ^ swizzle<ROW>(myRow + STEP * i);
+        return mine * 8 < D ? mine * 8 : 0;
+    };
+    uint32_t laneOff[TURNS];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            gone |= rows[i] < 0 ? 1u << i : 0u;
-            const int mine = piece ^ swizzle<ROW>(myRow + STEP * i);
-            const int64_t from = ((int64_t)max(rows[i], 0) * D + (mine * 8 < D ? mine * 8 : 0)) * 2;
-            dmaLoad16((const int8_t *)a.key + from, lds + stage * 2 * KB * ROW + i * 4096);
-            dmaLoad16((const int8_t *)a.value + from, lds + stage * 2 * KB * ROW + KB * ROW + i * 4096);
+    for (int i = 0; i < TURNS; i++) laneOff[i] = ((uint32_t)(myRow - waveRow) * (uint32_t)rowElems + (uint32_t)pieceOf(i)) * 2;
+    uint32_t pages[PER];
+    // the pages are asked for a block ahead; by scalar loads, which do not come back in order with the others
+    auto askPages = [&](int b) {
+        if constexpr (PAGED) {
+            const int j0 = blockStart(p, span, max(min(b, span.to - 1), 0));
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const uint32_t at = (uint32_t)max(min(j0 + STEP * i + waveRow, c.capacity - 1), 0);
+                pages[i] = ((const __attribute__((address_space(4))) uint32_t *)(uintptr_t)c.pages)[(int64_t)it.seq * c.P + fastDiv(at, c.ps)];
+            }
+        }
+    };
+    auto send = [&](int stage, int b) {
+        const int j0 = blockStart(p, span, b);
+        const unsigned to = lds + stage * 2 * KB * ROW;
+        bool whole = together && b < span.to && j0 + KB <= it.w.length;
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) whole = whole & (pages[i] < (uint32_t)c.NP);
+        }
+        gone = 0;
+        unpaged = false;
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const uint32_t at = (uint32_t)(j0 + STEP * i + waveRow);
+                uint32_t first;
+                if constexpr (PAGED) first = (pages[i] * (uint32_t)c.KVH + (uint32_t)it.head) * (uint32_t)c.PS + (at - fastDiv(at, c.ps) * c.ps.d);
+                else first = (at + (uint32_t)it.w.begin) * (uint32_t)c.KVH + (uint32_t)it.head;
+                const uint64_t from = (uint64_t)first * ((uint32_t)D * 2u);
+                dmaLoad16((const int8_t *)a.key + from, laneOff[i % TURNS], to + i * 4096);
+                dmaLoad16((const int8_t *)a.value + from, laneOff[i % TURNS], to + KB * ROW + i * 4096);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const KeyAsk<PAGED> asking = askKey<PAGED>(a, it, j0 + myRow + STEP * i, b < span.to);
+                const int row = keyRow(a, it, asking);
+                gone |= row < 0 ? 1u << i : 0u;
+                if constexpr (PAGED) unpaged |= asking.page.in & (row < 0);
+                const int64_t from = ((int64_t)max(row, 0) * D + pieceOf(i)) * 2;
+                dmaLoad16((const int8_t *)a.key + from, to + i * 4096);
+                dmaLoad16((const int8_t *)a.value + from, to + KB * ROW + i * 4096);
+            }
         }
     };
     auto flag = [&](int stage) {
@@ -835,7 +863,27 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         }
         if constexpr (PAGED) flag(stage);
     };
-    // int8: through registers, where they become bf16
+    // int8: through registers, where they become bf16, every lane's rows looked up a block ahead
+    int rows[PER], scaleRow = -1;
+    KeyAsk<PAGED> asked[PER], scaleAsked;
+    v2i kreg[PER], vreg[PER];
+    float sreg = 0.0f;
+    bool holes = false;  // unpaged, of the rows that were looked up
+    auto ask = [&](int b) {
+        const int j0 = blockStart(p, span, b);
+#pragma unroll
+        for (int i = 0; i < PER; i++) asked[i] = askKey<PAGED>(a, it, j0 + myRow + STEP * i, b < span.to);
+        if constexpr (Q8) scaleAsked = askKey<PAGED>(a, it, j0 + (tid & (KB - 1)), b < span.to);
+    };
+    auto resolve = [&]() {
+        holes = false;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            rows[i] = keyRow(a, it, asked[i]);
+            if constexpr (PAGED) holes |= asked[i].page.in & (rows[i] < 0);
+        }
+        if constexpr (Q8) scaleRow = keyRow(a, it, scaleAsked);
+    };
     auto fetch = [&]() {
         gone = 0;
         unpaged = holes;
@@ -860,11 +908,16 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         flag(stage);
     };
 
-    ask(span.from);
-    resolve();
-    ask(span.from + 1);
-    if constexpr (Q8) fetch();
-    else send(0);
+    if constexpr (Q8) {
+        ask(span.from);
+        resolve();
+        ask(span.from + 1);
+        fetch();
+    } else {
+        askPages(span.from);
+        send(0, span.from);
+        askPages(span.from + 1);
+    }
     v8bf q[DT / 16];
     const int64_t at = rowAt(col);
 #pragma unroll
@@ -883,9 +936,8 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         } else {
             arrive(stage);
             __syncthreads();  // and everybody is done with the other buffer
-            resolve();
-            ask(b + 2);
-            send(stage ^ 1);
+            send(stage ^ 1, b + 1);
+            askPages(b + 2);
         }
         const int j0 = blockStart(p, span, b);
         if (!active || j0 > bottom) continue;
