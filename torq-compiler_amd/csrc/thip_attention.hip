@@ -738,7 +738,7 @@ constexpr int kTileWaves = DT == 256 ? Q8 ? 1 : 2 : 3;
 // (64 with heads of 128: 214 us).
 //
 // Bound by the waits of a wave for itself (products, the softmax of their results, products) and by vector instructions next to matrix ones: that
-// prompt takes 187 us, 690 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 197, 630.  Heads of 256 leave two waves a SIMD and LDS busy with the
+// prompt takes 183 us, 710 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 203, 610.  Heads of 256 leave two waves a SIMD and LDS busy with the
 // blocks that come (six prompts of up to 2048 tokens: 106 us, 360 TFLOP/s, where the longest tile alone takes 100 of them).
 template <int DT, bool PAGED, bool Q8>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
