@@ -250,17 +250,21 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     __syncthreads();
     if (!*last) return;
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // the first sums are under way while the factors are made
-    const int pieces = D >> 2;
+    // Several elements of a thread's and several parts at once, the first of them while the factors are made.
+    constexpr int ELEMS = ROWS == 128 ? 4 : 1, BATCH = ROWS == 128 ? 4 : 8;
+    const int pieces = D >> 2, all = rows * pieces;
     const uint32_t step = slotRow(a, p, a.c.KVH, 0);
-    v4f part[8];
-    auto getParts = [&](int e, int s) {
-        const int r = e / pieces;
-        const uint32_t from = slotRow(a, p, first, r) + (e - r * pieces) * 16;
+    v4f part[ELEMS][BATCH];
+    auto getParts = [&](int e0, int s) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) part[k] = get4(slots, from + min(s + k, it.splits - 1) * step);
+        for (int i = 0; i < ELEMS; i++) {
+            const int e = min(e0 + 256 * i, all - 1), r = e / pieces;
+            const uint32_t from = slotRow(a, p, first, r) + (e - r * pieces) * 16;
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) part[i][k] = get4(slots, from + min(s + k, it.splits - 1) * step);
+        }
     };
-    getParts(min(tid, rows * pieces - 1), 0);
+    getParts(tid, 0);
     {
         const int r = tid / LANES, mine = tid % LANES;
         v4f stats[EACH];
@@ -285,20 +289,29 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
         if (mine == 0) totals[r] = total == 0.0f ? 0.0f : 1.0f / total;
     }
     __syncthreads();
-    for (int e = tid; e < rows * pieces; e += 256) {
-        const int r = e / pieces, d = 4 * (e - r * pieces);
-        v4f sum{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < it.splits; s += 8) {
-            if (e != tid || s != 0) getParts(e, s);
+    for (int e0 = tid; e0 < all; e0 += 256 * ELEMS) {
+        v4f sum[ELEMS];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float f = s + k < it.splits ? factors[r * PARTS + s + k] : 0.0f;
-                if (s + k < it.splits) sum += f * part[k];
+        for (int i = 0; i < ELEMS; i++) sum[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < it.splits; s += BATCH) {
+            if (e0 != tid || s != 0) getParts(e0, s);
+#pragma unroll
+            for (int i = 0; i < ELEMS; i++) {
+                const int r = min(e0 + 256 * i, all - 1) / pieces;
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) {
+                    if (s + k < it.splits) sum[i] += factors[r * PARTS + s + k] * part[i][k];
+                }
             }
         }
-        const int mine = it.tile * ROWS + r, token = (int)fastDiv((uint32_t)mine, a.g);
-        *(v2i *)(a.out + ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + mine - token * a.G) * D + d) =
-            v2i{packBf16(sum[0] * totals[r], sum[1] * totals[r]), packBf16(sum[2] * totals[r], sum[3] * totals[r])};
+#pragma unroll
+        for (int i = 0; i < ELEMS; i++) {
+            const int e = e0 + 256 * i, r = e / pieces, d = 4 * (e - r * pieces);
+            if (e >= all) break;
+            const int mine = it.tile * ROWS + r, token = (int)fastDiv((uint32_t)mine, a.g);
+            *(v2i *)(a.out + ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + mine - token * a.G) * D + d) =
+                v2i{packBf16(sum[i][0] * totals[r], sum[i][1] * totals[r]), packBf16(sum[i][2] * totals[r], sum[i][3] * totals[r])};
+        }
     }
 }
 
