@@ -201,7 +201,8 @@ __device__ __forceinline__ int keyRow(const AttentionArgs &a, const Item &it, co
 
 // ---- partial results ---------------------------------------------------------------------------------------------------
 
-// A slot holds, for each row of a tile, D sums, then the maximum and the sum of weights.  They go from workgroup to workgroup, which may be on
+// A slot holds, for each row of a stream, D sums, then the maximum and the sum of weights; of a tile, the sums as a wave has them (16 bytes a lane,
+// the waves' one behind the other, so that what is stored and read is whole lines), then the two of each row.  They go from workgroup to workgroup, which may be on
 // different XCDs, past the caches, by loads and stores at the device's scope (a fence would write the XCD's whole L2 back).
 constexpr int kDeviceScope = 16;  // sc1
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t slotsOf(const AttentionArgs &a, const AttentionPlan &p) {
@@ -210,6 +211,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t slotsOf(const AttentionArgs &a
 __device__ __forceinline__ uint32_t slotRow(const AttentionArgs &a, const AttentionPlan &p, int slot, int r) {
     return (((uint32_t)slot << p.rowsLog) + (uint32_t)r) * (uint32_t)(a.c.D + 4) * 4u;
 }
+// Of a tile: the sums, and its rows' maxima and sums of weights.
+__device__ __forceinline__ uint32_t tileSums(const AttentionArgs &a, int slot) { return (uint32_t)slot * 128u * (uint32_t)(a.c.D + 4) * 4u; }
+__device__ __forceinline__ uint32_t tileStats(const AttentionArgs &a, int slot, int r) { return tileSums(a, slot) + 512u * (uint32_t)a.c.D + 16u * (uint32_t)r; }
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t to, uint32_t at, float x, float y, float z, float w) {
@@ -252,18 +256,22 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // Several elements of a thread's and several parts at once, the first of them while the factors are made.
     constexpr int ELEMS = ROWS == 128 ? 4 : 1, BATCH = ROWS == 128 ? 4 : 8;
-    const int pieces = D >> 2, all = rows * pieces;
-    const uint32_t step = slotRow(a, p, a.c.KVH, 0);
+    constexpr bool TILE = ROWS == 128;
+    const int pieces = D >> 2, all = TILE ? ((rows + 31) >> 5) * 8 * D : rows * pieces;
+    const uint32_t step = TILE ? tileSums(a, a.c.KVH) : slotRow(a, p, a.c.KVH, 0), sums = TILE ? tileSums(a, first) : slotRow(a, p, first, 0);
     v4f part[ELEMS][BATCH];
     auto getParts = [&](int e0, int s) {
 #pragma unroll
         for (int i = 0; i < ELEMS; i++) {
-            const int e = min(e0 + 256 * i, all - 1), r = e / pieces;
-            const uint32_t from = slotRow(a, p, first, r) + (e - r * pieces) * 16;
+            const int e = min(e0 + 256 * i, all - 1);
+            const uint32_t from = sums + (uint32_t)(TILE ? e : e + e / pieces) * 16u;  // a stream's rows are D + 4 long
 #pragma unroll
             for (int k = 0; k < BATCH; k++) part[i][k] = get4(slots, from + min(s + k, it.splits - 1) * step);
         }
     };
+    // row and first column of an element
+    auto rowOf = [&](int e) { return TILE ? e / (8 * D) * 32 + (e & 31) : e / pieces; };
+    auto columnOf = [&](int e, int r) { return TILE ? (e % (8 * D) >> 6) * 8 + ((e >> 5) & 1) * 4 : 4 * (e - r * pieces); };
     getParts(tid, 0);
     {
         const int r = tid / LANES, mine = tid % LANES;
@@ -272,7 +280,8 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
             const int s = e * LANES + mine;
-            stats[e] = get4(slots, slotRow(a, p, first + min(s, it.splits - 1) * a.c.KVH, min(r, rows - 1)) + D * 4);
+            const int slot = first + min(s, it.splits - 1) * a.c.KVH, row = min(r, rows - 1);
+            stats[e] = get4(slots, TILE ? tileStats(a, slot, row) : slotRow(a, p, slot, row) + D * 4);
             if (s >= it.splits) stats[e] = v4f{-INFINITY, 0.0f, 0.0f, 0.0f};
         }
 #pragma unroll
@@ -297,7 +306,7 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
             if (e0 != tid || s != 0) getParts(e0, s);
 #pragma unroll
             for (int i = 0; i < ELEMS; i++) {
-                const int r = min(e0 + 256 * i, all - 1) / pieces;
+                const int r = rowOf(min(e0 + 256 * i, all - 1));
 #pragma unroll
                 for (int k = 0; k < BATCH; k++) {
                     if (s + k < it.splits) sum[i] += factors[r * PARTS + s + k] * part[i][k];
@@ -306,8 +315,8 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
         }
 #pragma unroll
         for (int i = 0; i < ELEMS; i++) {
-            const int e = e0 + 256 * i, r = e / pieces, d = 4 * (e - r * pieces);
-            if (e >= all) break;
+            const int e = e0 + 256 * i, r = rowOf(e), d = columnOf(e, r);
+            if (e >= all || r >= rows) continue;
             const int mine = it.tile * ROWS + r, token = (int)fastDiv((uint32_t)mine, a.g);
             *(v2i *)(a.out + ((int64_t)(it.w.begin + token) * a.H + it.head * a.G + mine - token * a.G) * D + d) =
                 v2i{packBf16(sum[i][0] * totals[r], sum[i][1] * totals[r]), packBf16(sum[i][2] * totals[r], sum[i][3] * totals[r])};
@@ -392,7 +401,7 @@ __device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q
 }
 
 // A row of an item once more, key by key, and its result or partial result stored.  q: LDS of this wave, kMaxHeadDim floats.
-template <bool PAGED, bool Q8>
+template <bool TILE, bool PAGED, bool Q8>
 __device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const Item &it, const Span &span, int r, float *q) {
     const int lane = threadIdx.x & 63, D = a.c.D;
     const int inSeq = (it.tile << p.rowsLog) + r, token = (int)fastDiv((uint32_t)inSeq, a.g), h = it.head * a.G + inSeq - token * a.G;
@@ -413,13 +422,14 @@ __device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionP
         }
     } else {
         const auto slots = slotsOf(a, p);
-        const uint32_t at = slotRow(a, p, it.slot, r);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const int d = lane + 64 * e;
-            if (d < D) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[e]), slots, (int)at + d * 4, 0, kDeviceScope);
+            const uint32_t to = TILE ? tileSums(a, it.slot) + (uint32_t)((((r >> 5) * (D >> 3) + (d >> 3)) * 64 + ((d >> 2) & 1) * 32 + (r & 31)) * 4 + (d & 3)) * 4u
+                                     : slotRow(a, p, it.slot, r) + (uint32_t)d * 4u;
+            if (d < D) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[e]), slots, (int)to, 0, kDeviceScope);
         }
-        if (lane == 0) put4(slots, at + D * 4, m, l, 0.0f, 0.0f);
+        if (lane == 0) put4(slots, TILE ? tileStats(a, it.slot, r) : slotRow(a, p, it.slot, r) + D * 4, m, l, 0.0f, 0.0f);
     }
     __threadfence_block();
 }
@@ -728,7 +738,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     if constexpr (!Q8) {
         __syncthreads();
         for (int k = 0; k < 4; k++) {
-            if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
+            if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<false, PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
         }
     }
     if (it.slot >= 0) {
@@ -1099,20 +1109,19 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         __builtin_amdgcn_wave_barrier();
     } else if (col < rowsHere && !((again >> col) & 1)) {
         const auto slots = slotsOf(a, p);
-        const uint32_t to = slotRow(a, p, it.slot, wave * 32 + col);
+        const uint32_t to = tileSums(a, it.slot) + (uint32_t)(wave * (D >> 3) * 64 + lane) * 16u;
 #pragma unroll
         for (int t = 0; t < DT / 32; t++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int d = 32 * t + 8 * i + 4 * half;
-                if (d < D) put4(slots, to + d * 4, o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
+                if (32 * t + 8 * i < D) put4(slots, to + (4 * t + i) * 1024, o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
             }
         }
-        if (half == 0) put4(slots, to + D * 4, m, l, 0.0f, 0.0f);
+        if (half == 0) put4(slots, tileStats(a, it.slot, wave * 32 + col), m, l, 0.0f, 0.0f);
     }
     if constexpr (!Q8) {
         for (int r = 0; r < rowsHere; r++) {
-            if ((again >> r) & 1) redoRow<PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
+            if ((again >> r) & 1) redoRow<true, PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
         }
     }
     if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
