@@ -49,6 +49,7 @@ hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx);
 // device cuts the runs of long sequences so that there are about `items`, and the last workgroup of a tile to finish joins the parts.
 struct AttentionPlan {
     bool tiles;                  // attention_tiles, or attention_stream
+    bool fine;                   // weights of tiles in two parts
     int32_t rowsLog, keysLog;
     int32_t windowBlocks;        // blocks that a tile can see at most (with a window)
     int32_t minBlocks, maxParts; // blocks that a part has at least, and parts of a run at most
@@ -69,6 +70,9 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // take the same, with 64 streams took a third more (16 sequences of 4096 positions, four heads of 128: 56 us and 43); heads of 256 have the
     // slower tiles, and few rows of them too few (64 tokens over 4096 positions, four heads: 79 us in tiles, 42 in streams).
     p.tiles = rows > 32 * S && (D <= 128 || rows * KVH > 2048);
+    // The second part costs a prompt of 8192 tokens with 32 heads of 128 a third (174 us, 228 with it), four chunks of up to 512 a quarter (186, 234); the error of a
+    // result goes from 1.4 times that of its rounding alone to 1.0.  Over many rows that is what it is; over few it may be 1.7 times in one call.
+    p.fine = T * H < 8192;
     p.rowsLog = p.tiles ? 7 : 4;
     p.keysLog = p.tiles && D <= 64 ? 6 : 5;
     // Tiles: a part's results are 34 (heads of 64) to 133 KB that are written, read and joined.  So runs are cut only where some CUs would have one

@@ -11,8 +11,9 @@
 //
 // Times below are medians of the kernels in a trace.
 //
-// Weights are rounded to bf16 for the second product, by half a step of 2^-8 each, as a result of independent values is off by anyway; their
-// sum is kept of the unrounded ones.  int8 keys and values are whole numbers that bf16 holds, so the scales are applied in fp32: a
+// Weights go into the second product as two bf16, one and what it leaves, in streams and in tiles of few rows, where that costs nothing; as one in tiles
+// of many, where the second product's time counts (AttentionPlan::fine): off by half a step of 2^-8 each, which moves a result of independent values about as
+// far as its own rounding does. Their sum is kept of the unrounded ones.  int8 keys and values are whole numbers that bf16 holds, so the scales are applied in fp32: a
 // key's to its score, a value's to its weight.
 #include "thip_attention.h"
 #include "thip_attention_rows.h"
@@ -453,6 +454,11 @@ __device__ __forceinline__ float sumOverQuarters(float v) {
     return sumOverHalves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// What is left of x and y behind their bf16 in `word`, as bf16 again.
+__device__ __forceinline__ int restOf(int word, float x, float y) {
+    return packBf16(x - __uint_as_float((uint32_t)word << 16), y - __uint_as_float((uint32_t)word & 0xffff0000u));
+}
+
 // A weight times its value's scale; 0 where the weight is 0, whatever the scale of a masked position is.
 __device__ __forceinline__ float weigh(float weight, float scale) { return weight == 0.0f ? 0.0f : weight * scale; }
 
@@ -667,7 +673,15 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
                 for (int i = 0; i < 4; i++) s[k][i] = weigh(s[k][i], u[i]);
             }
         }
-        const v8bf weights = __builtin_bit_cast(v8bf, v4i{packBf16(s[0][0], s[0][1]), packBf16(s[0][2], s[0][3]), packBf16(s[1][0], s[1][1]), packBf16(s[1][2], s[1][3])});
+        // in two parts, what the first leaves being the second: the matrix units have the time
+        v4i high4, low4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = s[i >> 1][2 * (i & 1)], y = s[i >> 1][2 * (i & 1) + 1];
+            high4[i] = packBf16(x, y);
+            low4[i] = restOf(high4[i], x, y);
+        }
+        const v8bf weights = __builtin_bit_cast(v8bf, high4), rest = __builtin_bit_cast(v8bf, low4);
         // a lane's part of V: of four rows (quarter) and the four 16 on, eight bytes at a time; of eight rows at once where they are int8
         const int valueRow = Q8 ? 4 * quarter + ((col >> 1) & 3) + 16 * (col >> 3) : 4 * quarter + (col >> 2);
         const int valueAt = hold(wave * KB * ROW + valueRow * ROW + (((Q8 ? 0 : (col & 3) >> 1) ^ streamSwizzle<ROW, Q8>(valueRow)) << 4) + 8 * (col & 1));
@@ -682,6 +696,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
                 vw = __builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]});
             }
             o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vw, weights, o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vw, rest, o[t], 0, 0, 0);
         }
     }
     l = sumOverQuarters(l);
@@ -763,7 +778,7 @@ constexpr int kTileWaves = DT == 256 ? Q8 ? 1 : 2 : 3;
 // Bound by the waits of a wave for itself (products, the softmax of their results, products) and by vector instructions next to matrix ones: that
 // prompt takes 183 us, 710 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 203, 610.  Heads of 256 leave two waves a SIMD and LDS busy with the
 // blocks that come (six prompts of up to 2048 tokens: 106 us, 360 TFLOP/s, where the longest tile alone takes 100 of them).
-template <int DT, bool PAGED, bool Q8>
+template <int DT, bool PAGED, bool Q8, bool FINE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
 void attention_tiles(AttentionArgs a, AttentionPlan p) {
     constexpr int KB = DT >= 128 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
@@ -1064,12 +1079,20 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) w[e] = packBf16(s[k][8 * x + 2 * e], s[k][8 * x + 2 * e + 1]);
                 const v8bf weights = __builtin_bit_cast(v8bf, w);
+                v4i left{0, 0, 0, 0};
+                if constexpr (FINE) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) left[e] = restOf(w[e], s[k][8 * x + 2 * e], s[k][8 * x + 2 * e + 1]);
+                }
+                const v8bf rest = __builtin_bit_cast(v8bf, left);
 #pragma unroll
                 for (int t = 0; t < DT / 32; t++) {
                     // the rows eight on are swizzled by two chunks more
                     const v2i v0 = turn16(smem + chunkAt(valueAt, 4 * t) + (k * 32 + 16 * x) * ROW);
                     const v2i v1 = turn16(smem + chunkAt(valueAt, (4 * t) ^ 2) + (k * 32 + 16 * x + 8) * ROW);
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]}), weights, o[t], 0, 0, 0);
+                    const v8bf vw = __builtin_bit_cast(v8bf, v4i{v0[0], v0[1], v1[0], v1[1]});
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vw, weights, o[t], 0, 0, 0);
+                    if constexpr (FINE) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vw, rest, o[t], 0, 0, 0);
                 }
             }
         }
@@ -1163,12 +1186,17 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
         constexpr int KB = DT >= 128 ? 32 : 64;
         constexpr size_t tiles = 4 * KB * DT * 2 + 4 * KB * 4 + 16 + 2 * KB, streams = PAGED && DT <= 128 ? streamLds(DT, Q8) : 0, lds = tiles > streams ? tiles : streams;
         static_assert(lds >= (4 * kMaxHeadDim + 128 * 17 + 1) * 4, "what joins the parts");
-        auto kernel = attention_tiles<DT, PAGED, Q8>;
-        // asked for the kernel's name, as every executable does once on its device, the launcher configures it there
-        if (lds > 64 * 1024 && ctx.name) {
-            if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return e;
-        }
-        THIP_ENQUEUE(ctx, kernelLabel("attention_tiles", {DT, PAGED, Q8}), kernel, grid, dim3(256), lds, a, p);
+        auto enqueue = [&](auto fine) -> hipError_t {
+            constexpr bool FINE = decltype(fine)::value;
+            auto kernel = attention_tiles<DT, PAGED, Q8, FINE>;
+            // asked for the kernel's name, as every executable does once on its device, the launcher configures it there
+            if (lds > 64 * 1024 && ctx.name) {
+                if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return e;
+            }
+            THIP_ENQUEUE(ctx, kernelLabel("attention_tiles", {DT, PAGED, Q8, FINE}), kernel, grid, dim3(256), lds, a, p);
+            return hipSuccess;
+        };
+        if (hipError_t e = p.fine ? enqueue(std::true_type{}) : enqueue(std::false_type{})) return e;
     } else {
         constexpr size_t lds = streamLds(DT, Q8);
         static_assert(lds >= (4 * kMaxHeadDim + 16 * 65 + 1) * 4, "what joins the parts");
