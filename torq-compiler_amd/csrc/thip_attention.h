@@ -77,7 +77,7 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     p.keysLog = p.tiles && D <= 64 ? 6 : 5;
     // Tiles: a part's results are 34 (heads of 64) to 133 KB that are written, read and joined.  So runs are cut only where some CUs would have one
     // workgroup and others two (384 tiles: four chunks of up to 512 tokens, 32 heads of 128, over up to 8192 positions: 298 us whole, 213 in
-    // parts), and in parts of 2048 positions or more (parts of 512 cost a prompt of 2048 tokens with 16 heads of 128 another 13 us, with a
+    // parts then, 189 now), and in parts of 2048 positions or more (parts of 512 cost a prompt of 2048 tokens with 16 heads of 128 another 13 us, with a
     // window of 512 another 28); in shorter ones where full tiles leave half the CUs without any.
     p.items = p.tiles ? 512 : 1024;
     p.maxParts = p.tiles ? 16 : 64;

@@ -770,14 +770,14 @@ template <int DT, bool Q8>
 constexpr int kTileWaves = DT == 256 ? Q8 ? 1 : 2 : 3;
 
 // Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is on its way while
-// one is worked on, the rows of the block behind that are being looked up.  A wave's keys and values feed one product each from LDS, which gives
+// one is worked on, and the pages of the block behind that are asked for.  A wave's keys and values feed one product each from LDS, which gives
 // just what the matrix units take; 64 rows a wave halve that, but leave two waves a SIMD where three hide each other's softmax (8192 tokens,
 // 32 heads of 128, a window of 1024: 230 us for 195).  Blocks are as long as three workgroups a CU allow: 32 keys, 64 with heads of 64
 // (64 with heads of 128: 214 us).
 //
 // Bound by the waits of a wave for itself (products, the softmax of their results, products) and by vector instructions next to matrix ones: that
-// prompt takes 183 us, 710 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 203, 610.  Heads of 256 leave two waves a SIMD and LDS busy with the
-// blocks that come (six prompts of up to 2048 tokens: 106 us, 360 TFLOP/s, where the longest tile alone takes 100 of them).
+// prompt takes 177 us, 730 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 189, 660.  Heads of 256 leave two waves a SIMD and LDS busy with the
+// blocks that come (six prompts of up to 2048 tokens: 104 us, 360 TFLOP/s, where the longest tile alone takes 100 of them).
 template <int DT, bool PAGED, bool Q8, bool FINE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
 void attention_tiles(AttentionArgs a, AttentionPlan p) {
@@ -901,7 +901,8 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         }
         if constexpr (PAGED) flag(stage);
     };
-    // int8: through registers, where they become bf16, every lane's rows looked up a block ahead
+    // int8: through registers, where they become bf16, every lane's rows looked up a block ahead (23 single tokens and a prompt's 777 in one batch, 16 heads of
+    // 64 over 4, windows of 2048: 40 us)
     int rows[PER], scaleRow = -1;
     KeyAsk<PAGED> asked[PER], scaleAsked;
     v2i kreg[PER], vreg[PER];
