@@ -513,6 +513,18 @@ def test_gpu_single_tokens_among_prompts(device, case, see, quantised):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keys", ["rows", "bf16", "int8"])
+@pytest.mark.parametrize("D", [48, 128, 256])
+def test_gpu_many_rows(device, D, keys):
+    """So many rows (T times heads) that tiles round the weights once."""
+    b = Batch([(700, 1100), (1, 900), (0, 3), (400, 400), (17, 60)], D=D, H=8, KVH=2, page=16, quantised=keys == "int8", tail=2)
+    assert b.T * b.H >= 8192
+    b.query[::50, 1] = ref.to_bf16(np.float32(np.nan) * np.ones(D, dtype=np.float32))  # rows that are done again
+    built, before, want = attend(b, keys != "rows", window=300, sinks=5)
+    check_attention(b, built.run(device)["out"], before, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_gpu_holes_in_long_tables(device, D, quantised):
