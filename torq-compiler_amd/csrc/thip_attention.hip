@@ -329,7 +329,8 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
 
 // One row by one wave: a lane has the scores of one key of 64, then four of the result's elements (lane + 64 e).  A value is only touched
 // where the row sees its position, so what other positions hold, NaN and infinities among it, cannot come in: the tiles below multiply a
-// masked value by a weight of zero, and hand a row here where that left a NaN.  Adds positions [from, to) to o, m and l.
+// masked value, or the scale of one, by a weight of zero, and hand a row here where that left a NaN.  (A select by the weight would drop
+// the NaN of a position that the row sees with a weight too small for 32 bits.)  Adds positions [from, to) to o, m and l.
 // q: D floats of LDS, the row's query.
 template <bool PAGED, bool Q8>
 __device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, int pos, int from, int to, float *o, float *m, float *l) {
@@ -459,9 +460,6 @@ __device__ __forceinline__ int restOf(int word, float x, float y) {
     return packBf16(x - __uint_as_float((uint32_t)word << 16), y - __uint_as_float((uint32_t)word & 0xffff0000u));
 }
 
-// A weight times its value's scale; 0 where the weight is 0, whatever the scale of a masked position is.
-__device__ __forceinline__ float weigh(float weight, float scale) { return weight == 0.0f ? 0.0f : weight * scale; }
-
 // Four int8 as bf16, which holds them: the upper halves of their floats.
 __device__ __forceinline__ v2i wholeBf16(int w) {
     const uint32_t f0 = __float_as_uint((float)(int8_t)w), f1 = __float_as_uint((float)(int8_t)(w >> 8));
@@ -559,7 +557,11 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     };
     ask(span.from + wave);
     auto fetchScales = [&]() {
-        if constexpr (Q8) sreg = (lane < 32 ? a.key_scales : a.value_scales)[max((lane & 16) ? row1 : row0, 0)];
+        if constexpr (Q8) {
+            const int row = (lane & 16) ? row1 : row0;
+            sreg = (lane < 32 ? a.key_scales : a.value_scales)[max(row, 0)];
+            if (row < 0) sreg = 0.0f;
+        }
     };
 
     v8bf q[STEPS];
@@ -670,7 +672,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
             for (int k = 0; k < 2; k++) {
                 const v4f u = *(const v4f *)(scales + 32 + 16 * k + 4 * quarter);
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[k][i] = weigh(s[k][i], u[i]);
+                for (int i = 0; i < 4; i++) s[k][i] *= u[i];
             }
         }
         // in two parts, what the first leaves being the second: the matrix units have the time
@@ -730,7 +732,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
         for (int i = 0; i < 4; i++) odd |= sum[e][i] != sum[e][i];
     }
     // the rows of this wave that have a NaN: 4 wave .. 4 wave + 3, 16 lanes each
-    const uint64_t odds = Q8 ? 0 : __ballot(odd);
+    const uint64_t odds = __ballot(odd);
     if (r < span.rows && !((odds >> (16 * (r & 3))) & 0xffff)) {
         const int mine = r0 + r, tok = (int)fastDiv((uint32_t)mine, a.g);
         if (it.slot < 0) {
@@ -750,11 +752,9 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
             if (col == 0) put4(slots, to + D * 4, most, total, 0.0f, 0.0f);
         }
     }
-    if constexpr (!Q8) {
-        __syncthreads();
-        for (int k = 0; k < 4; k++) {
-            if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<false, PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
-        }
+    __syncthreads();
+    for (int k = 0; k < 4; k++) {
+        if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<false, PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
     }
     if (it.slot >= 0) {
         __syncthreads();
@@ -934,6 +934,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
             vreg[i] = *(const v2i *)((const int8_t *)a.value + from);
         }
         sreg = (tid & KB ? a.value_scales : a.key_scales)[max(scaleRow, 0)];
+        if (scaleRow < 0) sreg = 0.0f;
     };
     auto put = [&](int stage) {
         int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
@@ -1066,7 +1067,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
                 for (int i = 0; i < 4; i++) {
                     const v4f u = *(const v4f *)(scaleRoom + stage * 2 * KB + KB + k * 32 + 8 * i + 4 * half);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[k][4 * i + e] = weigh(s[k][4 * i + e], u[e]);
+                    for (int e = 0; e < 4; e++) s[k][4 * i + e] *= u[e];
                 }
             }
         }
@@ -1103,12 +1104,10 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
     l = sumOverHalves(l);
     // a masked value that was no number, or a row that sees one
     bool odd = false;
-    if constexpr (!Q8) {
 #pragma unroll
-        for (int t = 0; t < DT / 32; t++) {
+    for (int t = 0; t < DT / 32; t++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) odd |= o[t][i] != o[t][i];
-        }
+        for (int i = 0; i < 16; i++) odd |= o[t][i] != o[t][i];
     }
     const uint64_t odds = __ballot(odd);
     const uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
@@ -1143,10 +1142,8 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         }
         if (half == 0) put4(slots, tileStats(a, it.slot, wave * 32 + col), m, l, 0.0f, 0.0f);
     }
-    if constexpr (!Q8) {
-        for (int r = 0; r < rowsHere; r++) {
-            if ((again >> r) & 1) redoRow<true, PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
-        }
+    for (int r = 0; r < rowsHere; r++) {
+        if ((again >> r) & 1) redoRow<true, PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
     }
     if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
 }
