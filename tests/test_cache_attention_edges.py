@@ -73,3 +73,35 @@ def test_gpu_infinite_scales(device, case):
         if not see:
             assert np.isinf(want[0][:b.starts[-1]]).any()
         check_attention(b, built.run(device)["out"], before, want, str(see))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("case", FORMS, ids=_id)
+def test_gpu_values_next_to_the_largest(device, case, quantised):
+    """Values of about 2^121, with weights that grow by 2^7.6 along a run: their sums pass what 32 bits hold only where weights pass 1."""
+    b = Batch(quantised=quantised, page=16, garbage=False, **case)
+    _along(b, 0.0, 5.3, set(range(40)) | set(range(70, 120)) | set(range(200, 680)))
+    if quantised:
+        b.scales[1][:] = b.scales[1] * np.float32(2.0 ** 121)
+    else:
+        b.caches[1][:] = ref.to_bf16((ref.from_bf16(b.caches[1]) * 2.0 ** 121).astype(np.float32))
+    built, before, want = attend(b, True)
+    with np.errstate(invalid="ignore"):
+        assert np.nanmax(np.abs(want[0])) < 2.0 ** 126
+    check_attention(b, built.run(device)["out"], before, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_gpu_prompts_of_values_next_to_the_largest(device, D):
+    b = Batch([(90, 90), (3, 3), (200, 200)], D=D, H=4, KVH=2, tail=1)
+    sign = np.where(b.rng.random(D) < 0.5, -1.0, 1.0)
+    b.query[:] = ref.to_bf16(sign.astype(np.float32))
+    score = np.zeros(b.T)
+    for s, (n, _) in enumerate(b.sequences):
+        score[b.starts[s] + 40:b.starts[s] + n] = 5.3
+    b.key[:] = ref.to_bf16((score[:, None, None] / (D * b.scale) * sign).astype(np.float32))
+    b.value[:] = ref.to_bf16((ref.from_bf16(b.value) * 2.0 ** 121).astype(np.float32))
+    built, before, want = attend(b, False)
+    check_attention(b, built.run(device)["out"], before, want)

@@ -503,7 +503,10 @@ __device__ __forceinline__ int hold(int v) {
     return v;
 }
 
-constexpr float kSlack = 8.0f;  // how far (powers of two) a score may pass the running maximum before all is scaled down: weights stay below 2^8
+// What is taken off a row's scores is set this far (powers of two) above their maximum, so that all is scaled down only where a later one passes
+// that.  Above, not at it: weights then never pass 1, and sums of finite values no further than the definition's.  (What has less than 2^-118 of the
+// largest weight counts as nothing.)
+constexpr float kSlack = 8.0f;
 
 // ---- few rows: keys and values streamed -----------------------------------------------------------------------------------
 
@@ -651,8 +654,8 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
         }
         float high = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         high = maxOverQuarters(high) * scale;
-        if (__any(high > m + kSlack || (m == -INFINITY && high > m))) {
-            const float now = fmaxf(m, high), down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+        if (__any(high > m)) {
+            const float now = high > m ? high + kSlack : m, down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
             m = now;
             l *= down;
 #pragma unroll
@@ -1041,8 +1044,8 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
             for (int i = 0; i < 16; i++) high = fmaxf(high, s[k][i]);
         }
         high = maxOverHalves(high) * scale;
-        if (__any(high > m + kSlack || (m == -INFINITY && high > m))) {
-            const float now = fmaxf(m, high), down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+        if (__any(high > m)) {
+            const float now = high > m ? high + kSlack : m, down = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
             m = now;
             l *= down;
 #pragma unroll
