@@ -3,8 +3,11 @@ positions at the ends of what 32 bits hold, batches of very unequal sequences, a
 import numpy as np
 import pytest
 
+import desc_interp
 from oracle import attention as ref
-from test_cache_attention import Batch, attend, check_attention
+from oracle import programs as prog
+from test_cache_attention import Batch, Built, attend, check_attention
+from torq_compiler_amd import workloads as w
 
 U16 = np.uint16
 
@@ -105,3 +108,65 @@ def test_gpu_prompts_of_values_next_to_the_largest(device, D):
     b.value[:] = ref.to_bf16((ref.from_bf16(b.value) * 2.0 ** 121).astype(np.float32))
     built, before, want = attend(b, False)
     check_attention(b, built.run(device)["out"], before, want)
+
+
+# ---- programs around the ops ------------------------------------------------------------------------------------------
+
+def _transposed_cache(between, quantised=False):
+    """query times the transposed pages of a key cache, with `between` (an op, or none) where the transpose has been and the product has not; returns the
+    program, the batch and its bindings."""
+    b = Batch([(2, 20), (1, 9)], D=64, H=4, KVH=1, page=16, quantised=quantised, garbage=False)
+    built = Built()
+    pages = b.caches[0].shape[0]
+    k, v = built.bind("key", b.key), built.bind("value", b.value)
+    cache, scales = built.cache(b)
+    starts, lengths = built.rows(b)
+    x = b.normal(pages, 3, b.D)
+    a, query = built.bind("x", x), built.bind("query", b.query)
+    p = built.program
+    turned = p.transpose(p.view(cache[0], (pages, b.page, b.D)), (0, 2, 1))
+    if between == "write":
+        p.cache_write(k, v, *cache, starts, lengths, **scales)
+    elif between == "read":  # into the first rows of the key cache
+        other = built.bind("other_keys", b.caches[0].copy()), built.bind("other_values", b.caches[1].copy())
+        p.cache_read(*other, cache[2], starts, lengths, key=p.view(cache[0], (b.T, 1, b.D)), value=v, **scales)
+    elif between == "attention":
+        p.attention(query, k, v, starts, scale=b.scale, init=p.view(cache[0], (b.T, b.H, b.D)))
+    elif between == "elsewhere":  # what is written are other bindings
+        p.cache_read(*cache, starts, lengths, key=p.view(a, (b.T, 1, b.D)), value=v, **scales)
+    out = built.bind("product", np.zeros((pages, 3, b.page), U16))
+    p.matmul(built.values["x"], turned, np.array([0.0], np.float32), init=out, output_zp=0, output_min=w.NO_CLAMP[0], output_max=w.NO_CLAMP[1], shift=0)
+    if between == "behind":
+        p.cache_write(k, v, *cache, starts, lengths, **scales)
+    return built, b, x
+
+
+def _kinds(blob):
+    return [int(o["kind"]) for o in desc_interp.Descriptor(blob).ops]
+
+
+TRANSPOSE, DEC_MATMUL, WRITE, READ, ATTENTION = 1, 16, 17, 18, 19
+
+
+@pytest.mark.parametrize("between,record", [("write", WRITE), ("read", READ), ("attention", ATTENTION)])
+def test_transposes_stay_in_front_of_what_overwrites_their_input(between, record):
+    built, _, _ = _transposed_cache(between)
+    kinds = _kinds(built.program.serialize())
+    assert kinds[0] == TRANSPOSE and record in kinds[1:] and DEC_MATMUL not in kinds, kinds
+
+
+@pytest.mark.parametrize("between,kinds", [(None, [DEC_MATMUL]), ("behind", [DEC_MATMUL, WRITE]), ("elsewhere", [READ, DEC_MATMUL])])
+def test_transposes_of_what_stays_are_read_in_place(between, kinds):
+    built, _, _ = _transposed_cache(between)
+    assert _kinds(built.program.serialize()) == kinds
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("between", [None, "write", "read", "attention", "behind"])
+def test_gpu_products_see_the_cache_as_it_was(device, between):
+    built, b, x = _transposed_cache(between)
+    got = built.run(device)["product"]
+    turned = np.ascontiguousarray(b.caches[0].reshape(-1, b.page, b.D).transpose(0, 2, 1))
+    want = prog.orc.matmul_bf16(x, turned, np.array([0.0], np.float32))
+    mag = np.abs(ref.from_bf16(x)) @ np.abs(ref.from_bf16(turned))
+    prog.assert_bf16_close(got, want, str(between), magnitude=mag)

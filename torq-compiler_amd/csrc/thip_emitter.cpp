@@ -719,6 +719,7 @@ class Emitter {
     thip_status_t emitTable(const thip_hl_table_t &c, const std::vector<int32_t> &staticTable);
     // Operands of an integer elementwise op: element types, and the record's common fields.
     // Attention and its cache (thip_lm_*).
+    bool shareBytes(thip_value_t a, thip_value_t b) const;
     thip_status_t boundPart(thip_value_t id, const char *what, int32_t dtype, int32_t rank, bool written, DescRef *out);
     thip_status_t indexOperand(thip_value_t id, const char *what, int32_t rank, DescRef *out);
     thip_status_t batchOperands(thip_value_t starts, thip_value_t lengths, thip_value_t pages, bool cached, DescOp *op, CacheExt *ext);
@@ -2190,6 +2191,51 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
     return THIP_OK;
 }
 
+// What an op writes, whole or in part.
+static std::vector<thip_value_t> writtenBy(const HlOp &op) {
+    switch (op.kind) {
+    case kHlConv2d: return {op.u.conv.init};
+    case kHlDepthwise: return {op.u.dw.init};
+    case kHlFullyConnected: return {op.u.fc.init};
+    case kHlMatmul: return {op.u.mm.init};
+    case kHlMaxPool: return {op.u.mp.init};
+    case kHlAvgPool: return {op.u.ap.init};
+    case kHlAdd: return {op.u.add.init};
+    case kHlTranspose: return {op.u.tr.init};
+    case kHlExpandWeights: return {op.u.ew.init};
+    case kHlFma: return {op.u.fma.init};
+    case kHlMul: return {op.u.mul.init};
+    case kHlAct: return {op.u.act.init};
+    case kHlBinary: return {op.u.bin.init};
+    case kHlUnary: return {op.u.un.init};
+    case kHlShift: return {op.u.sh.init};
+    case kHlTable: return {op.u.tab.init};
+    case kLmCacheWrite: return {op.u.cw.key_cache, op.u.cw.value_cache, op.u.cw.key_scales, op.u.cw.value_scales};
+    case kLmCacheRead: return {op.u.cr.key, op.u.cr.value};
+    case kLmAttention: return {op.u.at.init};
+    }
+    return {};
+}
+
+// Whether two values have bytes in common: of one binding, or of one intermediate.
+bool Emitter::shareBytes(thip_value_t a, thip_value_t b) const {
+    const size_t n = prog_.values.size();
+    if (a < 0 || (size_t)a >= n || b < 0 || (size_t)b >= n) return false;
+    struct Range {
+        thip_value_t root;
+        int64_t begin, end;
+    };
+    auto rangeOf = [&](thip_value_t id) {
+        const Value &v = prog_.values[(size_t)id];
+        const int64_t size = (int64_t)elemSize(v.dtype), begin = v.kind == kValueView ? v.viewOffset * size : 0;
+        return Range{v.kind == kValueView ? v.base : id, begin, begin + v.numel() * size};
+    };
+    const Range x = rangeOf(a), y = rangeOf(b);
+    const Value &p = prog_.values[(size_t)x.root], &q = prog_.values[(size_t)y.root];
+    const bool same = x.root == y.root || (p.kind == kValueBinding && q.kind == kValueBinding && p.binding == q.binding);
+    return same && x.begin < y.end && y.begin < x.end;
+}
+
 void Emitter::planDecodeFolding() {
     foldedTranspose_.clear();
     consumed_.assign(prog_.ops.size(), 0);
@@ -2216,6 +2262,12 @@ void Emitter::planDecodeFolding() {
             if (a.dtype != THIP_DTYPE_BF16 || a.rank < 2 || a.rank > 3 || a.shape[a.rank - 2] > kDecMaxRows) break;
             const int64_t batches = std::max<int64_t>(a.rank == 3 ? a.shape[0] : 1, res.rank == 3 ? res.shape[0] : 1);
             if (batches > 65535 || a.shape[a.rank - 1] % 8 != 0) break;
+            // read by the matmul, the input has to be then what it was where the transpose stands
+            bool changed = false;
+            for (size_t w = t + 1; w < m; w++) {
+                for (thip_value_t v : writtenBy(prog_.ops[w])) changed = changed || shareBytes(v, tr.input);
+            }
+            if (changed) break;
             foldedTranspose_[tr.init] = t;
             break;
         }
