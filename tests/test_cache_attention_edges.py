@@ -170,3 +170,56 @@ def test_gpu_products_see_the_cache_as_it_was(device, between):
     want = prog.orc.matmul_bf16(x, turned, np.array([0.0], np.float32))
     mag = np.abs(ref.from_bf16(x)) @ np.abs(ref.from_bf16(turned))
     prog.assert_bf16_close(got, want, str(between), magnitude=mag)
+
+
+def _over_an_intermediate(op, query_too=False):
+    """An intermediate (rows that a transpose made) that attention, or a read of the cache, writes for the sequences' rows, then turned back into a
+    binding."""
+    b = Batch([(3, 20), (0, 5), (2, 9)], D=64, H=4, KVH=4, page=16, tail=4)
+    built = Built()
+    k, v = built.bind("key", b.key), built.bind("value", b.value)
+    cache, scales = built.cache(b)
+    starts, lengths = built.rows(b)
+    p = built.program
+    first = b.normal(b.T, b.H, b.D)
+    rows = p.transpose(built.bind("first", np.ascontiguousarray(first.transpose(0, 2, 1))), (0, 2, 1))
+    if op == "read":
+        p.cache_read(*cache, starts, lengths, key=rows, value=v, **scales)
+    else:
+        p.paged_attention(rows if query_too else built.bind("query", b.query), *cache, starts, lengths, scale=b.scale, init=rows, **scales)
+    p.transpose(rows, (0, 2, 1), init=built.bind("out", np.zeros((b.T, b.D, b.H), U16)))
+    return built, b, first
+
+
+@pytest.mark.parametrize("op,query_too", [("read", False), ("attention", False), ("attention", True)])
+def test_intermediates_are_written_in_place(op, query_too):
+    built, _, _ = _over_an_intermediate(op, query_too)
+    made, record, back = desc_interp.Descriptor(built.program.serialize()).ops
+    assert made["out"] == record["out"] and record["out"] == back["in0"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op,query_too", [("read", False), ("attention", False), ("attention", True)])
+def test_gpu_rows_of_no_sequence_stay_in_intermediates(device, op, query_too):
+    built, b, first = _over_an_intermediate(op, query_too)
+    got = np.ascontiguousarray(built.run(device, dispatches=3)["out"].transpose(0, 2, 1))
+    if op == "read":
+        assert np.array_equal(got, ref.cache_read(b.cache(), first, b.value, b.starts, b.lengths)[0])
+        assert np.array_equal(got[-4:], first[-4:])
+    else:
+        want = ref.attention(first if query_too else b.query, b.starts, b.scale, cache=b.cache(), lengths=b.lengths)
+        check_attention(b, got, first, want)
+
+
+def test_a_transposed_intermediate_that_attention_writes_is_no_operand_in_place():
+    """The product behind it reads what attention left there, not what the transpose was made of."""
+    b = Batch([(3, 3)], D=64, H=64, KVH=64)
+    built = Built()
+    p = built.program
+    turned = p.transpose(built.bind("first", b.normal(b.T, b.D, b.H)), (0, 2, 1))
+    p.attention(built.bind("query", b.query), built.bind("key", b.key), built.bind("value", b.value), built.bind("row_starts", b.starts), scale=b.scale,
+                init=turned)
+    p.matmul(built.bind("x", b.normal(b.T, 2, b.H)), turned, np.array([0.0], np.float32), init=built.bind("out", b.normal(b.T, 2, b.D)), output_zp=0,
+             output_min=w.NO_CLAMP[0], output_max=w.NO_CLAMP[1], shift=0)
+    kinds = _kinds(p.serialize())
+    assert kinds[:2] == [TRANSPOSE, ATTENTION] and DEC_MATMUL not in kinds, kinds

@@ -2044,7 +2044,12 @@ thip_status_t Emitter::rowOperand(thip_value_t id, const char *what, bool writte
         if (thip_status_t s = literalInput(id, what, out)) return s;
         if (state_[(size_t)id].nhwcOfNchw) return fail(THIP_UNIMPLEMENTED, "%s: an N,C,H,W intermediate", what);
     } else {
-        if (thip_status_t s = literalOutput(id, what, THIP_DTYPE_BF16, v->numel(), out)) return s;
+        if (v->kind == kValueTensor && state_[id].defined) {  // an intermediate that is there keeps its other rows: in place
+            if (state_[id].nhwcOfNchw) return fail(THIP_UNIMPLEMENTED, "%s: an N,C,H,W intermediate", what);
+            *out = state_[id].ref;
+        } else if (thip_status_t s = literalOutput(id, what, THIP_DTYPE_BF16, v->numel(), out)) {
+            return s;
+        }
         const Value &root = v->kind == kValueView ? prog_.values[(size_t)v->base] : *v;
         if (root.kind == kValueBinding) bindingRef(root, false);
     }
@@ -2644,8 +2649,9 @@ void Emitter::planExpandFolding() {
         case kHlShift: read(op.u.sh.input1); read(op.u.sh.input2); break;
         case kHlTable: read(op.u.tab.input); break;
         case kLmCacheWrite: read(op.u.cw.key); read(op.u.cw.value); break;
-        case kLmCacheRead: read(op.u.cr.key_cache); read(op.u.cr.value_cache); break;
-        case kLmAttention: read(op.u.at.query); read(op.u.at.key); read(op.u.at.value); break;
+        // what they write in part stays in part
+        case kLmCacheRead: read(op.u.cr.key_cache); read(op.u.cr.value_cache); read(op.u.cr.key); read(op.u.cr.value); break;
+        case kLmAttention: read(op.u.at.query); read(op.u.at.key); read(op.u.at.value); read(op.u.at.init); break;
         }
     }
     valueReads_ = reads;
