@@ -223,3 +223,20 @@ def test_a_transposed_intermediate_that_attention_writes_is_no_operand_in_place(
              output_min=w.NO_CLAMP[0], output_max=w.NO_CLAMP[1], shift=0)
     kinds = _kinds(p.serialize())
     assert kinds[:2] == [TRANSPOSE, ATTENTION] and DEC_MATMUL not in kinds, kinds
+
+
+# ---- the ends of 32 bits ------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 3])
+@pytest.mark.parametrize("case", [dict(sequences=[(5, 2), (9, 4), (8, 5), (3, 300)], D=64, H=4, KVH=2), dict(sequences=[(60, 20), (70, 69), (40, 90)], D=128, H=4, KVH=2),
+                                  dict(sequences=[(9, 4)], D=256, H=4, KVH=1)], ids=_id)
+def test_gpu_longest_windows(device, case, window, quantised):
+    """A window that takes in everything, where the first rows of a sequence stand before its position 0."""
+    b = Batch(quantised=quantised, page=16, **case)
+    for sinks in (0, 3):
+        built, before, want = attend(b, True, window=window, sinks=sinks)
+        plain = ref.attention(b.query, b.starts, b.scale, cache=b.cache(), lengths=b.lengths)[0]
+        assert np.array_equal(want[0], plain, equal_nan=True)
+        check_attention(b, built.run(device)["out"], before, want)

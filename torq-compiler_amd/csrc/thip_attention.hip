@@ -168,7 +168,7 @@ __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPl
     const int r0 = it.tile << p.rowsLog, keys = p.keys();
     s.rows = min(p.rows(), it.w.count * a.G - r0);
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
-    const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(top - a.window + 1, 0) : 0;
+    const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(max(top, -1) - a.window + 1, 0) : 0;  // rows below position 0 see nothing
     s.sinkBlocks = (min(min(a.sinks, low), high) + keys - 1) >> p.keysLog;
     s.windowBlock = max(low >> p.keysLog, s.sinkBlocks);
     const int all = s.sinkBlocks + max(((int)((uint32_t)high + (uint32_t)keys - 1) >> p.keysLog) - s.windowBlock, 0);
