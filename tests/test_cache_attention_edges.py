@@ -240,3 +240,36 @@ def test_gpu_longest_windows(device, case, window, quantised):
         plain = ref.attention(b.query, b.starts, b.scale, cache=b.cache(), lengths=b.lengths)[0]
         assert np.array_equal(want[0], plain, equal_nan=True)
         check_attention(b, built.run(device)["out"], before, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("rows", [1, 3, 60])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_gpu_last_positions_of_32_bits(device, D, rows, quantised):
+    """Tables of 2^31 - 8 positions (all of their entries the same page) with sequences that end there, or behind.  The reference has the same rows
+    a whole number of pages further down."""
+    page, P = 8 * 127 * 113, 3 * 5 * 29 * 43
+    assert page * P == 2 ** 31 - 8
+    rng = np.random.default_rng(D + rows)
+    b = Batch([(rows, 16)], D=D, H=4, KVH=1, page=16, quantised=quantised, garbage=False)
+    shape = (1, 1, page, D)
+    if quantised:
+        b.caches = [rng.integers(-127, 128, size=shape, dtype=np.int8) for _ in range(2)]
+        b.scales = [(rng.uniform(0.5, 1.5, size=shape[:3]) / 73).astype(np.float32) for _ in range(2)]
+        b.scales[1][0, 0, page - 25] = np.nan  # a row that sees it is done again
+    else:
+        b.caches = [b.normal(*shape) for _ in range(2)]
+        b.caches[1][0, 0, page - 25] = 0x7FC0
+    b.page, b.pages = page, np.zeros((1, P), dtype=np.int32)
+    for length in (2 ** 31 - 8, 2 ** 31 - 1, 2 ** 31 - 37):
+        for sinks in (0, 3):
+            b.pages, b.lengths = np.zeros((1, 1), dtype=np.int32), np.array([length - (P - 1) * page], dtype=np.int32)
+            near = ref.attention(b.query, b.starts, b.scale, window=16, sinks=sinks, cache=b.cache(), lengths=b.lengths)
+            b.pages, b.lengths = np.zeros((1, P), dtype=np.int32), np.array([length], dtype=np.int32)
+            built, out = Built(), b.normal(b.T, b.H, b.D)
+            q = built.bind("query", b.query)
+            cache, scales = built.cache(b)
+            starts, lengths = built.rows(b)
+            built.program.paged_attention(q, *cache, starts, lengths, init=built.bind("out", out), scale=b.scale, window=16, sinks=sinks, **scales)
+            check_attention(b, built.run(device)["out"], out, near, "%d %d" % (length, sinks))

@@ -169,9 +169,10 @@ __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPl
     s.rows = min(p.rows(), it.w.count * a.G - r0);
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
     const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(max(top, -1) - a.window + 1, 0) : 0;  // rows below position 0 see nothing
-    s.sinkBlocks = (min(min(a.sinks, low), high) + keys - 1) >> p.keysLog;
+    auto blocksTo = [&](int end) { return (int)(((uint32_t)end + (uint32_t)keys - 1) >> p.keysLog); };  // a last block may pass 2^31
+    s.sinkBlocks = blocksTo(min(min(a.sinks, low), high));
     s.windowBlock = max(low >> p.keysLog, s.sinkBlocks);
-    const int all = s.sinkBlocks + max(((int)((uint32_t)high + (uint32_t)keys - 1) >> p.keysLog) - s.windowBlock, 0);
+    const int all = s.sinkBlocks + max(blocksTo(high) - s.windowBlock, 0);
     s.from = min(it.splits > 1 ? it.split * it.part : 0, all);
     s.to = it.splits > 1 ? min(all, s.from + it.part) : all;
     return s;
@@ -330,72 +331,70 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
 // One row by one wave: a lane has the scores of one key of 64, then four of the result's elements (lane + 64 e).  A value is only touched
 // where the row sees its position, so what other positions hold, NaN and infinities among it, cannot come in: the tiles below multiply a
 // masked value, or the scale of one, by a weight of zero, and hand a row here where that left a NaN.  (A select by the weight would drop
-// the NaN of a position that the row sees with a weight too small for 32 bits.)  Adds positions [from, to) to o, m and l.
+// the NaN of a position that the row sees with a weight too small for 32 bits.)  Adds the `count` (up to 64) positions from `from` on to o, m and l.
 // q: D floats of LDS, the row's query.
 template <bool PAGED, bool Q8>
-__device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, int pos, int from, int to, float *o, float *m, float *l) {
+__device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, int pos, int from, int count, float *o, float *m, float *l) {
     const CacheArgs &c = a.c;
     const int lane = threadIdx.x & 63, D = c.D;
     float most = *m, sum = *l;
-    for (int base = from; base < to; base += 64) {
-        const int j = base + lane;
-        int row = -1;
-        if (j < to && sees(windowOf(a), sinksOf(a, pos), pos, j)) row = keyRow(a, it, askKey<PAGED>(a, it, j, true));
-        float s = -INFINITY, vs = 1.0f;
-        if (row >= 0) {
-            float dot = 0.0f;
-            if constexpr (Q8) {
-                const int8_t *k = (const int8_t *)a.key + (int64_t)row * D;
-                for (int d = 0; d < D; d += 16) {
-                    const v4i w = *(const v4i *)(k + d);
+    const int j = (int)((uint32_t)from + (uint32_t)lane);
+    int row = -1;
+    if (lane < count && sees(windowOf(a), sinksOf(a, pos), pos, j)) row = keyRow(a, it, askKey<PAGED>(a, it, j, true));
+    float s = -INFINITY, vs = 1.0f;
+    if (row >= 0) {
+        float dot = 0.0f;
+        if constexpr (Q8) {
+            const int8_t *k = (const int8_t *)a.key + (int64_t)row * D;
+            for (int d = 0; d < D; d += 16) {
+                const v4i w = *(const v4i *)(k + d);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) dot = fmaf((float)(int8_t)(w[i >> 2] >> (8 * (i & 3))), q[d + i], dot);
-                }
-                dot *= a.key_scales[row];
-                vs = a.value_scales[row];
-            } else {
-                const uint16_t *k = (const uint16_t *)a.key + (int64_t)row * D;
-                for (int d = 0; d < D; d += 8) {
-                    const v4i w = *(const v4i *)(k + d);
+                for (int i = 0; i < 16; i++) dot = fmaf((float)(int8_t)(w[i >> 2] >> (8 * (i & 3))), q[d + i], dot);
+            }
+            dot *= a.key_scales[row];
+            vs = a.value_scales[row];
+        } else {
+            const uint16_t *k = (const uint16_t *)a.key + (int64_t)row * D;
+            for (int d = 0; d < D; d += 8) {
+                const v4i w = *(const v4i *)(k + d);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        dot = fmaf(__uint_as_float((uint32_t)w[i] << 16), q[d + 2 * i], dot);
-                        dot = fmaf(__uint_as_float((uint32_t)w[i] & 0xffff0000u), q[d + 2 * i + 1], dot);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    dot = fmaf(__uint_as_float((uint32_t)w[i] << 16), q[d + 2 * i], dot);
+                    dot = fmaf(__uint_as_float((uint32_t)w[i] & 0xffff0000u), q[d + 2 * i + 1], dot);
                 }
             }
-            s = dot * (a.scale * kLog2e);
         }
-        uint64_t seen = __ballot(row >= 0);
-        if (seen == 0) continue;
-        float high = s;
+        s = dot * (a.scale * kLog2e);
+    }
+    uint64_t seen = __ballot(row >= 0);
+    if (seen == 0) return;
+    float high = s;
 #pragma unroll
-        for (int step = 1; step < 64; step *= 2) high = fmaxf(high, __shfl_xor(high, step));
-        const float now = fmaxf(most, high), shift = now == -INFINITY ? 0.0f : now;
-        const float down = exp2f(most - shift);  // most <= shift or -inf
-        const float p = row >= 0 ? exp2f(s - shift) : 0.0f;
-        float part = p;
+    for (int step = 1; step < 64; step *= 2) high = fmaxf(high, __shfl_xor(high, step));
+    const float now = fmaxf(most, high), shift = now == -INFINITY ? 0.0f : now;
+    const float down = exp2f(most - shift);  // most <= shift or -inf
+    const float p = row >= 0 ? exp2f(s - shift) : 0.0f;
+    float part = p;
 #pragma unroll
-        for (int step = 1; step < 64; step *= 2) part += __shfl_xor(part, step);
-        sum = sum * down + part;
-        most = now;
+    for (int step = 1; step < 64; step *= 2) part += __shfl_xor(part, step);
+    sum = sum * down + part;
+    most = now;
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] *= down;
-        while (seen) {
-            const int t = __builtin_ctzll(seen);
-            seen &= seen - 1;
-            const int64_t r = __builtin_amdgcn_readlane(row, t);
-            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), t));
-            const float u = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), t));
+    for (int e = 0; e < 4; e++) o[e] *= down;
+    while (seen) {
+        const int t = __builtin_ctzll(seen);
+        seen &= seen - 1;
+        const int64_t r = __builtin_amdgcn_readlane(row, t);
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), t));
+        const float u = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), t));
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int d = lane + 64 * e;
-                if (d >= D) continue;
-                float v;
-                if constexpr (Q8) v = (float)((const int8_t *)a.value)[r * D + d] * u;
-                else v = __uint_as_float((uint32_t)((const uint16_t *)a.value)[r * D + d] << 16);
-                o[e] = fmaf(w, v, o[e]);
-            }
+        for (int e = 0; e < 4; e++) {
+            const int d = lane + 64 * e;
+            if (d >= D) continue;
+            float v;
+            if constexpr (Q8) v = (float)((const int8_t *)a.value)[r * D + d] * u;
+            else v = __uint_as_float((uint32_t)((const uint16_t *)a.value)[r * D + d] << 16);
+            o[e] = fmaf(w, v, o[e]);
         }
     }
     *m = most;
@@ -414,7 +413,7 @@ __device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionP
     const int pos = it.w.first + token;
     for (int b = span.from; b < span.to; b++) {
         const int j = blockStart(p, span, b);
-        attendRow<PAGED, Q8>(a, q, it, pos, j, j + p.keys(), o, &m, &l);
+        attendRow<PAGED, Q8>(a, q, it, pos, j, p.keys(), o, &m, &l);
     }
     if (it.slot < 0) {
 #pragma unroll
@@ -855,7 +854,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
     auto send = [&](int stage, int b) {
         const int j0 = blockStart(p, span, b);
         const unsigned to = lds + stage * 2 * KB * ROW;
-        bool whole = together && b < span.to && j0 + KB <= it.w.length;
+        bool whole = together && b < span.to && j0 <= it.w.length - KB;
         if constexpr (PAGED) {
 #pragma unroll
             for (int i = 0; i < PER; i++) whole = whole & (pages[i] < (uint32_t)c.NP);
@@ -1016,7 +1015,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
                 }
             }
         }
-        bool whole = j0 + KB - 1 <= top && j0 + KB <= it.w.length && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        bool whole = j0 + KB - 1 <= top && j0 <= it.w.length - KB && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
         bool gaps = false;
         if constexpr (PAGED) gaps = __builtin_amdgcn_readfirstlane(*(const int *)(flagRoom + stage * 4)) != 0;
         if (!whole || gaps) {
