@@ -4,9 +4,11 @@ import numpy as np
 import pytest
 
 import desc_interp
+import torq_compiler_amd as thip
 from oracle import attention as ref
 from oracle import programs as prog
 from test_cache_attention import Batch, Built, attend, check_attention
+from torq_compiler_amd import runtime as rt
 from torq_compiler_amd import workloads as w
 
 U16 = np.uint16
@@ -273,3 +275,11 @@ def test_gpu_last_positions_of_32_bits(device, D, rows, quantised):
             starts, lengths = built.rows(b)
             built.program.paged_attention(q, *cache, starts, lengths, init=built.bind("out", out), scale=b.scale, window=16, sinks=sinks, **scales)
             check_attention(b, built.run(device)["out"], out, near, "%d %d" % (length, sinks))
+
+
+@pytest.mark.parametrize("see", [dict(window=2 ** 32), dict(window=2 ** 32 + 5), dict(sinks=2 ** 31), dict(window=-2 ** 32), dict(window=1.5)], ids=str)
+@pytest.mark.parametrize("cached", [False, True], ids=["rows", "cache"])
+def test_windows_that_a_field_would_not_hold_are_refused(see, cached):
+    with pytest.raises(thip.ThipError) as e:
+        attend(Batch([(2, 2)]), cached, **see)
+    assert e.value.code == rt.INVALID_ARGUMENT and "32 bits" in e.value.message

@@ -326,6 +326,13 @@ class Program:
     def _index_or_none(self, x):
         return rt.NO_VALUE if x is None else self._as_value(x).index
 
+    @staticmethod
+    def _positions(name, x):
+        """A number of positions for a field of 32 bits, which would take it modulo 2^32."""
+        if int(x) != x or not -2 ** 31 <= x < 2 ** 31:
+            raise rt.ThipError(rt.INVALID_ARGUMENT, "%s: %r is no whole number of 32 bits" % (name, x))
+        return int(x)
+
     def cache_write(self, key, value, key_cache, value_cache, pages, row_starts, lengths, *, key_scales=None, value_scales=None):
         """Stores the rows key, value [T, kv_heads, D] in the cache, in place; an int8 cache quantises them row by row and head by head."""
         op = rt.LmCacheWrite(key_cache.index, value_cache.index, self._index_or_none(key_scales), self._index_or_none(value_scales), key.index,
@@ -348,7 +355,8 @@ class Program:
         of its sequence before it, with a window the last `window` of these and the first `sinks`."""
         init = self._init_or_new(init, query.shape, np.uint16)
         op = rt.LmAttention(init.index, query.index, key.index, value.index, rt.NO_VALUE, rt.NO_VALUE, rt.NO_VALUE,
-                            self._as_value(row_starts).index, rt.NO_VALUE, scale, int(window), int(sinks))
+                            self._as_value(row_starts).index, rt.NO_VALUE, scale, self._positions("window", window),
+                            self._positions("sinks", sinks))
         rt.check(rt.lib().thip_lm_attention(self._h, ctypes.byref(op)))
         return init
 
@@ -358,7 +366,8 @@ class Program:
         init = self._init_or_new(init, query.shape, np.uint16)
         op = rt.LmAttention(init.index, query.index, key_cache.index, value_cache.index, self._index_or_none(key_scales),
                             self._index_or_none(value_scales), self._as_value(pages).index, self._as_value(row_starts).index,
-                            self._as_value(lengths).index, scale, int(window), int(sinks))
+                            self._as_value(lengths).index, scale, self._positions("window", window),
+                            self._positions("sinks", sinks))
         rt.check(rt.lib().thip_lm_attention(self._h, ctypes.byref(op)))
         return init
 
