@@ -559,11 +559,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     };
     ask(span.from + wave);
     auto fetchScales = [&]() {
-        if constexpr (Q8) {
-            const int row = (lane & 16) ? row1 : row0;
-            sreg = (lane < 32 ? a.key_scales : a.value_scales)[max(row, 0)];
-            if (row < 0) sreg = 0.0f;
-        }
+        if constexpr (Q8) sreg = (lane < 32 ? a.key_scales : a.value_scales)[max((lane & 16) ? row1 : row0, 0)];
     };
 
     v8bf q[STEPS];
@@ -609,7 +605,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
             *(v4i *)(smem + chunkAt(storeAt, 4 * i)) = vreg[0][i];
             *(v4i *)(smem + chunkAt(storeAt, 4 * i) + 16 * ROW) = vreg[1][i];
         }
-        if constexpr (Q8) scales[lane] = sreg;
+        if constexpr (Q8) scales[lane] = ((lane & 16) ? there1 : there0) ? sreg : 0.0f;  // here, where the load has come back
         __builtin_amdgcn_wave_barrier();
         const bool now0 = row0 >= 0, now1 = row1 >= 0;
         fetchScales();
@@ -756,7 +752,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     }
     __syncthreads();
     for (int k = 0; k < 4; k++) {
-        if (((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows) redoRow<false, PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
+        if (__builtin_expect(((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows, 0)) redoRow<false, PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
     }
     if (it.slot >= 0) {
         __syncthreads();
@@ -909,6 +905,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
     KeyAsk<PAGED> asked[PER], scaleAsked;
     v2i kreg[PER], vreg[PER];
     float sreg = 0.0f;
+    bool scaleGone = false;  // of sreg's position
     bool holes = false;  // unpaged, of the rows that were looked up
     auto ask = [&](int b) {
         const int j0 = blockStart(p, span, b);
@@ -936,7 +933,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
             vreg[i] = *(const v2i *)((const int8_t *)a.value + from);
         }
         sreg = (tid & KB ? a.value_scales : a.key_scales)[max(scaleRow, 0)];
-        if (scaleRow < 0) sreg = 0.0f;
+        scaleGone = scaleRow < 0;
     };
     auto put = [&](int stage) {
         int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
@@ -946,7 +943,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
             *(v8bf *)(keys + where) = wholeBf16x8(kreg[i][0], kreg[i][1]);
             *(v8bf *)(values + where) = wholeBf16x8(vreg[i][0], vreg[i][1]);
         }
-        if (tid < 2 * KB) scaleRoom[stage * 2 * KB + tid] = sreg;
+        if (tid < 2 * KB) scaleRoom[stage * 2 * KB + tid] = scaleGone ? 0.0f : sreg;
         flag(stage);
     };
 
@@ -1145,7 +1142,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         if (half == 0) put4(slots, tileStats(a, it.slot, wave * 32 + col), m, l, 0.0f, 0.0f);
     }
     for (int r = 0; r < rowsHere; r++) {
-        if ((again >> r) & 1) redoRow<true, PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
+        if (__builtin_expect((again >> r) & 1, 0)) redoRow<true, PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
     }
     if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
 }
