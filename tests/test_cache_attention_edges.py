@@ -1,10 +1,14 @@
 """Attention and its cache (thip_lm_*) where a row's result hangs on what is easily lost: numbers that are none, values next to the largest,
 positions at the ends of what 32 bits hold, batches of very unequal sequences, and the programs around the ops."""
+import ctypes
+import subprocess
+
 import numpy as np
 import pytest
 
 import desc_interp
 import torq_compiler_amd as thip
+from helpers import host_check
 from oracle import attention as ref
 from oracle import programs as prog
 from test_cache_attention import Batch, Built, attend, check_attention
@@ -283,3 +287,55 @@ def test_windows_that_a_field_would_not_hold_are_refused(see, cached):
     with pytest.raises(thip.ThipError) as e:
         attend(Batch([(2, 2)]), cached, **see)
     assert e.value.code == rt.INVALID_ARGUMENT and "32 bits" in e.value.message
+
+
+# ---- batches of very unequal sequences ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("seed", [1, 2])
+def test_shares_of_a_launch(tmp_path, seed):
+    done = subprocess.run([host_check("attention_plan", tmp_path), str(seed)], stdout=subprocess.PIPE, text=True, timeout=120)
+    assert done.returncode == 0 and int(done.stdout) > 500, done.stdout
+
+
+SKEWED = [
+    dict(sequences=[(1, 30)] * 40 + [(1, 3000)] + [(1, 50)] * 70 + [(0, 9)], D=16, H=8, KVH=8, page=16),              # streams, a long run in the first 64
+    dict(sequences=[(1, 3)] * 290 + [(2, 2500)] + [(0, 4)] * 10 + [(1, 9)] * 20, D=16, H=2, KVH=2, page=32, tail=2),      # more than 256
+    dict(sequences=[(1, 1 + i % 3) for i in range(4200)] + [(1, 500)] + [(1, 2)] * 3, D=16, H=1, KVH=1, page=8),          # groups of more than 64
+    dict(sequences=[(1, 40)] * 66 + [(300, 2600)] + [(3, 1200)] + [(40, 50)] * 12, D=32, H=8, KVH=2, page=24, tail=1),    # tiles, streams among them
+    dict(sequences=[(17, 100)] * 20 + [(17, 4100)] + [(17, 90)] * 50, D=16, H=16, KVH=8, page=16),                       # more than 384 tiles
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("case", SKEWED, ids=_id)
+def test_gpu_one_long_sequence_among_many(device, case, quantised):
+    b = Batch(quantised=quantised, garbage=False, **case)
+    for see in (dict(), dict(window=1500, sinks=3)):
+        built, before, want = attend(b, True, **see)
+        first = built.run(device)["out"]
+        check_attention(b, first, before, want)
+        assert np.array_equal(built.run(device, dispatches=3)["out"], first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SKEWED[:4], ids=_id)
+def test_gpu_after_many_starts_that_do_not_ascend(device, case):
+    """Starts that claim far more rows than there are, in batches of many sequences, leave nothing behind for the next dispatch."""
+    b = Batch(garbage=False, **case)
+    built, before, want = attend(b, True)
+    exe = thip.Executable(device, built.program.serialize())
+    ptrs = [device.upload(x) for _, x in built.arrays]
+    try:
+        names = [name for name, _ in built.arrays]
+        starts, out = ptrs[names.index("row_starts")], ptrs[names.index("out")]
+        odd = np.where(np.arange(len(b.starts)) % 2, b.T, 0).astype(np.int32)
+        for x in (odd, b.starts, b.starts[::-1].copy(), odd[::-1].copy(), b.starts):
+            for where, data in ((starts, x), (out, before)):  # the others claim rows behind the last sequence too
+                rt.check(rt.lib().thip_device_h2d(device.handle, ctypes.c_void_p(where), data.ctypes.data_as(ctypes.c_void_p), data.nbytes))
+            exe.run_device(ptrs, [a.nbytes for _, a in built.arrays])
+        check_attention(b, device.download(out, before.shape, before.dtype), before, want)
+    finally:
+        for p in ptrs:
+            device.free(p)
+        exe.close()

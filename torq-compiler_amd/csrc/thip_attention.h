@@ -2,6 +2,8 @@
 // validation and the launchers have to agree on.
 #pragma once
 
+#include <math.h>
+
 #include "thip_kernels.h"
 
 namespace thip {
@@ -45,8 +47,8 @@ struct AttentionArgs {
 hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx);
 
 // How a launch shares its work out.  An item is a tile of `rows` of a sequence's rows (a row: one query head of one token, the heads of a key
-// head next to one another) against a run of blocks of `keys` positions; a workgroup has one.  Where that makes too few items, the
-// device cuts the runs of long sequences so that there are about `items`, and the last workgroup of a tile to finish joins the parts.
+// head next to one another) against a run of blocks of `keys` positions; a workgroup has one.  The device cuts runs that
+// are longer than their share of the launch, so that there are about `items` of that share's length, and the last workgroup of a tile to finish joins the parts.
 struct AttentionPlan {
     bool tiles;                  // attention_tiles, or attention_stream
     bool fine;                   // weights of tiles in two parts
@@ -55,15 +57,36 @@ struct AttentionPlan {
     int32_t minBlocks, maxParts; // blocks that a part has at least, and parts of a run at most
     int32_t fewBlocks;           // the same where few tiles are full, and of a stream among tiles
     bool splits;                 // runs may be cut
-    int32_t items;
+    int32_t items, whole;        // the launch's blocks by these: a part's, and those up to which a tile's run stays whole
+    // A run of b blocks, in parts of B, is ceil(b / B) items, less than one more than b / B; the b / B of all are no more than `items`.  So there are fewer
+    // than `items` above one a run (of `grid`), and of runs that are cut (b > B), less than 2 b / B each, fewer than twice `items` (of `slots`).
     int64_t grid;                // items at most
-    int64_t slots;               // parts at most: one that is cut is of more than one run, so there are at most twice as many as asked for
+    int64_t slots;               // parts of runs that are cut at most
     FastDiv kvh;
     __host__ __device__ int32_t rows() const { return 1 << rowsLog; }
     __host__ __device__ int32_t keys() const { return 1 << keysLog; }
 };
-// capacity: positions that a sequence can have
-inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
+
+// Blocks of a part, and up to how many a run stays whole: of tiles, and of streams (among tiles, or alone).
+struct PartBlocks {
+    int32_t tile, tileWhole, stream;
+};
+// total: blocks of all tiles of a key head, those of streams among tiles counted a quarter; full: tiles that are more than a few rows.
+__host__ __device__ inline PartBlocks partBlocks(const AttentionPlan &p, float total, float full, int32_t KVH) {
+    const float all = total * (float)KVH * 1.001f;  // sums of 32 bits
+    const int32_t part = (int32_t)fminf(ceilf(all / (float)p.items), 1e8f), whole = (int32_t)fminf(ceilf(all / (float)p.whole), 1e8f);
+    const int32_t least = full * (float)KVH < 128.0f ? p.fewBlocks : p.minBlocks;
+    return {part > least ? part : least, whole > least ? whole : least, 4 * part > p.fewBlocks ? 4 * part : p.fewBlocks};
+}
+// Parts of a run.
+__host__ __device__ inline int32_t partsOf(const AttentionPlan &p, int32_t blocks, int32_t part, int32_t whole) {
+    if (!p.splits || blocks <= part || blocks <= whole) return 1;
+    const int32_t parts = (int32_t)(((uint32_t)blocks + (uint32_t)part - 1) / (uint32_t)part);
+    return parts < p.maxParts ? parts : p.maxParts;
+}
+// capacity: positions that a sequence can have; quantised: the cache is int8 (for the launch only, what is asked of a workspace is the same)
+inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks,
+                                   bool quantised = false) {
     AttentionPlan p;
     const int64_t G = H / KVH, rows = T * G;  // of one key head
     // Streams read a sequence's keys once for every 16 of its rows, tiles once for 128, at the rate of one wave's row block.  With 32 rows a sequence both
@@ -75,11 +98,18 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     p.fine = T * H < 8192;
     p.rowsLog = p.tiles ? 7 : 4;
     p.keysLog = p.tiles && D <= 64 ? 6 : 5;
-    // Tiles: a part's results are 34 (heads of 64) to 133 KB that are written, read and joined.  So runs are cut only where some CUs would have one
-    // workgroup and others two (384 tiles: four chunks of up to 512 tokens, 32 heads of 128, over up to 8192 positions: 298 us whole, 213 in
-    // parts then, 189 now), and in parts of 2048 positions or more (parts of 512 cost a prompt of 2048 tokens with 16 heads of 128 another 13 us, with a
-    // window of 512 another 28); in shorter ones where full tiles leave half the CUs without any.
+    // Tiles: a part's results are 34 (heads of 64) to 133 KB that are written, read and joined.  So parts are of 2048 positions or more (parts of 512 cost
+    // a prompt of 2048 tokens with 16 heads of 128 another 13 us, with a window of 512 another 28), shorter where full tiles leave half the CUs without any;
+    // and a run is cut only if it is longer than the launch's blocks shared out over `whole` tiles, half of those that are on the chip at once (three
+    // workgroups a CU, two with bf16 heads of 256): runs that are alike are cut where their halves still go all at once.  us, whole / cut, runs of 8192
+    // positions, 32 heads of 128 over 8: 264 tiles 309 / 214, 384 322 / 239, 432 322 / 338, 480 322 / 340; 16 heads of 256 over 4: 176 502 / 365,
+    // 264 508 / 563, 320 515 / 564; int8, of which one workgroup of heads of 256 has a CU: 192 654 / 681, 264 1207 / 1030, 360 1227 / 1036.  A third of the
+    // tiles with runs of 16384 and two thirds of 4096: 384 tiles 533 / 249, 720 553 / 410; heads of 256, 264 981 / 489, 512 989 / 686.
+    // Streams cost less to join and are cut wherever they are longer than their share: a token for each of 72 sequences, eight heads of 128, one of 32768
+    // positions and the others of 200: 457 / 40; all of up to 4096: 171 / 172.  That a table has room for long runs costs where there is none (256
+    // sequences of up to 128 positions, a table for 32768: 32 / 37).
     p.items = p.tiles ? 512 : 1024;
+    p.whole = D > 128 && !quantised ? 260 : 390;
     p.maxParts = p.tiles ? 16 : 64;
     const int64_t keys = p.keys();
     const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
@@ -94,8 +124,10 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     p.fewBlocks = p.tiles ? (int32_t)(256 / keys) : p.minBlocks;
     int64_t parts = (blocks + p.fewBlocks - 1) / p.fewBlocks;
     if (parts > p.maxParts) parts = p.maxParts;
-    p.splits = parts > 1 && most <= (p.tiles ? 384 : p.items / 2);
-    p.grid = p.splits ? (most * parts < most + 2 * p.items ? most * parts : most + 2 * p.items) : most;
+    // What is cut is settled on the device, where the lengths are.  (With more tiles than this sums of their parts might pass 31 bits where starts
+    // do not ascend.)
+    p.splits = parts > 1 && most <= 65536;
+    p.grid = p.splits ? (most * parts < most + p.items ? most * parts : most + p.items) : most;
     p.slots = p.splits ? (p.grid < 2 * p.items ? p.grid : 2 * p.items) : 0;
     p.kvh = makeFastDiv((uint32_t)KVH);
     return p;

@@ -41,10 +41,11 @@ struct SeqWork {
 };
 __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const AttentionPlan &p, int s) {
     const CacheArgs &c = a.c;
-    SeqWork w{0, 0, 0, 0, 0, 0};
-    if (s >= c.S) return w;
-    rowsOf(c, c.starts, s, &w.begin, &w.count);
-    w.first = firstPosition(c, s, w.count);
+    SeqWork w;
+    const int there = min(s, c.S - 1);  // without a branch: of several sequences the loads go out together
+    rowsOf(c, c.starts, there, &w.begin, &w.count);
+    w.first = firstPosition(c, there, w.count);
+    if (s >= c.S) w.count = 0;
     w.length = c.pages ? min(w.first + w.count, c.capacity) : w.count;
     w.tiles = (int)(((uint32_t)w.count * (uint32_t)a.G + (uint32_t)p.rows() - 1) >> p.rowsLog);
     w.blocks = (int)(((uint32_t)w.length + (uint32_t)p.keys() - 1) >> p.keysLog);
@@ -77,27 +78,11 @@ constexpr int kFewRows = 16;  // a stream's
 // Among tiles, a sequence with few rows goes as a stream does, four blocks at once.
 __device__ __forceinline__ bool goesByStream(const AttentionArgs &a, int count) { return a.c.pages && a.c.D <= 128 && count * a.G <= kFewRows; }
 
-// Blocks that a part has at least, of a tile and of a stream among tiles: so many that about p.items parts come of all that the tiles can see, given
-// for the first 64 sequences in `mine`; and no fewer than the plan says, which is fewer where full tiles leave half the CUs without any.
-// The same for every wave; a float that does not hold a sum makes it more.
-struct PartBlocks {
-    int tile, stream;
-};
-__device__ __forceinline__ PartBlocks blocksOfPart(const AttentionArgs &a, const AttentionPlan &p, const SeqWork &mine) {
-    float total = 0.0f, full = 0.0f;  // blocks; tiles of more than a few rows
-    SeqWork w = mine;
-    for (int base = 0;;) {
-        const bool light = p.tiles && goesByStream(a, w.count);
-        total += (float)w.tiles * (float)w.blocks * (light ? 0.25f : 1.0f);
-        if (w.count * a.G > kFewRows) full += (float)w.tiles;
-        base += 64;
-        if (base >= a.c.S) break;
-        w = measureSeq(a, p, base + (threadIdx.x & 63));
-    }
-    total = sumOfWave(total);
-    full = sumOfWave(full);
-    const int part = (int)fminf(ceilf(total * (float)a.c.KVH * 1.001f / (float)p.items), 1e8f);
-    return {max(part, full * (float)a.c.KVH < 128.0f ? p.fewBlocks : p.minBlocks), max(4 * part, p.fewBlocks)};
+// A sequence's part of what blocksOfPart is made of: blocks, and tiles of more than a few rows.
+__device__ __forceinline__ void addWork(const AttentionArgs &a, const AttentionPlan &p, const SeqWork &w, float *total, float *full) {
+    const bool light = p.tiles && goesByStream(a, w.count);
+    *total += (float)w.tiles * (float)w.blocks * (light ? 0.25f : 1.0f);
+    if (w.count * a.G > kFewRows) *full += (float)w.tiles;
 }
 
 struct Item {
@@ -106,20 +91,93 @@ struct Item {
     int slot;  // of its partial result; -1: the item is its rows' only one
 };
 
+// Items of a sequence, and those of them that are parts.
+__device__ __forceinline__ int itemsOf(const AttentionArgs &a, const AttentionPlan &p, const PartBlocks &part, const SeqWork &w, int *splits, int *cut) {
+    const bool light = p.tiles && goesByStream(a, w.count);
+    *splits = partsOf(p, w.blocks, light ? part.stream : part.tile, light ? 0 : part.tileWhole);
+    const int mine = w.tiles * *splits * a.c.KVH;
+    *cut = *splits > 1 ? mine : 0;
+    return mine;
+}
+
+// What a workgroup has in LDS while it looks for its item among more than 64 sequences.
+struct Survey {
+    float total[4], full[4];   // of each wave's
+    int items[64], parts[64];  // of each group of sequences
+};
+constexpr int kManyItems = 1 << 24;  // more than a launch with parts has: where sums stop that starts which do not ascend make too large
+
 // Item `index` of the launch.  Items lie sequence by sequence, a sequence's last tiles, which see most, first; key heads are next to one another, so
-// that workgroups of one XCD (every eighth) read the same keys where there are eight heads.  False: there is none.
-__device__ __forceinline__ bool findItem(const AttentionArgs &a, const AttentionPlan &p, int index, Item *out) {
-    const int lane = threadIdx.x & 63;
-    SeqWork w = measureSeq(a, p, lane);
-    const PartBlocks part = p.splits ? blocksOfPart(a, p, w) : PartBlocks{0x7fffffff, 0x7fffffff};
-    int items = 0, slots = 0;
-    for (int base = 0;;) {
-        int splits = 1;
-        const int own = p.tiles && goesByStream(a, w.count) ? part.stream : part.tile;
-        if (p.splits && w.blocks > own) splits = min(p.maxParts, (int)(((uint32_t)w.blocks + (uint32_t)own - 1) / (uint32_t)own));
-        const int mine = w.tiles * splits * a.c.KVH, cut = splits > 1 ? mine : 0;
-        const int before = items + sumUpTo(mine) - mine, cutBefore = p.splits ? slots + sumUpTo(cut) - cut : 0;
-        const uint64_t found = __ballot(mine > 0 && before <= index && index < before + mine);
+// that workgroups of one XCD (every eighth) read the same keys where there are eight heads.  Every wave of the workgroup comes to the same; false: there is
+// none.  room: LDS, of which nothing is kept.
+//
+// A lane takes a sequence.  Of up to 64 each wave sums up all of them.  Of more the four waves share the sums, first the blocks, which the parts' length
+// is made of, then the items of up to 64 groups; each goes on in the group that has its item.  A token for each of 1024 sequences of up to 128 positions,
+// eight heads of 128: 121 us; with each wave going through all of them, 64 at a time, 148.
+__device__ __forceinline__ bool findItem(const AttentionArgs &a, const AttentionPlan &p, int index, Item *out, void *room) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), S = a.c.S;
+    PartBlocks part{0, 0, 0};
+    int base = 0, end = S, before = 0, partsBefore = 0;  // sequences to look through, and what lies before them
+    SeqWork w;
+    if (S <= 64) {
+        w = measureSeq(a, p, lane);
+        if (p.splits) {
+            float total = 0.0f, full = 0.0f;
+            addWork(a, p, w, &total, &full);
+            part = partBlocks(p, sumOfWave(total), sumOfWave(full), a.c.KVH);
+        }
+    } else {
+        Survey *const held = (Survey *)room;
+        const SeqWork own = measureSeq(a, p, threadIdx.x);  // in both sums
+        if (p.splits) {
+            float total = 0.0f, full = 0.0f;
+            addWork(a, p, own, &total, &full);
+#pragma unroll 4
+            for (int s = threadIdx.x + 256; s < S; s += 256) addWork(a, p, measureSeq(a, p, s), &total, &full);
+            total = sumOfWave(total);
+            full = sumOfWave(full);
+            if (lane == 0) {
+                held->total[wave] = total;
+                held->full[wave] = full;
+            }
+            __syncthreads();
+            part = partBlocks(p, held->total[0] + held->total[1] + held->total[2] + held->total[3], held->full[0] + held->full[1] + held->full[2] + held->full[3], a.c.KVH);
+        }
+        const int group = 64 * ((S - 1) / (64 * 64) + 1), groups = (S - 1) / group + 1;
+        for (int g = wave; g < groups; g += 4) {
+            int items = 0, parts = 0;
+            for (int s = g * group; s < min((g + 1) * group, S); s += 64) {
+                int splits, cut;
+                const SeqWork one = s + lane == (int)threadIdx.x ? own : measureSeq(a, p, s + lane);
+                items += __builtin_amdgcn_readlane(sumUpTo(itemsOf(a, p, part, one, &splits, &cut)), 63);
+                if (p.splits) {
+                    parts += __builtin_amdgcn_readlane(sumUpTo(cut), 63);
+                    items = min(items, kManyItems);
+                    parts = min(parts, kManyItems);
+                }
+            }
+            if (lane == 0) {
+                held->items[g] = items;
+                held->parts[g] = parts;
+            }
+        }
+        __syncthreads();
+        const int items = lane < groups ? held->items[lane] : 0, parts = lane < groups ? held->parts[lane] : 0;
+        const int upTo = sumUpTo(items), partsUpTo = sumUpTo(parts);
+        const uint64_t found = __ballot(upTo - items <= index && index < upTo);
+        __syncthreads();
+        if (!found) return false;
+        const int g = __builtin_ctzll(found);
+        before = __builtin_amdgcn_readlane(upTo - items, g);
+        partsBefore = __builtin_amdgcn_readlane(partsUpTo - parts, g);
+        base = g * group;
+        end = min(base + group, S);
+        w = measureSeq(a, p, base + lane);
+    }
+    for (;;) {
+        int splits, cut;
+        const int mine = itemsOf(a, p, part, w, &splits, &cut), upTo = sumUpTo(mine), cutUpTo = p.splits ? sumUpTo(cut) : 0, at = index - before;
+        const uint64_t found = __ballot(upTo - mine <= at && at < upTo);
         if (found) {
             const int l = __builtin_ctzll(found);
             out->w.begin = __builtin_amdgcn_readlane(w.begin, l);
@@ -130,7 +188,7 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
             out->w.blocks = __builtin_amdgcn_readlane(w.blocks, l);
             out->seq = base + l;
             out->splits = __builtin_amdgcn_readlane(splits, l);
-            const uint32_t local = (uint32_t)(index - __builtin_amdgcn_readlane(before, l));
+            const uint32_t local = (uint32_t)(at - __builtin_amdgcn_readlane(upTo - mine, l));
             uint32_t rest = fastDiv(local, p.kvh);
             out->head = (int)(local - rest * (uint32_t)a.c.KVH);
             out->split = out->part = 0;
@@ -140,7 +198,7 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
                 out->split = (int)(rest - tile * (uint32_t)out->splits);
                 rest = tile;
                 out->part = (int)(((uint32_t)out->w.blocks + (uint32_t)out->splits - 1) / (uint32_t)out->splits);
-                out->slot = __builtin_amdgcn_readlane(cutBefore, l) + (int)local;
+                out->slot = partsBefore + __builtin_amdgcn_readlane(cutUpTo - cut, l) + (int)local;
             }
             out->tile = out->w.tiles - 1 - (int)rest;
             // starts that do not ascend may make more of them: a run whose parts would not all have a place, or a workgroup, is left out whole, or its
@@ -148,10 +206,11 @@ __device__ __forceinline__ bool findItem(const AttentionArgs &a, const Attention
             const int behind = (out->splits - 1 - out->split) * a.c.KVH;
             return out->splits == 1 || (out->slot + behind < p.slots && (int64_t)index + behind < p.grid);
         }
+        const int these = __builtin_amdgcn_readlane(upTo, 63);
         base += 64;
-        if (base >= a.c.S) return false;
-        items = __builtin_amdgcn_readlane(before + mine, 63);
-        slots = __builtin_amdgcn_readlane(cutBefore + cut, 63);
+        if (base >= end || at < these) return false;  // the second: sums that are too large
+        before += these;
+        partsBefore += __builtin_amdgcn_readlane(cutUpTo, 63);
         w = measureSeq(a, p, base + lane);
     }
 }
@@ -787,7 +846,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const CacheArgs &c = a.c;
     Item it;
-    if (!findItem(a, p, blockIdx.x, &it)) return;
+    if (!findItem(a, p, blockIdx.x, &it, smem)) return;
     // single tokens among prompts: a tile would have one wave at work, and that for one row of 32 in its products
     if constexpr (PAGED && DT <= 128) {
         if (goesByStream(a, it.w.count)) {
@@ -1149,8 +1208,9 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
 
 template <int DT, bool EXACT, bool PAGED, bool Q8>
 __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_stream(AttentionArgs a, AttentionPlan p) {
+    extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     Item it;
-    if (findItem(a, p, blockIdx.x, &it)) streamItem<DT, EXACT, PAGED, Q8>(a, p, it);
+    if (findItem(a, p, blockIdx.x, &it, smem)) streamItem<DT, EXACT, PAGED, Q8>(a, p, it);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------
@@ -1220,7 +1280,7 @@ static hipError_t byHeadDim(const AttentionArgs &a, const AttentionPlan &p, cons
 
 hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx) {
     if (hipError_t e = checkAttention(a)) return e;
-    const AttentionPlan p = attentionPlan(a.c.T, a.c.S, a.H, a.c.KVH, a.c.D, a.c.pages ? a.c.capacity : a.c.T, a.window, a.sinks);
+    const AttentionPlan p = attentionPlan(a.c.T, a.c.S, a.H, a.c.KVH, a.c.D, a.c.pages ? a.c.capacity : a.c.T, a.window, a.sinks, a.key_scales != nullptr);
     return !a.c.pages ? byHeadDim<false, false>(a, p, ctx) : a.key_scales ? byHeadDim<true, true>(a, p, ctx) : byHeadDim<true, false>(a, p, ctx);
 }
 
