@@ -61,7 +61,7 @@ static bool check(const std::vector<Seq> &seqs, int64_t KVH, int64_t G, int64_t 
     }
     if (made->items > p.grid || made->parts > p.slots) return false;
     const uint64_t bytes = attentionWorkspaceBytes(T, S, H, KVH, D, capacity, window, sinks);
-    return p.slots == 0 ? bytes == 0 : bytes >= (uint64_t)p.slots * ((uint64_t)p.rows() * (uint64_t)(D + 4) * 4 + 4);
+    return p.slots == 0 ? bytes == 0 : (uint64_t)p.slots * 4 <= kAttentionCounterBytes && bytes >= kAttentionCounterBytes + (uint64_t)p.slots * (uint64_t)(p.rows() * (D + 4) * 4);
 }
 
 int main(int argc, char **argv) {

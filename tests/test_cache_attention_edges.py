@@ -339,3 +339,44 @@ def test_gpu_after_many_starts_that_do_not_ascend(device, case):
         for p in ptrs:
             device.free(p)
         exe.close()
+
+
+def _two_attentions(quantised=False):
+    """A program of attentions of other sizes, two of which are cut into parts (tiles of heads of 128, then streams of heads of 64 with more parts), and the first
+    once more behind the others."""
+    big = Batch([(300, 3000), (1, 900)], D=128, H=4, KVH=1, page=64, quantised=quantised, seed=1)
+    few = Batch([(1, 2500), (2, 1900), (1, 30)], D=64, H=8, KVH=4, page=16, quantised=quantised, seed=2)
+    none = Batch([(9, 40)], D=64, H=2, KVH=1, page=16, quantised=quantised, seed=3)
+    built, wants = Built(), []
+    for i, b in enumerate((big, few, none, big)):
+        q, out = built.bind("query%d" % i, b.query), b.normal(b.T, b.H, b.D)
+        k, v = built.bind("k%d" % i, b.caches[0]), built.bind("v%d" % i, b.caches[1])
+        scales = dict(key_scales=built.bind("ks%d" % i, b.scales[0]), value_scales=built.bind("vs%d" % i, b.scales[1]))
+        built.program.paged_attention(q, k, v, built.bind("p%d" % i, b.pages), built.bind("s%d" % i, b.starts), built.bind("l%d" % i, b.lengths), scale=b.scale,
+                                      init=built.bind("out%d" % i, out), **scales)
+        wants.append((b, out))
+    return built, wants
+
+
+def test_attentions_of_a_program_have_one_workspace():
+    built, _ = _two_attentions()
+    d = desc_interp.Descriptor(built.program.serialize())
+    refs = [tuple(o["in1"].tolist()) for o in d.ops]
+    assert refs[0] == refs[1] == refs[3] and refs[0][0] == 2 and refs[2][0] == 0 and len(d.temps) == 1
+    alone = [Built(), Built()]
+    sizes = []
+    for built, case in zip(alone, (dict(sequences=[(300, 3000), (1, 900)], D=128, H=4, KVH=1, page=64), dict(sequences=[(1, 2500), (2, 1900), (1, 30)], D=64, H=8, KVH=4))):
+        sizes.append(int(desc_interp.Descriptor(attend(Batch(**case), True)[0].program.serialize()).temps["size"][0]))
+    assert int(d.temps["size"][0]) == max(sizes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+def test_gpu_attentions_one_after_another_in_one_workspace(device, quantised):
+    built, wants = _two_attentions(quantised)
+    first = built.run(device)
+    for i, (b, out) in enumerate(wants):
+        check_attention(b, first["out%d" % i], out, ref.attention(b.query, b.starts, b.scale, cache=b.cache(), lengths=b.lengths), str(i))
+    again = built.run(device, dispatches=4)  # replayed as a graph from the second on
+    for name in first:
+        assert np.array_equal(first[name], again[name], equal_nan=first[name].dtype == np.float32), name

@@ -133,11 +133,13 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     return p;
 }
 
-// Bytes of partial results that a launch of these sizes may keep: for each row of a slot D sums, a maximum and a sum of weights; and a counter for each
-// slot, 0 before and after every launch.
+// Bytes of partial results that a launch of these sizes may keep: a counter for each slot, 0 before and after every launch, and behind the counters of as
+// many slots as there can be, for each row of a slot D sums, a maximum and a sum of weights.  The counters lie alike whatever the sizes are: launches that
+// follow one another have one workspace, as long as the longest.
+constexpr uint64_t kAttentionCounterBytes = 4 * 2 * 1024;
 inline uint64_t attentionWorkspaceBytes(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
     const AttentionPlan p = attentionPlan(T, S, H, KVH, D, capacity, window, sinks);
-    return (uint64_t)p.slots * ((uint64_t)p.rows() * (uint64_t)(D + 4) * 4 + 4);
+    return p.slots ? kAttentionCounterBytes + (uint64_t)p.slots * (uint64_t)p.rows() * (uint64_t)(D + 4) * 4 : 0;
 }
 
 }  // namespace thip

@@ -267,7 +267,7 @@ __device__ __forceinline__ int keyRow(const AttentionArgs &a, const Item &it, co
 // different XCDs, past the caches, by loads and stores at the device's scope (a fence would write the XCD's whole L2 back).
 constexpr int kDeviceScope = 16;  // sc1
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t slotsOf(const AttentionArgs &a, const AttentionPlan &p) {
-    return __builtin_amdgcn_make_buffer_rsrc(a.work, 0, (int)((uint32_t)p.slots * (uint32_t)p.rows() * (uint32_t)(a.c.D + 4) * 4u), 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc(a.work + kAttentionCounterBytes, 0, (int)((uint32_t)p.slots * (uint32_t)p.rows() * (uint32_t)(a.c.D + 4) * 4u), 0x00020000);
 }
 __device__ __forceinline__ uint32_t slotRow(const AttentionArgs &a, const AttentionPlan &p, int slot, int r) {
     return (((uint32_t)slot << p.rowsLog) + (uint32_t)r) * (uint32_t)(a.c.D + 4) * 4u;
@@ -306,7 +306,7 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     constexpr int LANES = 256 / ROWS, EACH = PARTS / LANES;  // threads of a row, and parts of each
     const int tid = threadIdx.x, D = a.c.D, first = it.slot - it.split * a.c.KVH;
     const auto slots = slotsOf(a, p);
-    uint32_t *const counter = (uint32_t *)(a.work + slotRow(a, p, (int)p.slots, 0)) + first;
+    uint32_t *const counter = (uint32_t *)a.work + first;
     int *const last = (int *)room;
     float *const factors = room + 1, *const totals = factors + ROWS * PARTS;
     waitVmcnt<0>();  // this wave's part is where the others will look
@@ -1237,7 +1237,7 @@ constexpr size_t streamLds(int DT, bool Q8) {
 
 template <int DT, bool PAGED, bool Q8>
 static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &p, const LaunchCtx &ctx) {
-    if (p.grid > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (p.grid > 0x7fffffffLL || p.slots * 4 > (int64_t)kAttentionCounterBytes) return hipErrorInvalidValue;
     const dim3 grid((unsigned)p.grid);
     if (p.tiles) {
         constexpr int KB = DT >= 128 ? 32 : 64;

@@ -109,7 +109,7 @@ enum Kind : uint32_t {
     kKindCacheWrite = 17,
     kKindCacheRead = 18,
     // in0 = query, out, bias0 = float bits of the scale, K = window, Kp = sinks, w0 = 1: over a cache (0: over the rows, no CacheExt),
-    // in1 = an intermediate of the record's own for partial results (attentionWorkspaceBytes; none where that is 0)
+    // in1 = an intermediate for partial results, which only attention records have, one for all of a program (attentionWorkspaceBytes; none where that is 0)
     kKindAttention = 19,
 };
 

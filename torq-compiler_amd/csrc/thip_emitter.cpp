@@ -717,8 +717,8 @@ class Emitter {
     thip_status_t emitUnary(const thip_hl_elementwiseunary_t &c);
     thip_status_t emitShift(const thip_hl_elementwiseshift_t &c);
     thip_status_t emitTable(const thip_hl_table_t &c, const std::vector<int32_t> &staticTable);
-    // Operands of an integer elementwise op: element types, and the record's common fields.
     // Attention and its cache (thip_lm_*).
+    DescRef attentionWork_{kSpaceNone, 0, 0};
     bool shareBytes(thip_value_t a, thip_value_t b) const;
     thip_status_t boundPart(thip_value_t id, const char *what, int32_t dtype, int32_t rank, bool written, DescRef *out);
     thip_status_t indexOperand(thip_value_t id, const char *what, int32_t rank, DescRef *out);
@@ -728,6 +728,7 @@ class Emitter {
     thip_status_t emitCacheWrite(const thip_lm_cache_write_t &c);
     thip_status_t emitCacheRead(const thip_lm_cache_read_t &c);
     thip_status_t emitAttention(const thip_lm_attention_t &c);
+    // Operands of an integer elementwise op: element types, and the record's common fields.
     thip_status_t eltwiseCommon(const char *what, thip_value_t input, thip_value_t init, DescOp *op);
     thip_status_t emitAvgPoolBf16(const thip_hl_avg_pool2d_t &c);
     // ---- decode-shaped bf16 programs (at most 32 rows per matmul): fewer, wider launches -----------------------
@@ -2191,7 +2192,12 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
         all.push_back({op.bias, (uint64_t)T * op.W * D * 2, false, "value"});
     }
     if (thip_status_t s = checkApart(all)) return s;
-    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T, op.K, op.Kp)) op.in1 = newTemp(work);
+    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T, op.K, op.Kp)) {
+        // records run one after another: they have one workspace, as long as the longest of them needs
+        if (attentionWork_.space == kSpaceNone) attentionWork_ = newTemp(0);
+        temps_[attentionWork_.index] = std::max(temps_[attentionWork_.index], work);
+        op.in1 = attentionWork_;
+    }
     ops_.push_back(op);
     return THIP_OK;
 }
