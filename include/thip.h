@@ -403,7 +403,12 @@ thip_status_t thip_hl_elementwisebinary(thip_program_t *program, const thip_hl_e
 /* ---- Attention and its cache -------------------------------------------------------------------------------------
  * Operators that no TorqHL op stands for (the reference has neither a softmax nor a cache): what a decoder needs
  * between its linears.  Element types: queries, keys, values and results BF16; a cache BF16, or I8 with one F32 scale
- * for each position and head.  Sums, softmax statistics and scores are held in 32 bits.
+ * for each position and head.  Sums, softmax statistics and scores are held in 32 bits.  A softmax weight meets its
+ * value as two bf16, one and what it leaves (an error of 2^-16 of it), but rounded once to bf16 (2^-8) in records of
+ * T * heads >= 8192 rows, those of no sequence among them, that have more than 32 rows of a key head for each sequence
+ * (T * heads / kv_heads > 32 S), for sequences of more than 16 such rows (for all where D is above 128, or without a
+ * cache).  Which of the two, and the order of sums, follow from the operands' sizes and the lengths: the same call gives
+ * the same bits, a padded or differently batched one may differ by these roundings.
  *
  * Rows are packed: a tensor of T rows holds those of S sequences one behind the other.  row_starts is I32[S + 1],
  * ascending: sequence s has the n_s rows row_starts[s] .. row_starts[s + 1] - 1.  Rows behind the last sequence's are
@@ -458,7 +463,8 @@ typedef struct thip_lm_cache_read_t {
  * (window == 0, or j > p - window, or j < sinks):
  *     init = sum_j w_j value_j / sum_j w_j,  w_j = exp(scale * (query . key_j) - max over the seen ones),
  * and zeros where it sees nothing.  What lies at positions that a row does not see has no influence on it, whatever its
- * bits.  Either over the rows themselves -- key and value [T, kv_heads, D], pages and lengths THIP_NO_VALUE: row i of
+ * bits.  (Rows that see a NaN or an infinity, or have one masked next to what they see, are done a second time, key by
+ * key: right, but slow where there are many.)  Either over the rows themselves -- key and value [T, kv_heads, D], pages and lengths THIP_NO_VALUE: row i of
  * a sequence stands at position i, a prompt without a cache -- or over a cache, where key and value are the caches
  * (and key_scales, value_scales those of an I8 cache) and the new rows' keys and values are there already (thip_lm_cache_write
  * before it).  init may be the query's own bytes; no other operand may share bytes with init. */

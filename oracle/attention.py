@@ -90,14 +90,17 @@ def cache_read(cache, key, value, row_starts, lengths):
     return out
 
 
-def attention(query, row_starts, scale, window=0, sinks=0, key=None, value=None, cache=None, lengths=None):
+def attention(query, row_starts, scale, window=0, sinks=0, key=None, value=None, cache=None, lengths=None, fine=False, rounded=False):
     """(result, bound) of each row and head [T, heads, D] in 64 bits, NaN in the result of rows that are no sequence's.
 
     bound: how far a bf16 result may be that is computed as the definition says with sums, scores and statistics in 32 bits and weights
     rounded to bf16 before they meet the values.  With a half step of h16 = 2^-8 (bf16) and h32 = 2^-24: the weights' rounding moves the result by at
     most h16 A, A = sum w |v| / sum w; the result's own by h16 |o|; a score of D products summed in 32 bits, scaled and taken off the maximum, is off by
     at most e = (D + 4) h32 scale sum |q k| + 4 h32 (|s| + |m|), each weight by a factor of 1 + e + 4 h32 (the exponential), numerator and
-    denominator by that and n h32 for sums of n: 2 (e + 4 h32 + n h32) A in all; 5 % for their products."""
+    denominator by that and n h32 for sums of n: 2 (e + 4 h32 + n h32) A in all; 5 % for their products.
+    fine: weights (of int8, times the value's scale: another h32) go in as two bf16, one and what it leaves, which is off by h16 of at most h16: h16^2 A in
+    place of h16 A.
+    rounded: the result itself is of weights that are rounded to bf16 once, to see that a bound tells the two apart."""
     q = from_bf16(query)
     T, H, D = q.shape
     out, bound = np.full((T, H, D), np.nan), np.zeros((T, H, D))
@@ -127,8 +130,10 @@ def attention(query, row_starts, scale, window=0, sinks=0, key=None, value=None,
                 m = np.max(x)
                 w = np.exp(x - (m if m != -np.inf else 0.0))
                 total = w.sum()
+                if rounded:
+                    w = from_bf16(to_bf16(w.astype(np.float32)))
                 out[row, h] = w @ v / total if total != 0 else 0.0
                 A = w @ np.abs(v) / total if total != 0 else np.zeros(D)
                 off = (D + 4) * h32 * scale * np.max(np.abs(k) @ np.abs(q[row, h])) + 4 * h32 * 2 * np.max(np.abs(x))
-                bound[row, h] = 1.05 * (h16 * np.abs(out[row, h]) + A * (h16 + 2 * (off + 4 * h32 + len(x) * h32))) + 1e-38
+                bound[row, h] = 1.05 * (h16 * np.abs(out[row, h]) + A * ((h16 * h16 + h32 if fine else h16) + 2 * (off + 4 * h32 + len(x) * h32))) + 1e-38
     return out, bound

@@ -380,3 +380,60 @@ def test_gpu_attentions_one_after_another_in_one_workspace(device, quantised):
     again = built.run(device, dispatches=4)  # replayed as a graph from the second on
     for name in first:
         assert np.array_equal(first[name], again[name], equal_nan=first[name].dtype == np.float32), name
+
+
+# ---- weights in two parts -----------------------------------------------------------------------------------------------
+
+FINE = [
+    dict(sequences=[(1, 3), (2, 5), (1, 9), (3, 40), (1, 2)], D=64, H=8, KVH=2, page=16),     # streams
+    dict(sequences=[(1, 6), (2, 4), (4, 700)], D=128, H=8, KVH=2, page=16),
+    dict(sequences=[(1, 7), (3, 3)], D=256, H=16, KVH=4, page=16),
+    dict(sequences=[(70, 75), (40, 40)], D=64, H=4, KVH=2, page=16),                          # tiles of few rows
+    dict(sequences=[(50, 55), (1, 5), (60, 900)], D=128, H=8, KVH=2, page=16),
+    dict(sequences=[(140, 140)], D=256, H=16, KVH=1, page=16),
+    dict(sequences=[(300, 300), (1, 4), (250, 300)], D=64, H=16, KVH=8, page=16),             # as one, but for the sequence of one row
+]
+
+
+def _few_keys(b):
+    """Keys so small that the first rows' weights are alike: results there are sums of a few values, some next to nothing."""
+    b.caches[0] = (b.caches[0] // 40).astype(np.int8) if b.quantised else ref.to_bf16((ref.from_bf16(b.caches[0]) / 40).astype(np.float32))
+    b.key = ref.to_bf16((ref.from_bf16(b.key) / 40).astype(np.float32))
+
+
+def _is_fine(b, cached):
+    """Rows whose weights meet the values in two parts, as the header says."""
+    G = b.H // b.KVH
+    once = b.T * b.H >= 8192 and b.T * G > 32 * len(b.sequences)
+    fine = np.ones(b.T, dtype=bool)
+    for s, (n, _) in enumerate(b.sequences):
+        fine[b.starts[s]:b.starts[s + 1]] = not once or (cached and n * G <= 16 and b.D <= 128)
+    return fine
+
+
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("case", FINE[:6], ids=_id)
+def test_the_bound_tells_weights_rounded_once(case, quantised):
+    b = Batch(quantised=quantised, **case)
+    _few_keys(b)
+    over = dict(cache=b.cache(), lengths=b.lengths)
+    exact, bound = ref.attention(b.query, b.starts, b.scale, fine=True, **over)
+    once = ref.from_bf16(ref.to_bf16(ref.attention(b.query, b.starts, b.scale, rounded=True, **over)[0].astype(np.float32)))
+    plain = ref.from_bf16(ref.to_bf16(exact.astype(np.float32)))
+    assert (np.abs(once - exact) > bound).any() and (np.abs(plain - exact) <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keys", ["rows", "bf16", "int8"])
+@pytest.mark.parametrize("case", FINE, ids=_id)
+def test_gpu_weights_in_two_parts(device, case, keys):
+    b = Batch(quantised=keys == "int8", **case)
+    if keys == "rows":
+        b.lengths = np.array([n for n, _ in b.sequences], dtype=np.int32)
+    _few_keys(b)
+    built, before, (result, coarse) = attend(b, keys != "rows")
+    over = dict(cache=b.cache(), lengths=b.lengths) if keys != "rows" else dict(key=b.key, value=b.value)
+    bound = ref.attention(b.query, b.starts, b.scale, fine=True, **over)[1]
+    fine = _is_fine(b, keys != "rows")
+    assert fine.any() or (keys == "rows" and case is FINE[-1])  # without a cache nothing goes as a stream among tiles
+    check_attention(b, built.run(device)["out"], before, (result, np.where(fine[:, None, None], bound, coarse)))
