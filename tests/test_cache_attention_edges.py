@@ -437,3 +437,73 @@ def test_gpu_weights_in_two_parts(device, case, keys):
     fine = _is_fine(b, keys != "rows")
     assert fine.any() or (keys == "rows" and case is FINE[-1])  # without a cache nothing goes as a stream among tiles
     check_attention(b, built.run(device)["out"], before, (result, np.where(fine[:, None, None], bound, coarse)))
+
+
+# ---- a decoder's layers -------------------------------------------------------------------------------------------------
+
+def _layers(b, hidden, caches, expose, layers=2):
+    """Layers of grouped linears (int8 weights in blocks), a write into each layer's cache, attention over it, and the linear behind with the residual sum, in
+    one program; expose: queries, keys, values and what attention gave are bindings, else the program's own."""
+    rng = np.random.default_rng(17)
+    built = Built()
+    p, M = built.program, b.T
+    x = built.bind("x", ref.to_bf16(rng.standard_normal((M, hidden)).astype(np.float32)))
+    starts, lengths = built.rows(b)
+    pages = built.bind("pages", b.pages)
+    zero, noclamp = np.zeros(1, np.float32), dict(output_zp=0, output_min=w.NO_CLAMP[0], output_max=w.NO_CLAMP[1])
+    half = ref.to_bf16(np.array([0.70703125, 0.70703125], dtype=np.float32))
+
+    def linear(src, N, gain, init):
+        K = src.shape[1]
+        wq, scale, qbias = w._block_quantized(rng, K, N, 128, gain)
+        return p.matmul(src, p.expand_weights(wq, scale, qbias, block_size=128, output_min=w.NO_CLAMP[0], output_max=w.NO_CLAMP[1]), zero, init=init, shift=0, **noclamp)
+
+    def place(name, shape):
+        return built.bind(name, np.zeros(shape, U16)) if expose else p.tensor(shape, U16)
+
+    for i in range(layers):
+        names = ["%s%d" % (n, i) for n in ("query", "key", "value", "attended")]
+        q, k, v = (linear(x, h * b.D, 1.0, place(n, (M, h * b.D))) for n, h in zip(names, (b.H, b.KVH, b.KVH)))
+        q, k, v = (p.view(t, (M, h, b.D)) for t, h in zip((q, k, v), (b.H, b.KVH, b.KVH)))
+        cache = built.bind("key_cache%d" % i, caches[i][0]), built.bind("value_cache%d" % i, caches[i][1]), pages
+        scales = dict(key_scales=built.bind("key_scales%d" % i, caches[i][2]), value_scales=built.bind("value_scales%d" % i, caches[i][3]))
+        p.cache_write(k, v, *cache, starts, lengths, **scales)
+        y = p.paged_attention(q, *cache, starts, lengths, scale=b.scale, window=90, sinks=2, init=p.view(place(names[3], (M, b.H * b.D)), (M, b.H, b.D)), **scales)
+        o = linear(p.view(y, (M, b.H * b.D)), hidden, 1.0, p.tensor((M, hidden), U16))
+        last = i == layers - 1
+        x = p.add(x, o, half, zero, init=built.bind("out", np.zeros((M, hidden), U16)) if last else p.tensor((M, hidden), U16), shift_factor=0, **noclamp)
+    return built
+
+
+LAYERS = [dict(sequences=[(1, 1 + 13 * i) for i in range(7)], D=64, H=4, KVH=1, page=16), dict(sequences=[(1, 40 + 7 * i) for i in range(24)], D=128, H=4, KVH=2, page=16),
+          dict(sequences=[(3, 30), (1, 200), (2, 2)], D=256, H=4, KVH=1, page=32)]
+
+
+def test_a_layer_is_four_records():
+    b = Batch(**LAYERS[0])
+    caches = [b.caches + [None, None]] * 2
+    assert _kinds(_layers(b, 256, caches, False).program.serialize()) == [15, WRITE, ATTENTION, 15] * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("case", LAYERS, ids=_id)
+def test_gpu_layers_of_a_decoder(device, case, quantised):
+    """Each attention of the run is checked on the queries, keys and values that the linears gave it, each cache on what was written; the program with
+    intermediates of its own gives the same."""
+    b, hidden = Batch(quantised=quantised, **case), 256
+    other = Batch(quantised=quantised, seed=5, garbage=False, **case)  # the second layer's has the first one's pages
+    caches = [c.caches + list(c.scales) for c in (b, other)]
+    exposed = _layers(b, hidden, caches, True).run(device)
+    for i, start in enumerate((b, other)):
+        q, k, v, got = (exposed["%s%d" % (n, i)].reshape(b.T, -1, b.D) for n in ("query", "key", "value", "attended"))
+        cache = ref.Cache(start.caches[0], start.caches[1], b.pages, *start.scales)
+        written = ref.cache_write(cache, k, v, b.starts, b.lengths)
+        for name, x in zip(("key_cache", "value_cache", "key_scales", "value_scales"), written):
+            if x is not None:
+                assert np.array_equal(exposed["%s%d" % (name, i)], x, equal_nan=x.dtype == np.float32), (name, i)
+        cache = ref.Cache(written[0], written[1], b.pages, *written[2:])
+        want = ref.attention(q, b.starts, b.scale, window=90, sinks=2, cache=cache, lengths=b.lengths, fine=True)
+        check_attention(b, got, got, want, "layer %d" % i)
+    inside = _layers(b, hidden, caches, False).run(device, dispatches=3)
+    assert np.isfinite(ref.from_bf16(inside["out"])).all() and np.array_equal(inside["out"], exposed["out"])
