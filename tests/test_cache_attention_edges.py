@@ -1,6 +1,8 @@
 """Attention and its cache (thip_lm_*) where a row's result hangs on what is easily lost: numbers that are none, values next to the largest,
 positions at the ends of what 32 bits hold, batches of very unequal sequences, and the programs around the ops."""
 import ctypes
+import os
+import shutil
 import subprocess
 
 import numpy as np
@@ -507,3 +509,17 @@ def test_gpu_layers_of_a_decoder(device, case, quantised):
         check_attention(b, got, got, want, "layer %d" % i)
     inside = _layers(b, hidden, caches, False).run(device, dispatches=3)
     assert np.isfinite(ref.from_bf16(inside["out"])).all() and np.array_equal(inside["out"], exposed["out"])
+
+
+def test_programs_and_records_under_sanitizers(tmp_path):
+    """Random programs around a cache, and mutated copies of their descriptors, through the emitter and the validation built with the sanitizers."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    csrc, exe = os.path.join(root, "torq-compiler_amd", "csrc"), str(tmp_path / "attention_host")
+    built = subprocess.run([shutil.which("g++"), "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-static-libasan", "-fno-sanitize-recover=undefined", "-w",
+                            "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + csrc, os.path.join(root, "tests", "fuzz", "attention_host.cpp")] +
+                           [os.path.join(csrc, s) for s in ("thip_emitter.cpp", "thip_validate.cpp", "thip_status.cpp")] + ["-o", exe], stdout=subprocess.PIPE,
+                           stderr=subprocess.STDOUT, text=True)
+    assert built.returncode == 0, built.stdout[-3000:]
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:abort_on_error=0:verify_asan_link_order=0", UBSAN_OPTIONS="print_stacktrace=1")
+    done = subprocess.run([exe, "300", "1"], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env, timeout=300)
+    assert done.returncode == 0 and "runtime error" not in done.stdout and "AddressSanitizer" not in done.stdout, done.stdout[-4000:]
