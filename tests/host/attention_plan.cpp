@@ -53,6 +53,7 @@ static bool check(const std::vector<Seq> &seqs, int64_t KVH, int64_t G, int64_t 
     *made = Made{};
     for (int64_t s = 0; s < S; s++) {
         const int32_t n = partsOf(p, (int32_t)blocks[s], light[s] ? part.stream : part.tile, light[s] ? 0 : part.tileWhole);
+        if (p.splits && !p.tiles && blocks[s] > part.tile && n == 1) return false;  // streams are cut wherever they are longer than a part
         const int64_t each = (blocks[s] + n - 1) / n;
         if (n > 1 && (n > p.maxParts || each * n < blocks[s] || each < 1)) return false;
         made->items += tiles[s] * n * KVH;

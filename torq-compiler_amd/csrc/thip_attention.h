@@ -76,7 +76,7 @@ __host__ __device__ inline PartBlocks partBlocks(const AttentionPlan &p, float t
     const float all = total * (float)KVH * 1.001f;  // sums of 32 bits
     const int32_t part = (int32_t)fminf(ceilf(all / (float)p.items), 1e8f), whole = (int32_t)fminf(ceilf(all / (float)p.whole), 1e8f);
     const int32_t least = full * (float)KVH < 128.0f ? p.fewBlocks : p.minBlocks;
-    return {part > least ? part : least, whole > least ? whole : least, 4 * part > p.fewBlocks ? 4 * part : p.fewBlocks};
+    return {part > least ? part : least, p.tiles && whole > least ? whole : least, 4 * part > p.fewBlocks ? 4 * part : p.fewBlocks};
 }
 // Parts of a run.
 __host__ __device__ inline int32_t partsOf(const AttentionPlan &p, int32_t blocks, int32_t part, int32_t whole) {
@@ -106,7 +106,7 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // 264 508 / 563, 320 515 / 564; int8, of which one workgroup of heads of 256 has a CU: 192 654 / 681, 264 1207 / 1030, 360 1227 / 1036.  A third of the
     // tiles with runs of 16384 and two thirds of 4096: 384 tiles 533 / 249, 720 553 / 410; heads of 256, 264 981 / 489, 512 989 / 686.
     // Streams cost less to join and are cut wherever they are longer than their share: a token for each of 72 sequences, eight heads of 128, one of 32768
-    // positions and the others of 200: 457 / 40; all of up to 4096: 171 / 172.  That a table has room for long runs costs where there is none (256
+    // positions and the others of 200: 457 / 40; all of up to 4096: 171 / 166; 65 of up to 4096: 175 / 141.  That a table has room for long runs costs where there is none (256
     // sequences of up to 128 positions, a table for 32768: 32 / 37).
     p.items = p.tiles ? 512 : 1024;
     p.whole = D > 128 && !quantised ? 260 : 390;
