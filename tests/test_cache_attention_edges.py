@@ -523,3 +523,25 @@ def test_programs_and_records_under_sanitizers(tmp_path):
     env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:abort_on_error=0:verify_asan_link_order=0", UBSAN_OPTIONS="print_stacktrace=1")
     done = subprocess.run([exe, "300", "1"], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env, timeout=300)
     assert done.returncode == 0 and "runtime error" not in done.stdout and "AddressSanitizer" not in done.stdout, done.stdout[-4000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+def test_gpu_tables_that_are_constants(device, quantised):
+    """Starts, lengths and pages that a program carries itself, and tables that are parts of one binding."""
+    b = Batch([(1, 700), (40, 90), (0, 3), (2, 2)], D=64, H=4, KVH=2, page=16, quantised=quantised, tail=1)
+    want = ref.attention(b.query, b.starts, b.scale, cache=b.cache(), lengths=b.lengths)
+    S, P = b.pages.shape
+    for carried in (True, False):
+        built, out = Built(), b.normal(b.T, b.H, b.D)
+        q, p = built.bind("query", b.query), built.program
+        k, v = built.bind("key_cache", b.caches[0]), built.bind("value_cache", b.caches[1])
+        scales = dict(key_scales=built.bind("key_scales", b.scales[0]), value_scales=built.bind("value_scales", b.scales[1]))
+        if carried:
+            tables = b.pages, b.starts, b.lengths
+        else:
+            whole = built.bind("tables", np.concatenate([b.lengths, b.starts, b.pages.reshape(-1)]).astype(np.int32))
+            tables = p.view(whole, (S, P), 2 * S + 1), p.view(whole, (S + 1,), S), p.view(whole, (S,), 0)
+        p.paged_attention(q, k, v, *tables, scale=b.scale, init=built.bind("out", out), **scales)
+        for via in ("device", "host"):
+            check_attention(b, built.run(device, via)["out"], out, want, "%s %s" % (carried, via))
