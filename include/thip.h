@@ -464,7 +464,8 @@ typedef struct thip_lm_cache_read_t {
  *     init = sum_j w_j value_j / sum_j w_j,  w_j = exp(scale * (query . key_j) - max over the seen ones),
  * and zeros where it sees nothing.  What lies at positions that a row does not see has no influence on it, whatever its
  * bits.  (Rows that see a NaN or an infinity, or have one masked next to what they see, are done a second time, key by
- * key: right, but slow where there are many.)  Either over the rows themselves -- key and value [T, kv_heads, D], pages and lengths THIP_NO_VALUE: row i of
+ * key: right, but slow where there are many.)
+ * Either over the rows themselves -- key and value [T, kv_heads, D], pages and lengths THIP_NO_VALUE: row i of
  * a sequence stands at position i, a prompt without a cache -- or over a cache, where key and value are the caches
  * (and key_scales, value_scales those of an I8 cache) and the new rows' keys and values are there already (thip_lm_cache_write
  * before it).  init may be the query's own bytes; no other operand may share bytes with init. */

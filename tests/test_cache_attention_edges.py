@@ -545,3 +545,42 @@ def test_gpu_tables_that_are_constants(device, quantised):
         p.paged_attention(q, k, v, *tables, scale=b.scale, init=built.bind("out", out), **scales)
         for via in ("device", "host"):
             check_attention(b, built.run(device, via)["out"], out, want, "%s %s" % (carried, via))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keys", ["rows", "bf16", "int8"])
+@pytest.mark.parametrize("case", [dict(sequences=[(300, 300)], D=64, H=4, KVH=2), dict(sequences=[(90, 90), (5, 5)], D=256, H=2, KVH=1),
+                                  dict(sequences=[(60, 1500), (1, 900)], D=128, H=8, KVH=2)], ids=_id)
+def test_gpu_rows_of_nothing_but_nan(device, case, keys):
+    """Whole rows of NaN in keys or values, which every later row sees."""
+    if keys == "rows":  # prompts have no positions before their first row
+        case = dict(case, sequences=[(n, n) for n, _ in case["sequences"]])
+    for which in (0, 1):
+        b = Batch(quantised=keys == "int8", page=16, **case)
+        for s, (n, length) in enumerate(b.sequences):
+            for p in {2, 33, length - 2} & set(range(length)):
+                if keys == "rows":
+                    (b.key, b.value)[which][b.starts[s] + p] = 0x7FC0
+                elif keys == "int8":
+                    b.scales[which][b.pages[s, p // 16], :, p % 16] = np.nan
+                else:
+                    b.caches[which][b.pages[s, p // 16], :, p % 16] = 0x7FC0
+        for see in (dict(), dict(window=30, sinks=1)):
+            built, before, want = attend(b, keys != "rows", **see)
+            assert np.isnan(want[0]).any()
+            check_attention(b, built.run(device)["out"], before, want, "%d %s" % (which, see))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("later", [False, True], ids=["all", "first"])
+def test_gpu_values_behind_scores_of_minus_infinity(device, later):
+    """Keys that give scores of minus infinity, all of a row's or the first 100, one of them with a value of NaN: zeros where no weight is above 0, else NaN."""
+    b = Batch([(1, 200), (90, 120), (120, 120)], D=64, H=2, KVH=1, page=16)
+    b.query[:, :, 0] = 0x3F80
+    for s, (_, length) in enumerate(b.sequences):
+        for p in range(100 if later else length):
+            b.caches[0][b.pages[s, p // 16], 0, p % 16, 0] = 0xFF80
+        b.caches[1][b.pages[s, 2], 0, 3] = 0x7FC0
+    built, before, want = attend(b, True)
+    assert (want[0][b.starts[2] + 90] == 0).all() and (np.isnan(want[0][0]).all() if later else (want[0][0] == 0).all())
+    check_attention(b, built.run(device)["out"], before, want)

@@ -473,6 +473,11 @@ __device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionP
     for (int b = span.from; b < span.to; b++) {
         const int j = blockStart(p, span, b);
         attendRow<PAGED, Q8>(a, q, it, pos, j, p.keys(), o, &m, &l);
+        // Where no element is a number any more, nothing that follows makes it one.  (With no weight above 0 yet the result may still be zeros.)
+        bool lost = l != 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) lost &= lane + 64 * e >= D || o[e] != o[e];
+        if (__all(lost)) break;
     }
     if (it.slot < 0) {
 #pragma unroll
