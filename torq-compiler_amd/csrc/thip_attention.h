@@ -93,7 +93,7 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // take the same, with 64 streams took a third more (16 sequences of 4096 positions, four heads of 128: 56 us and 43); heads of 256 have the
     // slower tiles, and few rows of them too few (64 tokens over 4096 positions, four heads: 79 us in tiles, 42 in streams).
     p.tiles = rows > 32 * S && (D <= 128 || rows * KVH > 2048);
-    // The second part costs a prompt of 8192 tokens with 32 heads of 128 a third (174 us, 228 with it), four chunks of up to 512 a quarter (186, 234); the error of a
+    // The second part costs a prompt of 8192 tokens with 32 heads of 128 a third (153 us, 201 with it), four chunks of up to 512 a quarter (167, 210); the error of a
     // result goes from 1.4 times that of its rounding alone to 1.0.  Over many rows that is what it is; over few it may be 1.7 times in one call.
     p.fine = T * H < 8192;
     p.rowsLog = p.tiles ? 7 : 4;

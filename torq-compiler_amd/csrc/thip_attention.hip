@@ -9,7 +9,8 @@
 // product left them, which is the addresses of V's reads.  V's operand has a lane's values along the keys, across the rows that V lies in;
 // ds_read_b64_tr turns them on the way out of LDS.
 //
-// Times below are medians of the kernels in a trace.
+// Times below are means of calls one behind another, once the clocks have settled (the first ones after a pause take up to a tenth longer).  Where two
+// forms are compared, both are of one call's inputs again and again, which the last cache helps by a few percent.
 //
 // Weights go into the second product as two bf16, one and what it leaves, in streams and in tiles of few rows, where that costs nothing; as one in tiles
 // of many, where the second product's time counts (AttentionPlan::fine): off by half a step of 2^-8 each, which moves a result of independent values about as
@@ -576,8 +577,8 @@ constexpr float kSlack = 8.0f;
 // A tile of 16 rows (a token's heads, or a few tokens'); each of the four waves has blocks of 32 keys of its own, every fourth, and joins the
 // others at the end.  A wave waits for nobody: its keys go straight into the matrix operand's registers, its values through LDS of its own.
 // The registers are filled again as soon as their content is used, so a block's 2 x 32 rows are under way while the one before is worked on.
-// Bound by memory where there is much to read (a token for each of 16 sequences of up to 32768 positions, 32 heads of 128 over 8, int8, 770 MB: 157 us,
-// 4.9 TB/s, what a large copy reaches), else by a chain of loads: starts, table, keys, and what the parts wrote (1024 positions of one head
+// Bound by memory where there is much to read (a token for each of 16 sequences of up to 32768 positions, 32 heads of 128 over 8, int8, 770 MB: 152 us,
+// 5.1 TB/s, what a large copy reaches), else by a chain of loads: starts, table, keys, and what the parts wrote (1024 positions of one head
 // of 256: 10 us, of which 2 are the join).
 template <int DT, bool EXACT, bool PAGED, bool Q8>
 __device__ __forceinline__ void streamItem(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
@@ -834,12 +835,12 @@ constexpr int kTileWaves = DT == 256 ? Q8 ? 1 : 2 : 3;
 // Four waves of 32 rows each; keys and values of a block in LDS, two buffers in turn, one barrier a block.  The next block is on its way while
 // one is worked on, and the pages of the block behind that are asked for.  A wave's keys and values feed one product each from LDS, which gives
 // just what the matrix units take; 64 rows a wave halve that, but leave two waves a SIMD where three hide each other's softmax (8192 tokens,
-// 32 heads of 128, a window of 1024: 230 us for 195).  Blocks are as long as three workgroups a CU allow: 32 keys, 64 with heads of 64
-// (64 with heads of 128: 214 us).
+// 32 heads of 128, a window of 1024: 230 us where 32 rows took 195).  Blocks are as long as three workgroups a CU allow: 32 keys, 64 with heads of 64
+// (64 with heads of 128: 214 us for 195).
 //
 // Bound by the waits of a wave for itself (products, the softmax of their results, products) and by vector instructions next to matrix ones: that
-// prompt takes 177 us, 730 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 189, 660.  Heads of 256 leave two waves a SIMD and LDS busy with the
-// blocks that come (six prompts of up to 2048 tokens: 104 us, 360 TFLOP/s, where the longest tile alone takes 100 of them).
+// prompt takes 159 us, 810 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 169, 730.  Heads of 256 leave two waves a SIMD and LDS busy with the
+// blocks that come (six prompts of up to 2048 tokens: 99 us, 380 TFLOP/s, where the longest tile's blocks alone take nearly all of it).
 template <int DT, bool PAGED, bool Q8, bool FINE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
 void attention_tiles(AttentionArgs a, AttentionPlan p) {
@@ -964,7 +965,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         if constexpr (PAGED) flag(stage);
     };
     // int8: through registers, where they become bf16, every lane's rows looked up a block ahead (23 single tokens and a prompt's 777 in one batch, 16 heads of
-    // 64 over 4, windows of 2048: 40 us)
+    // 64 over 4, windows of 2048: 35 us)
     int rows[PER], scaleRow = -1;
     KeyAsk<PAGED> asked[PER], scaleAsked;
     v2i kreg[PER], vreg[PER];
