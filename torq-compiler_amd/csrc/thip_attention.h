@@ -67,7 +67,8 @@ struct AttentionPlan {
     __host__ __device__ int32_t keys() const { return 1 << keysLog; }
 };
 
-// Blocks of a part, and up to how many a run stays whole: of tiles, and of streams (among tiles, or alone).
+// Blocks of a part of a tile's run (of a stream's where the launch is of streams), up to how many a tile's run stays whole, and blocks of a part of a stream
+// among tiles.
 struct PartBlocks {
     int32_t tile, tileWhole, stream;
 };
@@ -78,12 +79,14 @@ __host__ __device__ inline PartBlocks partBlocks(const AttentionPlan &p, float t
     const int32_t least = full * (float)KVH < 128.0f ? p.fewBlocks : p.minBlocks;
     return {part > least ? part : least, p.tiles && whole > least ? whole : least, 4 * part > p.fewBlocks ? 4 * part : p.fewBlocks};
 }
+
 // Parts of a run.
 __host__ __device__ inline int32_t partsOf(const AttentionPlan &p, int32_t blocks, int32_t part, int32_t whole) {
     if (!p.splits || blocks <= part || blocks <= whole) return 1;
     const int32_t parts = (int32_t)(((uint32_t)blocks + (uint32_t)part - 1) / (uint32_t)part);
     return parts < p.maxParts ? parts : p.maxParts;
 }
+
 // capacity: positions that a sequence can have; quantised: the cache is int8 (for the launch only, what is asked of a workspace is the same)
 inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks,
                                    bool quantised = false) {
@@ -106,8 +109,8 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // 264 508 / 563, 320 515 / 564; int8, of which one workgroup of heads of 256 has a CU: 192 654 / 681, 264 1207 / 1030, 360 1227 / 1036.  A third of the
     // tiles with runs of 16384 and two thirds of 4096: 384 tiles 533 / 249, 720 553 / 410; heads of 256, 264 981 / 489, 512 989 / 686.
     // Streams cost less to join and are cut wherever they are longer than their share: a token for each of 72 sequences, eight heads of 128, one of 32768
-    // positions and the others of 200: 457 / 40; all of up to 4096: 171 / 166; 65 of up to 4096: 175 / 141.  That a table has room for long runs costs where there is none (256
-    // sequences of up to 128 positions, a table for 32768: 32 / 37).
+    // positions and the others of 200: 457 / 40; all of up to 4096: 171 / 166; 65 of up to 4096: 175 / 141.  That a table has room for long runs costs
+    // where there is none (256 sequences of up to 128 positions, a table for 32768: 32 / 37).
     p.items = p.tiles ? 512 : 1024;
     p.whole = D > 128 && !quantised ? 260 : 390;
     p.maxParts = p.tiles ? 16 : 64;
