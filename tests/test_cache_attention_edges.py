@@ -584,3 +584,32 @@ def test_gpu_values_behind_scores_of_minus_infinity(device, later):
     built, before, want = attend(b, True)
     assert (want[0][b.starts[2] + 90] == 0).all() and (np.isnan(want[0][0]).all() if later else (want[0][0] == 0).all())
     check_attention(b, built.run(device)["out"], before, want)
+
+
+def _product_over_its_operand():
+    """x times a transposed binding, into the bytes of that binding."""
+    rng = np.random.default_rng(3)
+    x, keys = (ref.to_bf16(rng.standard_normal(shape).astype(np.float32)) for shape in ((3, 4, 64), (3, 64, 64)))
+    built = Built()
+    a, whole = built.bind("x", x), built.bind("keys", keys)
+    p = built.program
+    p.matmul(a, p.transpose(whole, (0, 2, 1)), np.array([0.0], np.float32), init=p.view(whole, (3, 4, 64), 64), output_zp=0, output_min=w.NO_CLAMP[0],
+             output_max=w.NO_CLAMP[1], shift=0)
+    return built, x, keys
+
+
+def test_a_product_does_not_read_in_place_what_it_overwrites():
+    kinds = _kinds(_product_over_its_operand()[0].program.serialize())
+    assert TRANSPOSE in kinds and DEC_MATMUL not in kinds, kinds
+
+
+@pytest.mark.gpu
+def test_gpu_product_over_its_operand(device):
+    built, x, keys = _product_over_its_operand()
+    got = built.run(device)["keys"].reshape(-1)
+    turned = np.ascontiguousarray(keys.transpose(0, 2, 1))
+    want = prog.orc.matmul_bf16(x, turned, np.array([0.0], np.float32))
+    prog.assert_bf16_close(got[64:64 + 768].reshape(3, 4, 64), want, "over its operand", magnitude=np.abs(ref.from_bf16(x)) @ np.abs(ref.from_bf16(turned)))
+    rest = np.ones(got.size, dtype=bool)
+    rest[64:64 + 768] = False
+    assert np.array_equal(got[rest], keys.reshape(-1)[rest])

@@ -2273,9 +2273,9 @@ void Emitter::planDecodeFolding() {
             if (a.dtype != THIP_DTYPE_BF16 || a.rank < 2 || a.rank > 3 || a.shape[a.rank - 2] > kDecMaxRows) break;
             const int64_t batches = std::max<int64_t>(a.rank == 3 ? a.shape[0] : 1, res.rank == 3 ? res.shape[0] : 1);
             if (batches > 65535 || a.shape[a.rank - 1] % 8 != 0) break;
-            // read by the matmul, the input has to be then what it was where the transpose stands
+            // read by the matmul, the input has to be then what it was where the transpose stands, and stay so while the matmul writes its result
             bool changed = false;
-            for (size_t w = t + 1; w < m; w++) {
+            for (size_t w = t + 1; w <= m; w++) {
                 for (thip_value_t v : writtenBy(prog_.ops[w])) changed = changed || shareBytes(v, tr.input);
             }
             if (changed) break;
