@@ -1945,13 +1945,6 @@ thip_status_t Emitter::emitTransposeOp(const thip_hl_transpose_t &c) {
     return THIP_OK;
 }
 
-// ---- decode-shaped programs ------------------------------------------------------------------------------------
-// A decoder's step is a chain of some hundred small dependent ops on one to 32 rows: what it costs is the number of
-// launches and the memory round trips inside each.  The ops are therefore grouped: linears that read the same rows
-// become one record (query, key and value projections), two linears whose results meet in an add become one record
-// that computes both and adds (gate and up), the add behind a linear moves into its epilogue (residual connections),
-// and a transpose in front of a matmul's input2 is read in place.  THIP_NO_DECODE_FUSION leaves every op its own record.
-
 // ---- attention and its cache ------------------------------------------------------------------------------------------
 
 // A binding, or a view of one, in place.
@@ -2201,6 +2194,14 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
     ops_.push_back(op);
     return THIP_OK;
 }
+
+// ---- decode-shaped programs ------------------------------------------------------------------------------------
+// A decoder's step is a chain of some hundred small dependent ops on one to 32 rows: what it costs is the number of
+// launches and the memory round trips inside each.  The ops are therefore grouped: linears that read the same rows
+// become one record (query, key and value projections), two linears whose results meet in an add become one record
+// that computes both and adds (gate and up), the add behind a linear moves into its epilogue (residual connections),
+// and a transpose in front of a matmul's input2 is read in place, unless something writes its bytes before the matmul
+// is done.  THIP_NO_DECODE_FUSION leaves every op its own record.
 
 // What an op writes, whole or in part.
 static std::vector<thip_value_t> writtenBy(const HlOp &op) {
