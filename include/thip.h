@@ -400,7 +400,7 @@ thip_status_t thip_hl_table(thip_program_t *program, const thip_hl_table_t *op);
 thip_status_t thip_hl_act(thip_program_t *program, const thip_hl_act_t *op);
 thip_status_t thip_hl_elementwisebinary(thip_program_t *program, const thip_hl_elementwisebinary_t *op);
 
-/* ---- Attention and its cache -------------------------------------------------------------------------------------
+/* ---- Attention, its cache, norms and rotary positions ------------------------------------------------------------
  * Operators that no TorqHL op stands for (the reference has neither a softmax nor a cache): what a decoder needs
  * between its linears.  Element types: queries, keys, values and results BF16; a cache BF16, or I8 with one F32 scale
  * for each position and head.  Sums, softmax statistics and scores are held in 32 bits.  A softmax weight meets its
@@ -484,9 +484,95 @@ typedef struct thip_lm_attention_t {
     int32_t sinks;
 } thip_lm_attention_t;
 
+/* Attention of a tree of drafted tokens over a cache, all of its branches at once.  The rows of a sequence are its drafts; row i has place
+ * lengths[s] - n_s + i in the cache (where thip_lm_cache_write put its key and value), wherever it stands in the tree.  parents is I32[T], one entry a row:
+ * the row of its own sequence, counted from the sequence's first, that it follows, or -1 where it follows the last position before the tree,
+ * base - 1 with base = lengths[s] - n_s.  A parent comes before its children; an entry that is not below the row's own number counts as -1.  A row with d
+ * rows above it on its path stands at position base + d of the text, and sees the positions before the tree, j < base, and the rows of its path, itself
+ * among them, where (window == 0, or the seen one's position of the text > its own - window, or that position < sinks).  The rest is as in thip_lm_attention.
+ * What rows at places that are not there, or of a sequence behind its first THIP_LM_TREE_ROWS, see is nothing, and nobody sees them.  parents is a
+ * binding, a view of one, or a constant.  Its weights meet their values as thip_lm_attention says. */
+#define THIP_LM_TREE_ROWS 512
+typedef struct thip_lm_tree_attention_t {
+    thip_value_t init;
+    thip_value_t query;
+    thip_value_t key;
+    thip_value_t value;
+    thip_value_t key_scales;
+    thip_value_t value_scales;
+    thip_value_t pages;
+    thip_value_t row_starts;
+    thip_value_t lengths;
+    thip_value_t parents;
+    float scale; /* positive, at most 2e38 */
+    int32_t window;
+    int32_t sinks;
+} thip_lm_tree_attention_t;
+
+/* What was accepted of the drafts moves together: accepted is I32[S, K], for each sequence the rows of the accepted path in ascending order, counted from the
+ * sequence's first; a list ends with its K entries, or at the first that is no row of the sequence or not above the one before.  With base =
+ * lengths[s] - n_s, what the cache holds at position base + accepted[s][k] is then at position base + k (the bits, and those of the scales); the other
+ * positions keep what they hold.  An entry of which either position is not there moves nothing.  The next dispatch's lengths start from base and the number of
+ * accepted rows.  accepted is a binding, a view of one, or a constant; two sequences must not have the same place among their drafts. */
+typedef struct thip_lm_cache_keep_t {
+    thip_value_t key_cache;
+    thip_value_t value_cache;
+    thip_value_t key_scales;
+    thip_value_t value_scales;
+    thip_value_t accepted;
+    thip_value_t pages;
+    thip_value_t row_starts;
+    thip_value_t lengths;
+} thip_lm_cache_keep_t;
+
+/* Rotary positions: of each row and head of query [T, heads, D] and key [T, kv_heads, D], BF16, pair i of pairs is turned by the angle
+ * t = positions[axes[i]][row] * frequencies[i]:
+ *     (a, b) -> (a cos t - b sin t, b cos t + a sin t),
+ * where a pair is the elements i and pairs + i of a head, or 2 i and 2 i + 1 where interleaved is not 0.  Elements from 2 * pairs on stay as they are.
+ * positions is I32[axes, T] (a binding, a view of one, or a constant), any values; frequencies F32[pairs], a constant, radians a position, at most 16
+ * in magnitude; axes I32[pairs], a constant (0 up to the axes of positions), or THIP_NO_VALUE: axis 0 for all.  Angles are taken modulo a turn in whole
+ * numbers, to 2^-31 of one, so that far positions lose nothing; sines, cosines and sums are in 32 bits, a result is rounded once.  pairs is a multiple of 8, at
+ * most D / 2; D a multiple of 16 up to 256.  query_out and key_out may be the query's and the key's own bytes, or lie apart from all operands.  key and
+ * key_out are THIP_NO_VALUE where there is one tensor only. */
+typedef struct thip_lm_rotary_t {
+    thip_value_t query_out;
+    thip_value_t key_out;
+    thip_value_t query;
+    thip_value_t key;
+    thip_value_t positions;
+    thip_value_t frequencies;
+    thip_value_t axes;
+    int32_t interleaved;
+} thip_lm_rotary_t;
+
+/* The norms behind a block and before the next one, with the residual between them, row by row (the last dimension of input, N elements, 1 to 65536):
+ *     u = input, or norm(input, post_weight);   h = residual + residual_scale * gate * u;   residual_out = h;   init = norm(h, weight)
+ *     norm(x, w) = x / sqrt(mean(x^2) + eps) * (w + weight_offset)
+ * input and init BF16; residual and residual_out BF16 or F32, each on its own; all four of input's shape.  weight and post_weight [N], BF16 or F32.  gate
+ * BF16 [rows, N], [rows, 1], [1, N] or [1, 1], rows those of input (the product of its other dimensions).  THIP_NO_VALUE leaves out: residual (0),
+ * gate (1), post_weight (no norm of the input), residual_out, or init with its weight, one of the last two at most.  All is held in 32 bits
+ * between, rounded where it is stored: init is the norm of h before its rounding.  Squares that would pass 32 bits are taken of scaled values, so rows
+ * of any finite values have their norm.  init may be the input's own bytes, residual_out those of a residual of its type; operands share no bytes otherwise. */
+typedef struct thip_lm_norm_t {
+    thip_value_t init;
+    thip_value_t residual_out;
+    thip_value_t input;
+    thip_value_t residual;
+    thip_value_t post_weight;
+    thip_value_t gate;
+    thip_value_t weight;
+    float eps;           /* 0 or more, a number */
+    float weight_offset; /* a number; 1 where weights are held less one */
+    float residual_scale;
+} thip_lm_norm_t;
+
 thip_status_t thip_lm_cache_write(thip_program_t *program, const thip_lm_cache_write_t *op);
 thip_status_t thip_lm_cache_read(thip_program_t *program, const thip_lm_cache_read_t *op);
 thip_status_t thip_lm_attention(thip_program_t *program, const thip_lm_attention_t *op);
+thip_status_t thip_lm_tree_attention(thip_program_t *program, const thip_lm_tree_attention_t *op);
+thip_status_t thip_lm_cache_keep(thip_program_t *program, const thip_lm_cache_keep_t *op);
+thip_status_t thip_lm_rotary(thip_program_t *program, const thip_lm_rotary_t *op);
+thip_status_t thip_lm_norm(thip_program_t *program, const thip_lm_norm_t *op);
 
 /* Serialises the program (role of TargetBackend::serializeExecutable,
  * compiler/torq/Target/TorqTarget.cpp:115-151, and serializeTorqHW,

@@ -121,19 +121,76 @@ def attention(query, row_starts, scale, window=0, sinks=0, key=None, value=None,
         if not keys:
             out[row] = 0
             continue
-        keys, values = np.stack(keys, axis=1), np.stack(values, axis=1)  # [kv_heads, positions, D]
-        G = H // keys.shape[0]
-        for h in range(H):
-            k, v = keys[h // G], values[h // G]
-            with np.errstate(all="ignore"):
-                x = k @ q[row, h] * scale
-                m = np.max(x)
-                w = np.exp(x - (m if m != -np.inf else 0.0))
-                total = w.sum()
-                if rounded:
-                    w = from_bf16(to_bf16(w.astype(np.float32)))
-                out[row, h] = w @ v / total if total != 0 else 0.0
-                A = w @ np.abs(v) / total if total != 0 else np.zeros(D)
-                off = (D + 4) * h32 * scale * np.max(np.abs(k) @ np.abs(q[row, h])) + 4 * h32 * 2 * np.max(np.abs(x))
-                bound[row, h] = 1.05 * (h16 * np.abs(out[row, h]) + A * ((h16 * h16 + h32 if fine else h16) + 2 * (off + 4 * h32 + len(x) * h32))) + 1e-38
+        out[row], bound[row] = _weighed(q[row], np.stack(keys, axis=1), np.stack(values, axis=1), scale, fine, rounded)
     return out, bound
+
+
+def _weighed(q, keys, values, scale, fine, rounded):
+    """One row: q [H, D] over what it sees, keys and values [kv_heads, positions, D]; (result, bound) as attention() states them."""
+    (H, D), G = q.shape, q.shape[0] // keys.shape[0]
+    out, bound = np.zeros((H, D)), np.zeros((H, D))
+    h16, h32 = 2.0 ** -8, 2.0 ** -24
+    for h in range(H):
+        k, v = keys[h // G], values[h // G]
+        with np.errstate(all="ignore"):
+            x = k @ q[h] * scale
+            m = np.max(x)
+            w = np.exp(x - (m if m != -np.inf else 0.0))
+            total = w.sum()
+            if rounded:
+                w = from_bf16(to_bf16(w.astype(np.float32)))
+            out[h] = w @ v / total if total != 0 else 0.0
+            A = w @ np.abs(v) / total if total != 0 else np.zeros(D)
+            off = (D + 4) * h32 * scale * np.max(np.abs(k) @ np.abs(q[h])) + 4 * h32 * 2 * np.max(np.abs(x))
+            bound[h] = 1.05 * (h16 * np.abs(out[h]) + A * ((h16 * h16 + h32 if fine else h16) + 2 * (off + 4 * h32 + len(x) * h32))) + 1e-38
+    return out, bound
+
+
+TREE_ROWS = 512
+
+
+def tree_attention(query, row_starts, lengths, parents, cache, scale, window=0, sinks=0, fine=False, rounded=False):
+    """(result, bound) as attention() has them, of rows that are trees: row i of a sequence follows row parents[its row]."""
+    q = from_bf16(query)
+    T, H, D = q.shape
+    out, bound = np.full((T, H, D), np.nan), np.zeros((T, H, D))
+    for row, s, place in places(row_starts, lengths, T):
+        start = min(max(int(row_starts[s]), 0), T)
+        i = row - start
+        base = place - i
+        if place < 0 or i >= TREE_ROWS:
+            out[row] = 0
+            continue
+        path = [i]
+        while 0 <= int(parents[start + path[-1]]) < path[-1]:
+            path.append(int(parents[start + path[-1]]))
+        here = base + len(path) - 1
+        sees = lambda at: window == 0 or here - at < window or at < sinks  # noqa: E731
+        seen = [j for j in range(base) if sees(j)] + [base + r for back, r in enumerate(path) if sees(here - back)]
+        seen = sorted(j for j in seen if cache.find(s, j) is not None)
+        if not seen:
+            out[row] = 0
+            continue
+        keys = np.stack([cache.row(0, s, j) for j in seen], axis=1)
+        values = np.stack([cache.row(1, s, j) for j in seen], axis=1)
+        out[row], bound[row] = _weighed(q[row], keys, values, scale, fine, rounded)
+    return out, bound
+
+
+def cache_keep(cache, accepted, row_starts, lengths):
+    """Moves into copies; returns (key array, value array, key scales, value scales)."""
+    out = [a.copy() for a in cache.arrays] + [None if x is None else x.copy() for x in cache.scales]
+    for s in range(len(row_starts) - 1):
+        n = max(int(row_starts[s + 1]) - int(row_starts[s]), 0)
+        base, last = max(int(lengths[s]), 0) - n, -1
+        for k, r in enumerate(int(r) for r in accepted[s]):
+            if not last < r < n:
+                break
+            last = r
+            source, to = cache.find(s, base + r), cache.find(s, base + k)
+            if source is None or to is None:
+                continue
+            for x in out:
+                if x is not None:
+                    x[to[0], :, to[1]] = x[source[0], :, source[1]]
+    return out

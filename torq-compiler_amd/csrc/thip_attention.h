@@ -31,6 +31,17 @@ struct CacheRowsArgs {
 hipError_t launchCacheWrite(const CacheRowsArgs &a, const LaunchCtx &ctx);
 hipError_t launchCacheRead(const CacheRowsArgs &a, const LaunchCtx &ctx);
 
+// There is no tensor of rows, which row_starts would be kept inside of (CacheArgs::T).
+constexpr int32_t kNoRows = 0x7fffffff;
+struct CacheKeepArgs {
+    CacheArgs c;
+    const int32_t *accepted;               // [S][K]
+    int32_t K;
+    void *key_cache, *value_cache;
+    float *key_scales, *value_scales;      // null: the cache is bf16
+};
+hipError_t launchCacheKeep(const CacheKeepArgs &a, const LaunchCtx &ctx);
+
 struct AttentionArgs {
     CacheArgs c;
     const uint16_t *query;                 // [T][H][D]
@@ -43,6 +54,8 @@ struct AttentionArgs {
     int32_t window, sinks;                 // window 0: none (and sinks then 0)
     uint8_t *work;                         // attentionWorkspaceBytes
     size_t work_bytes;
+    const int32_t *parents;                // [T]: the rows are trees; null: they follow one another
+    int32_t tree_rows, tree_at;            // rows of a tree at most; where in LDS a workgroup has what it knows of its tree (set by the launch)
 };
 hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx);
 
@@ -88,8 +101,11 @@ __host__ __device__ inline int32_t partsOf(const AttentionPlan &p, int32_t block
 }
 
 // capacity: positions that a sequence can have; quantised: the cache is int8 (for the launch only, what is asked of a workspace is the same)
+// tree: rows of a tree at most (treeRows), 0: rows follow one another
+constexpr int kTreeRows = 512;  // THIP_LM_TREE_ROWS
+inline int64_t treeRows(int64_t T) { return T < kTreeRows ? T : kTreeRows; }
 inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks,
-                                   bool quantised = false) {
+                                   bool quantised = false, int64_t tree = 0) {
     AttentionPlan p;
     const int64_t G = H / KVH, rows = T * G;  // of one key head
     // Streams read a sequence's keys once for every 16 of its rows, tiles once for 128, at the rate of one wave's row block.  With 32 rows a sequence both
@@ -116,8 +132,9 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     p.maxParts = p.tiles ? 16 : 64;
     const int64_t keys = p.keys();
     const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
-    // a tile's window reaches over its own tokens too, and its first and last block need not be whole
-    const int64_t windowed = (sinks + keys - 1) / keys + (window + (p.rows() - 1) / G + keys) / keys + 1;
+    // a tile's window reaches over its own tokens too (in a tree, whose rows may all stand at its first position, over those before it), and its first and
+    // last block need not be whole
+    const int64_t windowed = (sinks + keys - 1) / keys + (window + (tree ? tree : (p.rows() - 1) / G) + keys) / keys + 1;
     p.windowBlocks = (int32_t)(windowed < 0x7fffffff ? windowed : 0x7fffffff);
     int64_t blocks = (capacity + keys - 1) / keys;
     if (window && windowed < blocks) blocks = windowed;
@@ -140,8 +157,9 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
 // many slots as there can be, for each row of a slot D sums, a maximum and a sum of weights.  The counters lie alike whatever the sizes are: launches that
 // follow one another have one workspace, as long as the longest.
 constexpr uint64_t kAttentionCounterBytes = 4 * 2 * 1024;
-inline uint64_t attentionWorkspaceBytes(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks) {
-    const AttentionPlan p = attentionPlan(T, S, H, KVH, D, capacity, window, sinks);
+inline uint64_t attentionWorkspaceBytes(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks,
+                                        int64_t tree = 0) {
+    const AttentionPlan p = attentionPlan(T, S, H, KVH, D, capacity, window, sinks, false, tree);
     return p.slots ? kAttentionCounterBytes + (uint64_t)p.slots * (uint64_t)p.rows() * (uint64_t)(D + 4) * 4 : 0;
 }
 

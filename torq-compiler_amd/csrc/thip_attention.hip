@@ -19,6 +19,7 @@
 #include "thip_attention.h"
 #include "thip_attention_rows.h"
 #include "thip_kernels_common.h"
+#include "thip_lanes.h"
 
 namespace thip {
 
@@ -53,13 +54,6 @@ __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const Atte
     if (a.window) w.blocks = min(w.blocks, p.windowBlocks);
     return w;
 }
-
-// A value moved within a wave's vector registers (what ds_bpermute does takes a trip to LDS, which counts where a workgroup's whole call is a few us);
-// 0 where there is none to come.
-template <int CONTROL, int ROWS = 0xf>
-__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, true); }
-template <int CONTROL, int ROWS = 0xf>
-__device__ __forceinline__ float moved(float v) { return __uint_as_float((uint32_t)moved<CONTROL, ROWS>((int)__float_as_uint(v))); }
 
 // Sum of the lanes up to this one.
 template <typename T>
@@ -223,11 +217,16 @@ struct Span {
     int sinkBlocks, windowBlock;
     int from, to;
 };
+template <bool TREE>
 __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
     Span s;
     const int r0 = it.tile << p.rowsLog, keys = p.keys();
     s.rows = min(p.rows(), it.w.count * a.G - r0);
-    const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
+    int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
+    if constexpr (TREE) {  // places; the rows may stand at any positions of the tree
+        top = it.w.first;
+        bottom = min(bottom, it.w.first + a.tree_rows - 1);
+    }
     const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(max(top, -1) - a.window + 1, 0) : 0;  // rows below position 0 see nothing
     auto blocksTo = [&](int end) { return (int)(((uint32_t)end + (uint32_t)keys - 1) >> p.keysLog); };  // a last block may pass 2^31
     s.sinkBlocks = blocksTo(min(min(a.sinks, low), high));
@@ -285,20 +284,6 @@ __device__ __forceinline__ v4f get4(__amdgpu_buffer_rsrc_t from, uint32_t at) {
     return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, 0, kDeviceScope));
 }
 
-__device__ __forceinline__ int packBf16(float lo, float hi) { return __builtin_bit_cast(int, __builtin_convertvector((v2f){lo, hi}, v2bf)); }
-
-// Of 2 or 16 lanes next to one another, the same in each.
-template <int LANES, typename F>
-__device__ __forceinline__ float overLanes(float v, F &&f) {
-    static_assert(LANES == 2 || LANES == 16);
-    v = f(v, moved<0xb1>(v));  // the neighbour
-    if constexpr (LANES == 16) {
-        v = f(v, moved<0x4e>(v));   // the other pair of four
-        v = f(v, moved<0x141>(v));  // the other four of eight, backwards
-        v = f(v, moved<0x140>(v));  // the other eight of 16, backwards
-    }
-    return v;
-}
 
 // Every thread of a workgroup that has stored its part: the last one of the run's to come here adds the parts, in their order, scaled to
 // their common maximum.  room: LDS that nobody uses any more, ROWS (PARTS + 1) floats and one.
@@ -386,6 +371,86 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     }
 }
 
+// ---- trees -------------------------------------------------------------------------------------------------------------
+
+// What a workgroup knows of its tree, in LDS: the parents of the sequence's rows, then for each token of its tile the position in the text at which it stands
+// (-1: it sees nothing) and a bit for each row of its path that it sees.  A path ascends from its row, parents below children, so a lane that follows it has
+// a word's bits together before it stores them; windows are taken off here, where a row's depth is known, and cost the blocks of keys nothing.
+struct Tree {
+    const int32_t *position;  // [tokens]
+    const uint32_t *seen;     // [tokens][stride]
+    int words, stride, token0;
+    bool all;                 // every row of the tile stands somewhere
+};
+__host__ __device__ constexpr int treeWords(int rows) { return (rows + 31) / 32; }
+__host__ __device__ constexpr int treeStride(int rows) { return treeWords(rows) | 1; }  // odd: 32 rows at one word are in as many banks
+__host__ __device__ constexpr int treeBytes(int rows, int tokens) { return 4 * (rows + tokens * (1 + treeStride(rows))); }
+
+// Every thread of the workgroup calls it.  paths: the item has keys of the tree, so the seen rows are asked for.
+__device__ __forceinline__ Tree plantTree(const AttentionArgs &a, const Item &it, int8_t *smem, int r0, int rows, bool paths) {
+    int32_t *const parents = (int32_t *)(smem + a.tree_at);
+    const int tid = threadIdx.x, count = min(it.w.count, a.tree_rows), base = it.w.first;
+    Tree t;
+    t.words = treeWords(a.tree_rows);
+    t.stride = treeStride(a.tree_rows);
+    t.token0 = (int)fastDiv((uint32_t)r0, a.g);
+    const int tokens = (int)fastDiv((uint32_t)(r0 + rows - 1), a.g) - t.token0 + 1;
+    int32_t *const position = parents + a.tree_rows;
+    uint32_t *const seen = (uint32_t *)(position + tokens);
+    t.position = position;
+    t.seen = seen;
+    t.all = base + t.token0 >= 0 && t.token0 + tokens <= count;
+    const bool walks = paths || a.window;
+    if (walks) {
+        for (int i = tid; i < min(count, t.token0 + tokens); i += 256) {
+            const int parent = a.parents[it.w.begin + i];
+            parents[i] = parent < i ? max(parent, -1) : -1;
+        }
+        __syncthreads();
+    }
+    if (tid < tokens) {
+        const int row = t.token0 + tid;
+        const bool stands = row < count && base + row >= 0;
+        int here = -1, depth = 0;
+        if (stands) {
+            if (a.window) {
+                for (int r = parents[row]; r >= 0; r = parents[r]) depth++;
+            }
+            here = base + (a.window ? depth : row);
+        }
+        position[tid] = here;
+        if (walks) {
+            // rows of the path below (row, depth) that the window still holds: those at low or above; with sinks those below `sinks` too
+            uint32_t word = 0;
+            int at = t.words - 1;
+            uint32_t *const mine = seen + tid * t.stride;
+            if (stands) {
+                for (int r = row, back = 0; r >= 0; r = parents[r], back++) {
+                    for (; at > r >> 5; at--) {
+                        mine[at] = word;
+                        word = 0;
+                    }
+                    if (a.window == 0 || back < a.window || here - back < a.sinks) word |= 1u << (r & 31);
+                }
+            }
+            for (; at >= 0; at--) {
+                mine[at] = word;
+                word = 0;
+            }
+        }
+    }
+    __syncthreads();
+    return t;
+}
+__device__ __forceinline__ int positionOf(const Tree &t, int token) { return t.position[token - t.token0]; }
+// Whether a token sees the rows of the tree from `first` on (it may lie before the tree), a bit each.
+__device__ __forceinline__ uint32_t seenFrom(const Tree &t, int token, int first) {
+    const uint32_t *const mine = t.seen + (token - t.token0) * t.stride;
+    const int w = first >> 5;
+    const uint32_t lo = (uint32_t)w < (uint32_t)t.words ? mine[w] : 0u, hi = (uint32_t)(w + 1) < (uint32_t)t.words ? mine[w + 1] : 0u;
+    return (uint32_t)((((uint64_t)hi << 32) | lo) >> (first & 31));
+}
+
 // ---- one row, key by key ----------------------------------------------------------------------------------------------
 
 // One row by one wave: a lane has the scores of one key of 64, then four of the result's elements (lane + 64 e).  A value is only touched
@@ -393,14 +458,18 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
 // masked value, or the scale of one, by a weight of zero, and hand a row here where that left a NaN.  (A select by the weight would drop
 // the NaN of a position that the row sees with a weight too small for 32 bits.)  Adds the `count` (up to 64) positions from `from` on to o, m and l.
 // q: D floats of LDS, the row's query.
-template <bool PAGED, bool Q8>
-__device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, int pos, int from, int count, float *o, float *m, float *l) {
+template <bool PAGED, bool Q8, bool TREE>
+__device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q, const Item &it, const Tree &tree, int token, int pos, int from, int count, float *o, float *m, float *l) {
     const CacheArgs &c = a.c;
     const int lane = threadIdx.x & 63, D = c.D;
     float most = *m, sum = *l;
     const int j = (int)((uint32_t)from + (uint32_t)lane);
     int row = -1;
-    if (lane < count && sees(windowOf(a), sinksOf(a, pos), pos, j)) row = keyRow(a, it, askKey<PAGED>(a, it, j, true));
+    bool see = lane < count && sees(windowOf(a), sinksOf(a, pos), pos, j);
+    if constexpr (TREE) {
+        if (j >= it.w.first) see = lane < count && (seenFrom(tree, token, j - it.w.first) & 1);
+    }
+    if (see) row = keyRow(a, it, askKey<PAGED>(a, it, j, true));
     float s = -INFINITY, vs = 1.0f;
     if (row >= 0) {
         float dot = 0.0f;
@@ -462,18 +531,19 @@ __device__ __forceinline__ void attendRow(const AttentionArgs &a, const float *q
 }
 
 // A row of an item once more, key by key, and its result or partial result stored.  q: LDS of this wave, kMaxHeadDim floats.
-template <bool TILE, bool PAGED, bool Q8>
-__device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const Item &it, const Span &span, int r, float *q) {
+template <bool TILE, bool PAGED, bool Q8, bool TREE>
+__device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionPlan &p, const Item &it, const Span &span, const Tree &tree, int r, float *q) {
     const int lane = threadIdx.x & 63, D = a.c.D;
     const int inSeq = (it.tile << p.rowsLog) + r, token = (int)fastDiv((uint32_t)inSeq, a.g), h = it.head * a.G + inSeq - token * a.G;
     const int64_t at = ((int64_t)(it.w.begin + token) * a.H + h) * D;
     for (int d = lane; d < D; d += 64) q[d] = __uint_as_float((uint32_t)a.query[at + d] << 16);
     __threadfence_block();
     float o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-    const int pos = it.w.first + token;
+    int pos = it.w.first + token;
+    if constexpr (TREE) pos = positionOf(tree, token);
     for (int b = span.from; b < span.to; b++) {
         const int j = blockStart(p, span, b);
-        attendRow<PAGED, Q8>(a, q, it, pos, j, p.keys(), o, &m, &l);
+        attendRow<PAGED, Q8, TREE>(a, q, it, tree, token, pos, j, p.keys(), o, &m, &l);
         // Where no element is a number any more, nothing that follows makes it one.  (With no weight above 0 yet the result may still be zeros.)
         bool lost = l != 0.0f;
 #pragma unroll
@@ -501,23 +571,6 @@ __device__ __forceinline__ void redoRow(const AttentionArgs &a, const AttentionP
 }
 
 // ---- small helpers of the tiles ---------------------------------------------------------------------------------------
-
-__device__ __forceinline__ float maxOverHalves(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sumOverHalves(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float maxOverQuarters(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return maxOverHalves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float sumOverQuarters(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return sumOverHalves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
 
 // What is left of x and y behind their bf16 in `word`, as bf16 again.
 __device__ __forceinline__ int restOf(int word, float x, float y) {
@@ -580,18 +633,18 @@ constexpr float kSlack = 8.0f;
 // Bound by memory where there is much to read (a token for each of 16 sequences of up to 32768 positions, 32 heads of 128 over 8, int8, 770 MB: 152 us,
 // 5.1 TB/s, what a large copy reaches), else by a chain of loads: starts, table, keys, and what the parts wrote (1024 positions of one head
 // of 256: 10 us, of which 2 are the join).
-template <int DT, bool EXACT, bool PAGED, bool Q8>
+template <int DT, bool EXACT, bool PAGED, bool Q8, bool TREE>
 __device__ __forceinline__ void streamItem(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
     constexpr int KB = 32, STEPS = DT / 32, ROW = DT * (Q8 ? 1 : 2), LOADS = ROW / 64;  // LOADS: 16-byte pieces of a row that one of four lanes has
     constexpr int JOIN = 16 * (DT + 4);  // floats of a wave's result
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
     const CacheArgs &c = a.c;
-    const Span span = spanOf(a, p, it);
+    const Span span = spanOf<TREE>(a, p, it);
     const int D = c.D, r0 = it.tile * 16;
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + span.rows - 1), a.g);
     const int inSeq = r0 + min(col, span.rows - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
-    const int pos = it.w.first + token;
+    int pos = it.w.first + token;
     float *const scales = (float *)(smem + 4 * KB * ROW) + wave * 2 * KB;
 
     // Loads are never skipped: a position that is not there is read as row 0, its value taken for zeros and its score for minus infinity; behind D
@@ -651,6 +704,11 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     fetchScales();
     fetch(a.value, vreg);
     fetch(a.key, kreg);
+    Tree tree{};
+    if constexpr (TREE) {
+        tree = plantTree(a, it, smem, r0, span.rows, span.to > span.from && blockStart(p, span, span.to - 1) + KB > it.w.first);
+        pos = positionOf(tree, token);
+    }
     for (int b = span.from + wave; b < span.to; b += 4) {
         const int j0 = blockStart(p, span, b);
         resolve();
@@ -698,16 +756,21 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
                 for (int i = 0; i < 4; i++) s[k][i] *= u[i];
             }
         }
-        const bool whole = j0 + KB - 1 <= top && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        const bool whole = (TREE ? tree.all && j0 + KB <= it.w.first : j0 + KB - 1 <= top) && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
         if (!whole || (gone0 | gone1)) {
             const uint32_t window = windowOf(a);
             const int sinks = sinksOf(a, pos);
+            uint32_t path = 0;  // of the 32 keys from j0 + 4 quarter on
+            if constexpr (TREE) {
+                if (j0 + KB > it.w.first) path = seenFrom(tree, token, j0 + 4 * quarter - it.w.first);
+            }
 #pragma unroll
             for (int k = 0; k < 2; k++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = 4 * quarter + i, j = j0 + 16 * k + key;
-                    const bool see = sees(window, sinks, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
+                    bool see = sees(window, sinks, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
+                    if constexpr (TREE) see = (j < it.w.first ? sees(window, sinks, pos, j) : ((path >> (16 * k + i)) & 1) != 0) & !(((k ? gone1 : gone0) >> key) & 1);
                     s[k][i] = see ? s[k][i] : -INFINITY;
                 }
             }
@@ -817,7 +880,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     }
     __syncthreads();
     for (int k = 0; k < 4; k++) {
-        if (__builtin_expect(((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows, 0)) redoRow<false, PAGED, Q8>(a, p, it, span, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
+        if (__builtin_expect(((odds >> (16 * k)) & 0xffff) && 4 * wave + k < span.rows, 0)) redoRow<false, PAGED, Q8, TREE>(a, p, it, span, tree, 4 * wave + k, (float *)smem + wave * kMaxHeadDim);
     }
     if (it.slot >= 0) {
         __syncthreads();
@@ -841,9 +904,8 @@ constexpr int kTileWaves = DT == 256 ? Q8 ? 1 : 2 : 3;
 // Bound by the waits of a wave for itself (products, the softmax of their results, products) and by vector instructions next to matrix ones: that
 // prompt takes 159 us, 810 TFLOP/s; four chunks of up to 512 tokens over up to 8192 positions 169, 730.  Heads of 256 leave two waves a SIMD and LDS busy with the
 // blocks that come (six prompts of up to 2048 tokens: 99 us, 380 TFLOP/s, where the longest tile's blocks alone take nearly all of it).
-template <int DT, bool PAGED, bool Q8, bool FINE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
-void attention_tiles(AttentionArgs a, AttentionPlan p) {
+template <int DT, bool PAGED, bool Q8, bool FINE, bool TREE>
+__device__ __forceinline__ void tileItem(const AttentionArgs &a, const AttentionPlan &p) {
     constexpr int KB = DT >= 128 ? 32 : 64, CH = DT / 8, PER = KB * CH / 256, STEP = 256 / CH, ROW = DT * 2;
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     float *const scaleRoom = (float *)(smem + 4 * KB * ROW);       // [2][keys, values][KB]
@@ -859,10 +921,10 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
             AttentionPlan stream = p;
             stream.keysLog = 5;
             it.part <<= p.keysLog - 5;
-            return streamItem<DT, false, PAGED, Q8>(a, stream, it);
+            return streamItem<DT, false, PAGED, Q8, TREE>(a, stream, it);
         }
     }
-    const Span span = spanOf(a, p, it);
+    const Span span = spanOf<TREE>(a, p, it);
     const int D = c.D, r0 = it.tile * 128 + wave * 32, rowsHere = min(32, span.rows - wave * 32);  // of this wave; none: <= 0
     const bool active = rowsHere > 0;
     const int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + max(rowsHere, 1) - 1), a.g);
@@ -871,7 +933,8 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         const int inSeq = r0 + min(column, max(rowsHere, 1) - 1), token = (int)fastDiv((uint32_t)inSeq, a.g);
         return ((int64_t)(it.w.begin + min(token, it.w.count - 1)) * a.H + it.head * a.G + inSeq - token * a.G) * D;
     };
-    const int pos = it.w.first + (int)fastDiv((uint32_t)(r0 + min(col, max(rowsHere, 1) - 1)), a.g);
+    const int token = (int)fastDiv((uint32_t)(r0 + min(col, max(rowsHere, 1) - 1)), a.g);
+    int pos = it.w.first + token;
 
     v16f o[DT / 32];
 #pragma unroll
@@ -1030,6 +1093,11 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         if (16 * t >= D) w = v4i{0, 0, 0, 0};
         q[t] = __builtin_bit_cast(v8bf, w);
     }
+    Tree tree{};
+    if constexpr (TREE) {
+        tree = plantTree(a, it, smem, it.tile * 128, span.rows, span.to > span.from && blockStart(p, span, span.to - 1) + KB > it.w.first);
+        pos = positionOf(tree, min(token, tree.token0 + (int)fastDiv((uint32_t)(it.tile * 128 + span.rows - 1), a.g) - tree.token0));
+    }
     for (int b = span.from, stage = 0; b < span.to; b++, stage ^= 1) {
         if constexpr (Q8) {
             resolve();
@@ -1077,7 +1145,7 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
                 }
             }
         }
-        bool whole = j0 + KB - 1 <= top && j0 <= it.w.length - KB && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        bool whole = (TREE ? tree.all && j0 + KB <= it.w.first : j0 + KB - 1 <= top) && j0 <= it.w.length - KB && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
         bool gaps = false;
         if constexpr (PAGED) gaps = __builtin_amdgcn_readfirstlane(*(const int *)(flagRoom + stage * 4)) != 0;
         if (!whole || gaps) {
@@ -1088,12 +1156,18 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int j = j0 + k * 32 + 8 * i + 4 * half;
+                    uint32_t path = 0;
+                    if constexpr (TREE) {
+                        if (j + 3 >= it.w.first) path = seenFrom(tree, token, j - it.w.first);
+                    }
                     uint32_t missing = 0;  // a byte a position
                     if constexpr (PAGED) missing = *(const uint32_t *)(absentRoom + stage * KB + k * 32 + 8 * i + 4 * half);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const bool there = PAGED ? !(missing & (0xffu << (8 * e))) : j + e < it.w.length;
-                        s[k][4 * i + e] = (sees(window, sinks, at, j + e) & there) ? s[k][4 * i + e] : -INFINITY;
+                        bool see = sees(window, sinks, at, j + e);
+                        if constexpr (TREE) see = j + e < it.w.first ? see : ((path >> e) & 1) != 0;
+                        s[k][4 * i + e] = (see & there) ? s[k][4 * i + e] : -INFINITY;
                     }
                 }
             }
@@ -1207,16 +1281,35 @@ void attention_tiles(AttentionArgs a, AttentionPlan p) {
         if (half == 0) put4(slots, tileStats(a, it.slot, wave * 32 + col), m, l, 0.0f, 0.0f);
     }
     for (int r = 0; r < rowsHere; r++) {
-        if (__builtin_expect((again >> r) & 1, 0)) redoRow<true, PAGED, Q8>(a, p, it, span, wave * 32 + r, (float *)room);
+        if (__builtin_expect((again >> r) & 1, 0)) redoRow<true, PAGED, Q8, TREE>(a, p, it, span, tree, wave * 32 + r, (float *)room);
     }
     if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
+}
+
+template <int DT, bool PAGED, bool Q8, bool FINE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
+void attention_tiles(AttentionArgs a, AttentionPlan p) {
+    tileItem<DT, PAGED, Q8, FINE, false>(a, p);
+}
+
+template <int DT, bool Q8, bool FINE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
+void tree_attention_tiles(AttentionArgs a, AttentionPlan p) {
+    tileItem<DT, true, Q8, FINE, true>(a, p);
 }
 
 template <int DT, bool EXACT, bool PAGED, bool Q8>
 __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_stream(AttentionArgs a, AttentionPlan p) {
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     Item it;
-    if (findItem(a, p, blockIdx.x, &it, smem)) streamItem<DT, EXACT, PAGED, Q8>(a, p, it);
+    if (findItem(a, p, blockIdx.x, &it, smem)) streamItem<DT, EXACT, PAGED, Q8, false>(a, p, it);
+}
+
+template <int DT, bool EXACT, bool Q8>
+__global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void tree_attention_stream(AttentionArgs a, AttentionPlan p) {
+    extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+    Item it;
+    if (findItem(a, p, blockIdx.x, &it, smem)) streamItem<DT, EXACT, true, Q8, true>(a, p, it);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------
@@ -1232,7 +1325,8 @@ static hipError_t checkAttention(const AttentionArgs &a) {
     } else if (a.key_scales) {
         return hipErrorInvalidValue;
     }
-    if (a.work_bytes < attentionWorkspaceBytes(c.T, c.S, a.H, c.KVH, c.D, c.pages ? c.capacity : c.T, a.window, a.sinks)) return hipErrorInvalidValue;
+    if (a.parents && (!c.pages || a.tree_rows != treeRows(c.T))) return hipErrorInvalidValue;
+    if (a.work_bytes < attentionWorkspaceBytes(c.T, c.S, a.H, c.KVH, c.D, c.pages ? c.capacity : c.T, a.window, a.sinks, a.parents ? a.tree_rows : 0)) return hipErrorInvalidValue;
     return hipSuccess;
 }
 
@@ -1251,6 +1345,19 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
         static_assert(lds >= (4 * kMaxHeadDim + 128 * 17 + 1) * 4, "what joins the parts");
         auto enqueue = [&](auto fine) -> hipError_t {
             constexpr bool FINE = decltype(fine)::value;
+            if constexpr (PAGED) {
+                if (a.parents) {
+                    AttentionArgs t = a;
+                    t.tree_at = lds;
+                    const int bytes = (int)lds + treeBytes(a.tree_rows, 128);
+                    auto kernel = tree_attention_tiles<DT, Q8, FINE>;
+                    if (ctx.name) {
+                        if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds + treeBytes(kTreeRows, 128))) return e;
+                    }
+                    THIP_ENQUEUE(ctx, kernelLabel("tree_attention_tiles", {DT, Q8, FINE}), kernel, grid, dim3(256), bytes, t, p);
+                    return hipSuccess;
+                }
+            }
             auto kernel = attention_tiles<DT, PAGED, Q8, FINE>;
             // asked for the kernel's name, as every executable does once on its device, the launcher configures it there
             if (lds > 64 * 1024 && ctx.name) {
@@ -1265,6 +1372,19 @@ static hipError_t enqueueAttention(const AttentionArgs &a, const AttentionPlan &
         static_assert(lds >= (4 * kMaxHeadDim + 16 * 65 + 1) * 4, "what joins the parts");
         auto enqueue = [&](auto exact) -> hipError_t {
             constexpr bool EXACT = decltype(exact)::value;
+            if constexpr (PAGED) {
+                if (a.parents) {
+                    AttentionArgs t = a;
+                    t.tree_at = lds;
+                    const int bytes = (int)lds + treeBytes(a.tree_rows, 16);
+                    auto kernel = tree_attention_stream<DT, EXACT, Q8>;
+                    if (ctx.name) {
+                        if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds + treeBytes(kTreeRows, 16))) return e;
+                    }
+                    THIP_ENQUEUE(ctx, kernelLabel("tree_attention_stream", {DT, EXACT, Q8}), kernel, grid, dim3(256), bytes, t, p);
+                    return hipSuccess;
+                }
+            }
             auto kernel = attention_stream<DT, EXACT, PAGED, Q8>;
             if (lds > 64 * 1024 && ctx.name) {
                 if (hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return e;
@@ -1286,7 +1406,8 @@ static hipError_t byHeadDim(const AttentionArgs &a, const AttentionPlan &p, cons
 
 hipError_t launchAttention(const AttentionArgs &a, const LaunchCtx &ctx) {
     if (hipError_t e = checkAttention(a)) return e;
-    const AttentionPlan p = attentionPlan(a.c.T, a.c.S, a.H, a.c.KVH, a.c.D, a.c.pages ? a.c.capacity : a.c.T, a.window, a.sinks, a.key_scales != nullptr);
+    const AttentionPlan p = attentionPlan(a.c.T, a.c.S, a.H, a.c.KVH, a.c.D, a.c.pages ? a.c.capacity : a.c.T, a.window, a.sinks, a.key_scales != nullptr,
+                                          a.parents ? a.tree_rows : 0);
     return !a.c.pages ? byHeadDim<false, false>(a, p, ctx) : a.key_scales ? byHeadDim<true, true>(a, p, ctx) : byHeadDim<true, false>(a, p, ctx);
 }
 

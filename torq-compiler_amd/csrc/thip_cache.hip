@@ -1,4 +1,4 @@
-// Rows of keys and values to and from a paged cache (thip_lm_cache_write, thip_lm_cache_read).
+// Rows of keys and values to and from a paged cache (thip_lm_cache_write, thip_lm_cache_read), and to other places of it (thip_lm_cache_keep).
 #include "thip_attention.h"
 #include "thip_attention_rows.h"
 #include "thip_kernels_common.h"
@@ -147,6 +147,63 @@ __global__ __launch_bounds__(256) void cache_read(CacheRowsArgs a, int rowsLog) 
     }
 }
 
+// The rows that a sequence keeps go to their places, in order.  A lane has one piece of 16 bytes (or a scale) of a head's key or value, of all of them: a row's
+// destination is behind no later row's source (its number in the list is not above its row's), so a lane that goes through the list in its order reads each source before
+// it is written over, without waiting for anybody, also with kKeepBatch of them under way.  First each lane of the wave looks up one entry's two places.
+// Bound by that chain of loads (starts, list, table, rows), one launch of a few us.
+constexpr int kKeepBatch = 8;
+
+template <bool Q8>
+__global__ __launch_bounds__(64) void cache_keep(CacheKeepArgs a, int chunks) {
+    const CacheArgs &c = a.c;
+    const int lane = threadIdx.x, seq = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - seq * chunks;
+    int begin, count;
+    rowsOf(c, c.starts, seq, &begin, &count);
+    const int base = firstPosition(c, seq, count);
+    // this lane's column: the keys' pieces, the values', then the scales of both
+    const int pieces = c.D / (Q8 ? 16 : 8), columns = c.KVH * pieces, column = chunk * 64 + lane;
+    const bool isScale = Q8 && column >= 2 * columns, isValue = isScale ? column >= 2 * columns + c.KVH : column >= columns;
+    const int inKind = column - (isScale ? 2 * columns : 0) - (isValue ? (isScale ? c.KVH : columns) : 0);
+    const int head = isScale ? inKind : inKind / pieces, piece = isScale ? 0 : inKind - head * pieces;
+    const bool idle = column >= 2 * columns + (Q8 ? 2 * c.KVH : 0);
+    int8_t *const rows = (int8_t *)(isValue ? a.value_cache : a.key_cache) + piece * 16;
+    float *const scales = isValue ? a.value_scales : a.key_scales;
+    const int64_t rowBytes = (int64_t)c.D * (Q8 ? 1 : 2);
+    const int32_t *const list = a.accepted + (int64_t)seq * a.K;
+    for (int k0 = 0; k0 < a.K; k0 += 64) {
+        const int k = k0 + lane;
+        const int row = k < a.K ? list[k] : -1, before = k > 0 && k < a.K ? list[k - 1] : -1;
+        const uint64_t wrong = __ballot(!(row > before && row < count));
+        const int here = wrong ? __builtin_ctzll(wrong) : 64;  // of these 64
+        int from = -1, to = -1;  // rows of the cache, of head 0
+        if (lane < here && row != k) {
+            from = cacheRow(c, seq, 0, base + row);
+            to = cacheRow(c, seq, 0, base + k);
+        }
+        const bool moves = from >= 0 && to >= 0;
+        for (int s = 0; s < here; s += kKeepBatch) {
+            if (!((__ballot(moves) >> s) & ((1u << kKeepBatch) - 1))) continue;
+            v4i held[kKeepBatch];
+            float scale[kKeepBatch];
+#pragma unroll
+            for (int u = 0; u < kKeepBatch; u++) {
+                const int64_t at = (int64_t)max(__builtin_amdgcn_readlane(from, s + u), 0) + (int64_t)head * c.PS;
+                if (idle) continue;
+                if (Q8 && isScale) scale[u] = scales[at];
+                else held[u] = *(const v4i *)(rows + at * rowBytes);
+            }
+#pragma unroll
+            for (int u = 0; u < kKeepBatch; u++) {
+                const int64_t at = (int64_t)max(__builtin_amdgcn_readlane(to, s + u), 0) + (int64_t)head * c.PS;
+                if (idle || !__builtin_amdgcn_readlane((int)moves, s + u)) continue;
+                if (Q8 && isScale) scales[at] = scale[u];
+                else *(v4i *)(rows + at * rowBytes) = held[u];
+            }
+        }
+        if (here < 64) break;
+    }
+}
+
 static hipError_t checkRows(const CacheRowsArgs &a) {
     const CacheArgs &c = a.c;
     if (c.T < 1 || c.S < 1 || c.KVH < 1 || c.D < 16 || c.D > kMaxHeadDim || c.D % 16 != 0 || c.P < 1 || c.NP < 1 || c.PS < 1) return hipErrorInvalidValue;
@@ -203,6 +260,21 @@ hipError_t launchCacheWrite(const CacheRowsArgs &a, const LaunchCtx &ctx) {
 hipError_t launchCacheRead(const CacheRowsArgs &a, const LaunchCtx &ctx) {
     if (hipError_t e = checkRows(a)) return e;
     return enqueueRows(a, false, ctx);
+}
+
+hipError_t launchCacheKeep(const CacheKeepArgs &a, const LaunchCtx &ctx) {
+    const CacheArgs &c = a.c;
+    if (c.T != kNoRows || c.S < 1 || a.K < 1 || c.KVH < 1 || c.D < 16 || c.D > kMaxHeadDim || c.D % 16 != 0 || c.P < 1 || c.NP < 1 || c.PS < 1) return hipErrorInvalidValue;
+    if ((int64_t)c.P * c.PS != c.capacity || (int64_t)c.NP * c.KVH * c.PS >= (1LL << 31)) return hipErrorInvalidValue;
+    if (!c.starts || !c.lengths || !c.pages || !a.accepted || !a.key_cache || !a.value_cache || !a.key_scales != !a.value_scales) return hipErrorInvalidValue;
+    if (((uintptr_t)a.key_cache | (uintptr_t)a.value_cache) & 15) return hipErrorInvalidValue;
+    const bool q8 = a.key_scales != nullptr;
+    const int64_t columns = 2 * (int64_t)c.KVH * (q8 ? c.D / 16 + 1 : c.D / 8), chunks = (columns - 1) / 64 + 1;
+    if (columns >= (1LL << 31) - 64 || chunks * c.S >= (1LL << 31)) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(chunks * c.S));
+    if (q8) THIP_ENQUEUE(ctx, kernelLabel("cache_keep", {1}), cache_keep<true>, grid, dim3(64), 0, a, (int)chunks);
+    else THIP_ENQUEUE(ctx, kernelLabel("cache_keep", {0}), cache_keep<false>, grid, dim3(64), 0, a, (int)chunks);
+    return ctx.name ? hipSuccess : hipGetLastError();
 }
 
 }  // namespace thip

@@ -111,6 +111,19 @@ enum Kind : uint32_t {
     // in0 = query, out, bias0 = float bits of the scale, K = window, Kp = sinks, w0 = 1: over a cache (0: over the rows, no CacheExt),
     // in1 = an intermediate for partial results, which only attention records have, one for all of a program (attentionWorkspaceBytes; none where that is 0)
     kKindAttention = 19,
+    // kKindAttention over a cache, of trees of drafts: table = a TreeExt
+    kKindTreeAttention = 20,
+    // Rows of a cache to other places of it: as kKindCacheWrite, but there are no rows; K = entries of a sequence's list, table = a TreeExt
+    // (rows = the lists), out = the key cache again
+    kKindCacheKeep = 21,
+    // in0 / in1 = query / key, out / weights = where they go, scale = positions [N][M], table = RotaryTurn [K] in the constant segment.  M = rows,
+    // N = axes, H / W = heads of query / key (0: there is no key), C = D, K = pairs, w0 = interleaved
+    kKindRotary = 22,
+    // in0 = input, in1 = residual, scale = gate, bias = post weights, weights = weights, table = where the sum goes, out = where the norm goes.  Any but in0
+    // may be missing, of the last two not both.  M = rows, C = row length, KH / KW = bytes of an element of the residual / the sum, SH / SW = of the
+    // weights / post weights, TR = gate rows, TS = gate columns (1: broadcast, 0: no gate), bias0 = float bits of eps, scale0 = of the
+    // weights' offset, w0 = of the residual scale
+    kKindNorm = 23,
 };
 
 // Operands of a record on a cache; bindings or constants, or none.
@@ -118,6 +131,21 @@ struct CacheExt {
     DescRef key_scales, value_scales, pages, lengths;
 };
 static_assert(sizeof(CacheExt) == 64, "CacheExt layout");
+
+// The same with what a record on drafted trees has: a row's parent each, or the accepted rows of each sequence.
+struct TreeExt {
+    CacheExt cache;
+    DescRef rows;
+};
+static_assert(sizeof(TreeExt) == 80, "TreeExt layout");
+
+// How a pair of elements turns from one position to the next: 2^-64 of a turn, modulo one, and the axis that its positions are of.
+struct RotaryTurn {
+    uint64_t step;
+    int32_t axis;
+    int32_t reserved;
+};
+static_assert(sizeof(RotaryTurn) == 16, "RotaryTurn layout");
 
 enum DecLinearFlags : int32_t {
     kDecPair = 1,         // two matrices of equal width; a workgroup owns the same columns of both, the add joins them

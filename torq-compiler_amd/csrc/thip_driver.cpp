@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "thip_attention.h"
+#include "thip_layer.h"
 #include "thip_chain_turn.h"
 #include "thip_descriptor.h"
 #include "thip_host_copy.h"
@@ -143,6 +144,10 @@ static const char *opKernelName(const DescOp &op) {
     case kKindCacheWrite: return "cache_write";
     case kKindCacheRead: return "cache_read";
     case kKindAttention: return "attention";
+    case kKindTreeAttention: return "tree_attention";
+    case kKindCacheKeep: return "cache_keep";
+    case kKindRotary: return "rotary";
+    case kKindNorm: return "norm";
     default: return "unknown";
     }
 }
@@ -350,16 +355,18 @@ static thip_status_t launchOp(thip_executable_t *e, uint32_t i, const DescOp &op
         err = launchDecMatmul(a, ctx);
         break;
     }
-    case kKindCacheWrite: case kKindCacheRead: case kKindAttention: {
-        const bool attends = op.kind == kKindAttention;
+    case kKindCacheWrite: case kKindCacheRead: case kKindAttention: case kKindTreeAttention: case kKindCacheKeep: {
+        const bool attends = op.kind == kKindAttention || op.kind == kKindTreeAttention;
         CacheArgs c;
         memset(&c, 0, sizeof(c));
         c.starts = (const int32_t *)resolve(e, op.scale, bp);
         c.T = op.M; c.S = op.N; c.KVH = op.W; c.D = op.C;
-        CacheExt x;
-        memset(&x, 0, sizeof(x));
+        TreeExt tree;
+        memset(&tree, 0, sizeof(tree));
+        CacheExt &x = tree.cache;
         if (!attends || op.w0 == 1) {
-            memcpy(&x, e->blob.data() + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset, sizeof(x));  // the host copy
+            const bool ofTree = op.kind == kKindTreeAttention || op.kind == kKindCacheKeep;
+            memcpy(&tree, e->blob.data() + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset, ofTree ? sizeof(tree) : sizeof(x));  // the host copy
             c.lengths = (const int32_t *)resolve(e, x.lengths, bp);
             c.pages = (const int32_t *)resolve(e, x.pages, bp);
             c.P = op.KW; c.NP = op.OH; c.PS = op.KH;
@@ -370,16 +377,39 @@ static thip_status_t launchOp(thip_executable_t *e, uint32_t i, const DescOp &op
         uint8_t *keys = resolve(e, op.weights, bp), *values = resolve(e, op.bias, bp);
         if (attends) {
             AttentionArgs a{c, (const uint16_t *)resolve(e, op.in0, bp), (uint16_t *)resolve(e, op.out, bp), keys, values, keyScales, valueScales,
-                            op.H, op.H / op.W, 0.0f, makeFastDiv((uint32_t)(op.H / op.W)), op.K, op.Kp, resolve(e, op.in1, bp), 0};
+                            op.H, op.H / op.W, 0.0f, makeFastDiv((uint32_t)(op.H / op.W)), op.K, op.Kp, resolve(e, op.in1, bp), 0, nullptr, 0, 0};
+            if (op.kind == kKindTreeAttention) {
+                a.parents = (const int32_t *)resolve(e, tree.rows, bp);
+                a.tree_rows = (int32_t)treeRows(op.M);
+            }
             memcpy(&a.scale, &op.bias0, 4);
             if (op.in1.space == kSpaceTemp) a.work_bytes = (size_t)(e->temps[op.in1.index].size - op.in1.offset);
             err = launchAttention(a, ctx);
+        } else if (op.kind == kKindCacheKeep) {
+            c.T = kNoRows;
+            err = launchCacheKeep({c, (const int32_t *)resolve(e, tree.rows, bp), op.K, keys, values, keyScales, valueScales}, ctx);
         } else {
             const bool write = op.kind == kKindCacheWrite;
             CacheRowsArgs a{c, (uint16_t *)resolve(e, write ? op.in0 : op.out, bp), (uint16_t *)resolve(e, op.in1, bp), keys, values, keyScales, valueScales,
                             makeFastDiv((uint32_t)op.W)};
             err = write ? launchCacheWrite(a, ctx) : launchCacheRead(a, ctx);
         }
+        break;
+    }
+    case kKindRotary: {
+        const RotaryArgs a{(const uint16_t *)resolve(e, op.in0, bp), (const uint16_t *)resolve(e, op.in1, bp), (uint16_t *)resolve(e, op.out, bp), (uint16_t *)resolve(e, op.weights, bp),
+                           (const int32_t *)resolve(e, op.scale, bp), (const RotaryTurn *)resolve(e, op.table, bp), op.M, op.H, op.W, op.C, op.K, op.w0};
+        err = launchRotary(a, ctx);
+        break;
+    }
+    case kKindNorm: {
+        NormArgs a{(const uint16_t *)resolve(e, op.in0, bp), resolve(e, op.in1, bp), (const uint16_t *)resolve(e, op.scale, bp), resolve(e, op.bias, bp), resolve(e, op.weights, bp),
+                   resolve(e, op.table, bp), (uint16_t *)resolve(e, op.out, bp), op.M, op.C, op.KH, op.KW, op.SH, op.SW,
+                   op.TR > 1 ? op.TS : 0, op.TS > 1 ? 1 : 0, 0.0f, 0.0f, 0.0f};
+        memcpy(&a.eps, &op.bias0, 4);
+        memcpy(&a.offset, &op.scale0, 4);
+        memcpy(&a.scale, &op.w0, 4);
+        err = launchNorm(a, ctx);
         break;
     }
     default: return fail(THIP_INTERNAL, "op %u has unknown kind %u", i, op.kind);
@@ -512,7 +542,9 @@ static thip_status_t dumpOpOutput(thip_executable_t *e, uint32_t i, uint8_t *con
     case kKindExpandWeights: shape = {op.K, op.Nn}; bf16(); break;
     case kKindCacheWrite: shape = {op.OH, op.W, op.KH, op.C}; if (op.gran == 2) bf16(); break;
     case kKindCacheRead: shape = {op.M, op.W, op.C}; bf16(); break;
-    case kKindAttention: shape = {op.M, op.H, op.C}; bf16(); break;
+    case kKindCacheKeep: shape = {op.OH, op.W, op.KH, op.C}; if (op.gran == 2) bf16(); break;
+    case kKindAttention: case kKindTreeAttention: case kKindRotary: shape = {op.M, op.H, op.C}; bf16(); break;
+    case kKindNorm: shape = {op.M, op.C}; bf16(); break;
     default: return THIP_OK;
     }
     size_t count = 1;

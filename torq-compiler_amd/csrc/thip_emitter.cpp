@@ -25,6 +25,7 @@
 #include "thip_attention.h"
 #include "thip_descriptor.h"
 #include "thip_kernels.h"
+#include "thip_layer.h"
 #include "thip_status.h"
 
 namespace thip {
@@ -49,7 +50,7 @@ struct Value {
     }
 };
 
-enum HlKind { kHlConv2d, kHlDepthwise, kHlFullyConnected, kHlMatmul, kHlMaxPool, kHlAvgPool, kHlAdd, kHlTranspose, kHlExpandWeights, kHlFma, kHlMul, kHlAct, kHlBinary, kHlUnary, kHlShift, kHlTable, kLmCacheWrite, kLmCacheRead, kLmAttention };
+enum HlKind { kHlConv2d, kHlDepthwise, kHlFullyConnected, kHlMatmul, kHlMaxPool, kHlAvgPool, kHlAdd, kHlTranspose, kHlExpandWeights, kHlFma, kHlMul, kHlAct, kHlBinary, kHlUnary, kHlShift, kHlTable, kLmCacheWrite, kLmCacheRead, kLmAttention, kLmTreeAttention, kLmCacheKeep, kLmRotary, kLmNorm };
 
 struct HlOp {
     HlKind kind;
@@ -73,6 +74,10 @@ struct HlOp {
         thip_lm_cache_write_t cw;
         thip_lm_cache_read_t cr;
         thip_lm_attention_t at;
+        thip_lm_tree_attention_t ta;
+        thip_lm_cache_keep_t ck;
+        thip_lm_rotary_t ro;
+        thip_lm_norm_t no;
     } u;
     std::string name;
     std::vector<int32_t> staticTable;  // torq_hl.table: the caller's static_table, copied
@@ -727,7 +732,12 @@ class Emitter {
     thip_status_t rowOperand(thip_value_t id, const char *what, bool written, int64_t T, int64_t heads, int64_t D, DescRef *out);
     thip_status_t emitCacheWrite(const thip_lm_cache_write_t &c);
     thip_status_t emitCacheRead(const thip_lm_cache_read_t &c);
-    thip_status_t emitAttention(const thip_lm_attention_t &c);
+    thip_status_t emitAttention(const thip_lm_attention_t &c, const thip_value_t *parents = nullptr);
+    thip_status_t emitTreeAttention(const thip_lm_tree_attention_t &c);
+    thip_status_t emitCacheKeep(const thip_lm_cache_keep_t &c);
+    thip_status_t writtenInPlace(thip_value_t id, const char *what, int32_t dtype, int64_t numel, DescRef *out);
+    thip_status_t emitRotary(const thip_lm_rotary_t &c);
+    thip_status_t emitNorm(const thip_lm_norm_t &c);
     // Operands of an integer elementwise op: element types, and the record's common fields.
     thip_status_t eltwiseCommon(const char *what, thip_value_t input, thip_value_t init, DescOp *op);
     thip_status_t emitAvgPoolBf16(const thip_hl_avg_pool2d_t &c);
@@ -2133,7 +2143,7 @@ thip_status_t Emitter::emitCacheRead(const thip_lm_cache_read_t &c) {
     return THIP_OK;
 }
 
-thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
+thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c, const thip_value_t *parents) {
     const Value *q, *k;
     if (thip_status_t s = checkValue(c.query, "query", &q)) return s;
     if (thip_status_t s = checkValue(c.key, "key", &k)) return s;
@@ -2174,23 +2184,242 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
     if (thip_status_t s = rowOperand(c.init, "init", true, T, H, D, &op.out)) return s;
     const uint64_t bytes = (uint64_t)T * H * D * 2;
     std::vector<Extent> all{{op.out, bytes, true, "init"}};
+    DescRef rows{kSpaceNone, 0, 0};
+    if (parents) {
+        if (thip_status_t s = indexOperand(*parents, "parents", 1, &rows)) return s;
+        if (prog_.values[(size_t)*parents].shape[0] != T) {
+            return fail(THIP_INVALID_ARGUMENT, "parents of %lld rows, query has %lld", (long long)prog_.values[(size_t)*parents].shape[0], (long long)T);
+        }
+        op.kind = kKindTreeAttention;
+        all.push_back({rows, (uint64_t)T * 4, false, "parents"});
+    }
     const bool inPlace = op.in0.space == op.out.space && op.in0.index == op.out.index && op.in0.offset == op.out.offset;
     if (!inPlace) all.push_back({op.in0, bytes, false, "query"});
     if (cached) {
         addExtents(op, ext, false, &all);
-        op.table = newConst(std::vector<CacheExt>{ext});
+        op.table = parents ? newConst(std::vector<TreeExt>{{ext, rows}}) : newConst(std::vector<CacheExt>{ext});
     } else {
         all.push_back({op.scale, ((uint64_t)op.N + 1) * 4, false, "row_starts"});
         all.push_back({op.weights, (uint64_t)T * op.W * D * 2, false, "key"});
         all.push_back({op.bias, (uint64_t)T * op.W * D * 2, false, "value"});
     }
     if (thip_status_t s = checkApart(all)) return s;
-    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T, op.K, op.Kp)) {
+    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T, op.K, op.Kp, parents ? treeRows(T) : 0)) {
         // records run one after another: they have one workspace, as long as the longest of them needs
         if (attentionWork_.space == kSpaceNone) attentionWork_ = newTemp(0);
         temps_[attentionWork_.index] = std::max(temps_[attentionWork_.index], work);
         op.in1 = attentionWork_;
     }
+    ops_.push_back(op);
+    return THIP_OK;
+}
+
+thip_status_t Emitter::emitTreeAttention(const thip_lm_tree_attention_t &c) {
+    // over a cache always: the rows of a tree have no order of their own
+    if (c.pages == THIP_NO_VALUE || c.lengths == THIP_NO_VALUE) return fail(THIP_INVALID_ARGUMENT, "a tree of drafts is over a cache: pages and lengths are missing");
+    const thip_lm_attention_t over{c.init, c.query, c.key, c.value, c.key_scales, c.value_scales, c.pages, c.row_starts, c.lengths, c.scale, c.window, c.sinks};
+    return emitAttention(over, &c.parents);
+}
+
+thip_status_t Emitter::emitCacheKeep(const thip_lm_cache_keep_t &c) {
+    DescOp op;
+    memset(&op, 0, sizeof(op));
+    TreeExt ext{};
+    op.kind = kKindCacheKeep;
+    if (thip_status_t s = batchOperands(c.row_starts, c.lengths, c.pages, true, &op, &ext.cache)) return s;
+    if (thip_status_t s = cacheOperands(c.key_cache, c.value_cache, c.key_scales, c.value_scales, true, &op, &ext.cache)) return s;
+    if (thip_status_t s = indexOperand(c.accepted, "accepted", 2, &ext.rows)) return s;
+    const Value &accepted = prog_.values[(size_t)c.accepted];
+    if (accepted.shape[0] != op.N) return fail(THIP_INVALID_ARGUMENT, "accepted rows of %lld sequences, row_starts has %d", (long long)accepted.shape[0], op.N);
+    if (!fitsInt32(accepted.shape[1] + 64)) return fail(THIP_UNIMPLEMENTED, "accepted: %lld entries for a sequence", (long long)accepted.shape[1]);
+    if (!fitsInt32((int64_t)op.N * ((2 * (int64_t)op.W * (op.C / 8 + 1) - 1) / 64 + 1))) return fail(THIP_UNIMPLEMENTED, "%d sequences of %d heads are too many", op.N, op.W);
+    op.K = (int32_t)accepted.shape[1];
+    op.out = op.weights;
+    std::vector<Extent> all{{ext.rows, (uint64_t)op.N * op.K * 4, false, "accepted"}};
+    addExtents(op, ext.cache, true, &all);
+    if (thip_status_t s = checkApart(all)) return s;
+    op.table = newConst(std::vector<TreeExt>{ext});
+    ops_.push_back(op);
+    return THIP_OK;
+}
+
+// ---- norms and rotary positions ---------------------------------------------------------------------------------------
+
+// What an op writes whole: an intermediate that is there already in place (it may be what the op reads).
+thip_status_t Emitter::writtenInPlace(thip_value_t id, const char *what, int32_t dtype, int64_t numel, DescRef *out) {
+    const Value *v;
+    if (thip_status_t s = checkValue(id, what, &v)) return s;
+    if (v->kind != kValueTensor || !state_[id].defined) return literalOutput(id, what, dtype, numel, out);
+    if (v->dtype != dtype || v->numel() != numel) return fail(THIP_INVALID_ARGUMENT, "%s: %lld elements of its type expected", what, (long long)numel);
+    if (state_[id].nhwcOfNchw) return fail(THIP_UNIMPLEMENTED, "%s: an N,C,H,W intermediate", what);
+    *out = state_[id].ref;
+    return THIP_OK;
+}
+
+thip_status_t Emitter::emitRotary(const thip_lm_rotary_t &c) {
+    const Value *q, *pos, *freq;
+    if (thip_status_t s = checkValue(c.query, "query", &q)) return s;
+    if (q->rank != 3) return fail(THIP_INVALID_ARGUMENT, "query: rank %d, expected 3", q->rank);
+    if ((c.key == THIP_NO_VALUE) != (c.key_out == THIP_NO_VALUE)) return fail(THIP_INVALID_ARGUMENT, "key and key_out come together");
+    const int64_t T = q->shape[0], H = q->shape[1], D = q->shape[2];
+    int64_t KVH = 0;
+    if (c.key != THIP_NO_VALUE) {
+        const Value *k;
+        if (thip_status_t s = checkValue(c.key, "key", &k)) return s;
+        if (k->rank != 3) return fail(THIP_INVALID_ARGUMENT, "key: rank %d, expected 3", k->rank);
+        KVH = k->shape[1];
+    }
+    if (!fitsInt32(T) || !fitsInt32(H) || !fitsInt32(T * H) || (KVH && (!fitsInt32(KVH) || !fitsInt32(T * KVH)))) return fail(THIP_UNIMPLEMENTED, "more than 2^31 rows");
+    if (D % 16 != 0 || D > kMaxHeadDim) return fail(THIP_UNIMPLEMENTED, "rows of %lld elements: multiples of 16 up to %d", (long long)D, kMaxHeadDim);
+    if ((H + KVH) * D >= (1 << 26)) return fail(THIP_UNIMPLEMENTED, "%lld heads of %lld elements", (long long)(H + KVH), (long long)D);
+    if (thip_status_t s = constantData(c.frequencies, "frequencies", THIP_DTYPE_F32, &freq)) return s;
+    const int64_t pairs = freq->numel();
+    if (freq->rank != 1 || pairs % 8 != 0 || 2 * pairs > D) {
+        return fail(THIP_INVALID_ARGUMENT, "frequencies of %lld pairs: a multiple of 8, at most half the %lld elements of a head", (long long)pairs, (long long)D);
+    }
+    DescOp op;
+    memset(&op, 0, sizeof(op));
+    op.kind = kKindRotary;
+    op.out_dtype = THIP_DTYPE_BF16;
+    if (thip_status_t s = indexOperand(c.positions, "positions", 2, &op.scale)) return s;
+    pos = &prog_.values[(size_t)c.positions];
+    if (pos->shape[1] != T || !fitsInt32(pos->shape[0])) return fail(THIP_INVALID_ARGUMENT, "positions: expected [axes, %lld]", (long long)T);
+    const int32_t *axes = nullptr;
+    if (c.axes != THIP_NO_VALUE) {
+        const Value *v;
+        if (thip_status_t s = constantData(c.axes, "axes", THIP_DTYPE_I32, &v)) return s;
+        if (v->rank != 1 || v->numel() != pairs) return fail(THIP_INVALID_ARGUMENT, "axes: expected [%lld]", (long long)pairs);
+        axes = (const int32_t *)v->data.data();
+    }
+    std::vector<RotaryTurn> turns((size_t)pairs);
+    for (int64_t i = 0; i < pairs; i++) {
+        float f;
+        memcpy(&f, freq->data.data() + 4 * i, 4);
+        if (!(fabsf(f) <= kMaxRotaryStep)) return fail(THIP_INVALID_ARGUMENT, "frequencies[%lld]: not a number of at most %g", (long long)i, (double)kMaxRotaryStep);
+        // in 64 bits of a turn, modulo one
+        const long double turn = (long double)f / 6.283185307179586476925286766559L, part = turn - floorl(turn);
+        turns[(size_t)i].step = part >= 1.0L ? 0 : (uint64_t)(part * 18446744073709551616.0L);
+        turns[(size_t)i].axis = axes ? axes[i] : 0;
+        if (turns[(size_t)i].axis < 0 || turns[(size_t)i].axis >= pos->shape[0]) {
+            return fail(THIP_INVALID_ARGUMENT, "axes[%lld] is %d, positions has %lld", (long long)i, turns[(size_t)i].axis, (long long)pos->shape[0]);
+        }
+        turns[(size_t)i].reserved = 0;
+    }
+    op.M = (int32_t)T;
+    op.N = (int32_t)pos->shape[0];
+    op.H = (int32_t)H;
+    op.W = (int32_t)KVH;
+    op.C = (int32_t)D;
+    op.K = (int32_t)pairs;
+    op.w0 = c.interleaved ? 1 : 0;
+    std::vector<Extent> all{{op.scale, (uint64_t)op.N * T * 4, false, "positions"}};
+    const auto rows = [&](thip_value_t from, thip_value_t to, const char *what, const char *whatOut, int64_t heads, DescRef *in, DescRef *out) -> thip_status_t {
+        if (thip_status_t s = rowOperand(from, what, false, T, heads, D, in)) return s;
+        const Value *v;
+        if (thip_status_t s = checkValue(to, whatOut, &v)) return s;
+        if (v->rank != 3 || v->shape[0] != T || v->shape[1] != heads || v->shape[2] != D) return fail(THIP_INVALID_ARGUMENT, "%s: expected [%lld, %lld, %lld]", whatOut, (long long)T, (long long)heads, (long long)D);
+        if (thip_status_t s = writtenInPlace(to, whatOut, THIP_DTYPE_BF16, T * heads * D, out)) return s;
+        if (out->offset & 15) return fail(THIP_UNIMPLEMENTED, "%s: a view at an offset that is no multiple of 16 bytes", whatOut);
+        const uint64_t bytes = (uint64_t)T * heads * D * 2;
+        all.push_back({*out, bytes, true, whatOut});
+        if (in->space != out->space || in->index != out->index || in->offset != out->offset) all.push_back({*in, bytes, false, what});
+        return THIP_OK;
+    };
+    if (thip_status_t s = rows(c.query, c.query_out, "query", "query_out", H, &op.in0, &op.out)) return s;
+    if (KVH) {
+        if (thip_status_t s = rows(c.key, c.key_out, "key", "key_out", KVH, &op.in1, &op.weights)) return s;
+    }
+    if (thip_status_t s = checkApart(all)) return s;
+    op.table = newConst(turns);
+    ops_.push_back(op);
+    return THIP_OK;
+}
+
+thip_status_t Emitter::emitNorm(const thip_lm_norm_t &c) {
+    const Value *x;
+    if (thip_status_t s = checkValue(c.input, "input", &x)) return s;
+    if (x->dtype != THIP_DTYPE_BF16) return fail(THIP_INVALID_ARGUMENT, "input: rows are bf16");
+    const int64_t N = x->shape[x->rank - 1], rows = x->numel() / N;
+    if (N > kMaxNormRow) return fail(THIP_UNIMPLEMENTED, "rows of %lld elements: up to %d", (long long)N, kMaxNormRow);
+    if (!fitsInt32(rows)) return fail(THIP_UNIMPLEMENTED, "input: more than 2^31 rows");
+    const auto number = [](float f) { return f - f == 0.0f; };
+    if (!(c.eps >= 0.0f) || !number(c.eps) || !number(c.weight_offset) || !number(c.residual_scale)) {
+        return fail(THIP_INVALID_ARGUMENT, "eps must be a number of 0 or more, weight_offset and residual_scale numbers");
+    }
+    if ((c.init == THIP_NO_VALUE) != (c.weight == THIP_NO_VALUE)) return fail(THIP_INVALID_ARGUMENT, "init and weight come together");
+    if (c.init == THIP_NO_VALUE && c.residual_out == THIP_NO_VALUE) return fail(THIP_INVALID_ARGUMENT, "neither init nor residual_out is given");
+    DescOp op;
+    memset(&op, 0, sizeof(op));
+    op.kind = kKindNorm;
+    op.out_dtype = THIP_DTYPE_BF16;
+    op.M = (int32_t)rows;
+    op.C = (int32_t)N;
+    memcpy(&op.bias0, &c.eps, 4);
+    memcpy(&op.scale0, &c.weight_offset, 4);
+    memcpy(&op.w0, &c.residual_scale, 4);
+    std::vector<Extent> all;
+    // an operand that is read; *bytes: of an element
+    const auto read = [&](thip_value_t id, const char *what, bool wide, bool whole, DescRef *out, int32_t *bytes) -> thip_status_t {
+        const Value *v;
+        if (thip_status_t s = checkValue(id, what, &v)) return s;
+        if (v->dtype != THIP_DTYPE_BF16 && !(wide && v->dtype == THIP_DTYPE_F32)) return fail(THIP_INVALID_ARGUMENT, "%s: wrong element type", what);
+        if (whole ? v->numel() != rows * N || v->shape[v->rank - 1] != N : v->rank != 1 || v->shape[0] != N) {
+            return fail(THIP_INVALID_ARGUMENT, "%s: expected %s of %lld elements", what, whole ? "rows like the input's," : "one row", (long long)N);
+        }
+        if (thip_status_t s = literalInput(id, what, out)) return s;
+        if (state_[(size_t)id].nhwcOfNchw) return fail(THIP_UNIMPLEMENTED, "%s: an N,C,H,W intermediate", what);
+        *bytes = (int32_t)elemSize(v->dtype);
+        return THIP_OK;
+    };
+    int32_t two;
+    if (thip_status_t s = read(c.input, "input", false, true, &op.in0, &two)) return s;
+    const uint64_t elems = (uint64_t)rows * N;
+    if (c.residual != THIP_NO_VALUE) {
+        if (thip_status_t s = read(c.residual, "residual", true, true, &op.in1, &op.KH)) return s;
+    }
+    if (c.post_weight != THIP_NO_VALUE) {
+        if (thip_status_t s = read(c.post_weight, "post_weight", true, false, &op.bias, &op.SW)) return s;
+        all.push_back({op.bias, (uint64_t)N * op.SW, false, "post_weight"});
+    }
+    if (c.weight != THIP_NO_VALUE) {
+        if (thip_status_t s = read(c.weight, "weight", true, false, &op.weights, &op.SH)) return s;
+        all.push_back({op.weights, (uint64_t)N * op.SH, false, "weight"});
+    }
+    if (c.gate != THIP_NO_VALUE) {
+        const Value *g;
+        if (thip_status_t s = checkValue(c.gate, "gate", &g)) return s;
+        if (g->dtype != THIP_DTYPE_BF16) return fail(THIP_INVALID_ARGUMENT, "gate: wrong element type");
+        if (g->rank != 2 || (g->shape[0] != rows && g->shape[0] != 1) || (g->shape[1] != N && g->shape[1] != 1)) {
+            return fail(THIP_INVALID_ARGUMENT, "gate: expected [%lld or 1, %lld or 1]", (long long)rows, (long long)N);
+        }
+        if (thip_status_t s = literalInput(c.gate, "gate", &op.scale)) return s;
+        op.TR = (int32_t)g->shape[0];
+        op.TS = (int32_t)g->shape[1];
+        all.push_back({op.scale, (uint64_t)g->numel() * 2, false, "gate"});
+    }
+    const auto same = [](const DescRef &a, const DescRef &b) { return a.space == b.space && a.index == b.index && a.offset == b.offset; };
+    const auto written = [&](thip_value_t id, const char *what, int32_t dtype, DescRef *out) -> thip_status_t {
+        const Value *v;
+        if (thip_status_t s = checkValue(id, what, &v)) return s;
+        if (v->shape[v->rank - 1] != N) return fail(THIP_INVALID_ARGUMENT, "%s: expected rows of %lld elements", what, (long long)N);
+        if (thip_status_t s = writtenInPlace(id, what, dtype, rows * N, out)) return s;
+        all.push_back({*out, elems * elemSize(dtype), true, what});
+        return THIP_OK;
+    };
+    if (c.residual_out != THIP_NO_VALUE) {
+        const Value *v;
+        if (thip_status_t s = checkValue(c.residual_out, "residual_out", &v)) return s;
+        if (v->dtype != THIP_DTYPE_BF16 && v->dtype != THIP_DTYPE_F32) return fail(THIP_INVALID_ARGUMENT, "residual_out: wrong element type");
+        if (thip_status_t s = written(c.residual_out, "residual_out", v->dtype, &op.table)) return s;
+        op.KW = (int32_t)elemSize(v->dtype);
+    }
+    if (c.init != THIP_NO_VALUE) {
+        if (thip_status_t s = written(c.init, "init", THIP_DTYPE_BF16, &op.out)) return s;
+    }
+    // a row is read whole before any of it is written: over its own bytes it may be
+    if (!same(op.in0, op.out)) all.push_back({op.in0, elems * 2, false, "input"});
+    if (c.residual != THIP_NO_VALUE && !(same(op.in1, op.table) && op.KH == op.KW)) all.push_back({op.in1, elems * op.KH, false, "residual"});
+    if (thip_status_t s = checkApart(all)) return s;
     ops_.push_back(op);
     return THIP_OK;
 }
@@ -2202,6 +2431,9 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c) {
 // that computes both and adds (gate and up), the add behind a linear moves into its epilogue (residual connections),
 // and a transpose in front of a matmul's input2 is read in place, unless something writes its bytes before the matmul
 // is done.  THIP_NO_DECODE_FUSION leaves every op its own record.
+
+// What a norm reads (some of it may be no value).
+static std::vector<thip_value_t> normReads(const thip_lm_norm_t &c) { return {c.input, c.residual, c.post_weight, c.gate, c.weight}; }
 
 // What an op writes, whole or in part.
 static std::vector<thip_value_t> writtenBy(const HlOp &op) {
@@ -2225,6 +2457,10 @@ static std::vector<thip_value_t> writtenBy(const HlOp &op) {
     case kLmCacheWrite: return {op.u.cw.key_cache, op.u.cw.value_cache, op.u.cw.key_scales, op.u.cw.value_scales};
     case kLmCacheRead: return {op.u.cr.key, op.u.cr.value};
     case kLmAttention: return {op.u.at.init};
+    case kLmTreeAttention: return {op.u.ta.init};
+    case kLmCacheKeep: return {op.u.ck.key_cache, op.u.ck.value_cache, op.u.ck.key_scales, op.u.ck.value_scales};
+    case kLmRotary: return {op.u.ro.query_out, op.u.ro.key_out};
+    case kLmNorm: return {op.u.no.init, op.u.no.residual_out};
     }
     return {};
 }
@@ -2599,6 +2835,10 @@ void Emitter::planChannelPadding() {
         case kLmCacheWrite: bar(op.u.cw.key); bar(op.u.cw.value); break;
         case kLmCacheRead: bar(op.u.cr.key); bar(op.u.cr.value); break;
         case kLmAttention: bar(op.u.at.query); bar(op.u.at.key); bar(op.u.at.value); bar(op.u.at.init); break;
+        case kLmTreeAttention: bar(op.u.ta.query); bar(op.u.ta.key); bar(op.u.ta.value); bar(op.u.ta.init); break;
+        case kLmCacheKeep: break;  // bindings only
+        case kLmRotary: bar(op.u.ro.query); bar(op.u.ro.key); bar(op.u.ro.query_out); bar(op.u.ro.key_out); break;
+        case kLmNorm: for (thip_value_t v : normReads(op.u.no)) bar(v); bar(op.u.no.init); bar(op.u.no.residual_out); break;
         }
     }
     // one verdict per group: every member an int8 rank-4 intermediate, all uses agreeing on C
@@ -2659,6 +2899,10 @@ void Emitter::planExpandFolding() {
         // what they write in part stays in part
         case kLmCacheRead: read(op.u.cr.key_cache); read(op.u.cr.value_cache); read(op.u.cr.key); read(op.u.cr.value); break;
         case kLmAttention: read(op.u.at.query); read(op.u.at.key); read(op.u.at.value); read(op.u.at.init); break;
+        case kLmTreeAttention: read(op.u.ta.query); read(op.u.ta.key); read(op.u.ta.value); read(op.u.ta.init); break;
+        case kLmCacheKeep: read(op.u.ck.key_cache); read(op.u.ck.value_cache); break;
+        case kLmRotary: read(op.u.ro.query); read(op.u.ro.key); break;
+        case kLmNorm: for (thip_value_t v : normReads(op.u.no)) read(v); break;
         }
     }
     valueReads_ = reads;
@@ -2751,6 +2995,10 @@ thip_status_t Emitter::run(void **outBlob, size_t *outSize) {
         case kLmCacheWrite: s = emitCacheWrite(op.u.cw); break;
         case kLmCacheRead: s = emitCacheRead(op.u.cr); break;
         case kLmAttention: s = emitAttention(op.u.at); break;
+        case kLmTreeAttention: s = emitTreeAttention(op.u.ta); break;
+        case kLmCacheKeep: s = emitCacheKeep(op.u.ck); break;
+        case kLmRotary: s = emitRotary(op.u.ro); break;
+        case kLmNorm: s = emitNorm(op.u.no); break;
         }
         if (s != THIP_OK) return s;
     }
@@ -2942,6 +3190,10 @@ THIP_DEFINE_HL(thip_hl_elementwiseshift, thip_hl_elementwiseshift_t, kHlShift, s
 THIP_DEFINE_HL(thip_lm_cache_write, thip_lm_cache_write_t, kLmCacheWrite, cw)
 THIP_DEFINE_HL(thip_lm_cache_read, thip_lm_cache_read_t, kLmCacheRead, cr)
 THIP_DEFINE_HL(thip_lm_attention, thip_lm_attention_t, kLmAttention, at)
+THIP_DEFINE_HL(thip_lm_tree_attention, thip_lm_tree_attention_t, kLmTreeAttention, ta)
+THIP_DEFINE_HL(thip_lm_cache_keep, thip_lm_cache_keep_t, kLmCacheKeep, ck)
+THIP_DEFINE_HL(thip_lm_rotary, thip_lm_rotary_t, kLmRotary, ro)
+THIP_DEFINE_HL(thip_lm_norm, thip_lm_norm_t, kLmNorm, no)
 
 thip_status_t thip_hl_table(thip_program_t *program, const thip_hl_table_t *op) {
     if (!program || !op) return fail(THIP_INVALID_ARGUMENT, "thip_hl_table: null argument");

@@ -9,6 +9,7 @@
 
 #include "thip_attention.h"
 #include "thip_kernels.h"
+#include "thip_layer.h"
 #include "thip_status.h"
 
 namespace thip {
@@ -410,9 +411,11 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
         if ((op.in0.offset & 15) || (op.weights.offset & 15) || (op.out.offset & 7)) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
         return need(op.out, mul(op.TB, op.M, op.Nn) * 2, "out");
     }
-    case kKindCacheWrite: case kKindCacheRead: case kKindAttention: {
-        const bool attends = op.kind == kKindAttention, cached = !attends || op.w0 == 1;
-        if (!positive({op.M, op.N, op.W, op.C}) || op.C % 16 != 0 || op.C > kMaxHeadDim || (op.gran != 2 && !(cached && op.gran == 1)) || mul(op.M, op.W) >= (1ull << 31)) {
+    case kKindCacheWrite: case kKindCacheRead: case kKindAttention: case kKindTreeAttention: case kKindCacheKeep: {
+        const bool keeps = op.kind == kKindCacheKeep, ofTree = op.kind == kKindTreeAttention || keeps;
+        const bool attends = op.kind == kKindAttention || op.kind == kKindTreeAttention, cached = !attends || op.w0 == 1;
+        if (ofTree && !cached) return fail(THIP_INVALID_ARGUMENT, "op %u: a tree without a cache", i);
+        if (!positive({keeps ? 1 : op.M, op.N, op.W, op.C}) || op.C % 16 != 0 || op.C > kMaxHeadDim || (op.gran != 2 && !(cached && op.gran == 1)) || mul(op.M, op.W) >= (1ull << 31)) {
             return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of packed rows", i);
         }
         const uint64_t rowBytes = mul(op.M, op.W, op.C) * 2;
@@ -423,7 +426,7 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
                 return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of a cache", i);
             }
             if (op.table.space != kSpaceConst) return fail(THIP_INVALID_ARGUMENT, "op %u: the cache's operands must be a constant", i);
-            if ((s = need(op.table, sizeof(CacheExt), "cache operands"))) return s;
+            if ((s = need(op.table, ofTree ? sizeof(TreeExt) : sizeof(CacheExt), "cache operands"))) return s;
             CacheExt x;
             memcpy(&x, e->blob + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset, sizeof(x));
             for (const DescRef *r : {&x.key_scales, &x.value_scales, &x.pages, &x.lengths}) {
@@ -442,7 +445,17 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
             }
             if ((s = need(op.weights, cacheBytes, "key cache"))) return s;
             if ((s = need(op.bias, cacheBytes, "value cache"))) return s;
-            if (op.kind == kKindCacheWrite && (op.weights.space != kSpaceBinding || op.bias.space != kSpaceBinding || (op.gran == 1 && (x.key_scales.space != kSpaceBinding || x.value_scales.space != kSpaceBinding)))) {
+            if (ofTree) {
+                TreeExt tree;
+                memcpy(&tree, e->blob + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset, sizeof(tree));
+                if ((s = checkLooseRef(e, i, tree.rows))) return s;
+                if (tree.rows.space == kSpaceTemp || (tree.rows.offset & 3)) return fail(THIP_INVALID_ARGUMENT, "op %u: bad operand of a tree", i);
+                if (keeps && (op.K <= 0 || op.K > 0x7fffffff - 64 || mul(op.N, (2 * (int64_t)op.W * (op.C / 8 + 1) - 1) / 64 + 1) >= (1ull << 31))) {
+                    return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of accepted rows", i);
+                }
+                if ((s = need(tree.rows, keeps ? mul(op.N, op.K) * 4 : (uint64_t)op.M * 4, "rows of a tree"))) return s;
+            }
+            if ((op.kind == kKindCacheWrite || keeps) && (op.weights.space != kSpaceBinding || op.bias.space != kSpaceBinding || (op.gran == 1 && (x.key_scales.space != kSpaceBinding || x.value_scales.space != kSpaceBinding)))) {
                 return fail(THIP_INVALID_ARGUMENT, "op %u: a cache that is written must be a binding", i);
             }
         } else {
@@ -455,16 +468,69 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
             if (op.H <= 0 || op.H % op.W != 0 || mul(op.M, op.H) >= (1ull << 31) || op.K < 0 || op.Kp < 0 || (op.w0 != 0 && op.w0 != 1) || !(scale > 0.0f) || scale > 2e38f) {  // times log2(e) it is a number too
                 return fail(THIP_INVALID_ARGUMENT, "op %u: bad attention record", i);
             }
-            if (const uint64_t work = attentionWorkspaceBytes(op.M, op.N, op.H, op.W, op.C, cached ? (int64_t)op.KW * op.KH : op.M, op.K, op.Kp)) {
+            if (const uint64_t work = attentionWorkspaceBytes(op.M, op.N, op.H, op.W, op.C, cached ? (int64_t)op.KW * op.KH : op.M, op.K, op.Kp, ofTree ? treeRows(op.M) : 0)) {
                 if (op.in1.space != kSpaceTemp || (op.in1.offset & 15)) return fail(THIP_INVALID_ARGUMENT, "op %u: bad workspace", i);
                 if ((s = need(op.in1, work, "workspace"))) return s;
             }
             if ((s = need(op.in0, mul(op.M, op.H, op.C) * 2, "query"))) return s;
             return need(op.out, mul(op.M, op.H, op.C) * 2, "out");
         }
+        if (keeps) return THIP_OK;
         if (op.in1.offset & 15) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
         if ((s = need(op.in1, rowBytes, "value rows"))) return s;
         return need(op.kind == kKindCacheWrite ? op.in0 : op.out, rowBytes, "key rows");
+    }
+    case kKindRotary: {
+        if (!positive({op.M, op.N, op.H, op.C, op.K}) || op.W < 0 || op.C % 16 != 0 || op.C > kMaxHeadDim || op.K % 8 != 0 || op.K > op.C / 2 ||
+            mul(op.M, op.H) >= (1ull << 31) || mul(op.M, op.W) >= (1ull << 31) || mul((int64_t)op.H + op.W, op.C) >= (1ull << 26)) {
+            return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of rotary positions", i);
+        }
+        if (((op.in0.offset | op.in1.offset | op.out.offset | op.weights.offset) & 15) || (op.scale.offset & 3)) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
+        if ((s = need(op.in0, mul(op.M, op.H, op.C) * 2, "query"))) return s;
+        if ((s = need(op.out, mul(op.M, op.H, op.C) * 2, "query out"))) return s;
+        if (op.W) {
+            if ((s = need(op.in1, mul(op.M, op.W, op.C) * 2, "key"))) return s;
+            if ((s = need(op.weights, mul(op.M, op.W, op.C) * 2, "key out"))) return s;
+        } else if (op.in1.space != kSpaceNone || op.weights.space != kSpaceNone) {
+            return fail(THIP_INVALID_ARGUMENT, "op %u: a key without heads", i);
+        }
+        if ((s = need(op.scale, mul(op.N, op.M) * 4, "positions"))) return s;
+        if (op.table.space != kSpaceConst || (op.table.offset & 7)) return fail(THIP_INVALID_ARGUMENT, "op %u: the steps must be a constant", i);
+        if ((s = need(op.table, (uint64_t)op.K * sizeof(RotaryTurn), "steps"))) return s;
+        for (int32_t k = 0; k < op.K; k++) {
+            RotaryTurn t;
+            memcpy(&t, e->blob + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset + (uint64_t)k * sizeof(t), sizeof(t));
+            if (t.axis < 0 || t.axis >= op.N) return fail(THIP_INVALID_ARGUMENT, "op %u: pair %d turns by axis %d of %d", i, k, t.axis, op.N);
+        }
+        return THIP_OK;
+    }
+    case kKindNorm: {
+        if (!positive({op.M, op.C}) || op.C > kMaxNormRow) return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of rows", i);
+        const bool sums = op.table.space != kSpaceNone, norms = op.out.space != kSpaceNone;
+        if ((!sums && !norms) || norms != (op.weights.space != kSpaceNone)) return fail(THIP_INVALID_ARGUMENT, "op %u: no result, or one without weights", i);
+        if ((s = need(op.in0, mul(op.M, op.C) * 2, "input"))) return s;
+        uint64_t odd = (op.in0.offset | op.out.offset | op.scale.offset) & 1;
+        const struct {
+            const DescRef &ref;
+            int32_t bytes;
+            uint64_t elems;
+            const char *name;
+        } parts[] = {{op.in1, op.KH, mul(op.M, op.C), "residual"}, {op.table, op.KW, mul(op.M, op.C), "sum"}, {op.weights, op.SH, (uint64_t)op.C, "weights"}, {op.bias, op.SW, (uint64_t)op.C, "post weights"}};
+        for (const auto &part : parts) {
+            if (part.ref.space == kSpaceNone) continue;
+            if (part.bytes != 2 && part.bytes != 4) return fail(THIP_INVALID_ARGUMENT, "op %u: %s of %d bytes an element", i, part.name, part.bytes);
+            if ((s = need(part.ref, part.elems * (uint64_t)part.bytes, part.name))) return s;
+            odd |= part.ref.offset & (uint64_t)(part.bytes - 1);
+        }
+        if (op.scale.space != kSpaceNone) {
+            if ((op.TR != 1 && op.TR != op.M) || (op.TS != 1 && op.TS != op.C)) return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of a gate", i);
+            if ((s = need(op.scale, mul(op.TR, op.TS) * 2, "gate"))) return s;
+        }
+        if (odd) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
+        float eps;
+        memcpy(&eps, &op.bias0, 4);
+        if (!(eps >= 0.0f) || eps - eps != 0.0f) return fail(THIP_INVALID_ARGUMENT, "op %u: bad eps", i);
+        return norms ? need(op.out, mul(op.M, op.C) * 2, "out") : THIP_OK;
     }
     default: return fail(THIP_INVALID_ARGUMENT, "op %u has unknown kind %u", i, op.kind);
     }

@@ -42,7 +42,7 @@ EXPORTED_SYMBOLS = [
     "thip_program_tensor", "thip_program_view", "thip_gemm_tile_choice", "thip_hl_conv2d", "thip_hl_depthwise_conv2d", "thip_hl_fully_connected",
     "thip_hl_matmul", "thip_hl_maxpool2d", "thip_hl_avg_pool2d", "thip_hl_add", "thip_hl_transpose", "thip_hl_expand_weights",
     "thip_hl_fma", "thip_hl_mul", "thip_hl_act", "thip_hl_elementwisebinary", "thip_hl_elementwiseunary", "thip_hl_elementwiseshift", "thip_hl_table",
-    "thip_lm_cache_write", "thip_lm_cache_read", "thip_lm_attention",
+    "thip_lm_cache_write", "thip_lm_cache_read", "thip_lm_attention", "thip_lm_tree_attention", "thip_lm_cache_keep", "thip_lm_rotary", "thip_lm_norm",
     "thip_program_serialize", "thip_blob_free",
     "thip_device_create", "thip_device_destroy", "thip_device_name", "thip_device_alloc",
     "thip_device_free", "thip_device_h2d", "thip_device_d2h", "thip_device_synchronize",
@@ -249,6 +249,25 @@ class LmAttention(ctypes.Structure):
                                                     "lengths")] + [("scale", ctypes.c_float), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
 
 
+class LmTreeAttention(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("init", "query", "key", "value", "key_scales", "value_scales", "pages", "row_starts", "lengths",
+                                                    "parents")] + [("scale", ctypes.c_float), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
+class LmCacheKeep(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("key_cache", "value_cache", "key_scales", "value_scales", "accepted", "pages", "row_starts",
+                                                    "lengths")]
+
+
+class LmRotary(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("query_out", "key_out", "query", "key", "positions", "frequencies", "axes", "interleaved")]
+
+
+class LmNorm(ctypes.Structure):
+    _fields_ = ([(name, ctypes.c_int32) for name in ("init", "residual_out", "input", "residual", "post_weight", "gate", "weight")] +
+                [(name, ctypes.c_float) for name in ("eps", "weight_offset", "residual_scale")])
+
+
 _lib = None
 
 
@@ -284,7 +303,9 @@ def lib():
                      ("thip_hl_add", HlAdd), ("thip_hl_transpose", HlTranspose),
                      ("thip_hl_expand_weights", HlExpandWeights), ("thip_hl_fma", HlFma), ("thip_hl_mul", HlMul),
                      ("thip_hl_act", HlAct), ("thip_hl_elementwisebinary", HlElementwiseBinary),
-                     ("thip_lm_cache_write", LmCacheWrite), ("thip_lm_cache_read", LmCacheRead), ("thip_lm_attention", LmAttention)]:
+                     ("thip_lm_cache_write", LmCacheWrite), ("thip_lm_cache_read", LmCacheRead), ("thip_lm_attention", LmAttention),
+                     ("thip_lm_tree_attention", LmTreeAttention), ("thip_lm_cache_keep", LmCacheKeep), ("thip_lm_rotary", LmRotary),
+                     ("thip_lm_norm", LmNorm)]:
         getattr(L, name).argtypes = [vp, P(st)]
     L.thip_program_serialize.argtypes = [vp, P(vp), P(sz)]
     L.thip_blob_free.argtypes = [vp]

@@ -371,6 +371,52 @@ class Program:
         rt.check(rt.lib().thip_lm_attention(self._h, ctypes.byref(op)))
         return init
 
+    def tree_attention(self, query, key_cache, value_cache, pages, row_starts, lengths, parents, *, scale, window=0, sinks=0, key_scales=None,
+                       value_scales=None, init=None):
+        """Attention of trees of drafted tokens, query [T, heads, D], over a paged cache that holds their keys and values already, row behind row; parents
+        (int32 [T]) says which row of its own sequence each follows, -1 the last position before the tree."""
+        init = self._init_or_new(init, query.shape, np.uint16)
+        op = rt.LmTreeAttention(init.index, query.index, key_cache.index, value_cache.index, self._index_or_none(key_scales),
+                                self._index_or_none(value_scales), self._as_value(pages).index, self._as_value(row_starts).index,
+                                self._as_value(lengths).index, self._as_value(parents).index, scale, self._positions("window", window),
+                                self._positions("sinks", sinks))
+        rt.check(rt.lib().thip_lm_tree_attention(self._h, ctypes.byref(op)))
+        return init
+
+    def cache_keep(self, key_cache, value_cache, pages, row_starts, lengths, accepted, *, key_scales=None, value_scales=None):
+        """Moves what the cache holds of the accepted drafts (int32 [S, K]: ascending rows of each sequence's tree, then -1) behind one another, in place."""
+        op = rt.LmCacheKeep(key_cache.index, value_cache.index, self._index_or_none(key_scales), self._index_or_none(value_scales),
+                            self._as_value(accepted).index, self._as_value(pages).index, self._as_value(row_starts).index,
+                            self._as_value(lengths).index)
+        rt.check(rt.lib().thip_lm_cache_keep(self._h, ctypes.byref(op)))
+
+    # ---- around a decoder's linears -----------------------------------------
+    def rotary(self, query, key, positions, frequencies, *, axes=None, interleaved=False, query_out=None, key_out=None):
+        """Turns the pairs of query's [T, heads, D] and key's [T, kv_heads, D] heads (key may be None) by positions (int32 [axes, T]) times frequencies
+        (float32 [pairs], a constant); axes (int32 [pairs], a constant) says which of the positions turn which pair.  Returns what query and key became."""
+        query_out = self._init_or_new(query_out, query.shape, np.uint16)
+        if key is not None:
+            key_out = self._init_or_new(key_out, key.shape, np.uint16)
+        if not isinstance(frequencies, Value):
+            frequencies = np.asarray(frequencies, dtype=np.float32)
+        if axes is not None and not isinstance(axes, Value):
+            axes = np.asarray(axes, dtype=np.int32)
+        op = rt.LmRotary(query_out.index, self._index_or_none(key_out), query.index, self._index_or_none(key), self._as_value(positions).index,
+                         self._as_value(frequencies).index, self._index_or_none(axes), int(bool(interleaved)))
+        rt.check(rt.lib().thip_lm_rotary(self._h, ctypes.byref(op)))
+        return query_out, key_out
+
+    def norm(self, input, weight, *, eps, weight_offset=0.0, residual=None, post_weight=None, gate=None, residual_scale=1.0, residual_out=None,
+             init=None):
+        """The norm before a block, of h = residual + residual_scale * gate * u, where u is input or, with post_weight, its own norm (the one behind the block
+        before); h goes to residual_out if that is given.  Returns the norm (None where weight is None, which leaves it out)."""
+        if weight is not None:
+            init = self._init_or_new(init, input.shape, np.uint16)
+        op = rt.LmNorm(self._index_or_none(init), self._index_or_none(residual_out), input.index, self._index_or_none(residual),
+                       self._index_or_none(post_weight), self._index_or_none(gate), self._index_or_none(weight), eps, weight_offset, residual_scale)
+        rt.check(rt.lib().thip_lm_norm(self._h, ctypes.byref(op)))
+        return init
+
     # ---- serialisation ------------------------------------------------------
     def serialize(self):
         """Returns the dispatch descriptor as ``bytes``."""
