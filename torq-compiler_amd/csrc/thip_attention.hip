@@ -1009,12 +1009,15 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
             }
         }
     };
+    // int8: a thread has 16 elements of rows qRow + Q_STEP i, which become two chunks
+    constexpr int Q_CH = DT / 16, Q_PER = KB * Q_CH / 256, Q_STEP = 256 / Q_CH;
+    const int qPiece = tid % Q_CH, qRow = tid / Q_CH, qPieceAt = qPiece * 16 < D ? qPiece * 16 : 0;
     auto flag = [&](int stage) {
         const bool some = __any(unpaged);
         if (lane == 0) flagRoom[stage * 4 + wave] = some;
-        if (piece == 0) {
+        if ((Q8 ? qPiece : piece) == 0) {
 #pragma unroll
-            for (int i = 0; i < PER; i++) absentRoom[stage * KB + myRow + STEP * i] = (gone >> i) & 1;
+            for (int i = 0; i < (Q8 ? Q_PER : PER); i++) absentRoom[stage * KB + (Q8 ? qRow + Q_STEP * i : myRow + STEP * i)] = (gone >> i) & 1;
         }
     };
     auto arrive = [&](int stage) {
@@ -1029,22 +1032,22 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
     };
     // int8: through registers, where they become bf16, every lane's rows looked up a block ahead (23 single tokens and a prompt's 777 in one batch, 16 heads of
     // 64 over 4, windows of 2048: 35 us)
-    int rows[PER], scaleRow = -1;
-    KeyAsk<PAGED> asked[PER], scaleAsked;
-    v2i kreg[PER], vreg[PER];
+    int rows[Q_PER], scaleRow = -1;
+    KeyAsk<PAGED> asked[Q_PER], scaleAsked;
+    v4i kreg[Q_PER], vreg[Q_PER];
     float sreg = 0.0f;
     bool scaleGone = false;  // of sreg's position
     bool holes = false;  // unpaged, of the rows that were looked up
     auto ask = [&](int b) {
         const int j0 = blockStart(p, span, b);
 #pragma unroll
-        for (int i = 0; i < PER; i++) asked[i] = askKey<PAGED>(a, it, j0 + myRow + STEP * i, b < span.to);
+        for (int i = 0; i < Q_PER; i++) asked[i] = askKey<PAGED>(a, it, j0 + qRow + Q_STEP * i, b < span.to);
         if constexpr (Q8) scaleAsked = askKey<PAGED>(a, it, j0 + (tid & (KB - 1)), b < span.to);
     };
     auto resolve = [&]() {
         holes = false;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
+        for (int i = 0; i < Q_PER; i++) {
             rows[i] = keyRow(a, it, asked[i]);
             if constexpr (PAGED) holes |= asked[i].page.in & (rows[i] < 0);
         }
@@ -1054,11 +1057,11 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
         gone = 0;
         unpaged = holes;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
+        for (int i = 0; i < Q_PER; i++) {
             gone |= rows[i] < 0 ? 1u << i : 0u;
-            const int64_t from = (int64_t)max(rows[i], 0) * D + pieceAt;
-            kreg[i] = *(const v2i *)((const int8_t *)a.key + from);
-            vreg[i] = *(const v2i *)((const int8_t *)a.value + from);
+            const int64_t from = (int64_t)max(rows[i], 0) * D + qPieceAt;
+            kreg[i] = *(const v4i *)((const int8_t *)a.key + from);
+            vreg[i] = *(const v4i *)((const int8_t *)a.value + from);
         }
         sreg = (tid & KB ? a.value_scales : a.key_scales)[max(scaleRow, 0)];
         scaleGone = scaleRow < 0;
@@ -1066,10 +1069,14 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
     auto put = [&](int stage) {
         int8_t *const keys = smem + stage * 2 * KB * ROW, *const values = keys + KB * ROW;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int row = myRow + STEP * i, where = row * ROW + ((piece ^ swizzle<ROW>(row)) << 4);
-            *(v8bf *)(keys + where) = wholeBf16x8(kreg[i][0], kreg[i][1]);
-            *(v8bf *)(values + where) = wholeBf16x8(vreg[i][0], vreg[i][1]);
+        for (int i = 0; i < Q_PER; i++) {
+            const int row = qRow + Q_STEP * i;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int where = row * ROW + (((2 * qPiece + c) ^ swizzle<ROW>(row)) << 4);
+                *(v8bf *)(keys + where) = wholeBf16x8(kreg[i][2 * c], kreg[i][2 * c + 1]);
+                *(v8bf *)(values + where) = wholeBf16x8(vreg[i][2 * c], vreg[i][2 * c + 1]);
+            }
         }
         if (tid < 2 * KB) scaleRoom[stage * 2 * KB + tid] = scaleGone ? 0.0f : sreg;
         flag(stage);
