@@ -1,7 +1,8 @@
 // Rotary positions of a query's and a key's heads (thip_lm_rotary).
 //
 // (a, b) -> (a cos t - b sin t, b cos t + a sin t), t the position times the pair's step.  A workgroup has a few tokens: their sines and cosines once, in LDS, then
-// all of their heads by them, 16 elements a thread at a time.  Bound by memory.
+// all of their heads by them, 16 elements a thread at a time.  Bound by memory (8192 tokens, 40 heads of 128, 168 MB: 32.9 us, 5.1 TB/s), of few tokens by the launch
+// (16 tokens of 5 heads of 256: 2.3 us, with the first elements fetched behind the angles 3.9).
 #include "thip_layer.h"
 #include "thip_kernels_common.h"
 #include "thip_lanes.h"
@@ -29,11 +30,33 @@ __device__ __forceinline__ v2f cosSin(uint32_t turn) {
     return v2f{(quarter == 1 || quarter == 2) ? -cc : cc, quarter & 2 ? -ss : ss};
 }
 
-// COPY: elements behind the pairs are copied.  Where the results lie in place of the operands they are there already.
 template <bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary(RotaryArgs a, int tokens, int pieces, FastDiv byPieces, FastDiv byHeads, FastDiv byPairs) {
     __shared__ float cosines[kMaxTokens * kMaxPairs], sines[kMaxTokens * kMaxPairs];
-    const int first = (int)blockIdx.x * tokens, here = min(tokens, a.T - first), heads = a.H + a.KVH, turned = a.pairs >> 3;
+    const int first = (int)blockIdx.x * tokens, here = min(tokens, a.T - first), heads = a.H + a.KVH, turned = a.pairs >> 3, all = here * heads * pieces;
+    // A piece: 16 elements of a head, eight pairs, or those behind the pairs as they are.
+    struct Held {
+        v4i x, y;
+        uint16_t *x_to, *y_to;
+        int angle;  // of its first pair in LDS; -1: none
+    };
+    auto fetch = [&](int i) {
+        Held h;
+        const int row = (int)fastDiv((uint32_t)i, byPieces), piece = i - row * pieces, token = (int)fastDiv((uint32_t)row, byHeads), head = row - token * heads;
+        const bool isKey = head >= a.H, turns = piece < turned;
+        const int64_t at = (isKey ? (int64_t)(first + token) * a.KVH + head - a.H : (int64_t)(first + token) * a.H + head) * a.D;
+        const int lo = INTERLEAVED || !turns ? 16 * piece : 8 * piece, hi = INTERLEAVED || !turns ? lo + 8 : a.pairs + 8 * piece;
+        const uint16_t *const from = (isKey ? a.key : a.query) + at;
+        h.x = *(const v4i *)(from + lo);
+        h.y = *(const v4i *)(from + hi);
+        h.x_to = (isKey ? a.key_out : a.query_out) + at + lo;
+        h.y_to = h.x_to + (hi - lo);
+        h.angle = turns ? token * a.pairs + 8 * piece : -1;
+        return h;
+    };
+    // the first pieces are on their way while the angles are made, each next one while one is turned
+    Held next;
+    if ((int)threadIdx.x < all) next = fetch(threadIdx.x);
     for (int i = threadIdx.x; i < here * a.pairs; i += 256) {
         const int token = (int)fastDiv((uint32_t)i, byPairs), pair = i - token * a.pairs;
         const RotaryTurn t = a.turns[pair];
@@ -42,38 +65,30 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs a, int tokens, int piec
         sines[i] = cs[1];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < here * heads * pieces; i += 256) {
-        const int row = (int)fastDiv((uint32_t)i, byPieces), piece = i - row * pieces, token = (int)fastDiv((uint32_t)row, byHeads), head = row - token * heads;
-        const bool isKey = head >= a.H;
-        const int64_t at = (isKey ? (int64_t)(first + token) * a.KVH + head - a.H : (int64_t)(first + token) * a.H + head) * a.D;
-        const uint16_t *const from = (isKey ? a.key : a.query) + at;
-        uint16_t *const to = (isKey ? a.key_out : a.query_out) + at;
-        const bool turns = piece < turned;
-        const int lo = INTERLEAVED || !turns ? 16 * piece : 8 * piece, hi = INTERLEAVED || !turns ? lo + 8 : a.pairs + 8 * piece;
-        v4i x = *(const v4i *)(from + lo), y = *(const v4i *)(from + hi);
-        if (turns) {
-            const float *const c = cosines + token * a.pairs + 8 * piece, *const s = sines + token * a.pairs + 8 * piece;
+    for (int i = threadIdx.x; i < all; i += 256) {
+        Held h = next;
+        if (i + 256 < all) next = fetch(i + 256);
+        if (h.angle >= 0) {
+            const float *const c = cosines + h.angle, *const s = sines + h.angle;
             if constexpr (INTERLEAVED) {
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const uint32_t w = (uint32_t)(k < 4 ? x[k] : y[k - 4]);
+                    const uint32_t w = (uint32_t)(k < 4 ? h.x[k] : h.y[k - 4]);
                     const float p = __uint_as_float(w << 16), q = __uint_as_float(w & 0xffff0000u);
-                    const int turned2 = packBf16(p * c[k] - q * s[k], q * c[k] + p * s[k]);
-                    if (k < 4) x[k] = turned2;
-                    else y[k - 4] = turned2;
+                    (k < 4 ? h.x : h.y)[k & 3] = packBf16(p * c[k] - q * s[k], q * c[k] + p * s[k]);
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const float p0 = __uint_as_float((uint32_t)x[k] << 16), p1 = __uint_as_float((uint32_t)x[k] & 0xffff0000u);
-                    const float q0 = __uint_as_float((uint32_t)y[k] << 16), q1 = __uint_as_float((uint32_t)y[k] & 0xffff0000u);
-                    x[k] = packBf16(p0 * c[2 * k] - q0 * s[2 * k], p1 * c[2 * k + 1] - q1 * s[2 * k + 1]);
-                    y[k] = packBf16(q0 * c[2 * k] + p0 * s[2 * k], q1 * c[2 * k + 1] + p1 * s[2 * k + 1]);
+                    const float p0 = __uint_as_float((uint32_t)h.x[k] << 16), p1 = __uint_as_float((uint32_t)h.x[k] & 0xffff0000u);
+                    const float q0 = __uint_as_float((uint32_t)h.y[k] << 16), q1 = __uint_as_float((uint32_t)h.y[k] & 0xffff0000u);
+                    h.x[k] = packBf16(p0 * c[2 * k] - q0 * s[2 * k], p1 * c[2 * k + 1] - q1 * s[2 * k + 1]);
+                    h.y[k] = packBf16(q0 * c[2 * k] + p0 * s[2 * k], q1 * c[2 * k + 1] + p1 * s[2 * k + 1]);
                 }
             }
         }
-        *(v4i *)(to + lo) = x;
-        *(v4i *)(to + hi) = y;
+        *(v4i *)h.x_to = h.x;
+        *(v4i *)h.y_to = h.y;
     }
 }
 
@@ -84,8 +99,11 @@ hipError_t launchRotary(const RotaryArgs &a, const LaunchCtx &ctx) {
     if (((uintptr_t)a.query | (uintptr_t)a.key | (uintptr_t)a.query_out | (uintptr_t)a.key_out) & 15) return hipErrorInvalidValue;
     const bool inPlace = a.query == a.query_out && a.key == a.key_out;
     const int pieces = inPlace ? a.pairs / 8 : a.D / 16, heads = a.H + a.KVH;
-    // enough for a few pieces a thread
+    // A workgroup has about four pieces a thread where there are tokens for 512 of them (8192 tokens, 40 heads of 128: 32.9 us; two a thread 33.8, eight 35.5),
+    // else fewer (777 tokens, 32 heads of 80: 3.5 us by 389 workgroups, 3.9 by 195).
     int tokens = 1024 / (pieces * heads);
+    const int share = (a.T - 1) / 512 + 1;
+    tokens = tokens < share ? tokens : share;
     tokens = tokens < 1 ? 1 : tokens > kMaxTokens ? kMaxTokens : tokens;
     const dim3 grid((unsigned)((a.T - 1) / tokens + 1));
     const FastDiv byPieces = makeFastDiv((uint32_t)pieces), byHeads = makeFastDiv((uint32_t)heads), byPairs = makeFastDiv((uint32_t)a.pairs);
