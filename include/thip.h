@@ -545,7 +545,7 @@ typedef struct thip_lm_rotary_t {
     int32_t interleaved;
 } thip_lm_rotary_t;
 
-/* The norms behind a block and before the next one, with the residual between them, row by row (the last dimension of input, N elements, 1 to 65536):
+/* The norms behind a block and before the next one, with the residual between them, row by row (the last dimension of input, N elements, 1 to 32768):
  *     u = input, or norm(input, post_weight);   h = residual + residual_scale * gate * u;   residual_out = h;   init = norm(h, weight)
  *     norm(x, w) = x / sqrt(mean(x^2) + eps) * (w + weight_offset)
  * input and init BF16; residual and residual_out BF16 or F32, each on its own; all four of input's shape.  weight and post_weight [N], BF16 or F32.  gate

@@ -6,7 +6,7 @@
 
 namespace thip {
 
-constexpr int kMaxNormRow = 65536;       // elements of a row
+constexpr int kMaxNormRow = 32768;       // elements of a row
 constexpr float kMaxRotaryStep = 16.0f;  // radians a position
 
 struct NormArgs {
