@@ -2,12 +2,14 @@
 64-bit definition (oracle/attention.py, which derives the bound that is held), and a decoder's layers that check a tree and keep its accepted path."""
 import ctypes
 import struct
+import subprocess
 
 import numpy as np
 import pytest
 
 import desc_interp
 import torq_compiler_amd as thip
+from helpers import host_check
 from oracle import attention as ref
 from oracle import layer
 from test_cache_attention import Batch, Built, _operands, _serialize_error, check_attention
@@ -192,6 +194,13 @@ def test_the_bound_tells_trees_apart():
     # a chain is attention of a chunk
     chain = ref.tree_attention(b.query, b.starts, b.lengths, plant(b, "chain"), b.cache(), b.scale, window=9, sinks=2)[0]
     assert np.allclose(chain, ref.attention(b.query, b.starts, b.scale, 9, 2, cache=b.cache(), lengths=b.lengths)[0], rtol=1e-12, atol=1e-14)
+
+
+@pytest.mark.parametrize("seed", [1, 2])
+def test_shares_of_a_launch(tmp_path, seed):
+    """The parts of a run that is cut have all of its blocks, whatever the trees, their windows and the text before them are (tests/host/tree_plan.cpp)."""
+    run = subprocess.run([host_check("tree_plan", tmp_path), str(seed)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert run.returncode == 0 and int(run.stdout) > 1000, run.stdout[-2000:]
 
 
 # ---- what is kept -------------------------------------------------------------------------------------------------------

@@ -100,7 +100,7 @@ __host__ __device__ inline int32_t partsOf(const AttentionPlan &p, int32_t block
     return parts < p.maxParts ? parts : p.maxParts;
 }
 
-// capacity: positions that a sequence can have; quantised: the cache is int8 (for the launch only, what is asked of a workspace is the same)
+// capacity: positions that a sequence can have; quantised: the cache is int8 (but for trees the launch only knows it, what is asked of a workspace is the same)
 // tree: rows of a tree at most (treeRows), 0: rows follow one another
 constexpr int kTreeRows = 512;  // THIP_LM_TREE_ROWS
 inline int64_t treeRows(int64_t T) { return T < kTreeRows ? T : kTreeRows; }
@@ -112,6 +112,17 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // take the same, with 64 streams took a third more (16 sequences of 4096 positions, four heads of 128: 56 us and 43); heads of 256 have the
     // slower tiles, and few rows of them too few (64 tokens over 4096 positions, four heads: 79 us in tiles, 42 in streams).
     p.tiles = rows > 32 * S && (D <= 128 || rows * KVH > 2048);
+    // The rows of a tree have all of the text before it to read, so few tiles are few workgroups with long runs, and streams the faster: up to 64 full tiles
+    // (of heads above 128 32, of int8 128), but where the reading takes longer than the runs do, and a tile spares it for more streams than its work costs (four; of
+    // int8, which streams read the better, six).  us, streams / tiles, by rows a sequence: 48 rows, four key heads of 128, 2479 positions 13 / 29; 512, one, 7323
+    // 21 / 46; 37, 32 sequences, eight of 80, 761 28 / 34; 342, 20 sequences, eight of 80, 434 84 / 40; 254, three sequences, eight of 256 166 / 85; 204, eight
+    // sequences, eight of 256, 3131 of int8 187 / 221; 104, 18 sequences, four of 128, 2191 59 / 40; 117, seven sequences, four of 128, 18648 260 / 120; 42, 46
+    // sequences, two of 128, 12317 of int8 128 / 245.
+    if (tree) {
+        const int64_t each = (rows - 1) / S + 1, streams = (each + 15) / 16, tiles = (each + 127) / 128, blocks = (window && window < capacity ? window : capacity) / 32;
+        p.tiles = rows > 32 * S && (rows * KVH >= (D <= 128 ? 64 : quantised ? 128 : 32) * 128 ||
+                                    (streams > (quantised ? 6 : 4) * tiles && tiles * S * KVH * blocks >= (quantised ? 16384 : 2048)));
+    }
     // The second part costs a prompt of 8192 tokens with 32 heads of 128 a third (153 us, 201 with it), four chunks of up to 512 a quarter (167, 210); the error of a
     // result goes from 1.4 times that of its rounding alone to 1.0.  Over many rows that is what it is; over few it may be 1.7 times in one call.
     p.fine = T * H < 8192;
@@ -127,8 +138,11 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // Streams cost less to join and are cut wherever they are longer than their share: a token for each of 72 sequences, eight heads of 128, one of 32768
     // positions and the others of 200: 457 / 40; all of up to 4096: 171 / 166; 65 of up to 4096: 175 / 141.  That a table has room for long runs costs
     // where there is none (256 sequences of up to 128 positions, a table for 32768: 32 / 37).
-    p.items = p.tiles ? 512 : 1024;
-    p.whole = D > 128 && !quantised ? 260 : 390;
+    // Trees: parts of 512 positions or more (eight of up to 200 rows, four heads of 64, windows of 1024: 50 / 37; a window of 40 positions, whose 16 blocks are left
+    // whole, 25 / 41 cut), and of heads above 64 so that 640 are on the chip, nothing whole that is longer (16 of up to 64 rows over up to 8192 positions of int8,
+    // 32 heads of 128 over 8: 212 / 184; two of 250 rows over 7835, 96: 112 / 98).
+    p.items = !p.tiles ? 1024 : tree && D > 64 ? 640 : 512;
+    p.whole = tree && D > 64 ? 640 : D > 128 && !quantised ? 260 : 390;
     p.maxParts = p.tiles ? 16 : 64;
     const int64_t keys = p.keys();
     const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
@@ -140,8 +154,9 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     if (window && windowed < blocks) blocks = windowed;
     // Streams: a wave of a workgroup has a block at least, but two of them none where all the parts then still are few (a token of one sequence of
     // 1024 positions with one head of 256: 12.3 us in parts of four blocks, 11.2 of two; of 32 such with a window of 512: 12 and 13.5)
-    p.minBlocks = p.tiles ? (int32_t)(2048 / keys) : most * blocks <= 256 ? 2 : 4;
-    p.fewBlocks = p.tiles ? (int32_t)(256 / keys) : p.minBlocks;
+    // (A tree's 16 rows are all there to be joined: 16 of one sequence over 1024 positions, four heads of 256, 17.6 and 16.8.)
+    p.minBlocks = p.tiles ? (int32_t)((tree ? 512 : 2048) / keys) : most * blocks <= 256 && !tree ? 2 : 4;
+    p.fewBlocks = p.tiles ? (int32_t)((tree ? 512 : 256) / keys) : p.minBlocks;
     int64_t parts = (blocks + p.fewBlocks - 1) / p.fewBlocks;
     if (parts > p.maxParts) parts = p.maxParts;
     // What is cut is settled on the device, where the lengths are.  (With more tiles than this sums of their parts might pass 31 bits where starts
@@ -158,8 +173,8 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
 // follow one another have one workspace, as long as the longest.
 constexpr uint64_t kAttentionCounterBytes = 4 * 2 * 1024;
 inline uint64_t attentionWorkspaceBytes(int64_t T, int64_t S, int64_t H, int64_t KVH, int64_t D, int64_t capacity, int64_t window, int64_t sinks,
-                                        int64_t tree = 0) {
-    const AttentionPlan p = attentionPlan(T, S, H, KVH, D, capacity, window, sinks, false, tree);
+                                        int64_t tree = 0, bool quantised = false) {
+    const AttentionPlan p = attentionPlan(T, S, H, KVH, D, capacity, window, sinks, quantised, tree);
     return p.slots ? kAttentionCounterBytes + (uint64_t)p.slots * (uint64_t)p.rows() * (uint64_t)(D + 4) * 4 : 0;
 }
 

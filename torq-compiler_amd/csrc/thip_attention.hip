@@ -1333,7 +1333,7 @@ static hipError_t checkAttention(const AttentionArgs &a) {
         return hipErrorInvalidValue;
     }
     if (a.parents && (!c.pages || a.tree_rows != treeRows(c.T))) return hipErrorInvalidValue;
-    if (a.work_bytes < attentionWorkspaceBytes(c.T, c.S, a.H, c.KVH, c.D, c.pages ? c.capacity : c.T, a.window, a.sinks, a.parents ? a.tree_rows : 0)) return hipErrorInvalidValue;
+    if (a.work_bytes < attentionWorkspaceBytes(c.T, c.S, a.H, c.KVH, c.D, c.pages ? c.capacity : c.T, a.window, a.sinks, a.parents ? a.tree_rows : 0, a.parents && a.key_scales)) return hipErrorInvalidValue;
     return hipSuccess;
 }
 

@@ -2204,7 +2204,7 @@ thip_status_t Emitter::emitAttention(const thip_lm_attention_t &c, const thip_va
         all.push_back({op.bias, (uint64_t)T * op.W * D * 2, false, "value"});
     }
     if (thip_status_t s = checkApart(all)) return s;
-    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T, op.K, op.Kp, parents ? treeRows(T) : 0)) {
+    if (const uint64_t work = attentionWorkspaceBytes(T, op.N, H, op.W, D, cached ? (int64_t)op.KW * op.KH : T, op.K, op.Kp, parents ? treeRows(T) : 0, parents && op.gran == 1)) {
         // records run one after another: they have one workspace, as long as the longest of them needs
         if (attentionWork_.space == kSpaceNone) attentionWork_ = newTemp(0);
         temps_[attentionWork_.index] = std::max(temps_[attentionWork_.index], work);
