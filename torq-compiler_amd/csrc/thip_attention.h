@@ -68,7 +68,8 @@ struct AttentionPlan {
     int32_t rowsLog, keysLog;
     int32_t windowBlocks;        // blocks that a tile can see at most (with a window)
     int32_t minBlocks, maxParts; // blocks that a part has at least, and parts of a run at most
-    int32_t fewBlocks;           // the same where few tiles are full, and of a stream among tiles
+    int32_t fewBlocks;           // the same where few tiles are full, and of a stream among tiles; of trees' streams where the launch has less than manyBlocks
+    int32_t manyBlocks, shortRun; // (0: no streams of trees) and the blocks of a run that stays whole
     bool splits;                 // runs may be cut
     int32_t items, whole;        // the launch's blocks by these: a part's, and those up to which a tile's run stays whole
     // A run of b blocks, in parts of B, is ceil(b / B) items, less than one more than b / B; the b / B of all are no more than `items`.  So there are fewer
@@ -89,8 +90,8 @@ struct PartBlocks {
 __host__ __device__ inline PartBlocks partBlocks(const AttentionPlan &p, float total, float full, int32_t KVH) {
     const float all = total * (float)KVH * 1.001f;  // sums of 32 bits
     const int32_t part = (int32_t)fminf(ceilf(all / (float)p.items), 1e8f), whole = (int32_t)fminf(ceilf(all / (float)p.whole), 1e8f);
-    const int32_t least = full * (float)KVH < 128.0f ? p.fewBlocks : p.minBlocks;
-    return {part > least ? part : least, p.tiles && whole > least ? whole : least, 4 * part > p.fewBlocks ? 4 * part : p.fewBlocks};
+    const int32_t least = (p.manyBlocks ? all < (float)p.manyBlocks : full * (float)KVH < 128.0f) ? p.fewBlocks : p.minBlocks;
+    return {part > least ? part : least, p.tiles && whole > least ? whole : p.shortRun > least ? p.shortRun : least, 4 * part > p.fewBlocks ? 4 * part : p.fewBlocks};
 }
 
 // Parts of a run.
@@ -143,7 +144,7 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // 32 heads of 128 over 8: 212 / 184; two of 250 rows over 7835, 96: 112 / 98).
     p.items = !p.tiles ? 1024 : tree && D > 64 ? 640 : 512;
     p.whole = tree && D > 64 ? 640 : D > 128 && !quantised ? 260 : 390;
-    p.maxParts = p.tiles ? 16 : 64;
+    p.maxParts = p.tiles ? 16 : tree ? 32 : 64;
     const int64_t keys = p.keys();
     const int64_t most = (rows / p.rows() + (S < T ? S : T)) * KVH;
     // a tile's window reaches over its own tokens too (in a tree, whose rows may all stand at its first position, over those before it), and its first and
@@ -154,9 +155,14 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     if (window && windowed < blocks) blocks = windowed;
     // Streams: a wave of a workgroup has a block at least, but two of them none where all the parts then still are few (a token of one sequence of
     // 1024 positions with one head of 256: 12.3 us in parts of four blocks, 11.2 of two; of 32 such with a window of 512: 12 and 13.5)
-    // (A tree's 16 rows are all there to be joined: 16 of one sequence over 1024 positions, four heads of 256, 17.6 and 16.8.)
-    p.minBlocks = p.tiles ? (int32_t)((tree ? 512 : 2048) / keys) : most * blocks <= 256 && !tree ? 2 : 4;
-    p.fewBlocks = p.tiles ? (int32_t)((tree ? 512 : 256) / keys) : p.minBlocks;
+    // Trees' streams: 16 rows that are all there cost more to join than a token's few.  So parts are of eight blocks where those of four would be more workgroups than go
+    // at once (two a CU, one of bf16 heads above 128), a run of up to eight stays whole, and one has up to 32.  us: 42 rows of two sequences over 2286 positions,
+    // eight key heads of 80, 20.8 in parts of four, 14.9 of eight; 27 of 12 sequences over 1122, two of 256, 31 / 20; 64 of one sequence over 1024, one of 256, 16.7 /
+    // 19.5; eight of 15 sequences, windows of 61, two of 96, 9.2 / 6.6 whole; 25 of one over 15087, two of 96, 64 parts 23.2, 32 18.4, 16 19.3.
+    p.minBlocks = p.tiles ? (int32_t)((tree ? 512 : 2048) / keys) : tree ? 8 : most * blocks <= 256 ? 2 : 4;
+    p.fewBlocks = p.tiles ? (int32_t)((tree ? 512 : 256) / keys) : tree ? 4 : p.minBlocks;
+    p.manyBlocks = tree && !p.tiles ? (D > 128 && !quantised ? 1024 : 2048) : 0;
+    p.shortRun = tree && !p.tiles ? 8 : 0;
     int64_t parts = (blocks + p.fewBlocks - 1) / p.fewBlocks;
     if (parts > p.maxParts) parts = p.maxParts;
     // What is cut is settled on the device, where the lengths are.  (With more tiles than this sums of their parts might pass 31 bits where starts

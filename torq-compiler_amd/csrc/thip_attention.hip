@@ -287,7 +287,7 @@ __device__ __forceinline__ v4f get4(__amdgpu_buffer_rsrc_t from, uint32_t at) {
 
 // Every thread of a workgroup that has stored its part: the last one of the run's to come here adds the parts, in their order, scaled to
 // their common maximum.  room: LDS that nobody uses any more, ROWS (PARTS + 1) floats and one.
-template <int ROWS, int PARTS>
+template <int ROWS, int PARTS, int ELEMS>
 __device__ __forceinline__ void joinParts(const AttentionArgs &a, const AttentionPlan &p, const Item &it, int rows, float *room) {
     constexpr int LANES = 256 / ROWS, EACH = PARTS / LANES;  // threads of a row, and parts of each
     const int tid = threadIdx.x, D = a.c.D, first = it.slot - it.split * a.c.KVH;
@@ -302,7 +302,7 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     if (!*last) return;
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // Several elements of a thread's and several parts at once, the first of them while the factors are made.
-    constexpr int ELEMS = ROWS == 128 ? 4 : 1, BATCH = ROWS == 128 ? 4 : 8;
+    constexpr int BATCH = ROWS == 128 ? 4 : 8;
     constexpr bool TILE = ROWS == 128;
     const int pieces = D >> 2, all = TILE ? ((rows + 31) >> 5) * 8 * D : rows * pieces;
     const uint32_t step = TILE ? tileSums(a, a.c.KVH) : slotRow(a, p, a.c.KVH, 0), sums = TILE ? tileSums(a, first) : slotRow(a, p, first, 0);
@@ -310,6 +310,7 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     auto getParts = [&](int e0, int s) {
 #pragma unroll
         for (int i = 0; i < ELEMS; i++) {
+            if (ROWS < 128 && e0 - tid + 256 * i >= all) continue;
             const int e = min(e0 + 256 * i, all - 1);
             const uint32_t from = sums + (uint32_t)(TILE ? e : e + e / pieces) * 16u;  // a stream's rows are D + 4 long
 #pragma unroll
@@ -884,7 +885,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     }
     if (it.slot >= 0) {
         __syncthreads();
-        joinParts<16, 64>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
+        joinParts<16, 64, TREE && DT == 256 ? 4 : 1>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
     }
 }
 
@@ -1290,7 +1291,7 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
     for (int r = 0; r < rowsHere; r++) {
         if (__builtin_expect((again >> r) & 1, 0)) redoRow<true, PAGED, Q8, TREE>(a, p, it, span, tree, wave * 32 + r, (float *)room);
     }
-    if (it.slot >= 0) joinParts<128, 16>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
+    if (it.slot >= 0) joinParts<128, 16, 4>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
 }
 
 template <int DT, bool PAGED, bool Q8, bool FINE>
