@@ -1,6 +1,8 @@
 """Trees of drafted tokens over a paged cache (thip_lm_tree_attention, thip_lm_cache_keep): records and refusals on the CPU, results on the GPU against the
 64-bit definition (oracle/attention.py, which derives the bound that is held), and a decoder's layers that check a tree and keep its accepted path."""
 import ctypes
+import os
+import shutil
 import struct
 import subprocess
 
@@ -14,6 +16,7 @@ from oracle import attention as ref
 from oracle import layer
 from test_cache_attention import Batch, Built, _operands, _serialize_error, check_attention
 from torq_compiler_amd import runtime as rt
+from torq_compiler_amd import workloads as w
 
 U16, I32 = np.uint16, np.int32
 KIND_TREE, KIND_KEEP = 20, 21
@@ -410,3 +413,144 @@ def test_changed_records_are_refused_or_stay_inside():
             blob[o:o + 4] = struct.pack("<I", value)
             assert status(blob) in (rt.OK, rt.INVALID_ARGUMENT)
         blob[o:o + 4] = old
+
+
+# ---- a decoder's layers that check a tree -------------------------------------------------------------------------------
+
+def _layers(b, hidden, caches, parents, accepted, expose, layers=2):
+    """Layers in one program: the norm before the block, grouped linears (int8 weights in blocks), norms of the heads, rotary positions of two axes, the cache's write,
+    attention of the tree, the linear behind, and its norm with the residual and the next layer's norm; at the end what was accepted moves together in every
+    layer's cache.  expose: what each op gives is a binding, else the program's own."""
+    rng = np.random.default_rng(19)
+    built = Built()
+    p, M = built.program, b.T
+    bf16 = lambda *shape: ref.to_bf16(rng.standard_normal(shape).astype(np.float32))  # noqa: E731
+    zero, noclamp = np.zeros(1, np.float32), dict(output_zp=0, output_min=w.NO_CLAMP[0], output_max=w.NO_CLAMP[1])
+
+    def linear(src, N, init):
+        wq, scale, qbias = w._block_quantized(rng, src.shape[1], N, 128, 1.0)
+        return p.matmul(src, p.expand_weights(wq, scale, qbias, block_size=128, output_min=w.NO_CLAMP[0], output_max=w.NO_CLAMP[1]), zero, init=init, shift=0, **noclamp)
+
+    def place(name, shape, dtype=U16):
+        return built.bind(name, np.zeros(shape, dtype)) if expose else p.tensor(shape, dtype)
+
+    positions = rng.integers(0, 10 ** 5, size=(2, M)).astype(I32)
+    frequencies = (10000.0 ** (-np.arange(b.D // 2) / (b.D // 2))).astype(np.float32)
+    axes = (np.arange(b.D // 2) // 3 % 2).astype(I32)
+    held = dict(positions=positions, frequencies=frequencies, axes=axes, norms=[])
+    stream = built.bind("stream", rng.standard_normal((M, hidden)).astype(np.float32))  # the residual, in 32 bits
+    x = built.bind("x", bf16(M, hidden))
+    starts, lengths = built.rows(b)
+    pages, up = built.bind("pages", b.pages), built.bind("parents", parents)
+    turned = built.bind("positions", positions)
+    kept = []
+    for i in range(layers):
+        weights = [bf16(n) for n in (b.D, b.D, hidden, hidden)]
+        held["norms"].append(weights)
+        q, k, v = (linear(x, h * b.D, place("%s%d" % (n, i), (M, h * b.D))) for n, h in zip(("q", "k", "v"), (b.H, b.KVH, b.KVH)))
+        q, k, v = (p.view(t, (M, h, b.D)) for t, h in zip((q, k, v), (b.H, b.KVH, b.KVH)))
+        q = p.norm(q, weights[0], eps=1e-6, init=place("qn%d" % i, (M, b.H, b.D)))
+        k = p.norm(k, weights[1], eps=1e-6, init=place("kn%d" % i, (M, b.KVH, b.D)))
+        q, k = p.rotary(q, k, turned, frequencies, axes=axes, query_out=place("qr%d" % i, (M, b.H, b.D)) if expose else q,
+                        key_out=place("kr%d" % i, (M, b.KVH, b.D)) if expose else k)
+        cache = built.bind("key_cache%d" % i, caches[i][0]), built.bind("value_cache%d" % i, caches[i][1]), pages
+        scales = dict(key_scales=built.bind("key_scales%d" % i, caches[i][2]), value_scales=built.bind("value_scales%d" % i, caches[i][3]))
+        kept.append((cache, scales))
+        p.cache_write(k, v, *cache, starts, lengths, **scales)
+        y = p.tree_attention(q, *cache, starts, lengths, up, scale=b.scale, window=90, sinks=2, init=p.view(place("y%d" % i, (M, b.H * b.D)), (M, b.H, b.D)), **scales)
+        o = linear(p.view(y, (M, b.H * b.D)), hidden, place("o%d" % i, (M, hidden)))
+        after = place("stream%d" % i, (M, hidden), np.float32) if expose else stream
+        x = p.norm(o, weights[3], eps=1e-6, weight_offset=1.0, post_weight=weights[2], residual=stream, residual_out=after, residual_scale=0.5,
+                   init=built.bind("out", np.zeros((M, hidden), U16)) if i == layers - 1 else place("x%d" % i, (M, hidden)))
+        stream = after
+    if accepted is not None:
+        rows = built.bind("accepted", accepted)
+        for cache, scales in kept:
+            p.cache_keep(*cache, starts, lengths, rows, **scales)
+    return built, held
+
+
+LAYERS = [dict(sequences=[(1, 9), (5, 30), (3, 90)], D=64, H=4, KVH=1, page=16), dict(sequences=[(8, 40), (16, 200)], D=128, H=4, KVH=2, page=16, tail=2),
+          dict(sequences=[(13, 130), (1, 1)], D=256, H=4, KVH=1, page=32)]
+
+
+def test_a_layer_s_records():
+    b = Batch(**LAYERS[0])
+    caches = [b.caches + [None, None]] * 2
+    built, _ = _layers(b, 256, caches, plant(b), np.zeros((3, 2), I32), False)
+    assert [int(o["kind"]) for o in desc_interp.Descriptor(built.program.serialize()).ops] == [15, 23, 23, 22, 17, KIND_TREE, 15, 23] * 2 + [KIND_KEEP] * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("case", LAYERS, ids=_id)
+def test_gpu_layers_that_check_a_tree(device, case, quantised):
+    """Each op of the run is checked on what the ops before it gave; the program with intermediates of its own, some of them written in place, gives the same."""
+    b, hidden = Batch(quantised=quantised, **case), 256
+    other = Batch(quantised=quantised, seed=5, garbage=False, **case)  # the second layer's has the first one's pages
+    caches = [c.caches + list(c.scales) for c in (b, other)]
+    parents = plant(b)
+    built, held = _layers(b, hidden, caches, parents, None, True)
+    got = built.run(device)
+
+    def near(name, want):
+        result, bound = want
+        have = layer.wide(got[name]).reshape(result.shape)
+        assert (np.abs(have - result) <= bound).all(), name
+
+    stream = dict(built.arrays)["stream"]
+    for i, start in enumerate((b, other)):
+        qw, kw, post, pre = held["norms"][i]
+        for n, weight in (("q", qw), ("k", kw)):
+            near("%sn%d" % (n, i), layer.norm(got["%s%d" % (n, i)].reshape(-1, b.D), weight, eps=1e-6)[0])
+            near("%sr%d" % (n, i), layer.rotary(got["%sn%d" % (n, i)].reshape(b.T, -1, b.D), held["positions"], held["frequencies"], held["axes"]))
+        cache = ref.Cache(start.caches[0], start.caches[1], b.pages, *start.scales)
+        written = ref.cache_write(cache, got["kr%d" % i].reshape(b.T, -1, b.D), got["v%d" % i].reshape(b.T, -1, b.D), b.starts, b.lengths)
+        for name, x in zip(("key_cache", "value_cache", "key_scales", "value_scales"), written):
+            if x is not None:
+                assert np.array_equal(got["%s%d" % (name, i)], x, equal_nan=x.dtype == np.float32), (name, i)
+        cache = ref.Cache(written[0], written[1], b.pages, *written[2:])
+        y = got["y%d" % i].reshape(b.T, b.H, b.D)
+        check_attention(b, y, y, ref.tree_attention(got["qr%d" % i].reshape(b.T, -1, b.D), b.starts, b.lengths, parents, cache, b.scale, 90, 2, fine=True), "layer %d" % i)
+        out = "out" if i else "x0"
+        normed, sums = layer.norm(got["o%d" % i], pre, eps=1e-6, weight_offset=1.0, post_weight=post, residual=stream, residual_scale=0.5, sum_dtype=np.float32)
+        near(out, normed)
+        near("stream%d" % i, sums)
+        stream = got["stream%d" % i]
+    inside, _ = _layers(b, hidden, caches, parents, None, False)
+    assert np.array_equal(inside.run(device)["out"], got["out"])
+    # and with what was accepted moved behind: the caches are those of the rows' own order
+    accepted = _accept(b, 6, "some", b.rng)
+    moved = _layers(b, hidden, caches, parents, accepted, False)[0].run(device)
+    assert np.array_equal(moved["out"], got["out"])
+    for i in range(2):
+        cache = ref.Cache(got["key_cache%d" % i], got["value_cache%d" % i], b.pages, got.get("key_scales%d" % i), got.get("value_scales%d" % i))
+        for name, x in zip(("key_cache", "value_cache", "key_scales", "value_scales"), ref.cache_keep(cache, accepted, b.starts, b.lengths)):
+            if x is not None:
+                assert np.array_equal(moved["%s%d" % (name, i)], x, equal_nan=x.dtype == np.float32), (name, i)
+
+
+@pytest.mark.gpu
+def test_gpu_layers_without_an_allocation(device):
+    """The same program enqueued kernel by kernel, without a graph and without an allocation, and replayed: the bits of each dispatch on fresh buffers."""
+    b = Batch(**LAYERS[1])
+    caches = [b.caches + [None, None], [x.copy() for x in b.caches] + [None, None]]
+    built, _ = _layers(b, 256, caches, plant(b), _accept(b, 4, "some", b.rng), False)
+    first = built.run(device)
+    again = built.run(device, "noalloc")
+    for name in ("out", "key_cache0", "value_cache1", "stream"):
+        assert np.array_equal(first[name], again[name]), name
+
+
+def test_programs_and_records_under_sanitizers(tmp_path):
+    """Random programs of these ops, and mutated copies of their descriptors, through the emitter and the validation built with the sanitizers."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    csrc, exe = os.path.join(root, "torq-compiler_amd", "csrc"), str(tmp_path / "layer_host")
+    built = subprocess.run([shutil.which("g++"), "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-static-libasan", "-fno-sanitize-recover=undefined", "-w",
+                            "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + csrc, os.path.join(root, "tests", "fuzz", "layer_host.cpp")] +
+                           [os.path.join(csrc, s) for s in ("thip_emitter.cpp", "thip_validate.cpp", "thip_status.cpp")] + ["-o", exe], stdout=subprocess.PIPE,
+                           stderr=subprocess.STDOUT, text=True)
+    assert built.returncode == 0, built.stdout[-3000:]
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:abort_on_error=0:verify_asan_link_order=0", UBSAN_OPTIONS="print_stacktrace=1")
+    done = subprocess.run([exe, "400", "1"], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env, timeout=300)
+    assert done.returncode == 0 and "runtime error" not in done.stdout and "AddressSanitizer" not in done.stdout, done.stdout[-4000:]
