@@ -532,7 +532,7 @@ typedef struct thip_lm_cache_keep_t {
  * positions is I32[axes, T] (a binding, a view of one, or a constant), any values; frequencies F32[pairs], a constant, radians a position, at most 16
  * in magnitude; axes I32[pairs], a constant (0 up to the axes of positions), or THIP_NO_VALUE: axis 0 for all.  Angles are taken modulo a turn in whole
  * numbers, to 2^-31 of one, so that far positions lose nothing; sines, cosines and sums are in 32 bits, a result is rounded once.  pairs is a multiple of 8, at
- * most D / 2; D a multiple of 16 up to 256.  query_out and key_out may be the query's and the key's own bytes, or lie apart from all operands.  key and
+ * most D / 2; D a multiple of 16 up to 256, T below 2^27.  query_out and key_out may be the query's and the key's own bytes, or lie apart from all operands.  key and
  * key_out are THIP_NO_VALUE where there is one tensor only. */
 typedef struct thip_lm_rotary_t {
     thip_value_t query_out;

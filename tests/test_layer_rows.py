@@ -457,6 +457,7 @@ ROTARY_REFUSED = [
     ({}, dict(axes=np.full(32, -1, I32)), rt.INVALID_ARGUMENT, "axes[0]"),
     (dict(query=((4, 1 << 21, 64), U16), query_out=((4, 1 << 21, 64), U16)), {}, rt.UNIMPLEMENTED, "heads"),
     (dict(T=1 << 31), {}, rt.UNIMPLEMENTED, "2^31"),
+    (dict(T=1 << 27, H=1), {}, rt.UNIMPLEMENTED, "2^27"),
 ]
 
 

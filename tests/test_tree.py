@@ -187,6 +187,74 @@ def test_gpu_many_sequences_of_trees(device):
         check_attention(b, built.run(device)["out"], before, want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("rows,D", [(1, 64), (3, 128), (60, 64), (60, 128), (60, 256), (600, 128)])
+def test_gpu_last_positions_of_32_bits(device, rows, D, quantised):
+    """Tables of 2^31 - 8 positions (all of their entries the same page) with trees that end there, or behind; the reference has the same rows a whole number of
+    pages further down."""
+    page, P = 8 * 127 * 113, 3 * 5 * 29 * 43
+    assert page * P == 2 ** 31 - 8
+    b = Batch([(rows, 16)], D=D, H=4, KVH=1, page=16, quantised=quantised, garbage=False)
+    shape = (1, 1, page, D)
+    if quantised:
+        b.caches = [b.rng.integers(-127, 128, size=shape, dtype=np.int8) for _ in range(2)]
+        b.scales = [(b.rng.uniform(0.5, 1.5, size=shape[:3]) / 73).astype(np.float32) for _ in range(2)]
+        b.scales[1][0, 0, page - 25] = np.nan  # a row that sees it is done again
+    else:
+        b.caches = [b.normal(*shape) for _ in range(2)]
+        b.caches[1][0, 0, page - 25] = 0x7FC0
+    parents = plant(b)
+    for length in (2 ** 31 - 8, 2 ** 31 - 1, 2 ** 31 - 37):
+        see = dict(window=16, sinks=3 if length % 2 else 0)
+        b.page, b.pages, b.lengths = page, np.zeros((1, 1), dtype=I32), np.array([length - (P - 1) * page], dtype=I32)
+        near = ref.tree_attention(b.query, b.starts, b.lengths, parents, b.cache(), b.scale, **see)
+        b.pages, b.lengths = np.zeros((1, P), dtype=I32), np.array([length], dtype=I32)
+        built, out = Built(), b.normal(b.T, b.H, b.D)
+        q = built.bind("query", b.query)
+        cache, scales = built.cache(b)
+        starts, lengths = built.rows(b)
+        built.program.tree_attention(q, *cache, starts, lengths, built.bind("parents", parents), init=built.bind("out", out), scale=b.scale, **see, **scales)
+        check_attention(b, built.run(device)["out"], out, near, str(length))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("case", [TREES[2], TREES[3], TREES[10], dict(sequences=[(120, 3000)] * 3, D=128, H=32, KVH=4, page=16)], ids=_id)
+def test_gpu_results_over_the_queries(device, case, quantised):
+    """init is the query's own bytes, also where runs are cut into parts."""
+    b = Batch(quantised=quantised, **case)
+    parents = plant(b)
+    built = Built()
+    q = built.bind("query", b.query)
+    cache, scales = built.cache(b)
+    starts, lengths = built.rows(b)
+    built.program.tree_attention(q, *cache, starts, lengths, built.bind("parents", parents), init=q, scale=b.scale, **scales)
+    check_attention(b, built.run(device)["query"], b.query, ref.tree_attention(b.query, b.starts, b.lengths, parents, b.cache(), b.scale))
+
+
+@pytest.mark.gpu
+def test_gpu_two_programs_at_once(device):
+    """Two executables dispatched from a thread each, their runs cut into parts: each has its own workspace, and the results are those of one alone."""
+    import threading
+    batches = [Batch([(16, 3000 + 100 * i), (40, 900)], D=128, H=8, KVH=2, page=16, quantised=i == 1, seed=i) for i in range(2)]
+    made = [attend_tree(b, plant(b)) for b in batches]
+    alone = [m[0].run(device)["out"] for m in made]
+    together = [None, None]
+
+    def work(i):
+        together[i] = made[i][0].run(device, dispatches=40)["out"]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        check_attention(batches[i], alone[i], made[i][1], made[i][2])
+        assert np.array_equal(alone[i], together[i])
+
+
 def test_the_bound_tells_trees_apart():
     """A row that took a neighbour's path would be seen."""
     b = Batch([(12, 40)], D=64, H=2, KVH=1)

@@ -222,11 +222,9 @@ __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPl
     Span s;
     const int r0 = it.tile << p.rowsLog, keys = p.keys();
     s.rows = min(p.rows(), it.w.count * a.G - r0);
-    int top = it.w.first + (int)fastDiv((uint32_t)r0, a.g), bottom = it.w.first + (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
-    if constexpr (TREE) {  // places; the rows may stand at any positions of the tree
-        top = it.w.first;
-        bottom = min(bottom, it.w.first + a.tree_rows - 1);
-    }
+    const int last = (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
+    // of a tree places, whose rows may stand at any positions from the first on
+    const int top = it.w.first + (TREE ? 0 : (int)fastDiv((uint32_t)r0, a.g)), bottom = it.w.first + (TREE ? min(last, a.tree_rows - 1) : last);
     const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(max(top, -1) - a.window + 1, 0) : 0;  // rows below position 0 see nothing
     auto blocksTo = [&](int end) { return (int)(((uint32_t)end + (uint32_t)keys - 1) >> p.keysLog); };  // a last block may pass 2^31
     s.sinkBlocks = blocksTo(min(min(a.sinks, low), high));
@@ -707,7 +705,7 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
     fetch(a.key, kreg);
     Tree tree{};
     if constexpr (TREE) {
-        tree = plantTree(a, it, smem, r0, span.rows, span.to > span.from && blockStart(p, span, span.to - 1) + KB > it.w.first);
+        tree = plantTree(a, it, smem, r0, span.rows, span.to > span.from && blockStart(p, span, span.to - 1) > it.w.first - KB);  // a block may end at 2^31
         pos = positionOf(tree, token);
     }
     for (int b = span.from + wave; b < span.to; b += 4) {
@@ -757,13 +755,13 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
                 for (int i = 0; i < 4; i++) s[k][i] *= u[i];
             }
         }
-        const bool whole = (TREE ? tree.all && j0 + KB <= it.w.first : j0 + KB - 1 <= top) && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        const bool whole = (TREE ? tree.all && j0 <= it.w.first - KB : j0 + KB - 1 <= top) && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
         if (!whole || (gone0 | gone1)) {
             const uint32_t window = windowOf(a);
             const int sinks = sinksOf(a, pos);
             uint32_t path = 0;  // of the 32 keys from j0 + 4 quarter on
             if constexpr (TREE) {
-                if (j0 + KB > it.w.first) path = seenFrom(tree, token, j0 + 4 * quarter - it.w.first);
+                if (j0 > it.w.first - KB) path = seenFrom(tree, token, j0 + 4 * quarter - it.w.first);
             }
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -1103,7 +1101,7 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
     }
     Tree tree{};
     if constexpr (TREE) {
-        tree = plantTree(a, it, smem, it.tile * 128, span.rows, span.to > span.from && blockStart(p, span, span.to - 1) + KB > it.w.first);
+        tree = plantTree(a, it, smem, it.tile * 128, span.rows, span.to > span.from && blockStart(p, span, span.to - 1) > it.w.first - KB);
         pos = positionOf(tree, min(token, tree.token0 + (int)fastDiv((uint32_t)(it.tile * 128 + span.rows - 1), a.g) - tree.token0));
     }
     for (int b = span.from, stage = 0; b < span.to; b++, stage ^= 1) {
@@ -1153,7 +1151,7 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
                 }
             }
         }
-        bool whole = (TREE ? tree.all && j0 + KB <= it.w.first : j0 + KB - 1 <= top) && j0 <= it.w.length - KB && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        bool whole = (TREE ? tree.all && j0 <= it.w.first - KB : j0 + KB - 1 <= top) && j0 <= it.w.length - KB && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
         bool gaps = false;
         if constexpr (PAGED) gaps = __builtin_amdgcn_readfirstlane(*(const int *)(flagRoom + stage * 4)) != 0;
         if (!whole || gaps) {

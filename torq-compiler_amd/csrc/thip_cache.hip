@@ -270,7 +270,7 @@ hipError_t launchCacheKeep(const CacheKeepArgs &a, const LaunchCtx &ctx) {
     if (((uintptr_t)a.key_cache | (uintptr_t)a.value_cache) & 15) return hipErrorInvalidValue;
     const bool q8 = a.key_scales != nullptr;
     const int64_t columns = 2 * (int64_t)c.KVH * (q8 ? c.D / 16 + 1 : c.D / 8), chunks = (columns - 1) / 64 + 1;
-    if (columns >= (1LL << 31) - 64 || chunks * c.S >= (1LL << 31)) return hipErrorInvalidValue;
+    if (columns >= (1LL << 31) - 64 || chunks * c.S >= (1LL << 26)) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(chunks * c.S));
     if (q8) THIP_ENQUEUE(ctx, kernelLabel("cache_keep", {1}), cache_keep<true>, grid, dim3(64), 0, a, (int)chunks);
     else THIP_ENQUEUE(ctx, kernelLabel("cache_keep", {0}), cache_keep<false>, grid, dim3(64), 0, a, (int)chunks);

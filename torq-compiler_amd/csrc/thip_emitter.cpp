@@ -2232,7 +2232,7 @@ thip_status_t Emitter::emitCacheKeep(const thip_lm_cache_keep_t &c) {
     const Value &accepted = prog_.values[(size_t)c.accepted];
     if (accepted.shape[0] != op.N) return fail(THIP_INVALID_ARGUMENT, "accepted rows of %lld sequences, row_starts has %d", (long long)accepted.shape[0], op.N);
     if (!fitsInt32(accepted.shape[1] + 64)) return fail(THIP_UNIMPLEMENTED, "accepted: %lld entries for a sequence", (long long)accepted.shape[1]);
-    if (!fitsInt32((int64_t)op.N * ((2 * (int64_t)op.W * (op.C / 8 + 1) - 1) / 64 + 1))) return fail(THIP_UNIMPLEMENTED, "%d sequences of %d heads are too many", op.N, op.W);
+    if ((int64_t)op.N * ((2 * (int64_t)op.W * (op.C / 8 + 1) - 1) / 64 + 1) >= (1 << 26)) return fail(THIP_UNIMPLEMENTED, "%d sequences of %d heads are too many", op.N, op.W);
     op.K = (int32_t)accepted.shape[1];
     op.out = op.weights;
     std::vector<Extent> all{{ext.rows, (uint64_t)op.N * op.K * 4, false, "accepted"}};
@@ -2272,6 +2272,7 @@ thip_status_t Emitter::emitRotary(const thip_lm_rotary_t &c) {
     if (!fitsInt32(T) || !fitsInt32(H) || !fitsInt32(T * H) || (KVH && (!fitsInt32(KVH) || !fitsInt32(T * KVH)))) return fail(THIP_UNIMPLEMENTED, "more than 2^31 rows");
     if (D % 16 != 0 || D > kMaxHeadDim) return fail(THIP_UNIMPLEMENTED, "rows of %lld elements: multiples of 16 up to %d", (long long)D, kMaxHeadDim);
     if ((H + KVH) * D >= (1 << 26)) return fail(THIP_UNIMPLEMENTED, "%lld heads of %lld elements", (long long)(H + KVH), (long long)D);
+    if (T >= 1 << 27) return fail(THIP_UNIMPLEMENTED, "query: %lld rows, up to 2^27 are", (long long)T);
     if (thip_status_t s = constantData(c.frequencies, "frequencies", THIP_DTYPE_F32, &freq)) return s;
     const int64_t pairs = freq->numel();
     if (freq->rank != 1 || pairs % 8 != 0 || 2 * pairs > D) {

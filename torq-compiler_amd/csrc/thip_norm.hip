@@ -142,6 +142,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : 256) void norm(NormArgs a, int
     auto part = [&](const void *from, int64_t at, int e, int bytes) { return fetch<KIND>((const int8_t *)from + at * bytes, columnOf(e), a.N, bytes); };
     Piece post[EACH], weight[EACH];
     for (int t = 0; t < turns; t++) {
+        if (LANES > 64 && t > 0) __syncthreads();  // what the row before had in the room has been read
         int64_t row = ((int64_t)t * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / LANES;
         const bool idle = row >= a.rows;  // takes part in the sums of its wave, and stores nothing
         if (idle) row = a.rows - 1;
@@ -227,9 +228,9 @@ hipError_t launchNorm(const NormArgs &a, const LaunchCtx &ctx) {
         constexpr RowKind KIND = decltype(kind)::value;
         constexpr bool WIDE = decltype(wide)::value;
         // rows of a wave at most go by several a workgroup, with the weights in its registers, where there would be more than 4096 workgroups (131072 rows of 128
-        // 12.5 us, a workgroup for each of its rows 13.3, 2048 workgroups 12.9)
+        // 12.5 us, a workgroup for each of its rows 13.3, 2048 workgroups 12.9); longer rows where a grid would have no room for them
         const int64_t groups = ((int64_t)a.rows - 1) / ROWS + 1;
-        const int turns = LANES > 64 ? 1 : (int)((groups - 1) / 4096 + 1);
+        const int turns = (int)((groups - 1) / (LANES > 64 ? 1 << 20 : 4096) + 1);
         const dim3 grid((unsigned)((groups - 1) / turns + 1));
         THIP_ENQUEUE(ctx, kernelLabel("norm", {LANES, EACH, KIND, WIDE}), (norm<LANES, EACH, KIND, WIDE>), grid, dim3(THREADS), 0, a, turns);
     };

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs a, int tokens, int piec
 
 hipError_t launchRotary(const RotaryArgs &a, const LaunchCtx &ctx) {
     if (a.T < 1 || a.H < 1 || a.KVH < 0 || a.D < 16 || a.D > 2 * kMaxPairs || a.D % 16 != 0 || a.pairs < 8 || a.pairs % 8 != 0 || 2 * a.pairs > a.D) return hipErrorInvalidValue;
-    if ((int64_t)a.T * a.H >= (1LL << 31) || (int64_t)a.T * a.KVH >= (1LL << 31) || (int64_t)(a.H + a.KVH) * a.D >= (1LL << 26)) return hipErrorInvalidValue;
+    if (a.T >= 1 << 27 || (int64_t)a.T * a.H >= (1LL << 31) || (int64_t)a.T * a.KVH >= (1LL << 31) || (int64_t)(a.H + a.KVH) * a.D >= (1LL << 26)) return hipErrorInvalidValue;
     if (!a.query || !a.query_out || !a.positions || !a.turns || (a.KVH > 0) != (a.key != nullptr) || !a.key != !a.key_out) return hipErrorInvalidValue;
     if (((uintptr_t)a.query | (uintptr_t)a.key | (uintptr_t)a.query_out | (uintptr_t)a.key_out) & 15) return hipErrorInvalidValue;
     const bool inPlace = a.query == a.query_out && a.key == a.key_out;

@@ -450,7 +450,7 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
                 memcpy(&tree, e->blob + e->header.data_offset + e->consts[op.table.index].offset + op.table.offset, sizeof(tree));
                 if ((s = checkLooseRef(e, i, tree.rows))) return s;
                 if (tree.rows.space == kSpaceTemp || (tree.rows.offset & 3)) return fail(THIP_INVALID_ARGUMENT, "op %u: bad operand of a tree", i);
-                if (keeps && (op.K <= 0 || op.K > 0x7fffffff - 64 || mul(op.N, (2 * (int64_t)op.W * (op.C / 8 + 1) - 1) / 64 + 1) >= (1ull << 31))) {
+                if (keeps && (op.K <= 0 || op.K > 0x7fffffff - 64 || mul(op.N, (2 * (int64_t)op.W * (op.C / 8 + 1) - 1) / 64 + 1) >= (1ull << 26))) {
                     return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of accepted rows", i);
                 }
                 if ((s = need(tree.rows, keeps ? mul(op.N, op.K) * 4 : (uint64_t)op.M * 4, "rows of a tree"))) return s;
@@ -482,7 +482,7 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
     }
     case kKindRotary: {
         if (!positive({op.M, op.N, op.H, op.C, op.K}) || op.W < 0 || op.C % 16 != 0 || op.C > kMaxHeadDim || op.K % 8 != 0 || op.K > op.C / 2 ||
-            mul(op.M, op.H) >= (1ull << 31) || mul(op.M, op.W) >= (1ull << 31) || mul((int64_t)op.H + op.W, op.C) >= (1ull << 26)) {
+            op.M >= 1 << 27 || mul(op.M, op.H) >= (1ull << 31) || mul(op.M, op.W) >= (1ull << 31) || mul((int64_t)op.H + op.W, op.C) >= (1ull << 26)) {
             return fail(THIP_INVALID_ARGUMENT, "op %u: bad extents of rotary positions", i);
         }
         if (((op.in0.offset | op.in1.offset | op.out.offset | op.weights.offset) & 15) || (op.scale.offset & 3)) return fail(THIP_INVALID_ARGUMENT, "op %u: misaligned operand", i);
