@@ -547,3 +547,28 @@ def test_changed_records_are_refused_or_stay_inside():
             assert status(blob) == rt.INVALID_ARGUMENT
             blob[o:o + 4] = old
     assert status(blob) == rt.OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1544, 1601])
+def test_gpu_norm_of_more_rows_than_workgroups(device, N):
+    """Workgroups that go through several rows of more than a wave: the rows of each turn, and that of two turns' scales apart (large values in one, small in the other)."""
+    rng = np.random.default_rng(N)
+    rows = 65536 + 65536 // 2 + 1
+    some = bf16(rng, 1024, N)
+    x = np.tile(some, (rows // 1024 + 1, 1))[:rows]
+    odd = np.array([5, 65536 + 5, 65536 + 6, 70000])
+    x[odd] = ref.to_bf16((ref.from_bf16(x[odd]) * np.array([2.0 ** 70, 2.0 ** -70, 2.0 ** 80, 0.0])[:, None]).astype(F32))
+    a = dict(input=x, weight=bf16(rng, N), post_weight=bf16(rng, N))
+    built = Built()
+    v = {name: built.bind(name, y) for name, y in a.items()}
+    built.program.norm(v["input"], v["weight"], post_weight=v["post_weight"], eps=1e-6, init=built.bind("out", np.zeros((rows, N), U16)))
+    got = built.run(device)["out"]
+    look = np.unique(np.concatenate([odd, odd - 1, odd + 1, [0, 65535, 65536, rows - 2, rows - 1], rng.integers(0, rows, 300)]))
+    within(got[look], ref.norm(x[look], a["weight"], eps=1e-6, post_weight=a["post_weight"])[0], "some rows")
+    plain = np.ones(rows, dtype=bool)
+    plain[odd] = False
+    first = got[1024:2048]  # the same rows again and again: the same bits
+    for r in range(0, rows - 1024, 1024):
+        same = plain[r:r + 1024]
+        assert np.array_equal(got[r:r + 1024][same], first[same]), r

@@ -230,7 +230,7 @@ hipError_t launchNorm(const NormArgs &a, const LaunchCtx &ctx) {
         // rows of a wave at most go by several a workgroup, with the weights in its registers, where there would be more than 4096 workgroups (131072 rows of 128
         // 12.5 us, a workgroup for each of its rows 13.3, 2048 workgroups 12.9); longer rows where a grid would have no room for them
         const int64_t groups = ((int64_t)a.rows - 1) / ROWS + 1;
-        const int turns = (int)((groups - 1) / (LANES > 64 ? 1 << 20 : 4096) + 1);
+        const int turns = (int)((groups - 1) / (LANES > 64 ? 1 << 16 : 4096) + 1);
         const dim3 grid((unsigned)((groups - 1) / turns + 1));
         THIP_ENQUEUE(ctx, kernelLabel("norm", {LANES, EACH, KIND, WIDE}), (norm<LANES, EACH, KIND, WIDE>), grid, dim3(THREADS), 0, a, turns);
     };
