@@ -551,8 +551,8 @@ def test_changed_records_are_refused_or_stay_inside():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("N", [1544, 1601])
-def test_gpu_norm_of_more_rows_than_workgroups(device, N):
-    """Workgroups that go through several rows of more than a wave: the rows of each turn, and that of two turns' scales apart (large values in one, small in the other)."""
+def test_gpu_norm_of_rows_for_a_wider_grid(device, N):
+    """So many rows of more than a wave that the grid has two dimensions: the same bits for the same row wherever it lies, rows far apart in size next to others."""
     rng = np.random.default_rng(N)
     rows = 65536 + 65536 // 2 + 1
     some = bf16(rng, 1024, N)

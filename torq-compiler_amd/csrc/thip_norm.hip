@@ -142,8 +142,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : 256) void norm(NormArgs a, int
     auto part = [&](const void *from, int64_t at, int e, int bytes) { return fetch<KIND>((const int8_t *)from + at * bytes, columnOf(e), a.N, bytes); };
     Piece post[EACH], weight[EACH];
     for (int t = 0; t < turns; t++) {
-        if (LANES > 64 && t > 0) __syncthreads();  // what the row before had in the room has been read
-        int64_t row = ((int64_t)t * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / LANES;
+        int64_t row = (((int64_t)t * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / LANES;
         const bool idle = row >= a.rows;  // takes part in the sums of its wave, and stores nothing
         if (idle) row = a.rows - 1;
         const int64_t begin = row * a.N;
@@ -223,21 +222,26 @@ hipError_t launchNorm(const NormArgs &a, const LaunchCtx &ctx) {
     if (a.rows < 1 || a.N < 1 || a.N > kMaxNormRow || !a.input || (!a.sum && !a.out) || !a.out != !a.weight) return hipErrorInvalidValue;
     const auto size = [](const void *p, int bytes) { return !p || bytes == 2 || bytes == 4; };
     if (!size(a.residual, a.residual_bytes) || !size(a.sum, a.sum_bytes) || !size(a.weight, a.weight_bytes) || !size(a.post_weight, a.post_bytes)) return hipErrorInvalidValue;
-    const auto enqueueWidth = [&](auto lanes, auto each, auto kind, auto wide) {
+    bool fits = true;
+    const auto enqueueWidth = [&](auto lanes, auto each, auto kind, auto wideCode) {
         constexpr int LANES = decltype(lanes)::value, EACH = decltype(each)::value, THREADS = LANES > 64 ? LANES : 256, ROWS = THREADS / LANES;
         constexpr RowKind KIND = decltype(kind)::value;
-        constexpr bool WIDE = decltype(wide)::value;
+        constexpr bool WIDE = decltype(wideCode)::value;
         // rows of a wave at most go by several a workgroup, with the weights in its registers, where there would be more than 4096 workgroups (131072 rows of 128
-        // 12.5 us, a workgroup for each of its rows 13.3, 2048 workgroups 12.9); longer rows where a grid would have no room for them
+        // 12.5 us, a workgroup for each of its rows 13.3, 2048 workgroups 12.9).  A long row has a workgroup, and
+        // many of them a grid of two dimensions, as one holds 2^32 threads.
         const int64_t groups = ((int64_t)a.rows - 1) / ROWS + 1;
-        const int turns = (int)((groups - 1) / (LANES > 64 ? 1 << 16 : 4096) + 1);
-        const dim3 grid((unsigned)((groups - 1) / turns + 1));
+        const int turns = LANES > 64 ? 1 : (int)((groups - 1) / 4096 + 1);
+        const int64_t blocks = (groups - 1) / turns + 1, high = (blocks - 1) / 32768 + 1;
+        fits = high <= 65535;
+        if (!fits) return;
+        const dim3 grid((unsigned)((blocks - 1) / high + 1), (unsigned)high);
         THIP_ENQUEUE(ctx, kernelLabel("norm", {LANES, EACH, KIND, WIDE}), (norm<LANES, EACH, KIND, WIDE>), grid, dim3(THREADS), 0, a, turns);
     };
     using std::integral_constant;
-    const bool wide = (a.residual && a.residual_bytes == 4) || (a.sum && a.sum_bytes == 4) || (a.weight && a.weight_bytes == 4) || (a.post_weight && a.post_bytes == 4);
+    const bool wideRows = (a.residual && a.residual_bytes == 4) || (a.sum && a.sum_bytes == 4) || (a.weight && a.weight_bytes == 4) || (a.post_weight && a.post_bytes == 4);
     const auto enqueueKind = [&](auto lanes, auto each, auto kind) {
-        if (wide) enqueueWidth(lanes, each, kind, std::true_type{});
+        if (wideRows) enqueueWidth(lanes, each, kind, std::true_type{});
         else enqueueWidth(lanes, each, kind, std::false_type{});
     };
     const auto enqueue = [&](auto lanes, auto each) {
@@ -262,6 +266,7 @@ hipError_t launchNorm(const NormArgs &a, const LaunchCtx &ctx) {
     else if (pieces <= 1024) enqueue(integral_constant<int, 512>{}, integral_constant<int, 2>{});
     else if (pieces <= 2048) enqueue(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
     else enqueue(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+    if (!fits) return hipErrorInvalidValue;
     return ctx.name ? hipSuccess : hipGetLastError();
 }
 
