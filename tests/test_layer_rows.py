@@ -11,9 +11,10 @@ import torq_compiler_amd as thip
 from oracle import layer as ref
 from test_cache_attention import Built, _serialize_error
 from torq_compiler_amd import runtime as rt
+from torq_compiler_amd.workloads import NO_CLAMP
 
 U16, F32, I32 = np.uint16, np.float32, np.int32
-KIND_ROTARY, KIND_NORM = 22, 23
+KIND_TRANSPOSE, KIND_EXPAND, KIND_ROTARY, KIND_NORM = 1, 13, 22, 23
 
 
 def _id(case):
@@ -317,6 +318,63 @@ def test_norm_refused_calls():
 
     assert _serialize_error(undefined)[0] == rt.FAILED_PRECONDITION
     assert rt.lib().thip_lm_norm(None, None) == rt.INVALID_ARGUMENT
+
+
+def _written_over(by, what):
+    """A product of x [4, 64] and what an op in front of it made (a transpose, expanded weights), written over by a norm or a rotary turn.  The program and its operands."""
+    rng = np.random.default_rng(9)
+    built = Built()
+    x, other = bf16(rng, 4, 64), bf16(rng, 64, 48)
+    p = built.program
+    made = p.tensor((64, 48), U16)
+    if what == "transpose":
+        p.transpose(built.bind("source", bf16(rng, 48, 64)), (1, 0), init=made)
+    else:
+        scale, bias = bf16(rng, 2, 48), np.zeros((2, 48), F32)
+        p.expand_weights(rng.integers(-128, 128, (64, 48)).astype(np.int8), scale, bias, block_size=32, output_min=NO_CLAMP[0], output_max=NO_CLAMP[1], init=made)
+    v = built.bind("other", other)
+    if by == "norm":
+        weight = ref.to_bf16(np.ones(48, F32))
+        p.norm(v, built.bind("weight", weight), eps=1e-6, init=made)
+        held = ref.to_bf16(ref.norm(other, weight, eps=1e-6, weight_offset=0.0)[0][0].astype(F32))
+    elif by == "sum":
+        p.norm(v, None, eps=1e-6, residual_out=made)
+        held = other
+    out = built.bind("out", np.zeros((4, 48), U16))
+    p.matmul(built.bind("x", x), made, np.array([0.0], F32), init=out, output_zp=0, output_min=NO_CLAMP[0], output_max=NO_CLAMP[1], shift=0)
+    return built, x, held
+
+
+@pytest.mark.parametrize("by", ["norm", "sum"])
+@pytest.mark.parametrize("what", ["transpose", "expand"])
+def test_norm_over_what_a_product_would_have_folded(by, what):
+    """The op whose result is written over stays a record of its own: a product that took it into itself would read what was there before."""
+    built, _, _ = _written_over(by, what)
+    kinds = [int(o["kind"]) for o in desc_interp.Descriptor(built.program.serialize()).ops]
+    assert kinds[:2] == [dict(transpose=KIND_TRANSPOSE, expand=KIND_EXPAND)[what], KIND_NORM], kinds
+
+
+def test_rotary_over_what_a_product_would_have_folded():
+    p = thip.Program()
+    made = p.transpose(p.binding(0, (3, 48, 64), U16), (0, 2, 1))
+    p.rotary(p.binding(1, (3, 64, 48), U16), None, p.binding(2, (1, 3), I32), np.ones(8, F32), query_out=made)
+    p.matmul(p.binding(3, (3, 4, 64), U16), made, np.array([0.0], F32), init=p.binding(4, (3, 4, 48), U16), output_zp=0, output_min=NO_CLAMP[0],
+             output_max=NO_CLAMP[1], shift=0)
+    kinds = [int(o["kind"]) for o in desc_interp.Descriptor(p.serialize()).ops]
+    assert kinds[:2] == [KIND_TRANSPOSE, KIND_ROTARY], kinds
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", ["norm", "sum"])
+@pytest.mark.parametrize("what", ["transpose", "expand"])
+def test_gpu_norm_over_what_a_product_would_have_folded(device, by, what):
+    built, x, held = _written_over(by, what)
+    got = ref.wide(built.run(device, "device")["out"])
+    # of each operand of the sum half a step of bf16 (the norm's), of the result another, of 64 products the sum's roundings in 32 bits
+    a, b = ref.wide(x), ref.wide(held)
+    want, size = a @ b, np.abs(a) @ np.abs(b)
+    bound = size * (2.0 ** -8 * (2 if by == "norm" else 0) + 64 * 2.0 ** -24) + np.abs(want) * 2.0 ** -8
+    assert (np.abs(got - want) <= bound * 1.01).all()
 
 
 # ---- rotary positions ---------------------------------------------------------------------------------------------------

@@ -2902,8 +2902,9 @@ void Emitter::planExpandFolding() {
         case kLmAttention: read(op.u.at.query); read(op.u.at.key); read(op.u.at.value); read(op.u.at.init); break;
         case kLmTreeAttention: read(op.u.ta.query); read(op.u.ta.key); read(op.u.ta.value); read(op.u.ta.init); break;
         case kLmCacheKeep: read(op.u.ck.key_cache); read(op.u.ck.value_cache); break;
-        case kLmRotary: read(op.u.ro.query); read(op.u.ro.key); break;
-        case kLmNorm: for (thip_value_t v : normReads(op.u.no)) read(v); break;
+        // what they write over has a use before and one behind, and no op's result may be taken for what is read there
+        case kLmRotary: read(op.u.ro.query); read(op.u.ro.key); read(op.u.ro.query_out); read(op.u.ro.key_out); break;
+        case kLmNorm: for (thip_value_t v : normReads(op.u.no)) read(v); read(op.u.no.init); read(op.u.no.residual_out); break;
         }
     }
     valueReads_ = reads;
