@@ -282,7 +282,6 @@ __device__ __forceinline__ v4f get4(__amdgpu_buffer_rsrc_t from, uint32_t at) {
     return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, 0, kDeviceScope));
 }
 
-
 // Every thread of a workgroup that has stored its part: the last one of the run's to come here adds the parts, in their order, scaled to
 // their common maximum.  room: LDS that nobody uses any more, ROWS (PARTS + 1) floats and one.
 template <int ROWS, int PARTS, int ELEMS>
@@ -299,7 +298,9 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     __syncthreads();
     if (!*last) return;
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // Several elements of a thread's and several parts at once, the first of them while the factors are made.
+    // Several elements of a thread's and several parts at once, the first of them while the factors are made.  Of a stream's 16 rows one element, as
+    // the registers of more leave room for fewer workgroups (trees of 42 rows over 2286 positions, eight key heads of 80: 16.1 us, with four 17.8); but four in
+    // trees' heads of 256, of which a CU has one workgroup in any case, and 16 rows' parts to join (16 rows over 1024 positions 17.3 us, with four 16.8).
     constexpr int BATCH = ROWS == 128 ? 4 : 8;
     constexpr bool TILE = ROWS == 128;
     const int pieces = D >> 2, all = TILE ? ((rows + 31) >> 5) * 8 * D : rows * pieces;
@@ -308,7 +309,7 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
     auto getParts = [&](int e0, int s) {
 #pragma unroll
         for (int i = 0; i < ELEMS; i++) {
-            if (ROWS < 128 && e0 - tid + 256 * i >= all) continue;
+            if (ROWS < 128 && ELEMS > 1 && e0 - tid + 256 * i >= all) continue;
             const int e = min(e0 + 256 * i, all - 1);
             const uint32_t from = sums + (uint32_t)(TILE ? e : e + e / pieces) * 16u;  // a stream's rows are D + 4 long
 #pragma unroll
@@ -1292,9 +1293,13 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
     if (it.slot >= 0) joinParts<128, 16, 4>(a, p, it, span.rows, (float *)smem + 4 * kMaxHeadDim);
 }
 
+// What a plan has for trees is known to the other kernels when they are compiled: a call of few us waits for each instruction more.
+__device__ __forceinline__ void withoutTrees(AttentionPlan *p) { p->manyBlocks = p->shortRun = 0; }
+
 template <int DT, bool PAGED, bool Q8, bool FINE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
 void attention_tiles(AttentionArgs a, AttentionPlan p) {
+    withoutTrees(&p);
     tileItem<DT, PAGED, Q8, FINE, false>(a, p);
 }
 
@@ -1308,6 +1313,7 @@ template <int DT, bool EXACT, bool PAGED, bool Q8>
 __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_stream(AttentionArgs a, AttentionPlan p) {
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     Item it;
+    withoutTrees(&p);
     if (findItem(a, p, blockIdx.x, &it, smem)) streamItem<DT, EXACT, PAGED, Q8, false>(a, p, it);
 }
 
