@@ -41,6 +41,7 @@ __device__ __forceinline__ bool sees(uint32_t window, int sinks, int p, int j) {
 struct SeqWork {
     int begin, count, first, length, tiles, blocks;
 };
+__device__ __forceinline__ int blocksTo(const AttentionPlan &p, int end) { return (int)(((uint32_t)end + (uint32_t)p.keys() - 1) >> p.keysLog); }  // a last block may pass 2^31
 __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const AttentionPlan &p, int s) {
     const CacheArgs &c = a.c;
     SeqWork w;
@@ -50,8 +51,15 @@ __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const Atte
     if (s >= c.S) w.count = 0;
     w.length = c.pages ? min(w.first + w.count, c.capacity) : w.count;
     w.tiles = (int)(((uint32_t)w.count * (uint32_t)a.G + (uint32_t)p.rows() - 1) >> p.rowsLog);
-    w.blocks = (int)(((uint32_t)w.length + (uint32_t)p.keys() - 1) >> p.keysLog);
+    w.blocks = blocksTo(p, w.length);
     if (a.window) w.blocks = min(w.blocks, p.windowBlocks);
+    if (a.window && a.tree_rows) {
+        // what the last tile reads (spanOf); trees of a batch differ, and parts that are cut for the widest would be left empty (eight of up to 200 rows, windows
+        // of 1024: 37.2 us, so 36.7; 33 to 60 tokens of ten sequences, eight heads of 128, windows of 40 41 and 25)
+        const int high = max(min(w.first + min(w.count, a.tree_rows), w.length), 0), low = max(max(w.first, -1) - a.window + 1, 0);
+        const int sinkBlocks = blocksTo(p, min(min(a.sinks, low), high));
+        w.blocks = min(w.blocks, sinkBlocks + max(blocksTo(p, high) - max(low >> p.keysLog, sinkBlocks), 0));
+    }
     return w;
 }
 
@@ -220,16 +228,15 @@ struct Span {
 template <bool TREE>
 __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPlan &p, const Item &it) {
     Span s;
-    const int r0 = it.tile << p.rowsLog, keys = p.keys();
+    const int r0 = it.tile << p.rowsLog;
     s.rows = min(p.rows(), it.w.count * a.G - r0);
     const int last = (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
     // of a tree places, whose rows may stand at any positions from the first on
     const int top = it.w.first + (TREE ? 0 : (int)fastDiv((uint32_t)r0, a.g)), bottom = it.w.first + (TREE ? min(last, a.tree_rows - 1) : last);
     const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(max(top, -1) - a.window + 1, 0) : 0;  // rows below position 0 see nothing
-    auto blocksTo = [&](int end) { return (int)(((uint32_t)end + (uint32_t)keys - 1) >> p.keysLog); };  // a last block may pass 2^31
-    s.sinkBlocks = blocksTo(min(min(a.sinks, low), high));
+    s.sinkBlocks = blocksTo(p, min(min(a.sinks, low), high));
     s.windowBlock = max(low >> p.keysLog, s.sinkBlocks);
-    const int all = s.sinkBlocks + max(blocksTo(high) - s.windowBlock, 0);
+    const int all = s.sinkBlocks + max(blocksTo(p, high) - s.windowBlock, 0);
     s.from = min(it.splits > 1 ? it.split * it.part : 0, all);
     s.to = it.splits > 1 ? min(all, s.from + it.part) : all;
     return s;
@@ -373,73 +380,90 @@ __device__ __forceinline__ void joinParts(const AttentionArgs &a, const Attentio
 
 // ---- trees -------------------------------------------------------------------------------------------------------------
 
-// What a workgroup knows of its tree, in LDS: the parents of the sequence's rows, then for each token of its tile the position in the text at which it stands
-// (-1: it sees nothing) and a bit for each row of its path that it sees.  A path ascends from its row, parents below children, so a lane that follows it has
-// a word's bits together before it stores them; windows are taken off here, where a row's depth is known, and cost the blocks of keys nothing.
+// What a workgroup knows of its tree, in LDS: for each row of the sequence up to its tile's last where the run of rows that ends in it begins (each the next one's
+// parent, all in one word of a path) and that one's parent; then for each token of its tile the position in the text at which it stands (-1: it sees nothing) and a bit for
+// each row of its path that it sees.  A lane follows its token's path by runs, so that a chain takes a step a word; windows are taken off here, where a row's depth is
+// known, and cost the blocks of keys nothing.  (Row by row, with the words held back until they were whole: eight trees of 200 rows over 264 positions, 16 heads of 64 over
+// 4: 22.2 us, so 21.3.)
 struct Tree {
     const int32_t *position;  // [tokens]
     const uint32_t *seen;     // [tokens][stride]
     int words, stride, token0;
     bool all;                 // every row of the tile stands somewhere
+    int bottom;               // with a window: none of them stands further down
 };
 __host__ __device__ constexpr int treeWords(int rows) { return (rows + 31) / 32; }
 __host__ __device__ constexpr int treeStride(int rows) { return treeWords(rows) | 1; }  // odd: 32 rows at one word are in as many banks
-__host__ __device__ constexpr int treeBytes(int rows, int tokens) { return 4 * (rows + tokens * (1 + treeStride(rows))); }
+__host__ __device__ constexpr int treeBytes(int rows, int tokens) { return 4 * (1 + rows + tokens * (1 + treeStride(rows))); }
 
 // Every thread of the workgroup calls it.  paths: the item has keys of the tree, so the seen rows are asked for.
 __device__ __forceinline__ Tree plantTree(const AttentionArgs &a, const Item &it, int8_t *smem, int r0, int rows, bool paths) {
-    int32_t *const parents = (int32_t *)(smem + a.tree_at);
-    const int tid = threadIdx.x, count = min(it.w.count, a.tree_rows), base = it.w.first;
+    int32_t *const deepest = (int32_t *)(smem + a.tree_at);
+    uint32_t *const runs = (uint32_t *)(deepest + 1);  // a row's run: its first row, the parent of that + 1 in the upper half
+    const int tid = threadIdx.x, lane = tid & 63, count = min(it.w.count, a.tree_rows), base = it.w.first;
     Tree t;
     t.words = treeWords(a.tree_rows);
     t.stride = treeStride(a.tree_rows);
     t.token0 = (int)fastDiv((uint32_t)r0, a.g);
     const int tokens = (int)fastDiv((uint32_t)(r0 + rows - 1), a.g) - t.token0 + 1;
-    int32_t *const position = parents + a.tree_rows;
+    int32_t *const position = (int32_t *)(runs + a.tree_rows);
     uint32_t *const seen = (uint32_t *)(position + tokens);
     t.position = position;
     t.seen = seen;
     t.all = base + t.token0 >= 0 && t.token0 + tokens <= count;
     const bool walks = paths || a.window;
     if (walks) {
-        for (int i = tid; i < min(count, t.token0 + tokens); i += 256) {
-            const int parent = a.parents[it.w.begin + i];
-            parents[i] = parent < i ? max(parent, -1) : -1;
+        const int needed = min(count, t.token0 + tokens);
+        for (int first = tid - lane; first < needed; first += 256) {
+            const int i = first + lane;
+            int parent = i < needed ? a.parents[it.w.begin + i] : -1;
+            parent = parent < i ? max(parent, -1) : -1;
+            const uint64_t linked = __ballot((lane & 31) && parent == i - 1);
+            const uint32_t ends = ~(uint32_t)(linked >> (lane & 32)) & ((2u << (lane & 31)) - 1);  // rows of the word up to this one that begin a run
+            const int begin = (lane & 32) + 31 - __builtin_clz(ends);
+            const int above = __shfl(parent, begin);
+            if (i < needed) runs[i] = (uint32_t)(first + begin) | (uint32_t)(above + 1) << 16;
         }
+        if (paths) {
+            for (int i = tid; i < tokens * t.stride; i += 256) seen[i] = 0;
+        }
+        if (tid == 0) *deepest = -1;
         __syncthreads();
     }
     if (tid < tokens) {
         const int row = t.token0 + tid;
         const bool stands = row < count && base + row >= 0;
-        int here = -1, depth = 0;
+        uint32_t *const mine = seen + tid * t.stride;
+        int here = -1, depth = -1;
+        auto bits = [](int from, int to) { return (2u << (to & 31)) - (1u << (from & 31)); };
         if (stands) {
-            if (a.window) {
-                for (int r = parents[row]; r >= 0; r = parents[r]) depth++;
+            if (walks) {
+                for (int r = row; r >= 0;) {
+                    const uint32_t run = runs[r];
+                    const int first = (int)(run & 0xffff);
+                    if (paths) __hip_atomic_fetch_or(mine + (r >> 5), bits(first, r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    depth += r - first + 1;
+                    r = (int)(run >> 16) - 1;
+                }
             }
             here = base + (a.window ? depth : row);
         }
         position[tid] = here;
-        if (walks) {
-            // rows of the path below (row, depth) that the window still holds: those at low or above; with sinks those below `sinks` too
-            uint32_t word = 0;
-            int at = t.words - 1;
-            uint32_t *const mine = seen + tid * t.stride;
-            if (stands) {
-                for (int r = row, back = 0; r >= 0; r = parents[r], back++) {
-                    for (; at > r >> 5; at--) {
-                        mine[at] = word;
-                        word = 0;
-                    }
-                    if (a.window == 0 || back < a.window || here - back < a.sinks) word |= 1u << (r & 31);
-                }
-            }
-            for (; at >= 0; at--) {
-                mine[at] = word;
-                word = 0;
+        if (a.window) __hip_atomic_fetch_max(deepest, here, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (paths && a.window && depth >= a.window) {
+            // rows of the path that lie `back` below this one: those from the window's end on are not seen, up to those of the first positions
+            const int last = here < a.sinks ? -1 : here - a.sinks;
+            for (int r = row, back = 0; r >= 0;) {
+                const uint32_t run = runs[r];
+                const int first = (int)(run & 0xffff), from = max(back, a.window), to = min(back + r - first, last);
+                if (from <= to) __hip_atomic_fetch_and(mine + (r >> 5), ~bits(r - (to - back), r - (from - back)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                back += r - first + 1;
+                r = (int)(run >> 16) - 1;
             }
         }
     }
     __syncthreads();
+    t.bottom = a.window ? __builtin_amdgcn_readfirstlane(*deepest) : 0;
     return t;
 }
 __device__ __forceinline__ int positionOf(const Tree &t, int token) { return t.position[token - t.token0]; }
@@ -449,6 +473,19 @@ __device__ __forceinline__ uint32_t seenFrom(const Tree &t, int token, int first
     const int w = first >> 5;
     const uint32_t lo = (uint32_t)w < (uint32_t)t.words ? mine[w] : 0u, hi = (uint32_t)(w + 1) < (uint32_t)t.words ? mine[w + 1] : 0u;
     return (uint32_t)((((uint64_t)hi << 32) | lo) >> (first & 31));
+}
+
+// Which of the 32 positions from `from` on a token at `pos` sees, a bit each: those of the text in front of the tree that are in its window or among the first ones, and the
+// tree's (near: there may be some).  In words: where a lane read and compared four at a time, the trees above took 21.3 us, so 16.5 (a chunk of as many rows 12.3); with
+// windows of 1024 over up to 4096 positions 35.2 and 31.3; 16 trees of up to 64 rows over up to 8192 positions of int8, 32 heads of 128 over 8, 171 and 159.
+__device__ __forceinline__ uint32_t seenBits(const AttentionArgs &a, const Tree &t, const Item &it, int token, int pos, int from, bool near) {
+    const auto upTo = [&](int end) {  // the positions before `end`; a last block may pass 2^31
+        const int n = (int)((uint32_t)end - (uint32_t)from);
+        return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+    };
+    uint32_t text = pos < 0 ? 0u : upTo(it.w.first);
+    if (a.window) text &= ~upTo(max(pos - a.window + 1, 0)) | upTo(a.sinks);
+    return near ? text | seenFrom(t, token, (int)((uint32_t)from - (uint32_t)it.w.first)) : text;
 }
 
 // ---- one row, key by key ----------------------------------------------------------------------------------------------
@@ -756,21 +793,19 @@ __device__ __forceinline__ void streamItem(const AttentionArgs &a, const Attenti
                 for (int i = 0; i < 4; i++) s[k][i] *= u[i];
             }
         }
-        const bool whole = (TREE ? tree.all && j0 <= it.w.first - KB : j0 + KB - 1 <= top) && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        const bool whole = (TREE ? tree.all && j0 <= it.w.first - KB : j0 + KB - 1 <= top) && (a.window == 0 || (TREE ? min(bottom, tree.bottom) : bottom) - j0 < a.window || j0 + KB <= a.sinks);
         if (!whole || (gone0 | gone1)) {
             const uint32_t window = windowOf(a);
             const int sinks = sinksOf(a, pos);
-            uint32_t path = 0;  // of the 32 keys from j0 + 4 quarter on
-            if constexpr (TREE) {
-                if (j0 > it.w.first - KB) path = seenFrom(tree, token, j0 + 4 * quarter - it.w.first);
-            }
+            uint32_t seen = 0;  // of the 32 keys from j0 + 4 quarter on
+            if constexpr (TREE) seen = seenBits(a, tree, it, token, pos, j0 + 4 * quarter, j0 > it.w.first - KB);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = 4 * quarter + i, j = j0 + 16 * k + key;
                     bool see = sees(window, sinks, pos, j) & !(((k ? gone1 : gone0) >> key) & 1);
-                    if constexpr (TREE) see = (j < it.w.first ? sees(window, sinks, pos, j) : ((path >> (16 * k + i)) & 1) != 0) & !(((k ? gone1 : gone0) >> key) & 1);
+                    if constexpr (TREE) see = ((seen >> (16 * k + i)) & 1) & !(((k ? gone1 : gone0) >> key) & 1);
                     s[k][i] = see ? s[k][i] : -INFINITY;
                 }
             }
@@ -1152,7 +1187,7 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
                 }
             }
         }
-        bool whole = (TREE ? tree.all && j0 <= it.w.first - KB : j0 + KB - 1 <= top) && j0 <= it.w.length - KB && (a.window == 0 || bottom - j0 < a.window || j0 + KB <= a.sinks);
+        bool whole = (TREE ? tree.all && j0 <= it.w.first - KB : j0 + KB - 1 <= top) && j0 <= it.w.length - KB && (a.window == 0 || (TREE ? min(bottom, tree.bottom) : bottom) - j0 < a.window || j0 + KB <= a.sinks);
         bool gaps = false;
         if constexpr (PAGED) gaps = __builtin_amdgcn_readfirstlane(*(const int *)(flagRoom + stage * 4)) != 0;
         if (!whole || gaps) {
@@ -1160,20 +1195,18 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
             const uint32_t window = windowOf(a);
 #pragma unroll
             for (int k = 0; k < KB / 32; k++) {
+                uint32_t seen = 0;  // of the 32 keys from j0 + 32 k + 4 half on
+                if constexpr (TREE) seen = seenBits(a, tree, it, token, at, j0 + 32 * k + 4 * half, j0 > it.w.first - KB);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int j = j0 + k * 32 + 8 * i + 4 * half;
-                    uint32_t path = 0;
-                    if constexpr (TREE) {
-                        if (j + 3 >= it.w.first) path = seenFrom(tree, token, j - it.w.first);
-                    }
                     uint32_t missing = 0;  // a byte a position
                     if constexpr (PAGED) missing = *(const uint32_t *)(absentRoom + stage * KB + k * 32 + 8 * i + 4 * half);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const bool there = PAGED ? !(missing & (0xffu << (8 * e))) : j + e < it.w.length;
                         bool see = sees(window, sinks, at, j + e);
-                        if constexpr (TREE) see = j + e < it.w.first ? see : ((path >> e) & 1) != 0;
+                        if constexpr (TREE) see = (seen >> (8 * i + e)) & 1;
                         s[k][4 * i + e] = (see & there) ? s[k][4 * i + e] : -INFINITY;
                     }
                 }
@@ -1294,12 +1327,12 @@ __device__ __forceinline__ void tileItem(const AttentionArgs &a, const Attention
 }
 
 // What a plan has for trees is known to the other kernels when they are compiled: a call of few us waits for each instruction more.
-__device__ __forceinline__ void withoutTrees(AttentionPlan *p) { p->manyBlocks = p->shortRun = 0; }
+__device__ __forceinline__ void withoutTrees(AttentionArgs *a, AttentionPlan *p) { a->tree_rows = p->manyBlocks = p->shortRun = 0; }
 
 template <int DT, bool PAGED, bool Q8, bool FINE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTileWaves<DT, Q8>, kTileWaves<DT, Q8>)))
 void attention_tiles(AttentionArgs a, AttentionPlan p) {
-    withoutTrees(&p);
+    withoutTrees(&a, &p);
     tileItem<DT, PAGED, Q8, FINE, false>(a, p);
 }
 
@@ -1313,7 +1346,7 @@ template <int DT, bool EXACT, bool PAGED, bool Q8>
 __global__ __launch_bounds__(256, DT == 256 && !Q8 ? 1 : 2) void attention_stream(AttentionArgs a, AttentionPlan p) {
     extern __shared__ __attribute__((aligned(16))) int8_t smem[];
     Item it;
-    withoutTrees(&p);
+    withoutTrees(&a, &p);
     if (findItem(a, p, blockIdx.x, &it, smem)) streamItem<DT, EXACT, PAGED, Q8, false>(a, p, it);
 }
 
