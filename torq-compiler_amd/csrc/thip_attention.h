@@ -115,10 +115,9 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     p.tiles = rows > 32 * S && (D <= 128 || rows * KVH > 2048);
     // The rows of a tree have all of the text before it to read, so few tiles are few workgroups with long runs, and streams the faster: up to 64 full tiles
     // (of heads above 128 32, of int8 128), but where the reading takes longer than the runs do, and a tile spares it for more streams than its work costs (four; of
-    // int8, which streams read the better, six).  us, streams / tiles, by rows a sequence: 48 rows, four key heads of 128, 2479 positions 13 / 29; 512, one, 7323
-    // 21 / 46; 37, 32 sequences, eight of 80, 761 28 / 34; 342, 20 sequences, eight of 80, 434 84 / 40; 254, three sequences, eight of 256 166 / 85; 204, eight
-    // sequences, eight of 256, 3131 of int8 187 / 221; 104, 18 sequences, four of 128, 2191 59 / 40; 117, seven sequences, four of 128, 18648 260 / 120; 42, 46
-    // sequences, two of 128, 12317 of int8 128 / 245.
+    // int8, which streams read the better, six).  us, streams / tiles, by rows a sequence: 48 rows, four key heads of 128, 2479 positions of int8 13 / 39; 512, one, 7323
+    // 17 / 50; 342, 20 sequences, eight of 80, 434 69 / 37; 254, three sequences, eight of 256 167 / 78; 204, eight sequences, eight of 256, 3131 of int8 188 / 213; 117,
+    // seven sequences, four of 128, 18648 260 / 122; 42, 46 sequences, two of 128, 12317 of int8 126 / 207.  Not the faster side: 37, 32 sequences, eight of 80, 761 of int8 30 / 34.
     if (tree) {
         const int64_t each = (rows - 1) / S + 1, streams = (each + 15) / 16, tiles = (each + 127) / 128, blocks = (window && window < capacity ? window : capacity) / 32;
         p.tiles = rows > 32 * S && (rows * KVH >= (D <= 128 ? 64 : quantised ? 128 : 32) * 128 ||
@@ -139,9 +138,9 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // Streams cost less to join and are cut wherever they are longer than their share: a token for each of 72 sequences, eight heads of 128, one of 32768
     // positions and the others of 200: 457 / 40; all of up to 4096: 171 / 166; 65 of up to 4096: 175 / 141.  That a table has room for long runs costs
     // where there is none (256 sequences of up to 128 positions, a table for 32768: 32 / 37).
-    // Trees: parts of 512 positions or more (eight of up to 200 rows, four heads of 64, windows of 1024: 50 / 37; a window of 40 positions, whose 16 blocks are left
-    // whole, 25 / 41 cut), and of heads above 64 so that 640 are on the chip, nothing whole that is longer (16 of up to 64 rows over up to 8192 positions of int8,
-    // 32 heads of 128 over 8: 212 / 184; two of 250 rows over 7835, 96: 112 / 98).
+    // Trees: parts of 512 positions or more (eight of up to 200 rows, four heads of 64, windows of 1024: 31.4, of 256 31.8, of 1024 32.9, of 2048 40.6), and of heads above 64
+    // so that 640 are on the chip, nothing whole that is longer (16 of up to 64 rows over up to 8192 positions of int8, 32 heads of 128 over 8: 185 with up to half of
+    // that whole, so 159).
     p.items = !p.tiles ? 1024 : tree && D > 64 ? 640 : 512;
     p.whole = tree && D > 64 ? 640 : D > 128 && !quantised ? 260 : 390;
     p.maxParts = p.tiles ? 16 : tree ? 32 : 64;
@@ -157,8 +156,8 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     // 1024 positions with one head of 256: 12.3 us in parts of four blocks, 11.2 of two; of 32 such with a window of 512: 12 and 13.5)
     // Trees' streams: 16 rows that are all there cost more to join than a token's few.  So parts are of eight blocks where those of four would be more workgroups than go
     // at once (two a CU, one of bf16 heads above 128), a run of up to eight stays whole, and one has up to 32.  us: 42 rows of two sequences over 2286 positions,
-    // eight key heads of 80, 20.8 in parts of four, 14.9 of eight; 27 of 12 sequences over 1122, two of 256, 31 / 20; 64 of one sequence over 1024, one of 256, 16.7 /
-    // 19.5; eight of 15 sequences, windows of 61, two of 96, 9.2 / 6.6 whole; 25 of one over 15087, two of 96, 64 parts 23.2, 32 18.4, 16 19.3.
+    // eight key heads of 80, 16.3 in parts of four, 14.3 of eight; 27 of 12 sequences over 1122, two of 256, 32 / 20; 64 of one sequence over 1024, one of 256, 16.7 /
+    // 19.3; 16 of 15 sequences over up to 256, two of 96, 9.6 / 8.7 whole; 25 of one over 15087, two of 96, 64 parts 21.7, 32 17.9, 16 19.7.
     p.minBlocks = p.tiles ? (int32_t)((tree ? 512 : 2048) / keys) : tree ? 8 : most * blocks <= 256 ? 2 : 4;
     p.fewBlocks = p.tiles ? (int32_t)((tree ? 512 : 256) / keys) : tree ? 4 : p.minBlocks;
     p.manyBlocks = tree && !p.tiles ? (D > 128 && !quantised ? 1024 : 2048) : 0;
