@@ -713,7 +713,8 @@ class Emitter {
     thip_status_t emitMaxPool(const thip_hl_maxpool2d_t &c);
     thip_status_t emitAvgPool(const thip_hl_avg_pool2d_t &c);
     thip_status_t emitAdd(const thip_hl_add_t &c);
-    thip_status_t emitTransposeOp(const thip_hl_transpose_t &c);
+    thip_status_t emitTransposeOp(const thip_hl_transpose_t &c, size_t at);
+    bool writtenBehind(size_t at, thip_value_t v) const;
     thip_status_t emitExpandWeights(const thip_hl_expand_weights_t &c);
     thip_status_t emitFma(const thip_hl_fma_t &c);
     thip_status_t emitMul(const thip_hl_mul_t &c);
@@ -1891,7 +1892,7 @@ thip_status_t Emitter::emitAdd(const thip_hl_add_t &c) {
     return THIP_OK;
 }
 
-thip_status_t Emitter::emitTransposeOp(const thip_hl_transpose_t &c) {
+thip_status_t Emitter::emitTransposeOp(const thip_hl_transpose_t &c, size_t at) {
     const char *what = "torq_hl.transpose";
     const Value *x, *init;
     if (thip_status_t s = checkValue(c.input, "torq_hl.transpose input", &x)) return s;
@@ -1924,8 +1925,8 @@ thip_status_t Emitter::emitTransposeOp(const thip_hl_transpose_t &c) {
     DescRef in;
     if (thip_status_t s = literalInput(c.input, "torq_hl.transpose input", &in)) return s;
     const bool inNhwcOfNchw = state_[c.input].nhwcOfNchw;
-    if (init->kind == kValueTensor) {
-        // Fold with the layout the producer already wrote.
+    // Fold with the layout the producer already wrote: the result is the input's own bytes, which nothing may write behind this (an op in place, or into a part).
+    if (init->kind == kValueTensor && !writtenBehind(at, c.input) && !writtenBehind(at, c.init)) {
         if (toNhwc && inNhwcOfNchw) {
             state_[c.init] = state_[c.input];
             state_[c.init].nhwcOfNchw = false;  // literal N,H,W,C now
@@ -2485,6 +2486,16 @@ bool Emitter::shareBytes(thip_value_t a, thip_value_t b) const {
     return same && x.begin < y.end && y.begin < x.end;
 }
 
+// Whether an op behind `at` writes bytes of a value.
+bool Emitter::writtenBehind(size_t at, thip_value_t v) const {
+    for (size_t w = at + 1; w < prog_.ops.size(); w++) {
+        for (thip_value_t written : writtenBy(prog_.ops[w])) {
+            if (shareBytes(written, v)) return true;
+        }
+    }
+    return false;
+}
+
 void Emitter::planDecodeFolding() {
     foldedTranspose_.clear();
     consumed_.assign(prog_.ops.size(), 0);
@@ -2985,7 +2996,7 @@ thip_status_t Emitter::run(void **outBlob, size_t *outSize) {
         case kHlMaxPool: s = emitMaxPool(op.u.mp); break;
         case kHlAvgPool: s = emitAvgPool(op.u.ap); break;
         case kHlAdd: s = emitAdd(op.u.add); break;
-        case kHlTranspose: s = emitTransposeOp(op.u.tr); break;
+        case kHlTranspose: s = emitTransposeOp(op.u.tr, at); break;
         case kHlExpandWeights: s = emitExpandWeights(op.u.ew); break;
         case kHlFma: s = emitFma(op.u.fma); break;
         case kHlMul: s = emitMul(op.u.mul); break;
