@@ -1,5 +1,7 @@
 """Transposes whose result lies in memory as their input does take no record: the result is the input's own bytes.  Where an op writes over either of the
-two, they have to be apart: records on the CPU, results on the GPU."""
+two, they have to be apart: records on the CPU, results on the GPU.  No record writes to a constant."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -10,7 +12,7 @@ from test_cache_attention import Built
 from torq_compiler_amd import runtime as rt
 
 U16, I32 = np.uint16, np.int32
-KIND_TRANSPOSE, KIND_NORM = 1, 23
+KIND_TRANSPOSE, KIND_READ, KIND_ROTARY, KIND_NORM = 1, 18, 22, 23
 SHAPE, TO, TURNED = (2, 4, 64, 1), (0, 3, 1, 2), (2, 1, 4, 64)  # rows, columns, channels: one channel, so the bytes stay
 
 
@@ -164,3 +166,34 @@ def test_programs_that_write_nothing_over_take_no_record_for_them():
     p.norm(back, p.constant(np.full(1, 0x3F80, U16)), eps=1.0, init=p.binding(2, SHAPE, U16))
     kinds = [int(o["kind"]) for o in desc_interp.Descriptor(p.serialize()).ops]
     assert kinds.count(KIND_NORM) == 2 and kinds[0] == KIND_NORM
+
+
+def test_records_that_write_to_a_constant_are_refused():
+    """What a norm, a rotary turn, an attention or a cache's read writes may not be a constant's bytes, which the next dispatch reads."""
+    p = thip.Program()
+    q = p.binding(0, (4, 2, 64), U16)
+    x = p.binding(1, (1, 512), U16)
+    p.norm(x, p.constant(np.zeros(512, U16)), eps=1e-6, residual=x, residual_out=p.binding(2, (1, 512), U16), init=p.binding(3, (1, 512), U16))
+    p.rotary(q, p.binding(4, (4, 2, 64), U16), np.zeros((1, 4), I32), np.ones(32, np.float32), query_out=p.binding(5, (4, 2, 64), U16), key_out=p.binding(6, (4, 2, 64), U16))
+    p.attention(q, q, q, p.binding(7, (2,), I32), scale=0.125, init=p.binding(8, (4, 2, 64), U16))
+    cache, pages, lengths = p.binding(9, (3, 2, 16, 64), U16), p.binding(10, (1, 3), I32), p.binding(11, (1,), I32)
+    p.tree_attention(q, cache, cache, pages, p.binding(7, (2,), I32), lengths, p.binding(12, (4,), I32), scale=0.125, init=p.binding(8, (4, 2, 64), U16))
+    p.cache_read(cache, cache, pages, p.binding(7, (2,), I32), lengths, key=p.binding(13, (4, 2, 64), U16), value=p.binding(14, (4, 2, 64), U16))
+    blob = bytearray(p.serialize())
+    d = desc_interp.Descriptor(bytes(blob))
+
+    def status():
+        words = (ctypes.c_uint64 * (len(blob) // 8 + 1))()  # 8-byte aligned
+        ctypes.memmove(words, bytes(blob), len(blob))
+        return rt.lib().thip_descriptor_validate(words, len(blob))
+
+    assert status() == rt.OK
+    assert [int(o["kind"]) for o in d.ops] == [KIND_NORM, KIND_ROTARY, 19, 20, KIND_READ]
+    constant = d.ops[0]["weights"].tobytes()  # as long as each result
+    for op, field in ((0, "out"), (0, "table"), (1, "out"), (1, "weights"), (2, "out"), (3, "out"), (4, "out"), (4, "in1")):
+        o = int(d.header["ops_offset"]) + op * d.ops.dtype.itemsize + d.ops.dtype.fields[field][1]
+        old = bytes(blob[o:o + 16])
+        blob[o:o + 16] = constant
+        assert status() == rt.INVALID_ARGUMENT, (op, field)
+        blob[o:o + 16] = old
+    assert status() == rt.OK

@@ -174,6 +174,11 @@ thip_status_t checkOpFootprint(const DescriptorView *e, uint32_t i) {
     };
     const uint64_t outElem = op.out_dtype == THIP_DTYPE_I32 ? 4 : op.out_dtype == THIP_DTYPE_I16 ? 2 : 1;
     thip_status_t s = THIP_OK;
+    // constants are uploaded once: what a dispatch wrote there the next one would read
+    const DescRef none{kSpaceNone, 0, 0};
+    for (const DescRef &r : {op.out, op.kind == kKindNorm ? op.table : none, op.kind == kKindRotary ? op.weights : none, op.kind == kKindCacheRead ? op.in1 : none}) {
+        if (r.space == kSpaceConst) return fail(THIP_INVALID_ARGUMENT, "op %u: writes to a constant", i);
+    }
     switch (op.kind) {
     case kKindTranspose: {
         if (!positive({op.TB, op.TR, op.TS})) return fail(THIP_INVALID_ARGUMENT, "op %u: bad transpose extents", i);
