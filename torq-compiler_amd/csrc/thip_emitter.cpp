@@ -138,6 +138,7 @@ class Emitter {
     std::vector<uint64_t> temps_;
     std::vector<std::vector<uint8_t>> consts_;
     std::map<uint32_t, DescBinding> bindings_;
+    std::map<uint32_t, std::vector<std::pair<uint64_t, uint64_t>>> writtenParts_;  // [begin, end) in bytes
     // Physical channel count of an intermediate whose channels are padded to a multiple of 16
     // (0 = stored as declared).  See planChannelPadding.
     std::vector<int> valueReads_;  // per value: how many op inputs name it (planExpandFolding fills it)
@@ -184,12 +185,27 @@ class Emitter {
         return DescRef{kSpaceConst, (uint32_t)(consts_.size() - 1), 0};
     }
 
-    DescRef bindingRef(const Value &v, bool written) {
+    // part: what of it is written, where that is not all.
+    DescRef bindingRef(const Value &v, bool written, const Value *part = nullptr) {
         DescBinding &b = bindings_[v.binding];
+        const uint64_t size = elemSize(v.dtype), begin = part ? (uint64_t)part->viewOffset * size : 0;
         b.id = v.binding;
         b.flags |= written ? kBindingWritten : kBindingRead;
-        b.size = std::max<uint64_t>(b.size, (uint64_t)v.numel() * elemSize(v.dtype));
+        b.size = std::max<uint64_t>(b.size, (uint64_t)v.numel() * size);
+        if (written) writtenParts_[v.binding].push_back({begin, begin + (uint64_t)(part ? part : &v)->numel() * size});
         return DescRef{kSpaceBinding, v.binding, 0};
+    }
+
+    // A binding of which only parts are written is read too: the rest keeps what it holds, also where the dispatch works on a copy on the device that comes back whole.
+    void markPartlyWritten() {
+        for (auto &kv : writtenParts_) {
+            std::sort(kv.second.begin(), kv.second.end());
+            uint64_t whole = 0;  // up to here
+            for (const auto &part : kv.second) {
+                if (part.first <= whole) whole = std::max(whole, part.second);
+            }
+            if (whole < bindings_[kv.first].size) bindings_[kv.first].flags |= kBindingRead;
+        }
     }
 
     // Reference to the bytes of an input value exactly as declared.
@@ -343,7 +359,7 @@ class Emitter {
                 if (state_[v->base].nhwcOfNchw) return fail(THIP_UNIMPLEMENTED, "%s: a view of an N,C,H,W intermediate", what);
                 *out = state_[v->base].ref;
             } else {
-                *out = bindingRef(b, true);
+                *out = bindingRef(b, true, v);
             }
             out->offset += (uint64_t)v->viewOffset * elemSize(dtype);
         } else if (v->kind == kValueTensor) {
@@ -3017,6 +3033,7 @@ thip_status_t Emitter::run(void **outBlob, size_t *outSize) {
     }
     if (ops_.empty()) return fail(THIP_INVALID_ARGUMENT, "program has no ops");
     fuseResidualAdd();
+    markPartlyWritten();
 
     // Binding ids must be dense 0..n-1 so the dispatch's binding table indexes directly.
     uint32_t bindingCount = 0;
