@@ -99,7 +99,8 @@ __device__ __forceinline__ float rowSum(float v, float *room) {
     return v;
 }
 
-// 1 / sqrt(mean(x^2) + eps).  Where the squares would leave 32 bits, x becomes x by a power of two, and the factor is that of this.
+// 1 / sqrt(mean(x^2) + eps).  Where the squares would leave 32 bits, they are taken of x by a power of two.  Small x becomes that, and the factor is that of this: what small x
+// is can pass 32 bits.  Large x stays, as its small elements would leave 32 bits by it, and the factor is scaled back (2^-128 at least, of which 32 bits hold 21).
 template <int LANES, int EACH>
 __device__ __forceinline__ float factorOf(float (&x)[EACH][8], float count, float eps, float *room) {
     float sum = 0.0f;
@@ -110,20 +111,24 @@ __device__ __forceinline__ float factorOf(float (&x)[EACH][8], float count, floa
     }
     float mean = rowSum<LANES>(sum, room) / count + eps;
     const bool odd = !(mean >= 0x1p-100f && mean <= 0x1p120f);
-    if (__builtin_expect(__any(odd), 0)) {  // the waves of a row have the same mean
-        const float by = !odd ? 1.0f : mean > 1.0f ? 0x1p-100f : 0x1p100f;
+    float back = 1.0f;
+    if (__builtin_expect(__any(odd), 0)) {  // the waves of a row have the same mean; factors of 1, as a selection takes registers (256 lanes of two pieces: 131, so 125)
+        const bool large = odd && mean > 1.0f;
+        const float up = odd && !large ? 0x1p100f : 1.0f;
+        back = large ? 0x1p-100f : 1.0f;
         sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[e][i] *= by;
-                sum = fmaf(x[e][i], x[e][i], sum);
+                x[e][i] *= up;
+                const float y = x[e][i] * back;
+                sum = fmaf(y, y, sum);
             }
         }
-        mean = rowSum<LANES>(sum, room + 16) / count + eps * by * by;
+        mean = rowSum<LANES>(sum, room + 16) / count + eps * up * up * back * back;
     }
-    return __builtin_amdgcn_rsqf(mean);
+    return __builtin_amdgcn_rsqf(mean) * back;
 }
 
 // LANES lanes a row, EACH pieces a lane: LANES apart, so that what a wave loads lies together.  All operands are asked for at once while registers last.
