@@ -1,9 +1,12 @@
 """Trees of drafted tokens whose rows go by tiles of 128 (thip_lm_tree_attention): what a key head's rows are so many for, or what there is so much text in front of, that
 the launch takes tree_attention_tiles.  Every test makes sure of that by the kernel's name."""
+import subprocess
+
 import numpy as np
 import pytest
 
 import torq_compiler_amd as thip
+from helpers import host_check
 from oracle import attention as ref
 from test_cache_attention import Batch, Built, check_attention
 from test_tree import attend_tree, plant
@@ -229,3 +232,14 @@ def test_gpu_last_positions_of_32_bits(device, D, H, quantised):
         starts, lengths = built.rows(b)
         built.program.tree_attention(q, *cache, starts, lengths, built.bind("parents", parents), init=built.bind("out", out), scale=b.scale, **see, **scales)
         check_attention(b, run(device, built)["out"], out, near, str(length))
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_blocks_of_a_tile(tmp_path, seed):
+    """By the kernels' own arithmetic: a tile reads every position that its rows can see, and the parts of a run that is cut have all of its blocks
+    (tests/host/tree_blocks.cpp); a count that were one block short is found."""
+    exe = host_check("tree_blocks", tmp_path)
+    run = subprocess.run([exe, str(seed)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert run.returncode == 0 and int(run.stdout) > 1000, run.stdout[-2000:]
+    short = subprocess.run([exe, str(seed), "short"], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert short.returncode == 1 and "FAIL" in short.stdout and "blocks, the sequence counts" in short.stdout, short.stdout[-2000:]

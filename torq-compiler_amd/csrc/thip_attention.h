@@ -81,6 +81,34 @@ struct AttentionPlan {
     __host__ __device__ int32_t keys() const { return 1 << keysLog; }
 };
 
+// Blocks in front of position `end`; a last block may pass 2^31.
+__host__ __device__ inline int32_t blocksTo(const AttentionPlan &p, int32_t end) { return (int32_t)(((uint32_t)end + (uint32_t)p.keys() - 1) >> p.keysLog); }
+
+// The blocks that rows at positions from `top` on (or at it) read, of which none sees a position behind `bottom`, of a sequence that has `length`: `sinks` blocks of the
+// first positions that stay visible, then those from `window`, where the first row's window begins, on.  Rows below position 0 see nothing.
+struct RowBlocks {
+    int32_t sinks, window, all;
+};
+__host__ __device__ inline RowBlocks rowBlocks(const AttentionPlan &p, int32_t window, int32_t sinks, int32_t top, int32_t bottom, int32_t length) {
+    const auto most = [](int32_t a, int32_t b) { return a > b ? a : b; };
+    const auto least = [](int32_t a, int32_t b) { return a < b ? a : b; };
+    const int32_t high = most(least(bottom + 1, length), 0), low = window ? most(most(top, -1) - window + 1, 0) : 0;
+    const int32_t first = blocksTo(p, least(least(sinks, low), high)), from = most(low >> p.keysLog, first);
+    return {first, from, first + most(blocksTo(p, high) - from, 0)};
+}
+
+// The blocks that a tile of a sequence can see at most.  treeRows: of its rows, those that can be a tree's; 0: rows follow one another.
+__host__ __device__ inline int32_t seqBlocks(const AttentionPlan &p, int32_t window, int32_t sinks, int32_t treeRows, int32_t first, int32_t count, int32_t length) {
+    const int32_t blocks = blocksTo(p, length);
+    if (!window) return blocks;
+    const int32_t some = blocks < p.windowBlocks ? blocks : p.windowBlocks;
+    if (!treeRows) return some;
+    // what the last tile reads; trees of a batch differ, and parts that are cut for the widest would be left empty (eight of up to 200 rows, windows
+    // of 1024: 37.2 us, so 36.7; 33 to 60 tokens of ten sequences, eight heads of 128, windows of 40 41 and 25)
+    const int32_t last = rowBlocks(p, window, sinks, first, first + (count < treeRows ? count : treeRows) - 1, length).all;
+    return some < last ? some : last;
+}
+
 // Blocks of a part of a tile's run (of a stream's where the launch is of streams), up to how many a tile's run stays whole, and blocks of a part of a stream
 // among tiles.
 struct PartBlocks {

@@ -41,7 +41,6 @@ __device__ __forceinline__ bool sees(uint32_t window, int sinks, int p, int j) {
 struct SeqWork {
     int begin, count, first, length, tiles, blocks;
 };
-__device__ __forceinline__ int blocksTo(const AttentionPlan &p, int end) { return (int)(((uint32_t)end + (uint32_t)p.keys() - 1) >> p.keysLog); }  // a last block may pass 2^31
 __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const AttentionPlan &p, int s) {
     const CacheArgs &c = a.c;
     SeqWork w;
@@ -51,15 +50,7 @@ __device__ __forceinline__ SeqWork measureSeq(const AttentionArgs &a, const Atte
     if (s >= c.S) w.count = 0;
     w.length = c.pages ? min(w.first + w.count, c.capacity) : w.count;
     w.tiles = (int)(((uint32_t)w.count * (uint32_t)a.G + (uint32_t)p.rows() - 1) >> p.rowsLog);
-    w.blocks = blocksTo(p, w.length);
-    if (a.window) w.blocks = min(w.blocks, p.windowBlocks);
-    if (a.window && a.tree_rows) {
-        // what the last tile reads (spanOf); trees of a batch differ, and parts that are cut for the widest would be left empty (eight of up to 200 rows, windows
-        // of 1024: 37.2 us, so 36.7; 33 to 60 tokens of ten sequences, eight heads of 128, windows of 40 41 and 25)
-        const int high = max(min(w.first + min(w.count, a.tree_rows), w.length), 0), low = max(max(w.first, -1) - a.window + 1, 0);
-        const int sinkBlocks = blocksTo(p, min(min(a.sinks, low), high));
-        w.blocks = min(w.blocks, sinkBlocks + max(blocksTo(p, high) - max(low >> p.keysLog, sinkBlocks), 0));
-    }
+    w.blocks = seqBlocks(p, a.window, a.sinks, a.tree_rows, w.first, w.count, w.length);
     return w;
 }
 
@@ -233,10 +224,10 @@ __device__ __forceinline__ Span spanOf(const AttentionArgs &a, const AttentionPl
     const int last = (int)fastDiv((uint32_t)(r0 + s.rows - 1), a.g);
     // of a tree places, whose rows may stand at any positions from the first on
     const int top = it.w.first + (TREE ? 0 : (int)fastDiv((uint32_t)r0, a.g)), bottom = it.w.first + (TREE ? min(last, a.tree_rows - 1) : last);
-    const int high = max(min(bottom + 1, it.w.length), 0), low = a.window ? max(max(top, -1) - a.window + 1, 0) : 0;  // rows below position 0 see nothing
-    s.sinkBlocks = blocksTo(p, min(min(a.sinks, low), high));
-    s.windowBlock = max(low >> p.keysLog, s.sinkBlocks);
-    const int all = s.sinkBlocks + max(blocksTo(p, high) - s.windowBlock, 0);
+    const RowBlocks blocks = rowBlocks(p, a.window, a.sinks, top, bottom, it.w.length);
+    s.sinkBlocks = blocks.sinks;
+    s.windowBlock = blocks.window;
+    const int all = blocks.all;
     s.from = min(it.splits > 1 ? it.split * it.part : 0, all);
     s.to = it.splits > 1 ? min(all, s.from + it.part) : all;
     return s;
