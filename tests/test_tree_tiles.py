@@ -243,3 +243,9 @@ def test_blocks_of_a_tile(tmp_path, seed):
     assert run.returncode == 0 and int(run.stdout) > 1000, run.stdout[-2000:]
     short = subprocess.run([exe, str(seed), "short"], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
     assert short.returncode == 1 and "FAIL" in short.stdout and "blocks, the sequence counts" in short.stdout, short.stdout[-2000:]
+
+
+def test_streams_or_tiles(tmp_path):
+    """The plan's choice next to what both sides took (tests/host/tree_rule.cpp)."""
+    done = subprocess.run([host_check("tree_rule", tmp_path)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=60)
+    assert done.returncode == 0, done.stdout

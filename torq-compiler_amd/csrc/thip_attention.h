@@ -143,13 +143,15 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     p.tiles = rows > 32 * S && (D <= 128 || rows * KVH > 2048);
     // The rows of a tree have all of the text before it to read, so few tiles are few workgroups with long runs, and streams the faster: up to 64 full tiles
     // (of heads above 128 32, of int8 128), but where the reading takes longer than the runs do, and a tile spares it for more streams than its work costs (four; of
-    // int8, which streams read the better, six).  us, streams / tiles, by rows a sequence: 48 rows, four key heads of 128, 2479 positions of int8 13 / 39; 512, one, 7323
-    // 17 / 50; 342, 20 sequences, eight of 80, 434 69 / 37; 254, three sequences, eight of 256 167 / 78; 204, eight sequences, eight of 256, 3131 of int8 188 / 213; 117,
-    // seven sequences, four of 128, 18648 260 / 122; 42, 46 sequences, two of 128, 12317 of int8 126 / 207.  Not the faster side: 37, 32 sequences, eight of 80, 761 of int8 30 / 34.
+    // int8, which streams read the better, six, and of its heads above 128, whose tiles are slow, where there are more blocks).  us, streams / tiles, by rows a sequence: 48 rows,
+    // four key heads of 128, 2479 positions of int8 13 / 39; 516, one, 7323 with a window of 2275 17 / 50; 343, 20 sequences, eight of 80, 645 68 / 36; 257, three sequences,
+    // eight of 256, 2909 166 / 77; 119, seven sequences, four of 128, 25556 260 / 121; 45, 46 sequences, two of 128, 19909 of int8 123 / 206; heads of 256 of int8: 205, eight
+    // sequences, eight key heads, 4330 (17280 blocks of tiles) 188 / 212; 1538, two, four, 8192 (26624) 296 / 284; 553, two, eight, 20000 (50080) 557 / 437.  Not the faster
+    // side: 37, 32 sequences, eight of 80, 1122 of int8, windows of 512, 31 / 34; 690, four sequences, eight of 256, 1024 of int8 81 / 90.
     if (tree) {
         const int64_t each = (rows - 1) / S + 1, streams = (each + 15) / 16, tiles = (each + 127) / 128, blocks = (window && window < capacity ? window : capacity) / 32;
         p.tiles = rows > 32 * S && (rows * KVH >= (D <= 128 ? 64 : quantised ? 128 : 32) * 128 ||
-                                    (streams > (quantised ? 6 : 4) * tiles && tiles * S * KVH * blocks >= (quantised ? 16384 : 2048)));
+                                    (streams > (quantised ? 6 : 4) * tiles && tiles * S * KVH * blocks >= (!quantised ? 2048 : D <= 128 ? 16384 : 24576)));
     }
     // The second part costs a prompt of 8192 tokens with 32 heads of 128 a third (153 us, 201 with it), four chunks of up to 512 a quarter (167, 210); the error of a
     // result goes from 1.4 times that of its rounding alone to 1.0.  Over many rows that is what it is; over few it may be 1.7 times in one call.
