@@ -490,8 +490,9 @@ typedef struct thip_lm_attention_t {
  * base - 1 with base = lengths[s] - n_s.  A parent comes before its children; an entry that is not below the row's own number counts as -1.  A row with d
  * rows above it on its path stands at position base + d of the text, and sees the positions before the tree, j < base, and the rows of its path, itself
  * among them, where (window == 0, or the seen one's position of the text > its own - window, or that position < sinks).  The rest is as in thip_lm_attention.
- * What rows at places that are not there, or of a sequence behind its first THIP_LM_TREE_ROWS, see is nothing, and nobody sees them.  parents is a
- * binding, a view of one, or a constant.  Its weights meet their values as thip_lm_attention says. */
+ * A row at a place below 0, or behind its sequence's first THIP_LM_TREE_ROWS, sees nothing, and nobody sees it.  A row whose place has no page, or lies behind the
+ * table's end, is seen by nobody, itself among them, and sees the rest of its path and the text.  parents is a binding, a view of one, or a constant.  Weights
+ * meet their values as thip_lm_attention says; over an I8 cache with D above 128 as two bf16 in most records of T * heads below 16384 too. */
 #define THIP_LM_TREE_ROWS 512
 typedef struct thip_lm_tree_attention_t {
     thip_value_t init;
@@ -552,7 +553,8 @@ typedef struct thip_lm_rotary_t {
  * BF16 [rows, N], [rows, 1], [1, N] or [1, 1], rows those of input (the product of its other dimensions).  THIP_NO_VALUE leaves out: residual (0),
  * gate (1), post_weight (no norm of the input), residual_out, or init with its weight, one of the last two at most.  All is held in 32 bits
  * between, rounded where it is stored: init is the norm of h before its rounding.  Squares that would pass 32 bits are taken of scaled values, so rows
- * of any finite values have their norm.  init may be the input's own bytes, residual_out those of a residual of its type; operands share no bytes otherwise. */
+ * of any finite values have their norm, small elements next to large ones theirs in full.  init may be the input's own bytes, residual_out those of a
+ * residual of its type; operands share no bytes otherwise. */
 typedef struct thip_lm_norm_t {
     thip_value_t init;
     thip_value_t residual_out;

@@ -155,6 +155,7 @@ inline AttentionPlan attentionPlan(int64_t T, int64_t S, int64_t H, int64_t KVH,
     }
     // The second part costs a prompt of 8192 tokens with 32 heads of 128 a third (153 us, 201 with it), four chunks of up to 512 a quarter (167, 210); the error of a
     // result goes from 1.4 times that of its rounding alone to 1.0.  Over many rows that is what it is; over few it may be 1.7 times in one call.
+    // Trees of as many rows pay 30.5 to 32.9 (eight of up to 200 rows, windows of 1024) and 159 to 230 (16 of up to 64 over int8: 25 registers spill, not 9).
     p.fine = T * H < 8192;
     p.rowsLog = p.tiles ? 7 : 4;
     p.keysLog = p.tiles && D <= 64 ? 6 : 5;

@@ -2,7 +2,9 @@
 //
 // h = r + s g u, u = x or x c(x) (p + o); out = h c(h) (w + o), c(x) = 1 / sqrt(mean(x^2) + eps).  One pass: a row lies in the registers of its lanes, in
 // pieces of eight elements that are neighbours, so each operand is read once and each result written once.  Bound by memory (4096 rows of 4096, the residual in 32
-// bits, 201 MB: 40 us, 5.1 TB/s), or, of few rows, by the launch and the chain from the loads over the sums to the stores (8 rows of 1152: 2.9 us).
+// bits, 201 MB: 40 us, 5.1 TB/s), or, of few rows, by the launch and the chain from the loads over the sums to the stores (8 rows of 1152: 2.9 us).  Of the longest rows
+// a lane's part does not quite fit: above 16384 elements, where an operand has 32 bits or the length is no multiple of 8, 6 to 42 of its registers lie in memory, above 8192
+// with both of these 10 (100 rows, a residual and both norms: of 32768 10.0 us, of 30001 14.7; with the residual in 32 bits 22.2 and 24.7).
 #include "thip_layer.h"
 #include "thip_kernels_common.h"
 #include "thip_lanes.h"
